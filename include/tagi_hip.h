@@ -606,6 +606,98 @@ int tagi_embedding_bwd(const float* tokens, const float* dmz, const float* dSz, 
                        int64_t padding_idx, float* ws, int64_t ws_bytes, tagi_stream_t stream);
 int64_t tagi_embedding_bwd_ws_bytes(int64_t n_tokens, int64_t V, int64_t D);
 
+/* Embedding lookup with a scale, and the parameter deltas of the table by sorted tokens (no
+ * counterpart in the reference, whose Embedding (embedding.py:88-150) has neither):
+ *   mz[t] = c mw[id_t],  Sz[t] = c^2 Sw[id_t]
+ *   dmw[v] = c Sw[v] sum_{id_t = v} dmz[t],  dSw[v] = (c Sw[v])^2 sum_{id_t = v} dSz[t]
+ * ids: n of the given type; float ids are cast toward zero. Ids equal to padding_idx or
+ * outside [0, V) look up zeros and add nothing. dmw/dSw (V, D) are overwritten whole. The
+ * sums' order is fixed by the ids (deterministic); the cost does not grow with V beyond
+ * writing the deltas. n may be 0. n, V < 2^31, D < 2^21. */
+enum { TAGI_IDS_F32 = 0, TAGI_IDS_I32 = 1, TAGI_IDS_I64 = 2 };
+int tagi_embedding_scaled_fwd(const void* ids, int id_type, const float* mw, const float* Sw,
+                              float* mz, float* Sz, int64_t n, int64_t V, int64_t D,
+                              int64_t padding_idx, double scale, tagi_stream_t stream);
+int tagi_embedding_sorted_bwd(const void* ids, int id_type, const float* dmz, const float* dSz,
+                              const float* Sw, float* dmw, float* dSw, int64_t n, int64_t V,
+                              int64_t D, int64_t padding_idx, double scale, void* ws,
+                              int64_t ws_bytes, tagi_stream_t stream);
+/* The same deltas with the capped update (parameters.py:58-96) applied in place to the rows
+ * that occur in ids; other rows, whose deltas are zero, are not touched. dmw/dSw may be NULL:
+ * the deltas are then applied without being stored. The same bits as
+ * tagi_embedding_sorted_bwd followed by tagi_capped_update, for positive variances. */
+int tagi_embedding_sorted_bwd_update(const void* ids, int id_type, const float* dmz,
+                                     const float* dSz, float* mw, float* Sw, float* dmw, float* dSw,
+                                     float cap_factor, int64_t n, int64_t V, int64_t D,
+                                     int64_t padding_idx, double scale, void* ws, int64_t ws_bytes,
+                                     tagi_stream_t stream);
+int64_t tagi_embedding_sorted_ws_bytes(int64_t n, int64_t V, int64_t D);
+
+/* Sum of two Gaussian streams and its RMSNorm (the sum is resblock.py:183-213, the norm
+ * rms_norm.py:93-110; any row length):
+ *   ms = ma + mr, Ss = Sa + Sr, inv = 1/sqrt(mean(ms^2 + Ss) + eps),
+ *   mz = ms inv g, Sz = inv^2 (Ss (g^2 + Sg) + Sg ms^2)
+ * Ss may be NULL (not stored); ms and inv_rms (rows) are what the backward reads. */
+int tagi_add_rmsnorm_fwd(const float* ma, const float* Sa, const float* mr, const float* Sr,
+                         const float* mw, const float* Sw, float* mz, float* Sz, float* ms,
+                         float* Ss, float* inv_rms, int64_t rows, int64_t D, float eps,
+                         tagi_stream_t stream);
+/* Its backward: deltas of both inputs (one pair, the same for both) from those at z and,
+ * optionally (both NULL without), those that reach the sum itself; and gamma deltas
+ * (rms_norm.py:115-134). */
+int tagi_add_rmsnorm_bwd(const float* dmz, const float* dSz, const float* dms, const float* dSs,
+                         const float* ms, const float* inv_rms, const float* mw, const float* Sw,
+                         float* dma, float* dSa, float* dmw, float* dSw, int64_t rows, int64_t D,
+                         void* ws, int64_t ws_bytes, tagi_stream_t stream);
+int64_t tagi_add_rmsnorm_bwd_ws_bytes(int64_t rows, int64_t D);
+
+/* Linear attention with a decay for each head on Gaussian moments (no counterpart in the
+ * reference). A head's state is D x D independent Gaussians, means M and variances P; with
+ * its decay g and the scale c:
+ *   M_t = g M_{t-1} + k v^T,  P_t = g^2 P_{t-1} + Sk (v^2 + Sv)^T + (k^2) Sv^T
+ *   mo = c M_t^T q,  So = c^2 [P_t^T (Sq + q^2) + (M_t.M_t)^T Sq]
+ * Element (b, t, h, d) of an operand lies at b sb + t st + h sh + d of its strides; a mean
+ * and its variance share them. decay: (H). lengths: NULL or B int32 / int64 (len_bytes 4 / 8)
+ * on the GPU; tokens from a sequence's length on add nothing, are not read and get zeros as
+ * outputs; lengths below 0 or above T count as 0 and T. init_m/init_S: NULL (zeros) or the
+ * state (B, H, D, D) before the first token, [.., d of k, d of v]; end_m/end_S: NULL or the
+ * state after each sequence's last token (the initial one where it is empty). The two pairs
+ * must not overlap. D <= 128. */
+typedef struct {
+  int64_t sb, st, sh;
+} tagi_heads;
+int tagi_linear_attention_fwd(const float* mq, const float* Sq, const float* mk, const float* Sk,
+                              const float* mv, const float* Sv, const tagi_heads* lq,
+                              const tagi_heads* lk, const tagi_heads* lv, const float* decay,
+                              const void* lengths, int len_bytes, const float* init_m,
+                              const float* init_S, float* mo, float* So, const tagi_heads* lo,
+                              float* end_m, float* end_S, int64_t B, int64_t T, int64_t H,
+                              int64_t D, double scale, void* ws, int64_t ws_bytes,
+                              tagi_stream_t stream);
+int64_t tagi_linear_attention_fwd_ws_bytes(int64_t B, int64_t T, int64_t H, int64_t D);
+/* Its backward from a zero initial state, each product's other operand held at its mean (as
+ * multihead_attention.py:209-267): with d = c dmo, e = c^2 dSo,
+ *   dq = M_t d, dSq = (M_t.M_t) e;  G_t = g G_{t+1} + q d^T, N_t = g^2 N_{t+1} + (q^2) e^T
+ *   dk = G_t v, dSk = N_t (v^2);  dv = G_t^T k, dSv = N_t^T (k^2)
+ * The six outputs share the strides lo. */
+int tagi_linear_attention_bwd(const float* mq, const float* mk, const float* mv,
+                              const tagi_heads* lq, const tagi_heads* lk, const tagi_heads* lv,
+                              const float* dmo, const float* dSo, const tagi_heads* ld,
+                              const float* decay, const void* lengths, int len_bytes, float* dmq,
+                              float* dSq, float* dmk, float* dSk, float* dmv, float* dSv,
+                              const tagi_heads* lo, int64_t B, int64_t T, int64_t H, int64_t D,
+                              double scale, void* ws, int64_t ws_bytes, tagi_stream_t stream);
+int64_t tagi_linear_attention_bwd_ws_bytes(int64_t B, int64_t T, int64_t H, int64_t D);
+/* One token of every sequence (operands (B, H, D); st is not read): the state (B, H, D, D) is
+ * advanced in place. active: NULL or B bytes; a sequence whose byte is 0 keeps its state and
+ * gets zeros. */
+int tagi_linear_attention_step(const float* mq, const float* Sq, const float* mk, const float* Sk,
+                               const float* mv, const float* Sv, const tagi_heads* lq,
+                               const tagi_heads* lk, const tagi_heads* lv, const float* decay,
+                               const uint8_t* active, float* state_m, float* state_S, float* mo,
+                               float* So, const tagi_heads* lo, int64_t B, int64_t H, int64_t D,
+                               double scale, tagi_stream_t stream);
+
 /* Sinusoidal positional encoding add (positional_encoding.py:62): out = ma + pe[:S]. */
 int tagi_pe_add(const float* ma, const float* pe, float* out, int64_t B, int64_t S, int64_t E,
                 tagi_stream_t stream);

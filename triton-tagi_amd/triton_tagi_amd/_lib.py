@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_uint64, c_void_p
 from pathlib import Path
 
 import torch
@@ -54,6 +54,7 @@ class Plan(ctypes.Structure):
 P = c_void_p
 I64 = c_int64
 F = c_float
+DBL = c_double
 class BnPending(ctypes.Structure):
     """tagi_bn_bwd_pending: one BatchNorm2D layer whose parameter deltas are still to form."""
 
@@ -62,10 +63,17 @@ class BnPending(ctypes.Structure):
     ] + [(n, c_void_p) for n in ("cSb", "cdmb", "cdSb")] + [("nblk", c_int64)]
 
 
+class Heads(ctypes.Structure):
+    """tagi_heads: element (b, t, h, d) at b*sb + t*st + h*sh + d."""
+
+    _fields_ = [(n, c_int64) for n in ("sb", "st", "sh")]
+
+
 VP = POINTER(TagiView)
 GP = POINTER(ConvGeom)
 BP = POINTER(BnPending)
 PP = POINTER(Plan)
+HP = POINTER(Heads)
 OP_FWD, OP_FWD_FIXED, OP_BWD_DELTA, OP_WGRAD = range(4)  # TAGI_OP_*
 
 # name -> (restype, argtypes)
@@ -137,6 +145,20 @@ _SIGS = {
     "tagi_bn_relu_bwd_bias_ws_bytes": (I64, [I64, I64, I64]),
     "tagi_bn_bwd_finalize_multi": (c_int, [BP, I64, P]),
     "tagi_rmsnorm_fwd": (c_int, [P, P, P, P, P, P, P, I64, I64, F, P]),
+    "tagi_embedding_scaled_fwd": (c_int, [P, c_int, P, P, P, P, I64, I64, I64, I64, DBL, P]),
+    "tagi_embedding_sorted_bwd": (c_int, [P, c_int, P, P, P, P, P, I64, I64, I64, I64, DBL, P, I64, P]),
+    "tagi_embedding_sorted_bwd_update": (c_int, [P, c_int, P, P, P, P, P, P, F, I64, I64, I64, I64, DBL, P, I64, P]),
+    "tagi_embedding_sorted_ws_bytes": (I64, [I64, I64, I64]),
+    "tagi_add_rmsnorm_fwd": (c_int, [P, P, P, P, P, P, P, P, P, P, P, I64, I64, F, P]),
+    "tagi_add_rmsnorm_bwd": (c_int, [P, P, P, P, P, P, P, P, P, P, P, P, I64, I64, P, I64, P]),
+    "tagi_add_rmsnorm_bwd_ws_bytes": (I64, [I64, I64]),
+    "tagi_linear_attention_fwd": (c_int, [P, P, P, P, P, P, HP, HP, HP, P, P, c_int, P, P, P, P, HP, P, P, I64, I64,
+                                          I64, I64, DBL, P, I64, P]),
+    "tagi_linear_attention_fwd_ws_bytes": (I64, [I64, I64, I64, I64]),
+    "tagi_linear_attention_bwd": (c_int, [P, P, P, HP, HP, HP, P, P, HP, P, P, c_int, P, P, P, P, P, P, HP, I64, I64,
+                                          I64, I64, DBL, P, I64, P]),
+    "tagi_linear_attention_bwd_ws_bytes": (I64, [I64, I64, I64, I64]),
+    "tagi_linear_attention_step": (c_int, [P, P, P, P, P, P, HP, HP, HP, P, P, P, P, P, P, HP, I64, I64, I64, DBL, P]),
     "tagi_rmsnorm_bwd": (c_int, [P, P, P, P, P, P, P, P, P, P, I64, I64, P, I64, P]),
     "tagi_rmsnorm_bwd_ws_bytes": (I64, [I64, I64]),
     "tagi_embedding_fwd": (c_int, [P, P, P, P, P, I64, I64, I64, I64, P]),
@@ -204,6 +226,17 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed (status {rc}): {last_error()}")
 
 
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``call`` with t's GPU as the current device (a launch on another device's stream is
+    refused by the runtime); nothing is switched when it is current already."""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args)
+
+
 _queries: dict = {}
 
 
@@ -251,6 +284,23 @@ def check(t: torch.Tensor, name: str, contiguous: bool = True) -> torch.Tensor:
         )
     if contiguous and not (t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last))):
         raise ValueError(f"{name}: tensor must be dense (contiguous or channels-last)")
+    return t
+
+
+def check_with(t: torch.Tensor, name: str, ref: torch.Tensor, shape=None) -> torch.Tensor:
+    """``check`` without a layout, and on ref's GPU; ``shape`` as well when given."""
+    check(t, name, contiguous=False)
+    if t.get_device() != ref.get_device():
+        raise ValueError(f"{name}: tensor is on {t.device}, expected {ref.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def check_in_place(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A tensor that a kernel writes: contiguous, so that no copy would take the writes."""
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: updated in place, must be contiguous")
     return t
 
 
