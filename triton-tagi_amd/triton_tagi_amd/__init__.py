@@ -16,12 +16,14 @@ from .layers import (
     Flatten,
     LayerNorm,
     Linear,
+    LinearAttention,
     MaxPool2D,
     MultiheadAttentionV2,
     PositionalEncoding,
     ReLU,
     Remax,
     ResBlock,
+    ResidualRMSNorm,
     RMSNorm,
 )
 from .checkpoint import RunDir, load_model
@@ -51,4 +53,5 @@ __all__ = [
     "init_weight_bias_norm", "compute_innovation", "get_cap_factor", "update_parameters", "EvenSoftplus",
     "LayerNorm", "MaxPool2D", "RunDir", "load_model", "HierarchicalSoftmax", "class_to_obs", "labels_to_hrc",
     "obs_to_class_probs", "get_predicted_labels", "compute_innovation_with_indices", "hrc_innovation",
+    "LinearAttention", "ResidualRMSNorm",
 ]

@@ -4,22 +4,44 @@ Forward: (mu, S) = (mw[cat], Sw[cat]) for the integer ids carried in ``ma`` (cas
 zero, like ``.long()``); ids equal to padding_idx give zeros. Backward accumulates
 delta_mw[cat] += delta_mu * Sw[cat], delta_Sw[cat] += delta_S * Sw[cat]^2 and returns
 zero input deltas (the index is discrete).
+
+Two additions without a counterpart in the reference: ``output_scale`` c multiplies the
+moments looked up (means by c, variances by c^2; with it the deltas sum c delta_mu Sw and
+(c Sw)^2 delta_S), and ``sorted_deltas`` forms the deltas by sorting the tokens instead of
+scanning them once per category, which a large table needs. Within ``update_in_backward``
+the sorted form applies the capped update to the rows that occur as it forms their deltas.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 from torch import Tensor
 
 from .. import _lib
 from ..base import LearnableLayer
+from ..kernels.embedding import embedding_lookup, embedding_param_deltas, embedding_update
 from ..param_init import gaussian_param_init
+from ..update import in_backward
 from ..update.parameters import update_parameters
 
 
 class Embedding(LearnableLayer):
     def __init__(self, num_embeddings: int, embedding_dim: int, input_size: int = 0, scale: float = 1.0,
-                 padding_idx: int = -1, device: str = "cuda") -> None:
+                 padding_idx: int = -1, device: str = "cuda", output_scale: float = 1.0,
+                 sorted_deltas: bool | None = None) -> None:
+        """``sorted_deltas``: None takes the sorted form where ``output_scale`` is not 1 (the
+        scan knows no scale) and the scan otherwise. The sorted form also takes integer ids."""
+        output_scale = float(output_scale)
+        if not math.isfinite(output_scale):
+            raise ValueError(f"output_scale must be finite, got {output_scale}")
+        if sorted_deltas is None:
+            sorted_deltas = output_scale != 1.0
+        if not sorted_deltas and output_scale != 1.0:
+            raise ValueError("an output_scale needs sorted_deltas")
+        self.output_scale = output_scale
+        self.sorted_deltas = bool(sorted_deltas)
         self.num_embeddings = num_embeddings
         self.embedding_dim = embedding_dim
         self.input_size = input_size
@@ -35,6 +57,9 @@ class Embedding(LearnableLayer):
     def forward(self, ma: Tensor, Sa: Tensor) -> tuple[Tensor, Tensor]:
         if ma.dim() == 3 and ma.shape[-1] == 1:
             ma = ma.squeeze(-1)
+        if self.sorted_deltas:
+            self.cat_idx = ma.contiguous()
+            return embedding_lookup(self.cat_idx, self.mw, self.Sw, self.output_scale, self.padding_idx)
         tokens = _lib.check(ma.contiguous(), "ma")
         self.cat_idx = tokens
         D = self.embedding_dim
@@ -54,6 +79,17 @@ class Embedding(LearnableLayer):
         """The parameter deltas of ``backward`` without the (zero) deltas of the token ids;
         returns the ids."""
         tokens = self.cat_idx
+        if self.sorted_deltas:
+            upd = in_backward.active()
+            if upd is not None:
+                self.delta_mw, self.delta_Sw = embedding_update(
+                    tokens, delta_mz, delta_Sz, self.mw, self.Sw, upd.cap_factor, self.output_scale, self.padding_idx,
+                    upd.keep_deltas)
+            else:
+                self.delta_mw, self.delta_Sw = embedding_param_deltas(
+                    tokens, delta_mz, delta_Sz, self.Sw, self.output_scale, self.padding_idx)
+            self._updated_in_backward = upd is not None
+            return tokens
         D = self.embedding_dim
         dm = _lib.check(delta_mz.reshape(-1, D).contiguous(), "delta_mz")
         dS = _lib.check(delta_Sz.reshape(-1, D).contiguous(), "delta_Sz")
@@ -71,6 +107,9 @@ class Embedding(LearnableLayer):
         return [(self.mw, self.Sw, self.delta_mw, self.delta_Sw)]
 
     def update(self, cap_factor: float) -> None:
+        if self._updated_in_backward:  # the backward pass applied it (update_in_backward)
+            self._updated_in_backward = False
+            return
         update_parameters(self.mw, self.Sw, self.delta_mw, self.delta_Sw, cap_factor)
 
     @property

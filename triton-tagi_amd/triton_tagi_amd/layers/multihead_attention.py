@@ -20,21 +20,18 @@ concatenates or splits tensors.
 
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
 from torch import Tensor
 
-from .. import _lib, _overlap
-from ..base import LearnableLayer
-from ..kernels.common import fused_backward_delta, linear_forward, linear_param_deltas
-from ..update.parameters import update_parameters_multi
-from .linear import Linear
+from .. import _lib
+from ..kernels.common import fused_backward_delta, linear_forward
+from ._qkv import QkvProjections
 from .remax import remax
 
 
-class MultiheadAttentionV2(LearnableLayer):
+class MultiheadAttentionV2(QkvProjections):
     def __init__(self, embed_dim: int, num_heads: int, seq_len: int, num_kv_heads: int | None = None,
                  bias: bool = False, gain_weight: float = 1.0, gain_bias: float = 1.0, init_method: str = "He",
                  pos_emb: str = "", use_causal_mask: bool = False, device: str = "cuda") -> None:
@@ -61,10 +58,7 @@ class MultiheadAttentionV2(LearnableLayer):
         self.q_output_size = num_heads * self.head_dim
         self.k_output_size = num_kv_heads * self.head_dim
         self.v_output_size = num_kv_heads * self.head_dim
-        kw = dict(device=device, init_method=init_method, gain_w=gain_weight, gain_b=gain_bias, bias=bias)
-        self.q_proj = Linear(embed_dim, self.q_output_size, **kw)
-        self.k_proj = Linear(embed_dim, self.k_output_size, **kw)
-        self.v_proj = Linear(embed_dim, self.v_output_size, **kw)
+        self._make_projections(self.q_output_size)
         self._scale = 1.0 / math.sqrt(self.head_dim)
         self._cache: dict | None = None
         self._attn_mu: Tensor | None = None
@@ -81,48 +75,6 @@ class MultiheadAttentionV2(LearnableLayer):
     @staticmethod
     def _score_view(S: int, transpose: bool = False):
         return _lib.view(1, S * S, 0, 1, S) if transpose else _lib.view(1, S * S, 0, S, 1)
-
-    def _projections(self):
-        return (self.q_proj, self.k_proj, self.v_proj)
-
-    _QKV_ATTRS = ("mw", "Sw", "mb", "Sb")
-
-    def _qkv_params(self) -> dict:
-        """The three projections' parameters side by side: (E, 3E) weights and (1, 3E)
-        biases, which the fused projection product and the update read directly. Each
-        projection's mw, Sw, mb, Sb are column views of them, so in-place changes to either
-        are seen by both (checkpoint restore copies in place). Built at the first forward;
-        rebuilt from the projections' tensors if any of them was replaced since."""
-        projs = self._projections()
-        bufs = getattr(self, "_qkv", None)
-        if bufs is not None and self._qkv_intact(bufs):
-            return bufs
-        bufs = {}
-        for attr in self._QKV_ATTRS:
-            parts = [getattr(p, attr) for p in projs]
-            if parts[0] is None:
-                continue
-            buf = torch.cat(parts, 1)
-            n = parts[0].shape[1]
-            for i, p in enumerate(projs):
-                setattr(p, attr, buf[:, i * n:(i + 1) * n])
-            bufs[attr] = buf
-        self._qkv = bufs
-        return bufs
-
-    def _qkv_intact(self, bufs: dict) -> bool:
-        for attr, buf in bufs.items():
-            n = buf.shape[1] // 3
-            for i, p in enumerate(self._projections()):
-                t = getattr(p, attr, None)
-                if not (isinstance(t, Tensor) and t.device == buf.device and t.dtype == buf.dtype
-                        and tuple(t.shape) == (buf.shape[0], n) and t.stride() == buf.stride()
-                        and t.data_ptr() == buf.data_ptr() + i * n * buf.element_size()):
-                    return False
-        return True
-
-    def sublayers(self) -> tuple:
-        return self._projections()
 
     def forward(self, ma: Tensor, Sa: Tensor) -> tuple[Tensor, Tensor]:
         B, S, E = ma.shape
@@ -235,49 +187,12 @@ class MultiheadAttentionV2(LearnableLayer):
                       D, sv, hL, hL, s, s * s, 0, st)
             _lib.call("tagi_bmm_shared", scaled_mu.data_ptr(), scaled_var.data_ptr(), q_m, dk_m, dk_S, B * H, S, S,
                       D, svt, hL, hL, s, s * s, 0, st)
-        # the three projections' parameter deltas in one product (on the side stream within
-        # a step when large), their input deltas in one product over the 3E deltas
-        # (the sum of the three projections' input deltas, multihead_attention.py:262-267)
-        projs = self._projections()
-        ma_in = c["ma_in"]
-        ctx = _overlap.active()
-        big = ma_in.shape[0] * E * L >= _overlap.MIN_MACS_LINEAR
-        side = ctx.fork(dev, ma_in, dqkv_m, dqkv_S, c["w_S"], c["b_S"]) if ctx is not None and big else None
-        with torch.cuda.stream(side) if side is not None else contextlib.nullcontext():
-            dmw, dSw, dmb, dSb = linear_param_deltas(ma_in, dqkv_m, dqkv_S, c["w_S"], c["b_S"])
-        # each projection's deltas are column views of the (E, 3E) ones, as its parameters
-        # are of the side-by-side buffers the update applies them to
-        self._qkv_deltas = (dmw, dSw, dmb, dSb)
-        for i, p in enumerate(projs):
-            cols = slice(i * E, (i + 1) * E)
-            p.delta_mw, p.delta_Sw = dmw[:, cols], dSw[:, cols]
-            if self.has_bias:
-                p.delta_mb, p.delta_Sb = dmb[:, cols], dSb[:, cols]
+        # the three projections' parameter deltas, then their input deltas in one product over
+        # the 3E deltas (the sum of the three projections' input deltas,
+        # multihead_attention.py:262-267)
+        self._projection_param_deltas(c, dqkv_m, dqkv_S)
         dma, dSa = fused_backward_delta(dqkv_m, dqkv_S, c["w_m"])
         return dma.reshape(B, S, E), dSa.reshape(B, S, E)
-
-    def _update_items(self):
-        return self.q_proj._update_items() + self.k_proj._update_items() + self.v_proj._update_items()
-
-    def _update_groups(self):
-        """The update over the side-by-side buffers: two groups (weights, biases) instead
-        of six, the same values element by element."""
-        bufs = getattr(self, "_qkv", None)
-        deltas = getattr(self, "_qkv_deltas", None)
-        if bufs is None or deltas is None or not self._qkv_intact(bufs):
-            return self._update_items()
-        dmw, dSw, dmb, dSb = deltas
-        groups = [(bufs["mw"], bufs["Sw"], dmw, dSw)]
-        if self.has_bias:
-            groups.append((bufs["mb"], bufs["Sb"], dmb, dSb))
-        return groups
-
-    def update(self, cap_factor: float) -> None:
-        update_parameters_multi(self._update_groups(), cap_factor)
-
-    @property
-    def num_parameters(self) -> int:
-        return self.q_proj.num_parameters + self.k_proj.num_parameters + self.v_proj.num_parameters
 
     def get_attention_scores(self) -> tuple[Tensor, Tensor]:
         if self._attn_mu is None:

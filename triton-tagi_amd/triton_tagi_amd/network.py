@@ -21,6 +21,7 @@ from .layers.embedding import Embedding
 from .layers.linear import Linear
 from .layers.fused import backward_chain, defer_bn_parameter_deltas, forward_chain
 from .layers.multihead_attention import MultiheadAttentionV2
+from .layers.serving import check_layers, run_prompt, run_step
 from .update.observation import compute_innovation, hrc_innovation
 from .update.in_backward import update_in_backward
 from .update.parameters import get_cap_factor, update_parameters_multi
@@ -76,6 +77,27 @@ class Sequential:
         else:
             Sa = torch.zeros_like(x)
         return forward_chain(self.layers, x, Sa)
+
+    def _serving_input(self, x: Tensor) -> tuple[Tensor, Tensor | None]:
+        check_layers(self.layers)
+        first = self.layers[0] if self.layers else None
+        return x, (None if isinstance(first, (Linear, Embedding)) else torch.zeros_like(x))
+
+    def prompt(self, x: Tensor, lengths: Tensor | None = None, states: list | None = None):
+        """Whole sequences through layers that carry states (LinearAttention, also inside
+        ResidualRMSNorm) and layers that act on each token by itself: (means, variances,
+        states after each sequence's last token). ``x`` (B, T) token ids or (B, T, features);
+        ``lengths`` (B,) ends the sequences of a padded batch; ``states`` continues earlier
+        ones (not written). Causal: the same moments as ``forward`` on whole sequences."""
+        return run_prompt(self.layers, *self._serving_input(x), lengths, states)
+
+    def decode(self, x: Tensor, states: list, active: Tensor | None = None) -> tuple[Tensor, Tensor]:
+        """The next token of every sequence, ``x`` (B, 1) ids or (B, 1, features): moments
+        (B, 1, ...). ``states`` (from ``prompt``) are advanced in place; ``active`` (B,):
+        sequences that are off keep theirs, and their outputs mean nothing."""
+        if x.dim() < 2 or x.shape[1] != 1:
+            raise ValueError(f"decode: expected one token of every sequence, (B, 1), got {tuple(x.shape)}")
+        return run_step(self.layers, *self._serving_input(x), states, active)
 
     def backward(self, delta_mu: Tensor, delta_var: Tensor) -> tuple[Tensor, Tensor]:
         return backward_chain(self.layers, delta_mu, delta_var)
