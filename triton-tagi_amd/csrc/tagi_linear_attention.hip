@@ -21,9 +21,9 @@
 // values each lane keeps.
 //
 // Decay without a multiplication per token: inside a group of 8 tokens the state is kept
-// divided by g^j (token j), the powers go into the token's vectors when they are staged,
-// and the state is multiplied by g^8 (as a two-part float: its rounding would repeat every
-// group) between groups. |g| < 0.05 would overflow the powers and decays token by token.
+// divided by g^j (token j), the powers go into the token's vectors when they are staged, and
+// the state is multiplied by g^8 between groups. |g| < 0.05 would overflow the powers and
+// decays token by token.
 #include "tagi_common.h"
 
 namespace tagi {
@@ -37,12 +37,13 @@ enum Mode { FWD = 0, DQ = 1, DK = 2, DV = 3 };
 // vectors staged per token, over i and over o
 constexpr int n_ivec(int m) { return m == FWD ? 6 : (m == DQ ? 3 : 4); }
 constexpr int n_ovec(int m) { return m == FWD ? 3 : (m == DQ ? 1 : 2); }
+constexpr int scan_threads(int di) { return di <= 4 ? 64 : 16 * di; }
 
 struct Args {
   // DQ/DK/DV read the means and the deltas (dm, dS) only
   const float *mq, *Sq, *mk, *Sk, *mv, *Sv, *dm, *dS;
   tagi_heads lq, lk, lv, ld, lo;  // strides; lo of the outputs
-  float *om, *oS;
+  float *om, *oS, *km, *kS, *vm, *vS;  // outputs (backward: of the queries, keys and values)
   const float* decay;
   const void* lengths;
   int len_bytes;
@@ -51,11 +52,10 @@ struct Args {
   float c, c2;
   int64_t L;     // tokens per chunk, a multiple of kTok
   int64_t nch;
-  const float *pre_m, *pre_S;  // state before each chunk (nch > 1), [bh][chunk][D][D]
-  int pre_t;                   // pre is stored [o][i]
+  // states before each chunk (nch > 1), [bh][chunk][D][D]: M, P; last token first: G, N
+  float *pre_m, *pre_S, *pre_g, *pre_n;
   const float *init_m, *init_S;  // state before the first token, or null
   float *end_m, *end_S;          // state after the last token, or null
-  float *sum_m, *sum_S;          // SUM kernels: each chunk's own contribution, [bh][chunk][i][o]
 };
 
 __device__ __forceinline__ int64_t seq_len(const Args& a, int64_t b) {
@@ -136,17 +136,17 @@ __device__ __forceinline__ float4 add4(float4 a, float4 b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
 
-// The scan of one (sequence, head, chunk) per block. SUM: no outputs, the chunk's own
-// contribution to the state is written instead.
-template <int MODE, int DI, int EO, bool VEC, bool SUM>
-__global__ void __launch_bounds__(DI <= 4 ? 64 : DI * 16) scan_kernel(Args a) {
-  constexpr int IP = 8 * DI;                     // padded head dimension
-  constexpr int NT = DI <= 4 ? 64 : DI * 16;     // threads: a wave per 8 * EO columns
+// The scan of one (sequence, head, chunk), one block.
+template <int MODE, int DI, int EO, bool VEC>
+__device__ __forceinline__ void scan(const Args& a, float4* lds) {
+  constexpr int IP = 8 * DI;                  // padded head dimension
+  constexpr int NT = scan_threads(DI);        // a wave per 8 * EO columns
   constexpr bool REV = MODE >= DK, TWO_STATES = MODE != DQ;
-  constexpr int NI = SUM ? (MODE == FWD ? 3 : (MODE == DQ ? 1 : 2)) : n_ivec(MODE), NO = n_ovec(MODE);
-  constexpr int C4 = IP / 4;                     // float4 chunks of a row
-  __shared__ float4 iv[NI][kTok][C4];
-  __shared__ float4 ov[NO][kTok][C4];
+  constexpr int NI = n_ivec(MODE), NO = n_ovec(MODE);
+  constexpr int C4 = IP / 4;                  // float4 chunks of a row
+  // staged vectors: [vector][token][chunk], those over i, then those over o
+  auto iv = [&](int v, int t, int c) -> float4& { return lds[(v * kTok + t) * C4 + c]; };
+  auto ov = [&](int v, int t, int c) -> float4& { return lds[((NI + v) * kTok + t) * C4 + c]; };
 
   const int64_t bid = blockIdx.x, ch = bid % a.nch, bh = bid / a.nch, b = bh / a.H;
   const int h = (int)(bh % a.H), D = a.D;
@@ -156,18 +156,21 @@ __global__ void __launch_bounds__(DI <= 4 ? 64 : DI * 16) scan_kernel(Args a) {
 
   const float g = a.decay[h];
   const bool grouped = fabsf(g) >= kGroupMin;
+  // Between groups the state is multiplied by the float nearest g^8. What that rounds off
+  // would repeat every group, so it is kept: the true state is the kept one times r (its
+  // square for the variances), and r goes into the staged powers like g^j does. A decay that
+  // goes token by token needs none of this: what it rounds off is gone a token later.
   const int per = grouped ? kTok : 1;  // tokens between decays
-  const double gd = (double)g;
-  const Two gm = two(ipow(gd, per)), gS = two(ipow(gd, 2 * per));  // between groups
+  const double gd = (double)g, gp = ipow(gd, per);
+  const float s1 = (float)gp, s2 = (float)(gp * gp);
+  const double e1 = grouped ? gp / (double)s1 : 1.0, e2 = grouped ? gp * gp / (double)s2 : 1.0;
+  const double i1 = 1.0 / e1, i2 = 1.0 / e2;
+  double r1 = 1.0, r2 = 1.0, q1 = 1.0, q2 = 1.0;  // r, r of the variances, and their inverses
 
   // this thread's part of a stage: token st, values 4 sc .. 4 sc + 3
   const int st = tid / C4, sc = tid % C4;
   const bool stager = st < kTok, inside = 4 * sc < D;
-  float up = 1.f, up2 = 1.f, dn = 1.f, dn2 = 1.f;  // g^-j, g^-2j, g^j, g^2j
-  if (grouped && stager) {
-    const double p = ipow(gd, st);
-    dn = (float)p, dn2 = (float)(p * p), up = (float)(1.0 / p), up2 = (float)(1.0 / (p * p));
-  }
+  const double pj = grouped && stager ? ipow(gd, st) : 1.0, ij = 1.0 / pj;  // g^j, g^-j
   const float4 z4 = make_float4(0.f, 0.f, 0.f, 0.f);
 
   const int64_t qb = b * a.lq.sb + h * a.lq.sh, kb = b * a.lk.sb + h * a.lk.sh, vb = b * a.lv.sb + h * a.lv.sh,
@@ -182,19 +185,16 @@ __global__ void __launch_bounds__(DI <= 4 ? 64 : DI * 16) scan_kernel(Args a) {
       const int64_t t = tok(r);
       const int c = 4 * sc;
       if constexpr (MODE == FWD) {
+        x0 = load4<VEC>(a.mq + qb + t * a.lq.st, c, D), x1 = load4<VEC>(a.Sq + qb + t * a.lq.st, c, D);
         x2 = load4<VEC>(a.mk + kb + t * a.lk.st, c, D), x3 = load4<VEC>(a.Sk + kb + t * a.lk.st, c, D);
         x4 = load4<VEC>(a.mv + vb + t * a.lv.st, c, D), x5 = load4<VEC>(a.Sv + vb + t * a.lv.st, c, D);
-        if constexpr (!SUM)
-          x0 = load4<VEC>(a.mq + qb + t * a.lq.st, c, D), x1 = load4<VEC>(a.Sq + qb + t * a.lq.st, c, D);
       } else if constexpr (MODE == DQ) {
         x0 = load4<VEC>(a.mv + vb + t * a.lv.st, c, D), x1 = load4<VEC>(a.mk + kb + t * a.lk.st, c, D);
-        if constexpr (!SUM)
-          x2 = load4<VEC>(a.dm + db + t * a.ld.st, c, D), x3 = load4<VEC>(a.dS + db + t * a.ld.st, c, D);
+        x2 = load4<VEC>(a.dm + db + t * a.ld.st, c, D), x3 = load4<VEC>(a.dS + db + t * a.ld.st, c, D);
       } else {
         x0 = load4<VEC>(a.mq + qb + t * a.lq.st, c, D);
         x1 = load4<VEC>(a.dm + db + t * a.ld.st, c, D), x2 = load4<VEC>(a.dS + db + t * a.ld.st, c, D);
-        if constexpr (!SUM)
-          x3 = MODE == DK ? load4<VEC>(a.mv + vb + t * a.lv.st, c, D) : load4<VEC>(a.mk + kb + t * a.lk.st, c, D);
+        x3 = MODE == DK ? load4<VEC>(a.mv + vb + t * a.lv.st, c, D) : load4<VEC>(a.mk + kb + t * a.lk.st, c, D);
       }
     } else {
       x0 = x1 = x2 = x3 = x4 = x5 = z4;  // nothing to add, and a dead token's output is zero
@@ -202,35 +202,33 @@ __global__ void __launch_bounds__(DI <= 4 ? 64 : DI * 16) scan_kernel(Args a) {
   };
   auto stage = [&]() {
     if (!stager) return;
+    const float dn = (float)(pj * r1), dn2 = (float)(pj * pj * r2);
+    const float up = (float)(ij * q1), up2 = (float)(ij * ij * q2);
     if constexpr (MODE == FWD) {
-      iv[0][st][sc] = mul4(x2, up);
-      iv[1][st][sc] = mul4(x3, up2);
-      iv[2][st][sc] = mul4(mul4(x2, x2), up2);
-      ov[0][st][sc] = x4;
-      ov[1][st][sc] = add4(mul4(x4, x4), x5);
-      ov[2][st][sc] = x5;
-      if constexpr (!SUM) {
-        iv[3][st][sc] = mul4(x0, a.c * dn);
-        iv[4][st][sc] = mul4(add4(x1, mul4(x0, x0)), a.c2 * dn2);
-        iv[5][st][sc] = mul4(x1, a.c2 * dn2);
-      }
+      iv(0, st, sc) = mul4(x2, up);
+      iv(1, st, sc) = mul4(x3, up2);
+      iv(2, st, sc) = mul4(mul4(x2, x2), up2);
+      iv(3, st, sc) = mul4(x0, a.c * dn);
+      iv(4, st, sc) = mul4(add4(x1, mul4(x0, x0)), a.c2 * dn2);
+      iv(5, st, sc) = mul4(x1, a.c2 * (dn * dn));  // of the squared means
+      ov(0, st, sc) = x4;
+      ov(1, st, sc) = add4(mul4(x4, x4), x5);
+      ov(2, st, sc) = x5;
     } else if constexpr (MODE == DQ) {
-      iv[0][st][sc] = mul4(x0, up);
-      ov[0][st][sc] = x1;
-      if constexpr (!SUM) {
-        iv[1][st][sc] = mul4(x2, a.c * dn);
-        iv[2][st][sc] = mul4(x3, a.c2 * dn2);
-      }
+      iv(0, st, sc) = mul4(x0, up);
+      iv(1, st, sc) = mul4(x2, a.c * dn);
+      iv(2, st, sc) = mul4(x3, a.c2 * (dn * dn));
+      ov(0, st, sc) = x1;
     } else {
       const float4 d = mul4(x1, a.c), e = mul4(x2, a.c2), q2 = mul4(x0, x0);
       if constexpr (MODE == DK) {
-        iv[0][st][sc] = mul4(d, up), iv[1][st][sc] = mul4(e, up2);
-        ov[0][st][sc] = x0, ov[1][st][sc] = q2;
+        iv(0, st, sc) = mul4(d, up), iv(1, st, sc) = mul4(e, up2);
+        ov(0, st, sc) = x0, ov(1, st, sc) = q2;
       } else {
-        iv[0][st][sc] = mul4(x0, up), iv[1][st][sc] = mul4(q2, up2);
-        ov[0][st][sc] = d, ov[1][st][sc] = e;
+        iv(0, st, sc) = mul4(x0, up), iv(1, st, sc) = mul4(q2, up2);
+        ov(0, st, sc) = d, ov(1, st, sc) = e;
       }
-      if constexpr (!SUM) iv[2][st][sc] = mul4(x3, dn), iv[3][st][sc] = mul4(mul4(x3, x3), dn2);
+      iv(2, st, sc) = mul4(x3, dn), iv(3, st, sc) = mul4(mul4(x3, x3), dn2);
     }
   };
 
@@ -245,12 +243,14 @@ __global__ void __launch_bounds__(DI <= 4 ? 64 : DI * 16) scan_kernel(Args a) {
       X[k][e] = 0.f;
       if constexpr (TWO_STATES) Y[k][e] = 0.f;
     }
-  const bool from_pre = !SUM && a.nch > 1;
-  const float* sm = from_pre ? a.pre_m : (SUM ? nullptr : a.init_m);
-  const float* sS = from_pre ? a.pre_S : (SUM ? nullptr : a.init_S);
+  fetch(0);
+  const bool from_pre = a.nch > 1;
+  const bool tr = from_pre && MODE != FWD && MODE != DV;  // DQ and DK hold the transposed state
+  const float* sm = from_pre ? (MODE == DQ || MODE == FWD ? a.pre_m : a.pre_g) : (MODE == FWD ? a.init_m : nullptr);
+  const float* sS = from_pre ? (MODE == FWD ? a.pre_S : a.pre_n) : (MODE == FWD ? a.init_S : nullptr);
   if (sm) {
     const int64_t base = (from_pre ? bh * a.nch + ch : bh) * (int64_t)D * D;
-    const bool tr = from_pre && a.pre_t;
+    const float d1 = cnt > 0 ? g : 1.f;  // to before the first token; an empty chunk hands on what it got
 #pragma unroll
     for (int k = 0; k < DI; ++k)
 #pragma unroll
@@ -258,140 +258,269 @@ __global__ void __launch_bounds__(DI <= 4 ? 64 : DI * 16) scan_kernel(Args a) {
         const int i = idx_i(k), o = idx_o(e);
         if (i < D && o < D) {
           const int64_t at = base + (tr ? (int64_t)o * D + i : (int64_t)i * D + o);
-          X[k][e] = sm[at];
-          if constexpr (TWO_STATES) Y[k][e] = sS[at];
+          X[k][e] = d1 * sm[at];
+          if constexpr (TWO_STATES) Y[k][e] = d1 * (d1 * sS[at]);
         }
       }
   }
 
-  fetch(0);
+  auto token = [&](int s0, int j) {
+    float w[NO][EO];
+#pragma unroll
+    for (int v = 0; v < NO; ++v) {
+      const float* p = reinterpret_cast<const float*>(&ov(v, j, 0)) + 8 * EO * wave + EO * og;
+#pragma unroll
+      for (int e = 0; e < EO; ++e) w[v][e] = p[e];
+    }
+    float pm[EO] = {}, ps[EO] = {};
+#pragma unroll
+    for (int k0 = 0; k0 < DI; k0 += (EO == 4 ? 4 : DI)) {
+      constexpr int KN = EO == 4 ? 4 : DI;
+      float u[NI][KN];
+#pragma unroll
+      for (int v = 0; v < NI; ++v) {
+        const float* p = reinterpret_cast<const float*>(&iv(v, j, 0)) + idx_i(k0);
+#pragma unroll
+        for (int k = 0; k < KN; ++k) u[v][k] = p[k];
+      }
+#pragma unroll
+      for (int k = 0; k < KN; ++k)
+#pragma unroll
+        for (int e = 0; e < EO; ++e) {
+          float& x = X[k0 + k][e];
+          x = fmaf(u[0][k], w[0][e], x);
+          if constexpr (MODE == FWD) {
+            float& y = Y[k0 + k][e];
+            y = fmaf(u[1][k], w[1][e], y);
+            y = fmaf(u[2][k], w[2][e], y);
+            pm[e] = fmaf(u[3][k], x, pm[e]);
+            ps[e] = fmaf(u[4][k], y, ps[e]);
+            ps[e] = fmaf(u[5][k], x * x, ps[e]);
+          } else if constexpr (MODE == DQ) {
+            pm[e] = fmaf(u[1][k], x, pm[e]);
+            ps[e] = fmaf(u[2][k], x * x, ps[e]);
+          } else {
+            float& y = Y[k0 + k][e];
+            y = fmaf(u[1][k], w[1][e], y);
+            pm[e] = fmaf(u[2][k], x, pm[e]);
+            ps[e] = fmaf(u[3][k], y, ps[e]);
+          }
+        }
+    }
+    const float r = group_sums<EO>(pm, ps, lane);
+    const int o = idx_o(0) + (EO == 4 ? 2 * (lane & 1) + ((lane >> 1) & 1) : (lane & 1));
+    const bool mine = EO == 4 || (lane & 2) == 0;
+    float* om = MODE == DK ? a.km : (MODE == DV ? a.vm : a.om);
+    float* oS = MODE == DK ? a.kS : (MODE == DV ? a.vS : a.oS);
+    if (mine && o < D) ((lane & 4) ? oS : om)[ob + tok(s0 + j) * a.lo.st + o] = r;
+  };
+
   for (int s0 = 0; s0 < cnt; s0 += kTok) {
     __syncthreads();
     stage();
     __syncthreads();
     fetch(s0 + kTok);
     const int m = min(kTok, cnt - s0);
-    for (int j = 0; j < m; ++j) {
-      if (!grouped || j == 0) {  // the state before the token, decayed
+#pragma unroll 1
+    for (int j0 = 0; j0 < m; j0 += per) {
+      if (s0 + j0) {
 #pragma unroll
         for (int k = 0; k < DI; ++k)
 #pragma unroll
           for (int e = 0; e < EO; ++e) {
-            // the first group starts from the true state: one decay, not a group's
-            X[k][e] = (s0 == 0 && j == 0) ? g * X[k][e] : scaled(gm, X[k][e]);
-            if constexpr (TWO_STATES) Y[k][e] = (s0 == 0 && j == 0) ? g * (g * Y[k][e]) : scaled(gS, Y[k][e]);
+            X[k][e] *= s1;
+            if constexpr (TWO_STATES) Y[k][e] *= s2;
           }
       }
-      float w[NO][EO];
-#pragma unroll
-      for (int v = 0; v < NO; ++v) {
-        const float* p = reinterpret_cast<const float*>(&ov[v][j][0]) + 8 * EO * wave + EO * og;
-#pragma unroll
-        for (int e = 0; e < EO; ++e) w[v][e] = p[e];
-      }
-      float pm[EO] = {}, ps[EO] = {};
-#pragma unroll
-      for (int k0 = 0; k0 < DI; k0 += (EO == 4 ? 4 : DI)) {
-        constexpr int KN = EO == 4 ? 4 : DI;
-        float u[NI][KN];
-#pragma unroll
-        for (int v = 0; v < NI; ++v) {
-          const float* p = reinterpret_cast<const float*>(&iv[v][j][0]) + idx_i(k0);
-#pragma unroll
-          for (int k = 0; k < KN; ++k) u[v][k] = p[k];
-        }
-#pragma unroll
-        for (int k = 0; k < KN; ++k)
-#pragma unroll
-          for (int e = 0; e < EO; ++e) {
-            float& x = X[k0 + k][e];
-            x = fmaf(u[0][k], w[0][e], x);
-            if constexpr (MODE == FWD) {
-              float& y = Y[k0 + k][e];
-              y = fmaf(u[1][k], w[1][e], y);
-              y = fmaf(u[2][k], w[2][e], y);
-              if constexpr (!SUM) {
-                pm[e] = fmaf(u[3][k], x, pm[e]);
-                ps[e] = fmaf(u[4][k], y, ps[e]);
-                ps[e] = fmaf(u[5][k], x * x, ps[e]);
-              }
-            } else if constexpr (MODE == DQ) {
-              if constexpr (!SUM) {
-                pm[e] = fmaf(u[1][k], x, pm[e]);
-                ps[e] = fmaf(u[2][k], x * x, ps[e]);
-              }
-            } else {
-              float& y = Y[k0 + k][e];
-              y = fmaf(u[1][k], w[1][e], y);
-              if constexpr (!SUM) {
-                pm[e] = fmaf(u[2][k], x, pm[e]);
-                ps[e] = fmaf(u[3][k], y, ps[e]);
-              }
-            }
-          }
-      }
-      if constexpr (!SUM) {
-        const float r = group_sums<EO>(pm, ps, lane);
-        const int o = idx_o(0) + (EO == 4 ? 2 * (lane & 1) + ((lane >> 1) & 1) : (lane & 1));
-        const bool mine = EO == 4 || (lane & 2) == 0;
-        if (mine && o < D) ((lane & 4) ? a.oS : a.om)[ob + tok(s0 + j) * a.lo.st + o] = r;
-      }
+      const int j1 = min(j0 + per, m);
+#pragma unroll 1
+      for (int j = j0; j < j1; ++j) token(s0, j);
     }
+    r1 *= e1, r2 *= e2, q1 *= i1, q2 *= i2;  // of the next group
   }
 
-  // back to the true state: the last token's power
-  const int last = (grouped && cnt > 0) ? (cnt - 1) % kTok : 0;
-  const Two fm = two(ipow(gd, last)), fS = two(ipow(gd, 2 * last));
-  float* em = SUM ? a.sum_m : a.end_m;
-  float* eS = SUM ? a.sum_S : a.end_S;
-  // the chunk of the last live token (the first one without any) holds the final state
-  const bool writes = SUM || (em && ch == (n > 0 ? (n - 1) / a.L : 0));
-  if (writes) {
-    const int64_t base = (SUM ? bh * a.nch + ch : bh) * (int64_t)D * D;
+  if constexpr (MODE == FWD) {
+    // the chunk of the last live token (the first one without any) holds the final state
+    if (a.end_m && ch == (n > 0 ? (n - 1) / a.L : 0)) {
+      const int last = (grouped && cnt > 0) ? (cnt - 1) % kTok : 0;
+      double f1 = 1.0, f2 = 1.0;  // back to the true state; r is one group ahead
+      if (grouped && cnt > 0) f1 = ipow(gd, last) * (r1 * i1), f2 = ipow(gd, 2 * last) * (r2 * i2);
+      const Two w1 = two(f1), w2 = two(f2);
+      const int64_t base = bh * (int64_t)D * D;
 #pragma unroll
-    for (int k = 0; k < DI; ++k)
+      for (int k = 0; k < DI; ++k)
 #pragma unroll
-      for (int e = 0; e < EO; ++e) {
-        const int i = idx_i(k), o = idx_o(e);
-        if (i < D && o < D) {
-          em[base + (int64_t)i * D + o] = scaled(fm, X[k][e]);
-          if constexpr (TWO_STATES) eS[base + (int64_t)i * D + o] = scaled(fS, Y[k][e]);
+        for (int e = 0; e < EO; ++e) {
+          const int i = idx_i(k), o = idx_o(e);
+          if (i < D && o < D) {
+            a.end_m[base + (int64_t)i * D + o] = scaled(w1, X[k][e]);
+            a.end_S[base + (int64_t)i * D + o] = scaled(w2, Y[k][e]);
+          }
         }
-      }
-  }
-  if constexpr (!SUM) {  // tokens past the sequence's end
-    const int64_t dead0 = max(t0, min(t1, n));
-    for (int64_t q = tid; q < (t1 - dead0) * D; q += NT) {
-      const int64_t at = ob + (dead0 + q / D) * a.lo.st + q % D;
-      a.om[at] = 0.f;
-      a.oS[at] = 0.f;
     }
+  }
+  // tokens past the sequence's end
+  float* om = MODE == DK ? a.km : (MODE == DV ? a.vm : a.om);
+  float* oS = MODE == DK ? a.kS : (MODE == DV ? a.vS : a.oS);
+  const int64_t dead0 = max(t0, min(t1, n));
+  for (int64_t q = tid; q < (t1 - dead0) * D; q += NT) {
+    const int64_t at = ob + (dead0 + q / D) * a.lo.st + q % D;
+    om[at] = 0.f;
+    oS[at] = 0.f;
   }
 }
 
-// Chunk contributions to the states before each chunk, in place: run = g^n run + sum (n the
-// chunk's live tokens; fewer than L only where every later chunk in scan order is empty, or,
-// last token first, where run is still zero).
-template <bool REV>
-__global__ void __launch_bounds__(256) carry_kernel(Args a, int two_states) {
+template <int DI, int EO, bool VEC>
+__global__ void __launch_bounds__(scan_threads(DI)) scan_fwd_kernel(Args a) {
+  __shared__ float4 lds[(n_ivec(FWD) + n_ovec(FWD)) * kTok * 2 * DI];
+  scan<FWD, DI, EO, VEC>(a, lds);
+}
+// The three backward scans are independent: one launch, blockIdx.y says which.
+template <int DI, int EO, bool VEC>
+__global__ void __launch_bounds__(scan_threads(DI)) scan_bwd_kernel(Args a) {
+  __shared__ float4 lds[(n_ivec(DK) + n_ovec(DK)) * kTok * 2 * DI];
+  if (blockIdx.y == 0)
+    scan<DK, DI, EO, VEC>(a, lds);
+  else if (blockIdx.y == 1)
+    scan<DV, DI, EO, VEC>(a, lds);
+  else
+    scan<DQ, DI, EO, VEC>(a, lds);
+}
+
+// ------------------------------------------------------------------- chunk contributions
+// A chunk's own share of the state after it, sum_t g^(tokens still to come) u_t w_t^T, is a
+// matrix product over the chunk's tokens: fp32 MFMAs (32 x 32 x 2, a token for each half of
+// the wave), operands straight from memory, 32 floats of a token per half wave. A wave forms
+// 32 rows and NO 32-column tiles. The powers of the decay run from the token that keeps 1,
+// in float64, so that neither a small decay nor a long chunk leaves the floats' range early.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <bool REV, bool SECOND, int NO>
+__device__ __forceinline__ void chunk_sum(const Args& a, int it, int ot) {
+  const int64_t bid = blockIdx.x, ch = bid % a.nch, bh = bid / a.nch, b = bh / a.H;
+  if (ch == (REV ? 0 : a.nch - 1)) return;  // no chunk comes after it
+  const int h = (int)(bh % a.H), D = a.D, lane = threadIdx.x & 63, half = lane >> 5, l5 = lane & 31;
+  const int64_t n = seq_len(a, b), t0 = ch * a.L, t1 = min(a.T, t0 + a.L), live = min(n, t1);
+  if (live <= t0) return;  // the carry does not read it
+  const int cnt = (int)(live - t0);
+  const int i = 32 * it + l5;
+  const bool iok = i < D;
+  // u: keys (REV: queries), w: values (REV: deltas), with their variances' counterparts
+  const tagi_heads lu = REV ? a.lq : a.lk, lw = REV ? a.ld : a.lv;
+  const float* um = (REV ? a.mq : a.mk) + b * lu.sb + h * lu.sh + i;
+  const float* uS = REV ? nullptr : a.Sk + b * lu.sb + h * lu.sh + i;
+  const float* wm = (REV ? a.dm : a.mv) + b * lw.sb + h * lw.sh;
+  const float* wS = (REV ? a.dS : a.Sv) + b * lw.sb + h * lw.sh;
+  const double g = (double)a.decay[h];
+  double p = half ? g : 1.0;
+  const double gg = g * g;
+  f32x16 X[NO] = {}, Y[NO] = {};
+  constexpr int U = 4;  // pairs of tokens whose loads are in flight together
+  for (int r0 = 0; r0 < cnt; r0 += 2 * U) {
+    float ku[U], ks[U], wv[U][NO], ws[U][NO];
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const int r = r0 + 2 * q + half;
+      const bool on = r < cnt;
+      const int64_t t = REV ? t0 + r : live - 1 - r;
+      ku[q] = on && iok ? um[t * lu.st] : 0.f;
+      ks[q] = SECOND && !REV && on && iok ? uS[t * lu.st] : 0.f;
+#pragma unroll
+      for (int o = 0; o < NO; ++o) {
+        const int oc = 32 * (ot + o) + l5;
+        const bool ok = on && oc < D;
+        wv[q][o] = ok ? wm[t * lw.st + oc] : 0.f;
+        ws[q][o] = SECOND && ok ? wS[t * lw.st + oc] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const float f1 = (float)p, f2 = (float)(p * p);
+      p *= gg;
+      const float c1 = REV ? a.c : 1.f, c2 = REV ? a.c2 : 1.f;
+      const float x = ku[q] * f1, k2 = ku[q] * ku[q] * f2, xs = ks[q] * f2;
+#pragma unroll
+      for (int o = 0; o < NO; ++o) {
+        X[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, c1 * wv[q][o], X[o], 0, 0, 0);
+        if constexpr (SECOND) {
+          Y[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(k2, c2 * ws[q][o], Y[o], 0, 0, 0);
+          if constexpr (!REV)
+            Y[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(xs, wv[q][o] * wv[q][o] + ws[q][o], Y[o], 0, 0, 0);
+        }
+      }
+    }
+  }
+  float* sm = REV ? a.pre_g : a.pre_m;
+  float* sS = REV ? a.pre_n : a.pre_S;
+  const int64_t base = (bh * a.nch + ch) * (int64_t)D * D;
+#pragma unroll
+  for (int o = 0; o < NO; ++o)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = 32 * it + 8 * (e >> 2) + 4 * half + (e & 3), col = 32 * (ot + o) + l5;
+      if (row < D && col < D) {
+        sm[base + (int64_t)row * D + col] = X[o][e];
+        if constexpr (SECOND) sS[base + (int64_t)row * D + col] = Y[o][e];
+      }
+    }
+}
+
+template <int NO>
+__global__ void __launch_bounds__(64) sum_fwd_kernel(Args a) {
+  chunk_sum<false, true, NO>(a, blockIdx.y, blockIdx.z * NO);
+}
+// Keys and values into the mean state, queries and deltas into the adjoint ones.
+template <int NO>
+__global__ void __launch_bounds__(64) sum_bwd_kernel(Args a) {
+  const int tiles = (a.D + 31) / 32;
+  if ((int)blockIdx.y < tiles)
+    chunk_sum<false, false, NO>(a, blockIdx.y, blockIdx.z * NO);
+  else
+    chunk_sum<true, true, NO>(a, blockIdx.y - tiles, blockIdx.z * NO);
+}
+
+// Chunk contributions to the states before each chunk, in place: run = g^L run + sum. A chunk
+// with fewer live tokens than L has only empty ones after it, or (last token first) an empty
+// run before it, so its own power is never needed.
+// A: chunks in flight, whose loads do not wait for each other's carry (128 chunks of 8 heads
+// of 64: 95 us one by one, 22 us sixteen at a time).
+template <bool REV, int A>
+__device__ __forceinline__ void carry(const Args& a, float* x, const float* init, bool second) {
   const int64_t DD = (int64_t)a.D * a.D, per = (DD + 255) / 256, bh = blockIdx.x / per, b = bh / a.H;
   const int64_t el = (blockIdx.x % per) * 256 + threadIdx.x;
   if (el >= DD) return;
   const int64_t n = seq_len(a, b);
   const double gL = ipow((double)a.decay[bh % a.H], a.L);
-  for (int s = 0; s < (two_states ? 2 : 1); ++s) {
-    const Two f = two(s ? gL * gL : gL);
-    float* x = (s ? a.sum_S : a.sum_m) + bh * a.nch * DD + el;
-    const float* init = s ? a.init_S : a.init_m;
-    float run = init ? init[bh * DD + el] : 0.f;
-    for (int64_t k = 0; k < a.nch; ++k) {
-      const int64_t ch = REV ? a.nch - 1 - k : k;
-      const bool live = ch * a.L < n, more = k + 1 < a.nch;
-      const float own = live && more ? x[ch * DD] : 0.f;  // the last chunk's is not formed
+  const Two f = two(second ? gL * gL : gL);
+  x += bh * a.nch * DD + el;
+  float run = init ? init[bh * DD + el] : 0.f;
+  for (int64_t k0 = 0; k0 < a.nch; k0 += A) {
+    float own[A];
+#pragma unroll
+    for (int j = 0; j < A; ++j) {
+      const int64_t ch = REV ? a.nch - 1 - k0 - j : k0 + j;
+      const bool use = k0 + j + 1 < a.nch && ch * a.L < n;  // the last chunk's is not formed
+      own[j] = use ? x[ch * DD] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < A; ++j) {
+      if (k0 + j >= a.nch) break;
+      const int64_t ch = REV ? a.nch - 1 - k0 - j : k0 + j;
       x[ch * DD] = run;
-      if (live) run = scaled(f, run) + own;
+      if (ch * a.L < n) run = scaled(f, run) + own[j];
     }
   }
+}
+template <int A>
+__global__ void __launch_bounds__(256) carry_fwd_kernel(Args a) {
+  carry<false, A>(a, blockIdx.y ? a.pre_S : a.pre_m, blockIdx.y ? a.init_S : a.init_m, blockIdx.y);
+}
+template <int A>
+__global__ void __launch_bounds__(256) carry_bwd_kernel(Args a) {
+  if (blockIdx.y == 0)
+    carry<false, A>(a, a.pre_m, nullptr, false);
+  else
+    carry<true, A>(a, blockIdx.y == 1 ? a.pre_g : a.pre_n, nullptr, blockIdx.y == 2);
 }
 
 // One token of every sequence: the state is read, advanced and written once.
@@ -500,29 +629,62 @@ Chunks chunks(int64_t B, int64_t T, int64_t H, int64_t D) {
   return c;
 }
 
-template <int MODE, bool SUM, bool VEC>
+template <bool BWD, bool VEC>
 void launch_scan_v(const Args& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.B * a.H * a.nch));
+  const dim3 grid((unsigned)(a.B * a.H * a.nch), BWD ? 3 : 1);
+#define TAGI_SCAN(DI, EO)                                                                                   \
+  do {                                                                                                      \
+    if constexpr (BWD)                                                                                      \
+      hipLaunchKernelGGL((scan_bwd_kernel<DI, EO, VEC>), grid, dim3(scan_threads(DI)), 0, s, a);            \
+    else                                                                                                    \
+      hipLaunchKernelGGL((scan_fwd_kernel<DI, EO, VEC>), grid, dim3(scan_threads(DI)), 0, s, a);            \
+  } while (0)
   if (a.D <= 16)
-    hipLaunchKernelGGL((scan_kernel<MODE, 2, 2, VEC, SUM>), grid, dim3(64), 0, s, a);
+    TAGI_SCAN(2, 2);
   else if (a.D <= 32)
-    hipLaunchKernelGGL((scan_kernel<MODE, 4, 4, VEC, SUM>), grid, dim3(64), 0, s, a);
+    TAGI_SCAN(4, 4);
   else if (a.D <= 64)
-    hipLaunchKernelGGL((scan_kernel<MODE, 8, 4, VEC, SUM>), grid, dim3(128), 0, s, a);
+    TAGI_SCAN(8, 4);
   else if (a.D <= 96)
-    hipLaunchKernelGGL((scan_kernel<MODE, 12, 4, VEC, SUM>), grid, dim3(192), 0, s, a);
+    TAGI_SCAN(12, 4);
   else
-    hipLaunchKernelGGL((scan_kernel<MODE, 16, 4, VEC, SUM>), grid, dim3(256), 0, s, a);
+    TAGI_SCAN(16, 4);
+#undef TAGI_SCAN
 }
-template <int MODE, bool SUM>
-void launch_scan(const Args& a, bool vec, hipStream_t s) {
-  vec ? launch_scan_v<MODE, SUM, true>(a, s) : launch_scan_v<MODE, SUM, false>(a, s);
-}
-template <bool REV>
-void launch_carry(const Args& a, bool two_states, hipStream_t s) {
-  const int64_t DD = (int64_t)a.D * a.D;
-  hipLaunchKernelGGL(carry_kernel<REV>, dim3((unsigned)(cdiv(DD, 256) * a.B * a.H)), dim3(256), 0, s, a,
-                     (int)two_states);
+
+// The states before every chunk, then the scans.
+template <bool BWD>
+void launch_all(const Args& a, bool vec, hipStream_t s) {
+  if (a.nch > 1) {
+    const int tiles = (int)cdiv(a.D, 32);
+    const unsigned x = (unsigned)(a.B * a.H * a.nch), y = BWD ? 2 * tiles : tiles;
+    if (tiles % 2 == 0) {
+      const dim3 grid(x, y, tiles / 2);
+      if constexpr (BWD)
+        hipLaunchKernelGGL(sum_bwd_kernel<2>, grid, dim3(64), 0, s, a);
+      else
+        hipLaunchKernelGGL(sum_fwd_kernel<2>, grid, dim3(64), 0, s, a);
+    } else {
+      const dim3 grid(x, y, tiles);
+      if constexpr (BWD)
+        hipLaunchKernelGGL(sum_bwd_kernel<1>, grid, dim3(64), 0, s, a);
+      else
+        hipLaunchKernelGGL(sum_fwd_kernel<1>, grid, dim3(64), 0, s, a);
+    }
+    const dim3 grid((unsigned)(cdiv((int64_t)a.D * a.D, 256) * a.B * a.H), BWD ? 3 : 2);
+    if constexpr (BWD) {
+      if (a.nch <= 4)
+        hipLaunchKernelGGL(carry_bwd_kernel<4>, grid, dim3(256), 0, s, a);
+      else
+        hipLaunchKernelGGL(carry_bwd_kernel<16>, grid, dim3(256), 0, s, a);
+    } else {
+      if (a.nch <= 4)
+        hipLaunchKernelGGL(carry_fwd_kernel<4>, grid, dim3(256), 0, s, a);
+      else
+        hipLaunchKernelGGL(carry_fwd_kernel<16>, grid, dim3(256), 0, s, a);
+    }
+  }
+  vec ? launch_scan_v<BWD, true>(a, s) : launch_scan_v<BWD, false>(a, s);
 }
 
 int check_sizes(const char* what, int64_t B, int64_t T, int64_t H, int64_t D) {
@@ -581,13 +743,10 @@ extern "C" int tagi_linear_attention_fwd(const float* mq, const float* Sq, const
   const bool vec = D % 4 == 0 && al4(*lq) && al4(*lk) && al4(*lv) && al16a(mq) && al16a(Sq) && al16a(mk) && al16a(Sk) &&
                    al16a(mv) && al16a(Sv);
   if (c.nch > 1) {
-    a.sum_m = static_cast<float*>(ws);
-    a.sum_S = a.sum_m + state_floats(B, H, D, c.nch);
-    launch_scan<FWD, true>(a, vec, s);
-    launch_carry<false>(a, true, s);
-    a.pre_m = a.sum_m, a.pre_S = a.sum_S, a.pre_t = 0;
+    a.pre_m = static_cast<float*>(ws);
+    a.pre_S = a.pre_m + state_floats(B, H, D, c.nch);
   }
-  launch_scan<FWD, false>(a, vec, s);
+  launch_all<false>(a, vec, s);
   return check_launch(what);
 }
 
@@ -618,23 +777,13 @@ extern "C" int tagi_linear_attention_bwd(const float* mq, const float* mk, const
   a.L = c.L, a.nch = c.nch;
   const bool vec = D % 4 == 0 && al4(*lq) && al4(*lk) && al4(*lv) && al4(*ld) && al16a(mq) && al16a(mk) && al16a(mv) &&
                    al16a(dmo) && al16a(dSo);
-  float *wM = nullptr, *wG = nullptr, *wN = nullptr;
+  a.om = dmq, a.oS = dSq, a.km = dmk, a.kS = dSk, a.vm = dmv, a.vS = dSv;
   if (c.nch > 1) {
     const int64_t n = state_floats(B, H, D, c.nch);
-    wM = static_cast<float*>(ws), wG = wM + n, wN = wG + n;
-    a.sum_m = wM;
-    launch_scan<DQ, true>(a, vec, s);
-    launch_carry<false>(a, false, s);
-    a.sum_m = wG, a.sum_S = wN;
-    launch_scan<DV, true>(a, vec, s);
-    launch_carry<true>(a, true, s);
+    a.pre_m = static_cast<float*>(ws);
+    a.pre_g = a.pre_m + n, a.pre_n = a.pre_g + n;
   }
-  a.pre_m = wM, a.pre_t = 0, a.om = dmq, a.oS = dSq;  // the transposed state, as DQ's own sums left it
-  launch_scan<DQ, false>(a, vec, s);
-  a.pre_m = wG, a.pre_S = wN, a.pre_t = 1, a.om = dmk, a.oS = dSk;
-  launch_scan<DK, false>(a, vec, s);
-  a.pre_t = 0, a.om = dmv, a.oS = dSv;
-  launch_scan<DV, false>(a, vec, s);
+  launch_all<true>(a, vec, s);
   return check_launch(what);
 }
 
