@@ -340,6 +340,40 @@ def test_linear_attention_long(dev, T):
     check_lin(dev, 2, T, 1, 65, seed=T, lengths=[T - 77, 300], state=True, decay=torch.tensor([0.99]))
 
 
+# enough heads (or, split along time, enough chunks) that a wavefront takes 32 columns of the
+# state, half as many that it takes 16; one for each padded head dimension
+WIDE = [(1024, 3, 2, 30), (512, 3, 2, 30), (1024, 9, 2, 16), (512, 9, 2, 61), (256, 9, 2, 64), (342, 9, 2, 90),
+        (171, 10, 2, 96), (256, 9, 2, 128), (128, 17, 2, 125), (32, 256, 8, 32), (8, 512, 8, 64), (6, 600, 7, 72),
+        (4, 512, 8, 128), (3, 700, 8, 57), (33, 130, 3, 100)]
+
+
+@pytest.mark.parametrize("B,T,H,D", WIDE)
+def test_linear_attention_many_heads(dev, B, T, H, D):
+    """As ``check_lin``, the float64 reference on the GPU (products and sums of tensors only)."""
+    from triton_tagi_amd.kernels import linear_attention, linear_attention_backward
+
+    x = [t.to(dev) for t in lin_inputs(B, T, H, D, B + T + D)]
+    dec, c = decays(H).to(dev), 0.4
+    r = g(B)
+    ln = torch.randint(0, T + 1, (B,), generator=r).to(dev) if B % 2 else None
+    dm, dS = torch.randn(B, T, H, D, generator=r).to(dev), -torch.rand(B, T, H, D, generator=r).to(dev)
+    mo, So, (M, P) = linear_attention(*x, dec, scale=c, lengths=ln, return_state=True)
+    bwd = linear_attention_backward(x[0], x[2], x[4], dm, dS, dec, scale=c, lengths=ln)
+    x64 = [t.double() for t in x]
+    ab = [t.abs() for t in x64]
+    k = (1.5 * T + D + 32) * U
+
+    with torch.device(dev):
+        ref = lin_reference(*x64, dec.double(), c, ln)
+        mag = lin_reference(*ab, dec.double(), c, ln)
+        refb = lin_backward_reference(x64[0], x64[2], x64[4], dm.double(), dS.double(), dec.double(), c, ln)
+        magb = lin_backward_reference(ab[0], ab[2], ab[4], dm.double().abs(), dS.double().abs(), dec.double(), c, ln)
+    for got, rf, mg, f, what in zip((mo, So, M, P), ref, mag, (1, 2, 1, 2), ("mo", "So", "M", "P")):
+        close(got, rf, f * k * d64(mg) + 1e-37, what)
+    for got, rf, mg, what in zip(bwd, refb, magb, ("dmq", "dSq", "dmk", "dSk", "dmv", "dSv")):
+        close(got, rf, (2 if what[1] == "S" else 1) * k * d64(mg) + 1e-37, what)
+
+
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("state", [False, True])
 def test_linear_attention_ragged(dev, dtype, state):

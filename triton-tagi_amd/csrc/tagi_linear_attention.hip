@@ -37,7 +37,7 @@ enum Mode { FWD = 0, DQ = 1, DK = 2, DV = 3 };
 // vectors staged per token, over i and over o
 constexpr int n_ivec(int m) { return m == FWD ? 6 : (m == DQ ? 3 : 4); }
 constexpr int n_ovec(int m) { return m == FWD ? 3 : (m == DQ ? 1 : 2); }
-constexpr int scan_threads(int di) { return di <= 4 ? 64 : 16 * di; }
+constexpr int scan_threads(int di, int eo) { return 64 * di / eo; }  // a wave per 8 eo columns of 8 di
 
 struct Args {
   // DQ/DK/DV read the means and the deltas (dm, dS) only
@@ -93,7 +93,7 @@ constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kXor7 = 0x141;  // quad_perm, quad_per
 
 // Sums over the 8 lanes of a group (lane & 7) of EO means and EO variances per lane. Lanes
 // with bit 2 set end with variances, the others with means; of the EO values the lane's
-// bit 0 (and, with four, bit 1) says which.
+// bit 0 (and, with four, bit 1) says which, lanes that differ in the bits left over agree.
 template <int EO>
 __device__ __forceinline__ float group_sums(const float* pm, const float* ps, int lane) {
   float r[EO];
@@ -103,17 +103,21 @@ __device__ __forceinline__ float group_sums(const float* pm, const float* ps, in
     const float keep = b2 ? ps[e] : pm[e], give = b2 ? pm[e] : ps[e];
     r[e] = keep + dpp<kXor7>(give);
   }
-  float h[EO / 2];
-#pragma unroll
-  for (int e = 0; e < EO / 2; ++e) {
-    const float keep = b0 ? r[EO / 2 + e] : r[e], give = b0 ? r[e] : r[EO / 2 + e];
-    h[e] = keep + dpp<kXor1>(give);
-  }
-  if constexpr (EO == 4) {
-    const float keep = b1 ? h[1] : h[0], give = b1 ? h[0] : h[1];
-    return keep + dpp<kXor2>(give);
+  if constexpr (EO == 1) {
+    r[0] += dpp<kXor1>(r[0]);
+    return r[0] + dpp<kXor2>(r[0]);
   } else {
-    return h[0] + dpp<kXor2>(h[0]);
+    float h[EO / 2];
+#pragma unroll
+    for (int e = 0; e < EO / 2; ++e) {
+      const float keep = b0 ? r[EO / 2 + e] : r[e], give = b0 ? r[e] : r[EO / 2 + e];
+      h[e] = keep + dpp<kXor1>(give);
+    }
+    if constexpr (EO == 2) return h[0] + dpp<kXor2>(h[0]);
+    if constexpr (EO == 4) {
+      const float keep = b1 ? h[1] : h[0], give = b1 ? h[0] : h[1];
+      return keep + dpp<kXor2>(give);
+    }
   }
 }
 
@@ -138,9 +142,9 @@ __device__ __forceinline__ float4 add4(float4 a, float4 b) {
 
 // The scan of one (sequence, head, chunk), one block.
 template <int MODE, int DI, int EO, bool VEC>
-__device__ __forceinline__ void scan(const Args& a, float4* lds) {
+__device__ __forceinline__ void scan(const Args& a, float4* lds, int64_t bid) {
   constexpr int IP = 8 * DI;                  // padded head dimension
-  constexpr int NT = scan_threads(DI);        // a wave per 8 * EO columns
+  constexpr int NT = scan_threads(DI, EO);
   constexpr bool REV = MODE >= DK, TWO_STATES = MODE != DQ;
   constexpr int NI = n_ivec(MODE), NO = n_ovec(MODE);
   constexpr int C4 = IP / 4;                  // float4 chunks of a row
@@ -148,7 +152,7 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds) {
   auto iv = [&](int v, int t, int c) -> float4& { return lds[(v * kTok + t) * C4 + c]; };
   auto ov = [&](int v, int t, int c) -> float4& { return lds[((NI + v) * kTok + t) * C4 + c]; };
 
-  const int64_t bid = blockIdx.x, ch = bid % a.nch, bh = bid / a.nch, b = bh / a.H;
+  const int64_t ch = bid % a.nch, bh = bid / a.nch, b = bh / a.H;
   const int h = (int)(bh % a.H), D = a.D;
   const int64_t n = seq_len(a, b), t0 = ch * a.L, t1 = min(a.T, t0 + a.L), live = min(n, t1);
   const int cnt = live > t0 ? (int)(live - t0) : 0;  // live tokens of the chunk
@@ -232,8 +236,9 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds) {
     }
   };
 
-  // state element (i, o): i = 32 (k / 4) + 4 ig + k % 4 (EO == 4), the o of this wave
-  auto idx_i = [&](int k) { return EO == 4 ? 32 * (k >> 2) + 4 * ig + (k & 3) : DI * ig + k; };
+  // state element (i, o): i = 32 (k / 4) + 4 ig + k % 4 (DI a multiple of 4), the o of this wave
+  constexpr int KN = DI % 4 == 0 ? 4 : DI;
+  auto idx_i = [&](int k) { return DI % 4 == 0 ? 32 * (k >> 2) + 4 * ig + (k & 3) : DI * ig + k; };
   auto idx_o = [&](int e) { return 8 * EO * wave + EO * og + e; };
   float X[DI][EO], Y[TWO_STATES ? DI : 1][EO];
 #pragma unroll
@@ -274,8 +279,7 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds) {
     }
     float pm[EO] = {}, ps[EO] = {};
 #pragma unroll
-    for (int k0 = 0; k0 < DI; k0 += (EO == 4 ? 4 : DI)) {
-      constexpr int KN = EO == 4 ? 4 : DI;
+    for (int k0 = 0; k0 < DI; k0 += KN) {
       float u[NI][KN];
 #pragma unroll
       for (int v = 0; v < NI; ++v) {
@@ -308,8 +312,8 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds) {
         }
     }
     const float r = group_sums<EO>(pm, ps, lane);
-    const int o = idx_o(0) + (EO == 4 ? 2 * (lane & 1) + ((lane >> 1) & 1) : (lane & 1));
-    const bool mine = EO == 4 || (lane & 2) == 0;
+    const int o = idx_o(0) + (EO == 4 ? 2 * (lane & 1) + ((lane >> 1) & 1) : (EO == 2 ? lane & 1 : 0));
+    const bool mine = EO == 4 || (lane & (EO == 2 ? 2 : 3)) == 0;
     float* om = MODE == DK ? a.km : (MODE == DV ? a.vm : a.om);
     float* oS = MODE == DK ? a.kS : (MODE == DV ? a.vS : a.oS);
     if (mine && o < D) ((lane & 4) ? oS : om)[ob + tok(s0 + j) * a.lo.st + o] = r;
@@ -371,20 +375,24 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds) {
 }
 
 template <int DI, int EO, bool VEC>
-__global__ void __launch_bounds__(scan_threads(DI)) scan_fwd_kernel(Args a) {
+__global__ void __launch_bounds__(scan_threads(DI, EO)) scan_fwd_kernel(Args a) {
   __shared__ float4 lds[(n_ivec(FWD) + n_ovec(FWD)) * kTok * 2 * DI];
-  scan<FWD, DI, EO, VEC>(a, lds);
+  scan<FWD, DI, EO, VEC>(a, lds, blockIdx.x);
 }
-// The three backward scans are independent: one launch, blockIdx.y says which.
+// The three backward scans are independent and read the same tensors: one launch, the three
+// blocks of a chunk 8 block numbers apart, so that they run at about the same time on one of
+// the 8 XCDs and find each other's reads in its L2.
 template <int DI, int EO, bool VEC>
-__global__ void __launch_bounds__(scan_threads(DI)) scan_bwd_kernel(Args a) {
+__global__ void __launch_bounds__(scan_threads(DI, EO)) scan_bwd_kernel(Args a) {
   __shared__ float4 lds[(n_ivec(DK) + n_ovec(DK)) * kTok * 2 * DI];
-  if (blockIdx.y == 0)
-    scan<DK, DI, EO, VEC>(a, lds);
-  else if (blockIdx.y == 1)
-    scan<DV, DI, EO, VEC>(a, lds);
+  const int64_t x = blockIdx.x, q = x >> 3, bid = (q / 3) * 8 + (x & 7);
+  if (bid >= a.B * a.H * a.nch) return;
+  if (q % 3 == 0)
+    scan<DK, DI, EO, VEC>(a, lds, bid);
+  else if (q % 3 == 1)
+    scan<DV, DI, EO, VEC>(a, lds, bid);
   else
-    scan<DQ, DI, EO, VEC>(a, lds);
+    scan<DQ, DI, EO, VEC>(a, lds, bid);
 }
 
 // ------------------------------------------------------------------- chunk contributions
@@ -415,40 +423,53 @@ __device__ __forceinline__ void chunk_sum(const Args& a, int it, int ot) {
   double p = half ? g : 1.0;
   const double gg = g * g;
   f32x16 X[NO] = {}, Y[NO] = {};
-  constexpr int U = 4;  // pairs of tokens whose loads are in flight together
-  for (int r0 = 0; r0 < cnt; r0 += 2 * U) {
+  constexpr int U = 4;  // pairs of tokens a stage; a stage's loads run during the one before
+  struct Stage {
     float ku[U], ks[U], wv[U][NO], ws[U][NO];
+  };
+  auto fetch = [&](Stage& f, int r0) {
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const int r = r0 + 2 * q + half;
       const bool on = r < cnt;
       const int64_t t = REV ? t0 + r : live - 1 - r;
-      ku[q] = on && iok ? um[t * lu.st] : 0.f;
-      ks[q] = SECOND && !REV && on && iok ? uS[t * lu.st] : 0.f;
+      f.ku[q] = on && iok ? um[t * lu.st] : 0.f;
+      if constexpr (SECOND && !REV) f.ks[q] = on && iok ? uS[t * lu.st] : 0.f;
 #pragma unroll
       for (int o = 0; o < NO; ++o) {
         const int oc = 32 * (ot + o) + l5;
         const bool ok = on && oc < D;
-        wv[q][o] = ok ? wm[t * lw.st + oc] : 0.f;
-        ws[q][o] = SECOND && ok ? wS[t * lw.st + oc] : 0.f;
+        f.wv[q][o] = ok ? wm[t * lw.st + oc] : 0.f;
+        if constexpr (SECOND) f.ws[q][o] = ok ? wS[t * lw.st + oc] : 0.f;
       }
     }
+  };
+  auto product = [&](const Stage& f) {
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const float f1 = (float)p, f2 = (float)(p * p);
       p *= gg;
       const float c1 = REV ? a.c : 1.f, c2 = REV ? a.c2 : 1.f;
-      const float x = ku[q] * f1, k2 = ku[q] * ku[q] * f2, xs = ks[q] * f2;
+      const float x = f.ku[q] * f1, k2 = f.ku[q] * f.ku[q] * f2;
 #pragma unroll
       for (int o = 0; o < NO; ++o) {
-        X[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, c1 * wv[q][o], X[o], 0, 0, 0);
+        X[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, c1 * f.wv[q][o], X[o], 0, 0, 0);
         if constexpr (SECOND) {
-          Y[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(k2, c2 * ws[q][o], Y[o], 0, 0, 0);
+          Y[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(k2, c2 * f.ws[q][o], Y[o], 0, 0, 0);
           if constexpr (!REV)
-            Y[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(xs, wv[q][o] * wv[q][o] + ws[q][o], Y[o], 0, 0, 0);
+            Y[o] = __builtin_amdgcn_mfma_f32_32x32x2f32(f.ks[q] * f2, f.wv[q][o] * f.wv[q][o] + f.ws[q][o], Y[o], 0, 0,
+                                                        0);
         }
       }
     }
+  };
+  Stage f0, f1;
+  fetch(f0, 0);
+  for (int r0 = 0; r0 < cnt; r0 += 4 * U) {  // fetches past the chunk's tokens are zeros
+    fetch(f1, r0 + 2 * U);
+    product(f0);
+    fetch(f0, r0 + 4 * U);
+    product(f1);
   }
   float* sm = REV ? a.pre_g : a.pre_m;
   float* sS = REV ? a.pre_n : a.pre_S;
@@ -605,56 +626,86 @@ __global__ void __launch_bounds__(256) step_kernel(Args a, const uint8_t* __rest
 inline bool al16a(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 inline bool al4(const tagi_heads& s) { return s.sb % 4 == 0 && s.st % 4 == 0 && s.sh % 4 == 0; }
 
-// Tokens per chunk. One chunk is one pass over the data, but a wavefront per (sequence, head,
-// 32 columns) leaves the GPU's 1024 SIMDs idle where these are few; chunks cost a pass that
-// sums each one's contribution and 16 bytes of state traffic an element. Two wavefronts for
-// each SIMD, chunks of 32 tokens at least. One prompt of 32768 tokens, 8 heads of 64 (us):
-// one chunk 22514, 1024 wavefronts 686, 2048 468, 4096 630.
-constexpr int64_t kWaves = 2048, kMinChunk = 32;
-int64_t chunk_len(int64_t heads, int64_t T, int64_t D) {
-  const int64_t waves = heads * cdiv(D, 32);
-  int64_t nch = cdiv(kWaves, waves);
-  if (nch > cdiv(T, kMinChunk)) nch = cdiv(T, kMinChunk);
-  if (nch < 1) nch = 1;
-  return cdiv(cdiv(T > 0 ? T : 1, nch), kTok) * kTok;
-}
-
+// Columns of a wavefront and tokens of a chunk. A wave per (sequence, head, 32 columns) is the
+// least work, but few of them leave the GPU's 1024 SIMDs idle. Narrower waves (16 or 8
+// columns) read the token's vectors more often; chunks cost a pass that sums each one's
+// contribution, the state traffic, and two launches. Measured (us, forward / backward; "n x c":
+// n chunks, c columns):
+//   64 x 256 tokens, 8 heads of 32:  1 x 8 62 / 114, 1 x 16 79 / 93, 1 x 32 - / 97, 4 x 32 78 / 104
+//   32 x 128 tokens, 8 heads of 64:  1 x 8 46 / 78, 1 x 16 56 / 65, 2 x 16 78 / 105
+//   2 x 4096 tokens, 16 heads of 64: 32 x 32 186 / 310, 16 x 32 - / 283, 16 x 16 195 / 318
+//   1 x 512 tokens, 8 heads of 64:   16 x 8 33 / 37, 16 x 16 37 / 39, 16 x 32 46 / 50
+//   1 x 2048 tokens, 4 heads of 128: 64 x 16 76 / 131, 32 x 32 - / 118, 64 x 32 87 / -
+//   1 x 64 tokens, 8 heads of 32:    1 x 8 17 / 25, 2 x 8 24 / 32
+// So: no chunks where waves of 8 columns (backward, whose three scans run side by side: 16)
+// reach 2048 (1024), in the widest that do; none below 128 tokens; else as many chunks as
+// bring 32-column waves there, of 32 tokens at least (backward: and of half a head's
+// features, its three states' traffic), with narrower waves where that falls short.
 struct Chunks {
   int64_t L, nch;
+  int cols;
 };
-Chunks chunks(int64_t B, int64_t T, int64_t H, int64_t D) {
-  Chunks c;
-  c.L = chunk_len(B * H, T, D);
-  c.nch = T > 0 ? cdiv(T, c.L) : 1;
+Chunks chunks(int64_t B, int64_t T, int64_t H, int64_t D, bool bwd) {
+  const int64_t heads = B * H, target = bwd ? 1024 : 2048, enough = bwd ? 512 : 2048;
+  const auto waves = [&](int cols) { return heads * cdiv(D, cols); };
+  Chunks c{cdiv(T > 0 ? T : 1, kTok) * kTok, 1, 8};
+  for (int cols = 32; cols >= (bwd ? 16 : 8); cols /= 2)
+    if (waves(cols) >= target) {
+      c.cols = cols;
+      return c;
+    }
+  if (T < 128) return c;
+  const int64_t least = bwd && D > 64 ? D / 2 : 32;
+  int64_t n = cdiv(target, waves(32));
+  if (n > T / least) n = T / least;
+  c.L = cdiv(cdiv(T, n), kTok) * kTok;
+  c.nch = cdiv(T, c.L);
+  for (c.cols = 32; c.cols > 8 && c.nch * waves(c.cols) < enough;) c.cols /= 2;
   return c;
 }
 
 template <bool BWD, bool VEC>
-void launch_scan_v(const Args& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.B * a.H * a.nch), BWD ? 3 : 1);
+void launch_scan_v(const Args& a, int cols, hipStream_t s) {
+  const int64_t n = a.B * a.H * a.nch;
+  const dim3 grid((unsigned)(BWD ? cdiv(n, 8) * 24 : n));
 #define TAGI_SCAN(DI, EO)                                                                                   \
   do {                                                                                                      \
     if constexpr (BWD)                                                                                      \
-      hipLaunchKernelGGL((scan_bwd_kernel<DI, EO, VEC>), grid, dim3(scan_threads(DI)), 0, s, a);            \
+      hipLaunchKernelGGL((scan_bwd_kernel<DI, EO, VEC>), grid, dim3(scan_threads(DI, EO)), 0, s, a);        \
     else                                                                                                    \
-      hipLaunchKernelGGL((scan_fwd_kernel<DI, EO, VEC>), grid, dim3(scan_threads(DI)), 0, s, a);            \
+      hipLaunchKernelGGL((scan_fwd_kernel<DI, EO, VEC>), grid, dim3(scan_threads(DI, EO)), 0, s, a);        \
+    return;                                                                                                 \
   } while (0)
-  if (a.D <= 16)
-    TAGI_SCAN(2, 2);
-  else if (a.D <= 32)
-    TAGI_SCAN(4, 4);
-  else if (a.D <= 64)
-    TAGI_SCAN(8, 4);
-  else if (a.D <= 96)
-    TAGI_SCAN(12, 4);
-  else
-    TAGI_SCAN(16, 4);
+#define TAGI_SCAN_COLS(DI)     \
+  do {                         \
+    if (cols == 8)             \
+      TAGI_SCAN(DI, 1);        \
+    else if (cols == 16)       \
+      TAGI_SCAN(DI, 2);        \
+    else                       \
+      TAGI_SCAN(DI, 4);        \
+  } while (0)
+  if (a.D <= 16) {
+    if (cols == 8)
+      TAGI_SCAN(2, 1);
+    else
+      TAGI_SCAN(2, 2);
+  } else if (a.D <= 32) {
+    TAGI_SCAN_COLS(4);
+  } else if (a.D <= 64) {
+    TAGI_SCAN_COLS(8);
+  } else if (a.D <= 96) {
+    TAGI_SCAN_COLS(12);
+  } else {
+    TAGI_SCAN_COLS(16);
+  }
 #undef TAGI_SCAN
+#undef TAGI_SCAN_COLS
 }
 
 // The states before every chunk, then the scans.
 template <bool BWD>
-void launch_all(const Args& a, bool vec, hipStream_t s) {
+void launch_all(const Args& a, int cols, bool vec, hipStream_t s) {
   if (a.nch > 1) {
     const int tiles = (int)cdiv(a.D, 32);
     const unsigned x = (unsigned)(a.B * a.H * a.nch), y = BWD ? 2 * tiles : tiles;
@@ -684,7 +735,7 @@ void launch_all(const Args& a, bool vec, hipStream_t s) {
         hipLaunchKernelGGL(carry_fwd_kernel<16>, grid, dim3(256), 0, s, a);
     }
   }
-  vec ? launch_scan_v<BWD, true>(a, s) : launch_scan_v<BWD, false>(a, s);
+  vec ? launch_scan_v<BWD, true>(a, cols, s) : launch_scan_v<BWD, false>(a, cols, s);
 }
 
 int check_sizes(const char* what, int64_t B, int64_t T, int64_t H, int64_t D) {
@@ -703,13 +754,13 @@ using namespace tagi;
 
 extern "C" int64_t tagi_linear_attention_fwd_ws_bytes(int64_t B, int64_t T, int64_t H, int64_t D) {
   if (B <= 0 || T <= 0 || H <= 0 || D <= 0) return 0;
-  const Chunks c = chunks(B, T, H, D);
+  const Chunks c = chunks(B, T, H, D, false);
   return c.nch > 1 ? 2 * state_floats(B, H, D, c.nch) * 4 : 0;
 }
 
 extern "C" int64_t tagi_linear_attention_bwd_ws_bytes(int64_t B, int64_t T, int64_t H, int64_t D) {
   if (B <= 0 || T <= 0 || H <= 0 || D <= 0) return 0;
-  const Chunks c = chunks(B, T, H, D);
+  const Chunks c = chunks(B, T, H, D, true);
   return c.nch > 1 ? 3 * state_floats(B, H, D, c.nch) * 4 : 0;
 }
 
@@ -728,8 +779,8 @@ extern "C" int tagi_linear_attention_fwd(const float* mq, const float* Sq, const
   TAGI_REQUIRE((init_m == nullptr) == (init_S == nullptr) && (end_m == nullptr) == (end_S == nullptr),
                "%s: a state is means and variances together", what);
   TAGI_REQUIRE(!lengths || len_bytes == 4 || len_bytes == 8, "%s: lengths are int32 or int64", what);
-  const Chunks c = chunks(B, T, H, D);
-  TAGI_REQUIRE(B * H * c.nch < (1ll << 31), "%s: too large", what);
+  const Chunks c = chunks(B, T, H, D, false);
+  TAGI_REQUIRE(B * H * c.nch < (1ll << 29), "%s: too large", what);
   TAGI_REQUIRE(c.nch == 1 || (ws && ws_bytes >= tagi_linear_attention_fwd_ws_bytes(B, T, H, D)),
                "%s: workspace too small", what);
   hipStream_t s = (hipStream_t)stream;
@@ -746,7 +797,7 @@ extern "C" int tagi_linear_attention_fwd(const float* mq, const float* Sq, const
     a.pre_m = static_cast<float*>(ws);
     a.pre_S = a.pre_m + state_floats(B, H, D, c.nch);
   }
-  launch_all<false>(a, vec, s);
+  launch_all<false>(a, c.cols, vec, s);
   return check_launch(what);
 }
 
@@ -763,8 +814,8 @@ extern "C" int tagi_linear_attention_bwd(const float* mq, const float* mk, const
   TAGI_REQUIRE(lq && lk && lv && ld && lo && decay && mq && mk && mv && dmo && dSo && dmq && dSq && dmk && dSk && dmv &&
                    dSv, "%s: null pointer", what);
   TAGI_REQUIRE(!lengths || len_bytes == 4 || len_bytes == 8, "%s: lengths are int32 or int64", what);
-  const Chunks c = chunks(B, T, H, D);
-  TAGI_REQUIRE(B * H * c.nch < (1ll << 31), "%s: too large", what);
+  const Chunks c = chunks(B, T, H, D, true);
+  TAGI_REQUIRE(B * H * c.nch < (1ll << 29), "%s: too large", what);
   TAGI_REQUIRE(c.nch == 1 || (ws && ws_bytes >= tagi_linear_attention_bwd_ws_bytes(B, T, H, D)),
                "%s: workspace too small", what);
   hipStream_t s = (hipStream_t)stream;
@@ -783,7 +834,7 @@ extern "C" int tagi_linear_attention_bwd(const float* mq, const float* mk, const
     a.pre_m = static_cast<float*>(ws);
     a.pre_g = a.pre_m + n, a.pre_n = a.pre_g + n;
   }
-  launch_all<true>(a, vec, s);
+  launch_all<true>(a, c.cols, vec, s);
   return check_launch(what);
 }
 
