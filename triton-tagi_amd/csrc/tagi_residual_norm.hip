@@ -11,78 +11,265 @@
 namespace tagi {
 namespace {
 
-constexpr int kThreads = 256;
+// Four consecutive floats at any 4-byte alignment: one 16-byte access on gfx950.
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// One block per row.
-__global__ void __launch_bounds__(kThreads) add_rms_norm_kernel(
+template <bool NT>
+__device__ __forceinline__ f4 ld(const float* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const f4*>(p));
+  return *reinterpret_cast<const f4*>(p);
+}
+template <bool NT>
+__device__ __forceinline__ void st(float* p, f4 v) {
+  if constexpr (NT)
+    __builtin_nontemporal_store(v, reinterpret_cast<f4*>(p));
+  else
+    *reinterpret_cast<f4*>(p) = v;
+}
+// The row's last chunk, which may hold fewer than four.
+__device__ __forceinline__ f4 ld_tail(const float* p, int left) {
+  f4 v = {p[0], 0.f, 0.f, 0.f};
+  if (left > 1) v.y = p[1];
+  if (left > 2) v.z = p[2];
+  return v;
+}
+__device__ __forceinline__ void st_tail(float* p, f4 v, int left) {
+  p[0] = v.x;
+  if (left > 1) p[1] = v.y;
+  if (left > 2) p[2] = v.z;
+}
+
+// Sum over the TPR threads of a row (a wave, or the whole block).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float x, float* red) {
+#pragma unroll
+  for (int w = 32; w > 0; w >>= 1) x += __shfl_xor(x, w);
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = red[0];
+#pragma unroll
+    for (int w = 1; w < TPR / 64; ++w) x += red[w];
+  }
+  return x;
+}
+
+// One pass: TPR threads hold a row's sums in registers (NV chunks of four each) between the
+// statistic and the output, so every input is read and every output written once. HBM bound:
+// 16384 x 4096 moves 2.15 GB in 380 us (5.65 TB/s;
+// a copy kernel reaches 6.26 here), 65536 x 256 537 MB in 93 us.
+template <int TPR, int NV, bool NT>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(
     const float* __restrict__ ma, const float* __restrict__ Sa, const float* __restrict__ mr,
     const float* __restrict__ Sr, const float* __restrict__ mw, const float* __restrict__ Sw, float* __restrict__ mz,
     float* __restrict__ Sz, float* __restrict__ ms, float* __restrict__ Ss, float* __restrict__ inv_rms, int64_t rows,
     int D, float eps) {
-  __shared__ float red[kThreads / 64];
+  __shared__ float red[TPR / 64];
+  constexpr int RPB = TPR < 256 ? 256 / TPR : 1;  // rows of a block
+  const int t = (int)threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * RPB + (int)threadIdx.x / TPR, o = row * D;
+  if (row >= rows) return;  // TPR > 64 has one row a block: no thread of it leaves
+  const int full = D >> 2, left = D & 3;
+  f4 m[NV], v[NV];
+  float acc = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = t + j * TPR;
+    m[j] = v[j] = f4{0.f, 0.f, 0.f, 0.f};
+    if (c < full) {
+      const int64_t at = o + 4 * c;
+      const f4 a = ld<NT>(ma + at), b = ld<NT>(mr + at), x = ld<NT>(Sa + at), y = ld<NT>(Sr + at);
+      m[j] = a + b, v[j] = x + y;
+    } else if (c == full && left) {
+      const int64_t at = o + 4 * c;
+      m[j] = ld_tail(ma + at, left) + ld_tail(mr + at, left), v[j] = ld_tail(Sa + at, left) + ld_tail(Sr + at, left);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const f4 q = m[j] * m[j] + v[j];
+    acc += (q.x + q.y) + (q.z + q.w);
+  }
+  const float inv = 1.f / sqrtf(row_sum<TPR>(acc, red) / (float)D + eps);
+  if (t == 0) inv_rms[row] = inv;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = t + j * TPR;
+    if (c > full || (c == full && !left)) continue;
+    const int64_t at = o + 4 * c;
+    const bool tail = c == full;
+    const f4 g = tail ? ld_tail(mw + 4 * c, left) : *reinterpret_cast<const f4*>(mw + 4 * c);
+    const f4 sg = tail ? ld_tail(Sw + 4 * c, left) : *reinterpret_cast<const f4*>(Sw + 4 * c);
+    const f4 z = m[j] * inv * g, s = inv * inv * (v[j] * (g * g + sg) + sg * (m[j] * m[j]));
+    if (tail) {
+      st_tail(ms + at, m[j], left), st_tail(mz + at, z, left), st_tail(Sz + at, s, left);
+      if (Ss) st_tail(Ss + at, v[j], left);
+    } else {
+      st<NT>(ms + at, m[j]), st<NT>(mz + at, z), st<NT>(Sz + at, s);
+      if (Ss) st<NT>(Ss + at, v[j]);
+    }
+  }
+}
+
+// Rows too long for registers: the inputs are read twice.
+__global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(
+    const float* __restrict__ ma, const float* __restrict__ Sa, const float* __restrict__ mr,
+    const float* __restrict__ Sr, const float* __restrict__ mw, const float* __restrict__ Sw, float* __restrict__ mz,
+    float* __restrict__ Sz, float* __restrict__ ms, float* __restrict__ Ss, float* __restrict__ inv_rms, int D,
+    float eps) {
+  __shared__ float red[16];
   const int64_t row = blockIdx.x, o = row * D;
   float acc = 0.f;
-  for (int c = threadIdx.x; c < D; c += kThreads) {
+  for (int c = threadIdx.x; c < D; c += 1024) {
     const float m = ma[o + c] + mr[o + c], v = Sa[o + c] + Sr[o + c];
-    ms[o + c] = m;
-    if (Ss) Ss[o + c] = v;
     acc += m * m + v;
   }
-  for (int w = 32; w > 0; w >>= 1) acc += __shfl_xor(acc, w);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
-  __syncthreads();
-  const float inv = 1.f / sqrtf((red[0] + red[1] + red[2] + red[3]) / (float)D + eps);
+  const float inv = 1.f / sqrtf(row_sum<1024>(acc, red) / (float)D + eps);
   if (threadIdx.x == 0) inv_rms[row] = inv;
-  for (int c = threadIdx.x; c < D; c += kThreads) {
+  for (int c = threadIdx.x; c < D; c += 1024) {
     const float m = ma[o + c] + mr[o + c], v = Sa[o + c] + Sr[o + c], g = mw[c], sg = Sw[c];
+    ms[o + c] = m;
+    if (Ss) Ss[o + c] = v;
     mz[o + c] = m * inv * g;
     Sz[o + c] = inv * inv * (v * (g * g + sg) + sg * (m * m));
   }
 }
 
-// Blocks own a range of rows and 256 columns; partial column sums go to ws[moment][block][D].
-__global__ void __launch_bounds__(kThreads) add_rms_norm_bwd_kernel(
+// Blocks own a range of rows and 4 CT columns (CT threads across, 256 / CT rows at a time);
+// a thread keeps the weights and sums of its four columns in registers over the range, the
+// threads of a column are joined in float64 through LDS, and one partial sum per block,
+// column and moment goes to ws[moment][block][D]. HBM bound: 16384 x 4096 with deltas at the
+// sum moves 1.88 GB in 342 us (5.5 TB/s).
+template <bool NT>
+__global__ void __launch_bounds__(256) add_rms_norm_bwd_kernel(
     const float* __restrict__ dmz, const float* __restrict__ dSz, const float* __restrict__ dms,
     const float* __restrict__ dSs, const float* __restrict__ ms, const float* __restrict__ inv_rms,
     const float* __restrict__ mw, float* __restrict__ dma, float* __restrict__ dSa, float* __restrict__ ws,
-    int64_t rows, int D) {
-  const int c = (int)blockIdx.y * kThreads + (int)threadIdx.x;
-  if (c >= D) return;
-  const int nblk = (int)gridDim.x;
+    int64_t rows, int D, int CT) {
+  __shared__ f4 red[2][256];
+  const int RG = 256 / CT, ct = (int)threadIdx.x % CT, rg = (int)threadIdx.x / CT;
+  const int c = 4 * ((int)blockIdx.y * CT + ct), nblk = (int)gridDim.x, left = D - c;
   const int64_t r0 = rows * blockIdx.x / nblk, r1 = rows * (blockIdx.x + 1) / nblk;
-  const float g = mw[c];
-  float am = 0.f, as = 0.f;
-  for (int64_t r = r0; r < r1; ++r) {
-    const int64_t o = r * D + c;
-    const float inv = inv_rms[r], k = inv * g, x = inv * ms[o], a = dmz[o], b = dSz[o];
-    dma[o] = a * k + (dms ? dms[o] : 0.f);
-    dSa[o] = b * (k * k) + (dSs ? dSs[o] : 0.f);
-    am += a * x;
-    as += b * (x * x);
+  f4 am = {0.f, 0.f, 0.f, 0.f}, as = am;
+  const bool live = left > 0 && rg < RG;
+  if (live && left >= 4) {
+    const f4 g = *reinterpret_cast<const f4*>(mw + c);
+#pragma unroll 2
+    for (int64_t r = r0 + rg; r < r1; r += RG) {
+      const int64_t o = r * D + c;
+      const float inv = inv_rms[r];
+      const f4 a = ld<NT>(dmz + o), b = ld<NT>(dSz + o), x = ld<NT>(ms + o) * inv, k = g * inv;
+      f4 u = a * k, w = b * (k * k);
+      if (dms) u += ld<NT>(dms + o), w += ld<NT>(dSs + o);
+      st<NT>(dma + o, u);
+      st<NT>(dSa + o, w);
+      am += a * x;
+      as += b * (x * x);
+    }
+  } else if (live) {
+    const f4 g = ld_tail(mw + c, left);
+    for (int64_t r = r0 + rg; r < r1; r += RG) {
+      const int64_t o = r * D + c;
+      const float inv = inv_rms[r];
+      const f4 a = ld_tail(dmz + o, left), b = ld_tail(dSz + o, left), x = ld_tail(ms + o, left) * inv, k = g * inv;
+      f4 u = a * k, w = b * (k * k);
+      if (dms) u += ld_tail(dms + o, left), w += ld_tail(dSs + o, left);
+      st_tail(dma + o, u, left);
+      st_tail(dSa + o, w, left);
+      am += a * x;
+      as += b * (x * x);
+    }
   }
-  ws[(int64_t)blockIdx.x * D + c] = am;
-  ws[((int64_t)nblk + blockIdx.x) * D + c] = as;
+  red[0][threadIdx.x] = am, red[1][threadIdx.x] = as;
+  __syncthreads();
+  // value e of column chunk q, moment w: the RG threads' sums in order
+  const float* f = reinterpret_cast<const float*>(&red[0][0]);
+  for (int i = threadIdx.x; i < 8 * CT; i += 256) {
+    const int w = i / (4 * CT), e = i % (4 * CT), col = 4 * (int)blockIdx.y * CT + e;
+    if (col >= D) continue;
+    double s = 0.0;
+    for (int r = 0; r < RG; ++r) s += f[w * 1024 + r * 4 * CT + e];
+    ws[((int64_t)w * nblk + blockIdx.x) * D + col] = (float)s;
+  }
 }
 
-__global__ void __launch_bounds__(kThreads) add_rms_norm_finalize_kernel(const float* __restrict__ ws,
-                                                                         const float* __restrict__ Sw,
-                                                                         float* __restrict__ dmw,
-                                                                         float* __restrict__ dSw, int D, int nblk) {
-  const int c = (int)blockIdx.x * kThreads + (int)threadIdx.x;
-  if (c >= D) return;
-  double m = 0.0, s = 0.0;
-  for (int b = 0; b < nblk; ++b) {
-    m += ws[(int64_t)b * D + c];
-    s += ws[((int64_t)nblk + b) * D + c];
+// 32 columns and 8 stretches of the blocks' partial sums at a time, in float64.
+__global__ void __launch_bounds__(256) add_rms_norm_finalize_kernel(const float* __restrict__ ws,
+                                                                    const float* __restrict__ Sw,
+                                                                    float* __restrict__ dmw, float* __restrict__ dSw,
+                                                                    int D, int nblk) {
+  __shared__ double red[8][32];
+  const int cl = threadIdx.x & 31, part = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + cl, w = blockIdx.y;
+  const int b0 = nblk * part / 8, b1 = nblk * (part + 1) / 8;
+  const float* p = ws + (int64_t)w * nblk * D + c;
+  double s = 0.0;
+  if (c < D) {
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) s += p[(int64_t)b * D];
   }
+  red[part][cl] = s;
+  __syncthreads();
+  if (part || c >= D) return;
+#pragma unroll
+  for (int q = 1; q < 8; ++q) s += red[q][cl];
   const float sg = Sw[c];
-  dmw[c] = sg * (float)m;
-  dSw[c] = sg * sg * (float)s;
+  if (w)
+    dSw[c] = sg * sg * (float)s;
+  else
+    dmw[c] = sg * (float)s;
 }
 
-int bwd_blocks(int64_t rows) {
-  const int64_t b = cdiv(rows, 32);
-  return (int)(b > 512 ? 512 : b);
+// Threads across a block's columns, and row ranges: up to 1024 blocks (16384 x 4096: 512 blocks
+// 333 us, 1024 342, 2048 375; 65536 x 256: 94, 90, 96), 4 rows a thread at least.
+struct BwdPlan {
+  int ct, chunks, nblk;
+};
+BwdPlan bwd_plan(int64_t rows, int64_t D) {
+  BwdPlan p;
+  const int64_t q = cdiv(D, 4);
+  p.ct = (int)(q < 256 ? q : 256);
+  p.chunks = (int)cdiv(q, p.ct);
+  const int64_t rg = 256 / p.ct;
+  int64_t n = cdiv(rows, rg * 4);
+  const int64_t most = p.chunks < 1024 ? 1024 / p.chunks : 1;
+  p.nblk = (int)(n > most ? most : n);
+  return p;
+}
+
+// Above this much traffic nothing a kernel reads or writes is still in the 256 MB last-level
+// cache when it is needed next, and the nontemporal policy reaches further
+// (16384 x 4096: forward 400 -> 380 us, backward 364 -> 342; 16384 x 1024: 120 -> 109, 105 -> 95).
+constexpr double kCacheBytes = 256e6;
+
+struct FwdArgs {
+  const float *ma, *Sa, *mr, *Sr, *mw, *Sw;
+  float *mz, *Sz, *ms, *Ss, *inv;
+  int64_t rows;
+  int D;
+  float eps;
+};
+template <int TPR, int NV>
+void launch_fwd(const FwdArgs& a, bool nt, hipStream_t s) {
+  const dim3 grid((unsigned)cdiv(a.rows, TPR < 256 ? 256 / TPR : 1)), block(TPR < 256 ? 256 : TPR);
+  if (nt)
+    hipLaunchKernelGGL((add_rms_norm_kernel<TPR, NV, true>), grid, block, 0, s, a.ma, a.Sa, a.mr, a.Sr, a.mw, a.Sw,
+                       a.mz, a.Sz, a.ms, a.Ss, a.inv, a.rows, a.D, a.eps);
+  else
+    hipLaunchKernelGGL((add_rms_norm_kernel<TPR, NV, false>), grid, block, 0, s, a.ma, a.Sa, a.mr, a.Sr, a.mw, a.Sw,
+                       a.mz, a.Sz, a.ms, a.Ss, a.inv, a.rows, a.D, a.eps);
+}
+// Chunks of four per thread: rounded up to a kernel that holds them, TPR * 32 values at most.
+template <int TPR>
+void launch_fwd_nv(const FwdArgs& a, bool nt, hipStream_t s) {
+  const int64_t nv = cdiv(cdiv(a.D, 4), TPR);
+  if (nv <= 1)
+    launch_fwd<TPR, 1>(a, nt, s);
+  else if (nv <= 2)
+    launch_fwd<TPR, 2>(a, nt, s);
+  else if (nv <= 4)
+    launch_fwd<TPR, 4>(a, nt, s);
+  else
+    launch_fwd<TPR, 8>(a, nt, s);
 }
 
 }  // namespace
@@ -100,14 +287,26 @@ extern "C" int tagi_add_rmsnorm_fwd(const float* ma, const float* Sa, const floa
   TAGI_REQUIRE(ma && Sa && mr && Sr && mw && Sw && mz && Sz && ms && inv_rms, "%s: null pointer", what);
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps(FAM_RMSNORM, s, 0.0, (Ss ? 32.0 : 28.0) * rows * D + 4.0 * rows);
-  hipLaunchKernelGGL(add_rms_norm_kernel, dim3((unsigned)rows), dim3(kThreads), 0, s, ma, Sa, mr, Sr, mw, Sw, mz, Sz,
-                     ms, Ss, inv_rms, rows, (int)D, eps);
+  const FwdArgs a{ma, Sa, mr, Sr, mw, Sw, mz, Sz, ms, Ss, inv_rms, rows, (int)D, eps};
+  const bool nt = 32.0 * rows * D > kCacheBytes;
+  // threads of a row: a wave for short rows, or for longer ones when there are rows enough to
+  // fill the GPU; more where few rows would wait on each thread's loads
+  const int64_t chunks = cdiv(D, 4);
+  if (chunks > 8 * 1024)
+    hipLaunchKernelGGL(add_rms_norm_long_kernel, dim3((unsigned)rows), dim3(1024), 0, s, ma, Sa, mr, Sr, mw, Sw, mz, Sz,
+                       ms, Ss, inv_rms, (int)D, eps);
+  else if (chunks <= 64 || (chunks <= 4 * 64 && rows >= 4096))
+    launch_fwd_nv<64>(a, nt, s);
+  else if (chunks <= 256 || (chunks <= 8 * 256 && rows >= 512))
+    launch_fwd_nv<256>(a, nt, s);
+  else
+    launch_fwd_nv<1024>(a, nt, s);
   return check_launch(what);
 }
 
 extern "C" int64_t tagi_add_rmsnorm_bwd_ws_bytes(int64_t rows, int64_t D) {
   if (rows <= 0 || D <= 0) return 0;
-  return (int64_t)bwd_blocks(rows) * 2 * D * (int64_t)sizeof(float);
+  return (int64_t)bwd_plan(rows, D).nblk * 2 * D * (int64_t)sizeof(float);
 }
 
 extern "C" int tagi_add_rmsnorm_bwd(const float* dmz, const float* dSz, const float* dms, const float* dSs,
@@ -123,11 +322,18 @@ extern "C" int tagi_add_rmsnorm_bwd(const float* dmz, const float* dSz, const fl
   TAGI_REQUIRE(ws_bytes >= tagi_add_rmsnorm_bwd_ws_bytes(rows, D), "%s: workspace too small", what);
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps(FAM_RMSNORM, s, 0.0, (dms ? 28.0 : 20.0) * rows * D);
-  const int nblk = bwd_blocks(rows);
-  if (rows > 0)
-    hipLaunchKernelGGL(add_rms_norm_bwd_kernel, dim3((unsigned)nblk, (unsigned)cdiv(D, kThreads)), dim3(kThreads), 0,
-                       s, dmz, dSz, dms, dSs, ms, inv_rms, mw, dma, dSa, static_cast<float*>(ws), rows, (int)D);
-  hipLaunchKernelGGL(add_rms_norm_finalize_kernel, dim3((unsigned)cdiv(D, kThreads)), dim3(kThreads), 0, s,
-                     static_cast<const float*>(ws), Sw, dmw, dSw, (int)D, nblk);
+  const BwdPlan p = bwd_plan(rows, D);
+  if (rows > 0) {
+    const dim3 grid((unsigned)p.nblk, (unsigned)p.chunks);
+    float* part = static_cast<float*>(ws);
+    if ((dms ? 28.0 : 20.0) * rows * D > kCacheBytes)
+      hipLaunchKernelGGL(add_rms_norm_bwd_kernel<true>, grid, dim3(256), 0, s, dmz, dSz, dms, dSs, ms, inv_rms, mw, dma,
+                         dSa, part, rows, (int)D, p.ct);
+    else
+      hipLaunchKernelGGL(add_rms_norm_bwd_kernel<false>, grid, dim3(256), 0, s, dmz, dSz, dms, dSs, ms, inv_rms, mw,
+                         dma, dSa, part, rows, (int)D, p.ct);
+  }
+  hipLaunchKernelGGL(add_rms_norm_finalize_kernel, dim3((unsigned)cdiv(D, 32), 2), dim3(256), 0, s,
+                     static_cast<const float*>(ws), Sw, dmw, dSw, (int)D, p.nblk);
   return check_launch(what);
 }
