@@ -21,6 +21,49 @@ constexpr int kMaxRadixBits = 10;
 
 inline bool al16e(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+// Four consecutive floats at any 4-byte alignment: one 16-byte access on gfx950.
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ f4 ld4(const float* p) { return *reinterpret_cast<const f4*>(p); }
+__device__ __forceinline__ void st4(float* p, f4 v) { *reinterpret_cast<f4*>(p) = v; }
+
+// A lane's columns of rows of D. The last lane of rows with D % 4 != 0 takes the row's last
+// four, so that every lane's loads are one access with no branch between them; only the
+// columns no other lane has (from `skip` on) are its own to store. Lanes past the row load its
+// first columns and store none: every lane of the wave stays active, as reading another
+// lane's register asks for. Rows shorter than four load a column at a time. (Rows of 390 with
+// a branch on the row's end instead: 101 us a pass against 70.)
+struct Cols {
+  int at, skip;  // first column; columns of it that are not the lane's own
+};
+__device__ __forceinline__ Cols columns(int chunk, int D) {
+  Cols c{4 * chunk, 0};
+  if (c.at >= D)
+    c.at = 0, c.skip = 4;
+  else if (c.at + 4 > D && D >= 4)
+    c.skip = c.at + 4 - D, c.at = D - 4;
+  return c;
+}
+template <bool WIDE>  // D >= 4
+__device__ __forceinline__ f4 ldc(const float* p, int D) {
+  if constexpr (WIDE) return ld4(p);
+  f4 v = {p[0], 0.f, 0.f, 0.f};
+  if (D > 1) v.y = p[1];
+  if (D > 2) v.z = p[2];
+  return v;
+}
+template <bool WIDE>
+__device__ __forceinline__ void stc(float* p, f4 v, int D, int skip) {
+  if (WIDE && skip == 0) {
+    st4(p, v);
+    return;
+  }
+  const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e >= skip && e < D) p[e] = x[e];
+}
+
 // The category of token t, or V (sorted behind every category) for padding and ids outside
 // the table. Float ids are cast toward zero; a NaN is outside.
 __device__ __forceinline__ uint32_t category(const void* ids, int type, int64_t t, int64_t V, int64_t pad) {
@@ -70,7 +113,7 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const void* __res
 // Least-significant-digit radix sort of (category, token index). Per digit: every block
 // counts its tile's digits; a wave per digit turns the blocks' counts into places; every
 // block writes its tile's pairs to them in order. Latency bound: 65536 tokens of 131071
-// categories take 2 digits of 9 bits, about KSORT us a digit. Up to kSmall tokens one block
+// categories take 2 digits of 9 bits, 18 us a digit. Up to kSmall tokens one block
 // does all of it in LDS (a launch instead of three per digit).
 constexpr int kSmall = 4096, kSmallBits = 8;
 
@@ -104,7 +147,28 @@ struct SortArgs {
   uint32_t* total;  // [digit]
   int64_t n, V, pad;
   int nblk, shift, bits;
+  // Zeros for the deltas of the rows that do not occur: the sort waits on latency, the fill on
+  // bandwidth, so each launch of the sort takes a share of it in blocks after its own `work`.
+  float* z0;
+  float* z1;
+  int64_t f0, f1;
+  int work;
 };
+
+__device__ __forceinline__ bool fills(const SortArgs& a) {
+  if ((int)blockIdx.x < a.work) return false;
+  const f4 z = {0.f, 0.f, 0.f, 0.f};
+  const int64_t threads = blockDim.x, step = (int64_t)(gridDim.x - a.work) * threads * 4;
+  for (int64_t i = a.f0 + ((int64_t)(blockIdx.x - a.work) * threads + threadIdx.x) * 4; i < a.f1; i += step) {
+    if (i + 4 <= a.f1) {
+      st4(a.z0 + i, z);
+      st4(a.z1 + i, z);
+    } else {
+      for (int64_t j = i; j < a.f1; ++j) a.z0[j] = a.z1[j] = 0.f;
+    }
+  }
+  return true;
+}
 
 __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int64_t i) {
   return a.first ? category(a.ids, a.type, i, a.V, a.pad) : a.kin[i];
@@ -122,6 +186,7 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, bool on, int bits) {
 
 template <int IT>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
+  if (fills(a)) return;
   __shared__ uint32_t cnt[1 << kMaxRadixBits];
   const int radix = 1 << a.bits;
   for (int d = threadIdx.x; d < radix; d += kSortThreads) cnt[d] = 0;
@@ -138,6 +203,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
 
 // One wave per digit: the blocks' counts become places within the digit.
 __global__ void __launch_bounds__(256) sort_places_kernel(SortArgs a) {
+  if (fills(a)) return;
   const int d = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (d >= 1 << a.bits) return;
   uint32_t* h = a.hist + (int64_t)d * a.nblk;
@@ -161,6 +227,7 @@ __global__ void __launch_bounds__(256) sort_places_kernel(SortArgs a) {
 // before it in this strip (a counter per wave and digit, and a ballot match within 64 pairs).
 template <int IT>
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) {
+  if (fills(a)) return;
   constexpr int W = kSortThreads / 64;
   __shared__ uint32_t cnt[W][1 << kMaxRadixBits];
   __shared__ uint32_t wsum[W];
@@ -183,6 +250,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
   uint32_t run = 0;
 #pragma unroll
   for (int r = 0; r < (1 << kMaxRadixBits) / kSortThreads; ++r) {
+    if (r * kSortThreads >= radix) break;
     const int d = r * kSortThreads + (int)threadIdx.x;
     const uint32_t c = d < radix ? a.total[d] : 0u;
     uint32_t x = c;
@@ -234,6 +302,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
 
 // The whole sort of up to kSmall tokens: 16 waves, strips of 256 tokens, digits of 8 bits.
 __global__ void __launch_bounds__(1024) sort_small_kernel(SortArgs a, int passes) {
+  if (fills(a)) return;
   constexpr int W = 16, IT = kSmall / 1024, R = 1 << kSmallBits;
   __shared__ uint32_t cnt[W][R];
   __shared__ uint32_t ks[kSmall], vs[kSmall];
@@ -322,54 +391,32 @@ struct SumArgs {
   float c, c2, cap;
 };
 
-// Four consecutive floats at any 4-byte alignment: one 16-byte access on gfx950.
-typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-
-__device__ __forceinline__ f4 ld4(const float* p, int left) {
-  if (left >= 4) return *reinterpret_cast<const f4*>(p);
-  f4 v = {p[0], 0.f, 0.f, 0.f};
-  if (left > 1) v.y = p[1];
-  if (left > 2) v.z = p[2];
-  return v;
-}
-__device__ __forceinline__ void st4(float* p, f4 v, int left) {
-  if (left >= 4) {
-    *reinterpret_cast<f4*>(p) = v;
-    return;
-  }
-  p[0] = v.x;
-  if (left > 1) p[1] = v.y;
-  if (left > 2) p[2] = v.z;
-}
-
-// The finished sums of up to 4 columns of a category: weighted, stored, applied.
-template <bool UPD>
-__device__ __forceinline__ void finish(const SumArgs& a, uint32_t cat, int col, f4 sm, f4 ss) {
-  const int64_t o = (int64_t)cat * a.D + col;
-  const int left = a.D - col;
-  f4 S = ld4(a.Sw + o, left);
+// The finished sums of a lane's columns of a category: weighted, stored, applied.
+template <bool UPD, bool WIDE>
+__device__ __forceinline__ void finish(const SumArgs& a, uint32_t cat, const Cols& c, f4 sm, f4 ss, f4 m, f4 S) {
+  const int64_t o = (int64_t)cat * a.D + c.at;
   const f4 dm = (sm * a.c) * S, dS = (ss * a.c2) * (S * S);
   if (!UPD || a.dmw) {
-    st4(a.dmw + o, dm, left);
-    st4(a.dSw + o, dS, left);
+    stc<WIDE>(a.dmw + o, dm, a.D, c.skip);
+    stc<WIDE>(a.dSw + o, dS, a.D, c.skip);
   }
   if constexpr (UPD) {
-    f4 m = ld4(a.mw + o, left);
     float mm[4] = {m.x, m.y, m.z, m.w}, vv[4] = {S.x, S.y, S.z, S.w};
     const float d[4] = {dm.x, dm.y, dm.z, dm.w}, e[4] = {dS.x, dS.y, dS.z, dS.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) capped(mm[i], vv[i], d[i], e[i], a.cap);
-    st4(a.mw + o, f4{mm[0], mm[1], mm[2], mm[3]}, left);
-    st4(a.Sw + o, f4{vv[0], vv[1], vv[2], vv[3]}, left);
+    stc<WIDE>(a.mw + o, f4{mm[0], mm[1], mm[2], mm[3]}, a.D, c.skip);
+    stc<WIDE>(a.Sw + o, f4{vv[0], vv[1], vv[2], vv[3]}, a.D, c.skip);
   }
 }
 
-// One wave per piece and 256 columns; the rows of kAhead tokens are loaded before they are
-// added, in order.
-constexpr int kAhead = 8;
-template <bool UPD>
+// One wave per piece and 256 columns; the rows of AHEAD tokens, and the table's rows of the
+// runs that end among them, are loaded before the tokens are added in order. Most categories
+// of a large table have one token: without that each would wait for its own row.
+template <bool UPD, bool WIDE, int AHEAD>
 __global__ void __launch_bounds__(64) embedding_sum_kernel(SumArgs a) {
-  const int lane = threadIdx.x, col = ((int)blockIdx.y * 64 + lane) * 4, P = a.piece, left = a.D - col;
+  const int lane = threadIdx.x, P = a.piece;
+  const Cols c = columns((int)blockIdx.y * 64 + lane, a.D);
   const int64_t p0 = (int64_t)blockIdx.x * P;
   const int cnt = (int)min((int64_t)P, a.n - p0);
   const uint32_t mykey = lane < cnt ? a.key[p0 + lane] : 0u, myval = lane < cnt ? a.val[p0 + lane] : 0u;
@@ -380,37 +427,44 @@ __global__ void __launch_bounds__(64) embedding_sum_kernel(SumArgs a) {
   int start = 0;  // first entry of the run being summed
   const uint64_t padding = __ballot(lane < cnt && mykey >= a.V);
   const int real = padding ? __ffsll((long long)padding) - 1 : cnt;  // padding sorts last
-  for (int j0 = 0; j0 < real; j0 += kAhead) {
-    f4 xm[kAhead], xs[kAhead];
+  const auto category_at = [&](int j) -> uint32_t {
+    return j < cnt ? (uint32_t)__builtin_amdgcn_readlane(mykey, j) : after;
+  };
+  for (int j0 = 0; j0 < real; j0 += AHEAD) {
+    f4 xm[AHEAD], xs[AHEAD], rm[UPD ? AHEAD : 1], rS[AHEAD];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      xm[u] = xs[u] = z;
-      if (j0 + u < real && left > 0) {
-        const int64_t at = (int64_t)(uint32_t)__builtin_amdgcn_readlane(myval, j0 + u) * a.D + col;
-        xm[u] = ld4(a.dmz + at, left);
-        xs[u] = ld4(a.dSz + at, left);
+    for (int u = 0; u < AHEAD; ++u) {
+      const int j = j0 + u;
+      xm[u] = xs[u] = rS[u] = z;
+      if constexpr (UPD) rm[u] = z;
+      if (j < real) {
+        const int64_t at = (int64_t)(uint32_t)__builtin_amdgcn_readlane(myval, j) * a.D + c.at;
+        xm[u] = ldc<WIDE>(a.dmz + at, a.D);
+        xs[u] = ldc<WIDE>(a.dSz + at, a.D);
+        const uint32_t cat = category_at(j);
+        if (category_at(j + 1) != cat) {
+          const int64_t o = (int64_t)cat * a.D + c.at;
+          rS[u] = ldc<WIDE>(a.Sw + o, a.D);
+          if constexpr (UPD) rm[u] = ldc<WIDE>(a.mw + o, a.D);
+        }
       }
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       const int j = j0 + u;
       if (j >= real) break;
       sm += xm[u];
       ss += xs[u];
-      const uint32_t cat = __builtin_amdgcn_readlane(mykey, j);
-      const bool last = j + 1 == cnt;
-      const uint32_t next = last ? after : (uint32_t)__builtin_amdgcn_readlane(mykey, j + 1);
-      const bool open_right = last && next == cat;
+      const uint32_t cat = category_at(j), next = category_at(j + 1);
+      const bool open_right = j + 1 == cnt && next == cat;
       if (next != cat || open_right) {
         const bool open_left = start == 0 && before == cat;
-        if (left > 0) {
-          if (open_left || open_right) {
-            float* p = a.part + (((int64_t)blockIdx.x * 2 + (open_left ? 0 : 1)) * 2) * a.D + col;
-            st4(p, sm, left);
-            st4(p + a.D, ss, left);
-          } else {
-            finish<UPD>(a, cat, col, sm, ss);
-          }
+        if (open_left || open_right) {
+          float* p = a.part + (((int64_t)blockIdx.x * 2 + (open_left ? 0 : 1)) * 2) * a.D + c.at;
+          stc<WIDE>(p, sm, a.D, c.skip);
+          stc<WIDE>(p + a.D, ss, a.D, c.skip);
+        } else {
+          finish<UPD, WIDE>(a, cat, c, sm, ss, rm[UPD ? u : 0], rS[u]);
         }
         sm = ss = z;
         start = j + 1;
@@ -423,60 +477,60 @@ __global__ void __launch_bounds__(64) embedding_sum_kernel(SumArgs a) {
 // sums, each of its waves a stretch of them in order and then the waves in order, in float64
 // (up to n / piece of them).
 constexpr int kJoinWaves = 4;
-template <bool UPD>
+template <bool UPD, bool WIDE>
 __global__ void __launch_bounds__(64 * kJoinWaves) embedding_join_kernel(SumArgs a) {
   __shared__ double red[kJoinWaves][8][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = ((int)blockIdx.y * 64 + lane) * 4, left = a.D - col;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Cols c = columns((int)blockIdx.y * 64 + lane, a.D);
   const int64_t p = blockIdx.x, P = a.piece, last = (p + 1) * P - 1;
   if (last + 1 >= a.n) return;  // the last piece's runs end in it
-  const uint32_t cat = a.key[last];
-  if (cat >= a.V || a.key[last + 1] != cat) return;
-  if (p > 0 && a.key[p * P] == cat && a.key[p * P - 1] == cat) return;  // started in an earlier piece
+  // the keys that decide, and those of the next 64 pieces, in one round trip
+  const auto first_key = [&](int64_t r) { return r < a.pieces ? a.key[r * P] : 0xffffffffu; };
+  const uint32_t cat = a.key[last], after = a.key[last + 1], head = a.key[p * P];
+  const uint32_t before = p > 0 ? a.key[p * P - 1] : 0xffffffffu;
+  uint32_t ahead = first_key(p + 1 + lane);
+  if (cat >= a.V || after != cat) return;
+  if (head == cat && before == cat) return;  // started in an earlier piece
+  const int64_t o = (int64_t)cat * a.D + c.at;
+  f4 S = {0.f, 0.f, 0.f, 0.f}, m = S;
+  if (wave == 0) {
+    S = ldc<WIDE>(a.Sw + o, a.D);
+    if constexpr (UPD) m = ldc<WIDE>(a.mw + o, a.D);
+  }
   // pieces p + 1 .. p + more hold the run's further partial sums
   int64_t more = 0;
   while (true) {
-    const int64_t r = p + 1 + more + lane;
-    const uint64_t off = ~__ballot(r < a.pieces && a.key[r * P] == cat);
+    const uint64_t off = ~__ballot(ahead == cat);
     if (off) {
       more += __ffsll((long long)off) - 1;
       break;
     }
     more += 64;
+    ahead = first_key(p + 1 + more + lane);
   }
   double s[8] = {};
-  if (left > 0) {
-    const int64_t q0 = (more + 1) * wave / kJoinWaves, q1 = (more + 1) * (wave + 1) / kJoinWaves;
-#pragma unroll 4
-    for (int64_t q = q0; q < q1; ++q) {
-      const float* x = a.part + ((p + q) * 2 + (q == 0 ? 1 : 0)) * 2 * a.D + col;
-      const f4 m = ld4(x, left), v = ld4(x + a.D, left);
-      s[0] += m.x, s[1] += m.y, s[2] += m.z, s[3] += m.w;
-      s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
-    }
-  }
+      const int64_t q0 = (more + 1) * wave / kJoinWaves, q1 = (more + 1) * (wave + 1) / kJoinWaves;
+#pragma unroll 8
+      for (int64_t q = q0; q < q1; ++q) {
+        const float* x = a.part + ((p + q) * 2 + (q == 0 ? 1 : 0)) * 2 * a.D + c.at;
+        const f4 y = ldc<WIDE>(x, a.D), v = ldc<WIDE>(x + a.D, a.D);
+        s[0] += y.x, s[1] += y.y, s[2] += y.z, s[3] += y.w;
+        s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
+      }
 #pragma unroll
   for (int e = 0; e < 8; ++e) red[wave][e][lane] = s[e];
   __syncthreads();
-  if (wave || left <= 0) return;
+  if (wave) return;
 #pragma unroll
   for (int w = 1; w < kJoinWaves; ++w)
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] += red[w][e][lane];
-  finish<UPD>(a, cat, col, f4{(float)s[0], (float)s[1], (float)s[2], (float)s[3]},
-              f4{(float)s[4], (float)s[5], (float)s[6], (float)s[7]});
-}
-
-__global__ void __launch_bounds__(256) zero2_kernel(float* __restrict__ x, float* __restrict__ y, int64_t n) {
-  const f4 z = {0.f, 0.f, 0.f, 0.f};
-  const int64_t step = (int64_t)gridDim.x * 1024;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += step) {
-    st4(x + i, z, n - i < 4 ? (int)(n - i) : 4);
-    st4(y + i, z, n - i < 4 ? (int)(n - i) : 4);
-  }
+  finish<UPD, WIDE>(a, cat, c, f4{(float)s[0], (float)s[1], (float)s[2], (float)s[3]},
+              f4{(float)s[4], (float)s[5], (float)s[6], (float)s[7]}, m, S);
 }
 
 // Tokens of a piece: as many as keep 2048 waves busy, 16 to 64. Shorter pieces leave more
-// partial sums (PIECE).
+// partial sums. (16384 tokens x 256: pieces of 64 25 us for the sums, of 16 7.)
 int piece_len(int64_t n, int64_t D) {
   const int64_t cols = cdiv(D, 256);
   int p = 64;
@@ -500,11 +554,12 @@ Layout layout(int64_t n, int64_t V, int64_t D) {
   return l;
 }
 
-template <bool UPD>
+constexpr int kAhead = 4;
+template <bool UPD, bool WIDE>
 void launch_sums(const SumArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)a.pieces, (unsigned)cdiv(a.D, 256));
-  hipLaunchKernelGGL((embedding_sum_kernel<UPD>), grid, dim3(64), 0, s, a);
-  if (a.pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<UPD>), grid, dim3(64 * kJoinWaves), 0, s, a);
+  hipLaunchKernelGGL((embedding_sum_kernel<UPD, WIDE, kAhead>), grid, dim3(64), 0, s, a);
+  if (a.pieces > 1) hipLaunchKernelGGL((embedding_join_kernel<UPD, WIDE>), grid, dim3(64 * kJoinWaves), 0, s, a);
 }
 
 int sorted_impl(const char* what, const void* ids, int type, const float* dmz, const float* dSz, float* mw, float* Sw,
@@ -518,8 +573,6 @@ int sorted_impl(const char* what, const void* ids, int type, const float* dmz, c
   const Layout l = layout(n, V, D);
   TAGI_REQUIRE(n == 0 || (ws && ws_bytes >= l.bytes), "%s: workspace too small", what);
   ProfScope ps(FAM_EMBEDDING, s, 0.0, 4.0 * n + 8.0 * n * D + (dmw ? 8.0 * V * D : 0.0));
-  if (dmw) hipLaunchKernelGGL(zero2_kernel, dim3(ew_blocks(cdiv(V * D, 4), 256)), dim3(256), 0, s, dmw, dSw, V * D);
-  if (n == 0) return check_launch(what);
   const SortPlan p = sort_plan(n, V);
   char* base = static_cast<char*>(ws);
   const int64_t na = pad16(4 * n);
@@ -529,25 +582,44 @@ int sorted_impl(const char* what, const void* ids, int type, const float* dmz, c
   a.ids = ids, a.type = type, a.n = n, a.V = V, a.pad = pad, a.nblk = (int)p.nblk, a.bits = p.bits;
   a.hist = reinterpret_cast<uint32_t*>(base + l.hist);
   a.total = reinterpret_cast<uint32_t*>(base + l.total);
-  if (n <= kSmall) {
+  a.z0 = dmw, a.z1 = dSw;
+  const bool small = n <= kSmall;
+  const int launches = small ? 1 : 3 * p.passes;
+  const int64_t share = dmw ? cdiv(cdiv(V * D, launches), 4) * 4 : 0;
+  int done = 0;
+  // the next launch's grid: `work` blocks, and those for its share of the zeros
+  const auto grid = [&](int64_t work, int threads) {
+    a.work = (int)work;
+    a.f0 = done * share, a.f1 = dmw ? (a.f0 + share < V * D ? a.f0 + share : V * D) : 0;
+    ++done;
+    int64_t fill = a.f1 > a.f0 ? cdiv(cdiv(a.f1 - a.f0, 4), threads) : 0;
+    if (fill > 1024) fill = 1024;
+    return dim3((unsigned)(work + fill));
+  };
+  if (small) {
     a.first = 1, a.kout = buf[0], a.vout = buf[1];
-    hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, s, a, (int)cdiv(key_bits(V), kSmallBits));
+    const dim3 g = grid(n > 0 ? 1 : 0, 1024);
+    if (g.x) hipLaunchKernelGGL(sort_small_kernel, g, dim3(1024), 0, s, a, (int)cdiv(key_bits(V), kSmallBits));
+    if (n == 0) return check_launch(what);
   } else {
     for (int k = 0; k < p.passes; ++k) {
       a.first = k == 0;
       a.kin = buf[2 * ((k + 1) & 1)], a.vin = buf[2 * ((k + 1) & 1) + 1];
       a.kout = buf[2 * (k & 1)], a.vout = buf[2 * (k & 1) + 1];
       a.shift = k * p.bits;
-      const dim3 grid((unsigned)p.nblk), block(kSortThreads), digits((unsigned)cdiv(1 << p.bits, 4));
+      const dim3 block(kSortThreads);
+      dim3 g = grid(p.nblk, kSortThreads);
       if (p.items == 4)
-        hipLaunchKernelGGL(sort_count_kernel<4>, grid, block, 0, s, a);
+        hipLaunchKernelGGL(sort_count_kernel<4>, g, block, 0, s, a);
       else
-        hipLaunchKernelGGL(sort_count_kernel<16>, grid, block, 0, s, a);
-      hipLaunchKernelGGL(sort_places_kernel, digits, dim3(256), 0, s, a);
+        hipLaunchKernelGGL(sort_count_kernel<16>, g, block, 0, s, a);
+      g = grid(cdiv(1 << p.bits, 4), kSortThreads);
+      hipLaunchKernelGGL(sort_places_kernel, g, block, 0, s, a);
+      g = grid(p.nblk, kSortThreads);
       if (p.items == 4)
-        hipLaunchKernelGGL(sort_scatter_kernel<4>, grid, block, 0, s, a);
+        hipLaunchKernelGGL(sort_scatter_kernel<4>, g, block, 0, s, a);
       else
-        hipLaunchKernelGGL(sort_scatter_kernel<16>, grid, block, 0, s, a);
+        hipLaunchKernelGGL(sort_scatter_kernel<16>, g, block, 0, s, a);
     }
   }
   SumArgs q{};
@@ -555,7 +627,10 @@ int sorted_impl(const char* what, const void* ids, int type, const float* dmz, c
   q.part = reinterpret_cast<float*>(base + l.part);
   q.mw = mw, q.Sw = Sw, q.dmw = dmw, q.dSw = dSw, q.n = n, q.V = V, q.D = (int)D;
   q.piece = piece_len(n, D), q.pieces = (int)cdiv(n, q.piece), q.c = (float)c, q.c2 = (float)(c * c), q.cap = cap;
-  upd ? launch_sums<true>(q, s) : launch_sums<false>(q, s);
+  if (D >= 4)
+    upd ? launch_sums<true, true>(q, s) : launch_sums<false, true>(q, s);
+  else
+    upd ? launch_sums<true, false>(q, s) : launch_sums<false, false>(q, s);
   return check_launch(what);
 }
 

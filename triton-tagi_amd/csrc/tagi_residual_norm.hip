@@ -26,17 +26,22 @@ __device__ __forceinline__ void st(float* p, f4 v) {
   else
     *reinterpret_cast<f4*>(p) = v;
 }
-// The row's last chunk, which may hold fewer than four.
-__device__ __forceinline__ f4 ld_tail(const float* p, int left) {
-  f4 v = {p[0], 0.f, 0.f, 0.f};
-  if (left > 1) v.y = p[1];
-  if (left > 2) v.z = p[2];
-  return v;
+// A thread's four columns. The last chunk of a row with D % 4 != 0 is the row's last four, of
+// which the first `skip` are the chunk's before as well: every load is one access with no
+// branch between them. Threads past the row take its first columns, all skipped. D >= 4.
+struct Cols {
+  int at, skip;
+};
+__device__ __forceinline__ Cols columns(int chunk, int D) {
+  Cols c{4 * chunk, 0};
+  if (c.at >= D)
+    c.at = 0, c.skip = 4;
+  else if (c.at + 4 > D)
+    c.skip = c.at + 4 - D, c.at = D - 4;
+  return c;
 }
-__device__ __forceinline__ void st_tail(float* p, f4 v, int left) {
-  p[0] = v.x;
-  if (left > 1) p[1] = v.y;
-  if (left > 2) p[2] = v.z;
+__device__ __forceinline__ f4 own(f4 v, int skip) {  // zeros for the skipped
+  return f4{skip > 0 ? 0.f : v.x, skip > 1 ? 0.f : v.y, skip > 2 ? 0.f : v.z, skip > 3 ? 0.f : v.w};
 }
 
 // Sum over the TPR threads of a row (a wave, or the whole block).
@@ -69,49 +74,36 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(
   const int t = (int)threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * RPB + (int)threadIdx.x / TPR, o = row * D;
   if (row >= rows) return;  // TPR > 64 has one row a block: no thread of it leaves
-  const int full = D >> 2, left = D & 3;
   f4 m[NV], v[NV];
   float acc = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = t + j * TPR;
-    m[j] = v[j] = f4{0.f, 0.f, 0.f, 0.f};
-    if (c < full) {
-      const int64_t at = o + 4 * c;
-      const f4 a = ld<NT>(ma + at), b = ld<NT>(mr + at), x = ld<NT>(Sa + at), y = ld<NT>(Sr + at);
-      m[j] = a + b, v[j] = x + y;
-    } else if (c == full && left) {
-      const int64_t at = o + 4 * c;
-      m[j] = ld_tail(ma + at, left) + ld_tail(mr + at, left), v[j] = ld_tail(Sa + at, left) + ld_tail(Sr + at, left);
-    }
+    const int64_t at = o + columns(t + j * TPR, D).at;
+    const f4 a = ld<NT>(ma + at), b = ld<NT>(mr + at), x = ld<NT>(Sa + at), y = ld<NT>(Sr + at);
+    m[j] = a + b, v[j] = x + y;
   }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const f4 q = m[j] * m[j] + v[j];
+    const f4 q = own(m[j] * m[j] + v[j], columns(t + j * TPR, D).skip);
     acc += (q.x + q.y) + (q.z + q.w);
   }
   const float inv = 1.f / sqrtf(row_sum<TPR>(acc, red) / (float)D + eps);
   if (t == 0) inv_rms[row] = inv;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = t + j * TPR;
-    if (c > full || (c == full && !left)) continue;
-    const int64_t at = o + 4 * c;
-    const bool tail = c == full;
-    const f4 g = tail ? ld_tail(mw + 4 * c, left) : *reinterpret_cast<const f4*>(mw + 4 * c);
-    const f4 sg = tail ? ld_tail(Sw + 4 * c, left) : *reinterpret_cast<const f4*>(Sw + 4 * c);
-    const f4 z = m[j] * inv * g, s = inv * inv * (v[j] * (g * g + sg) + sg * (m[j] * m[j]));
-    if (tail) {
-      st_tail(ms + at, m[j], left), st_tail(mz + at, z, left), st_tail(Sz + at, s, left);
-      if (Ss) st_tail(Ss + at, v[j], left);
-    } else {
-      st<NT>(ms + at, m[j]), st<NT>(mz + at, z), st<NT>(Sz + at, s);
-      if (Ss) st<NT>(Ss + at, v[j]);
-    }
+    const Cols c = columns(t + j * TPR, D);
+    if (c.skip == 4) continue;
+    const int64_t at = o + c.at;
+    const f4 g = *reinterpret_cast<const f4*>(mw + c.at), sg = *reinterpret_cast<const f4*>(Sw + c.at);
+    // columns of two threads get the same values from both
+    st<NT>(ms + at, m[j]);
+    if (Ss) st<NT>(Ss + at, v[j]);
+    st<NT>(mz + at, m[j] * inv * g);
+    st<NT>(Sz + at, inv * inv * (v[j] * (g * g + sg) + sg * (m[j] * m[j])));
   }
 }
 
-// Rows too long for registers: the inputs are read twice.
+// Rows too long for registers, or shorter than four: the inputs are read twice.
 __global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(
     const float* __restrict__ ma, const float* __restrict__ Sa, const float* __restrict__ mr,
     const float* __restrict__ Sr, const float* __restrict__ mw, const float* __restrict__ Sw, float* __restrict__ mz,
@@ -140,46 +132,51 @@ __global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(
 // threads of a column are joined in float64 through LDS, and one partial sum per block,
 // column and moment goes to ws[moment][block][D]. HBM bound: 16384 x 4096 with deltas at the
 // sum moves 1.88 GB in 342 us (5.5 TB/s).
-template <bool NT>
+template <bool NT, bool WIDE>
 __global__ void __launch_bounds__(256) add_rms_norm_bwd_kernel(
     const float* __restrict__ dmz, const float* __restrict__ dSz, const float* __restrict__ dms,
     const float* __restrict__ dSs, const float* __restrict__ ms, const float* __restrict__ inv_rms,
     const float* __restrict__ mw, float* __restrict__ dma, float* __restrict__ dSa, float* __restrict__ ws,
     int64_t rows, int D, int CT) {
   __shared__ f4 red[2][256];
-  const int RG = 256 / CT, ct = (int)threadIdx.x % CT, rg = (int)threadIdx.x / CT;
-  const int c = 4 * ((int)blockIdx.y * CT + ct), nblk = (int)gridDim.x, left = D - c;
+  const int RG = 256 / CT, ct = (int)threadIdx.x % CT, rg = (int)threadIdx.x / CT, nblk = (int)gridDim.x;
   const int64_t r0 = rows * blockIdx.x / nblk, r1 = rows * (blockIdx.x + 1) / nblk;
   f4 am = {0.f, 0.f, 0.f, 0.f}, as = am;
-  const bool live = left > 0 && rg < RG;
-  if (live && left >= 4) {
-    const f4 g = *reinterpret_cast<const f4*>(mw + c);
+  int skip = 4;
+  if constexpr (WIDE) {
+    const Cols c = columns((int)blockIdx.y * CT + ct, D);
+    skip = rg < RG ? c.skip : 4;
+    if (skip < 4) {
+      const f4 g = *reinterpret_cast<const f4*>(mw + c.at);
 #pragma unroll 2
-    for (int64_t r = r0 + rg; r < r1; r += RG) {
-      const int64_t o = r * D + c;
-      const float inv = inv_rms[r];
-      const f4 a = ld<NT>(dmz + o), b = ld<NT>(dSz + o), x = ld<NT>(ms + o) * inv, k = g * inv;
-      f4 u = a * k, w = b * (k * k);
-      if (dms) u += ld<NT>(dms + o), w += ld<NT>(dSs + o);
-      st<NT>(dma + o, u);
-      st<NT>(dSa + o, w);
-      am += a * x;
-      as += b * (x * x);
+      for (int64_t r = r0 + rg; r < r1; r += RG) {
+        const int64_t o = r * D + c.at;
+        const float inv = inv_rms[r];
+        const f4 a = ld<NT>(dmz + o), b = ld<NT>(dSz + o), x = ld<NT>(ms + o) * inv, k = g * inv;
+        f4 u = a * k, w = b * (k * k);
+        if (dms) u += ld<NT>(dms + o), w += ld<NT>(dSs + o);
+        st<NT>(dma + o, u);  // columns of two threads get the same values from both
+        st<NT>(dSa + o, w);
+        am += a * x;
+        as += b * (x * x);
+      }
     }
-  } else if (live) {
-    const f4 g = ld_tail(mw + c, left);
-    for (int64_t r = r0 + rg; r < r1; r += RG) {
-      const int64_t o = r * D + c;
-      const float inv = inv_rms[r];
-      const f4 a = ld_tail(dmz + o, left), b = ld_tail(dSz + o, left), x = ld_tail(ms + o, left) * inv, k = g * inv;
-      f4 u = a * k, w = b * (k * k);
-      if (dms) u += ld_tail(dms + o, left), w += ld_tail(dSs + o, left);
-      st_tail(dma + o, u, left);
-      st_tail(dSa + o, w, left);
-      am += a * x;
-      as += b * (x * x);
-    }
+  } else if (rg < RG) {  // rows of one to three values, one thread across
+    skip = 0;
+    for (int64_t r = r0 + rg; r < r1; r += RG)
+      for (int e = 0; e < D; ++e) {
+        const int64_t o = r * D + e;
+        const float inv = inv_rms[r], x = inv * ms[o], k = inv * mw[e], a = dmz[o], b = dSz[o];
+        dma[o] = a * k + (dms ? dms[o] : 0.f);
+        dSa[o] = b * (k * k) + (dSs ? dSs[o] : 0.f);
+        am[e] += a * x;
+        as[e] += b * (x * x);
+      }
   }
+  // the thread's own columns first
+  if (skip == 1) am = f4{am.y, am.z, am.w, 0.f}, as = f4{as.y, as.z, as.w, 0.f};
+  if (skip == 2) am = f4{am.z, am.w, 0.f, 0.f}, as = f4{as.z, as.w, 0.f, 0.f};
+  if (skip == 3) am = f4{am.w, 0.f, 0.f, 0.f}, as = f4{as.w, 0.f, 0.f, 0.f};
   red[0][threadIdx.x] = am, red[1][threadIdx.x] = as;
   __syncthreads();
   // value e of column chunk q, moment w: the RG threads' sums in order
@@ -292,7 +289,7 @@ extern "C" int tagi_add_rmsnorm_fwd(const float* ma, const float* Sa, const floa
   // threads of a row: a wave for short rows, or for longer ones when there are rows enough to
   // fill the GPU; more where few rows would wait on each thread's loads
   const int64_t chunks = cdiv(D, 4);
-  if (chunks > 8 * 1024)
+  if (chunks > 8 * 1024 || D < 4)
     hipLaunchKernelGGL(add_rms_norm_long_kernel, dim3((unsigned)rows), dim3(1024), 0, s, ma, Sa, mr, Sr, mw, Sw, mz, Sz,
                        ms, Ss, inv_rms, (int)D, eps);
   else if (chunks <= 64 || (chunks <= 4 * 64 && rows >= 4096))
@@ -326,12 +323,11 @@ extern "C" int tagi_add_rmsnorm_bwd(const float* dmz, const float* dSz, const fl
   if (rows > 0) {
     const dim3 grid((unsigned)p.nblk, (unsigned)p.chunks);
     float* part = static_cast<float*>(ws);
-    if ((dms ? 28.0 : 20.0) * rows * D > kCacheBytes)
-      hipLaunchKernelGGL(add_rms_norm_bwd_kernel<true>, grid, dim3(256), 0, s, dmz, dSz, dms, dSs, ms, inv_rms, mw, dma,
-                         dSa, part, rows, (int)D, p.ct);
-    else
-      hipLaunchKernelGGL(add_rms_norm_bwd_kernel<false>, grid, dim3(256), 0, s, dmz, dSz, dms, dSs, ms, inv_rms, mw,
-                         dma, dSa, part, rows, (int)D, p.ct);
+    const bool nt = (dms ? 28.0 : 20.0) * rows * D > kCacheBytes;
+    const auto kernel = D < 4 ? add_rms_norm_bwd_kernel<false, false>
+                              : (nt ? add_rms_norm_bwd_kernel<true, true> : add_rms_norm_bwd_kernel<false, true>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, dmz, dSz, dms, dSs, ms, inv_rms, mw, dma, dSa, part, rows, (int)D,
+                       p.ct);
   }
   hipLaunchKernelGGL(add_rms_norm_finalize_kernel, dim3((unsigned)cdiv(D, 32), 2), dim3(256), 0, s,
                      static_cast<const float*>(ws), Sw, dmw, dSw, (int)D, p.nblk);
