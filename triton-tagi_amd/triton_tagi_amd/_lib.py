@@ -226,11 +226,15 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed (status {rc}): {last_error()}")
 
 
+# torch.cuda.current_device without its initialisation check: a tensor on a GPU exists
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def call_on(t: torch.Tensor, name: str, *args) -> None:
     """``call`` with t's GPU as the current device (a launch on another device's stream is
     refused by the runtime); nothing is switched when it is current already."""
     dev = t.get_device()
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         call(name, *args)
     else:
         with torch.cuda.device(dev):
@@ -295,6 +299,15 @@ def check_with(t: torch.Tensor, name: str, ref: torch.Tensor, shape=None) -> tor
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     return t
+
+
+def dense_with(t: torch.Tensor, name: str, ref: torch.Tensor, shape) -> torch.Tensor:
+    """``check_with``, as a contiguous tensor. One test for the usual case: a small call
+    spends more on its arguments than on the GPU."""
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == ref.get_device()
+            and t.shape == shape and t.is_contiguous()):
+        return t
+    return check_with(t, name, ref, shape).contiguous()
 
 
 def check_in_place(t: torch.Tensor, name: str) -> torch.Tensor:

@@ -28,14 +28,14 @@ def _check_ids(ids: Tensor, ref: Tensor) -> tuple[Tensor, int]:
     kind = _ID_TYPES.get(ids.dtype)
     if kind is None:
         raise TypeError(f"ids: expected float32, int32 or int64, got {ids.dtype}")
-    if ids.device != ref.device:
+    if ids.get_device() != ref.get_device():
         raise ValueError(f"ids: tensor is on {ids.device}, the table on {ref.device}")
     return ids.contiguous(), kind
 
 
 def _check_table(t: Tensor, name: str) -> Tensor:
     _lib.check(t, name, contiguous=False)
-    if t.dim() != 2 or t.shape[0] == 0 or t.shape[1] == 0:
+    if t.dim() != 2 or t.numel() == 0:
         raise ValueError(f"{name}: expected a (categories, features) table, got {tuple(t.shape)}")
     return t
 
@@ -62,7 +62,7 @@ def embedding_lookup(ids: Tensor, mw: Tensor, Sw: Tensor, scale: float = 1.0,
                      padding_idx: int = -1) -> tuple[Tensor, Tensor]:
     """Moments (*ids.shape, D) of the rows ``ids`` of the table (mw, Sw), scaled."""
     mw = _check_table(mw, "mw").contiguous()
-    Sw = _lib.check_with(Sw, "Sw", mw, mw.shape).contiguous()
+    Sw = _lib.dense_with(Sw, "Sw", mw, mw.shape)
     ids, kind = _check_ids(ids, mw)
     scale = _check_scale(scale)
     V, D = mw.shape

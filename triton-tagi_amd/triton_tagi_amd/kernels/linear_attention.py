@@ -30,6 +30,11 @@ from .. import _lib
 
 def _pair(m: Tensor, S: Tensor, name: str, ref: Tensor, shape) -> tuple[Tensor, Tensor]:
     """A mean and its variance in one layout with a unit last stride."""
+    if (isinstance(m, Tensor) and isinstance(S, Tensor) and m.dtype is torch.float32 and S.dtype is torch.float32
+            and m.get_device() == ref.get_device() == S.get_device() and m.shape == shape == S.shape):
+        st = m.stride()
+        if st == S.stride() and (st[-1] == 1 or shape[-1] == 1):
+            return m, S
     _lib.check_with(m, "m" + name, ref, shape)
     _lib.check_with(S, "S" + name, ref, shape)
     if m.stride() != S.stride() or (m.stride(-1) != 1 and m.shape[-1] != 1):
@@ -47,16 +52,16 @@ def _heads(t: Tensor) -> _lib.Heads:
     return _lib.Heads(st[0], st[1], st[2]) if t.dim() == 4 else _lib.Heads(st[0], 0, st[1])
 
 
-def _shape(t: Tensor, dims: int) -> tuple:
+def _shape(t: Tensor, dims: int) -> torch.Size:
     _lib.check(t, "mq", contiguous=False)
     if t.dim() != dims or min(t.shape[-2:]) == 0:
         what = "(B, T, H, D)" if dims == 4 else "(B, H, D)"
         raise ValueError(f"mq: expected {what} with heads and features, got {tuple(t.shape)}")
-    return tuple(t.shape)
+    return t.shape
 
 
 def _decay(decay: Tensor, ref: Tensor, H: int) -> Tensor:
-    return _lib.check_with(decay, "decay", ref, (H,)).contiguous()
+    return _lib.dense_with(decay, "decay", ref, (H,))
 
 
 def _scale(scale: float) -> float:

@@ -27,9 +27,11 @@ def add_rms_norm(ma: Tensor, Sa: Tensor, mr: Tensor, Sr: Tensor, mw: Tensor, Sw:
     if ma.dim() < 1 or ma.shape[-1] == 0:
         raise ValueError(f"ma: rows must hold at least one feature, got {tuple(ma.shape)}")
     ma = ma.contiguous()
-    Sa, mr, Sr = (_lib.check_with(t, n, ma, ma.shape).contiguous() for t, n in ((Sa, "Sa"), (mr, "mr"), (Sr, "Sr")))
-    D, rows = ma.shape[-1], _rows(ma)
-    mw, Sw = (_lib.check_with(t, n, ma, (D,)).contiguous() for t, n in ((mw, "mw"), (Sw, "Sw")))
+    shape = ma.shape
+    D, rows = shape[-1], _rows(ma)
+    Sa, mr, Sr = (_lib.dense_with(Sa, "Sa", ma, shape), _lib.dense_with(mr, "mr", ma, shape),
+                  _lib.dense_with(Sr, "Sr", ma, shape))
+    mw, Sw = _lib.dense_with(mw, "mw", ma, (D,)), _lib.dense_with(Sw, "Sw", ma, (D,))
     mz, Sz, ms = torch.empty_like(ma), torch.empty_like(ma), torch.empty_like(ma)
     Ss = torch.empty_like(ma) if need_sum_var else None
     inv = torch.empty(rows, 1, device=ma.device, dtype=torch.float32)
@@ -52,15 +54,14 @@ def add_rms_norm_backward(delta_mz: Tensor, delta_Sz: Tensor, ms: Tensor, inv_rm
         raise ValueError("delta_ms and delta_Ss must be given together")
     ms = ms.contiguous()
     D, rows = ms.shape[-1], _rows(ms)
-    dm, dS = (_lib.check_with(t, n, ms, ms.shape).contiguous() for t, n in ((delta_mz, "delta_mz"),
-                                                                            (delta_Sz, "delta_Sz")))
+    dm, dS = _lib.dense_with(delta_mz, "delta_mz", ms, ms.shape), _lib.dense_with(delta_Sz, "delta_Sz", ms, ms.shape)
     if delta_ms is not None:
-        delta_ms, delta_Ss = (_lib.check_with(t, n, ms, ms.shape).contiguous()
-                              for t, n in ((delta_ms, "delta_ms"), (delta_Ss, "delta_Ss")))
+        delta_ms = _lib.dense_with(delta_ms, "delta_ms", ms, ms.shape)
+        delta_Ss = _lib.dense_with(delta_Ss, "delta_Ss", ms, ms.shape)
     inv = _lib.check_with(inv_rms, "inv_rms", ms).contiguous()
     if inv.numel() != rows:
         raise ValueError(f"inv_rms: expected {rows} rows, got {tuple(inv.shape)}")
-    mw, Sw = (_lib.check_with(t, n, ms, (D,)).contiguous() for t, n in ((mw, "mw"), (Sw, "Sw")))
+    mw, Sw = _lib.dense_with(mw, "mw", ms, (D,)), _lib.dense_with(Sw, "Sw", ms, (D,))
     dma, dSa = torch.empty_like(ms), torch.empty_like(ms)
     dmw, dSw = torch.empty_like(mw), torch.empty_like(mw)
     ws = _lib.workspace(_lib.query("tagi_add_rmsnorm_bwd_ws_bytes", rows, D), ms.device)
