@@ -646,7 +646,10 @@ struct Chunks {
   int cols;
 };
 Chunks chunks(int64_t B, int64_t T, int64_t H, int64_t D, bool bwd) {
-  const int64_t heads = B * H, target = bwd ? 1024 : 2048, enough = bwd ? 512 : 2048;
+  // three-wave blocks (65 to 96 features) fit a CU twice, not 2 2/3 times: 512 of them at once
+  // (7 x 777 tokens, 6 heads of 80: 11 chunks 152, 14 chunks 181)
+  const int64_t heads = B * H, full = D > 64 && D <= 96 ? 1536 : 2048, target = bwd ? 1024 : full;
+  const int64_t enough = bwd ? 512 : full;
   const auto waves = [&](int cols) { return heads * cdiv(D, cols); };
   Chunks c{cdiv(T > 0 ? T : 1, kTok) * kTok, 1, 8};
   for (int cols = 32; cols >= (bwd ? 16 : 8); cols /= 2)
