@@ -37,7 +37,7 @@ enum Mode { FWD = 0, DQ = 1, DK = 2, DV = 3 };
 // vectors staged per token, over i and over o
 constexpr int n_ivec(int m) { return m == FWD ? 6 : (m == DQ ? 3 : 4); }
 constexpr int n_ovec(int m) { return m == FWD ? 3 : (m == DQ ? 1 : 2); }
-constexpr int scan_threads(int di, int eo) { return 64 * di / eo; }  // a wave per 8 eo columns of 8 di
+constexpr int scan_threads(int ip, int ig, int eo) { return ip * ig / eo; }  // 64 per 64 eo / ig columns
 
 struct Args {
   // DQ/DK/DV read the means and the deltas (dm, dS) only
@@ -91,34 +91,22 @@ __device__ __forceinline__ float dpp(float x) {
 }
 constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kXor7 = 0x141;  // quad_perm, quad_perm, row_half_mirror
 
-// Sums over the 8 lanes of a group (lane & 7) of EO means and EO variances per lane. Lanes
-// with bit 2 set end with variances, the others with means; of the EO values the lane's
-// bit 0 (and, with four, bit 1) says which, lanes that differ in the bits left over agree.
-template <int EO>
+// Sums over the IG lanes of a group (consecutive lanes) of EO means and EO variances per lane.
+// Lanes whose bit IG / 2 is set end with variances, the others with means; with two columns
+// the lane's bit 0 says which, and lanes that differ in the bits left over agree.
+template <int IG, int EO>
 __device__ __forceinline__ float group_sums(const float* pm, const float* ps, int lane) {
+  const bool var = lane & (IG / 2), odd = lane & 1;
   float r[EO];
-  const bool b2 = lane & 4, b0 = lane & 1, b1 = lane & 2;
 #pragma unroll
   for (int e = 0; e < EO; ++e) {
-    const float keep = b2 ? ps[e] : pm[e], give = b2 ? pm[e] : ps[e];
-    r[e] = keep + dpp<kXor7>(give);
+    const float keep = var ? ps[e] : pm[e], give = var ? pm[e] : ps[e];
+    r[e] = keep + dpp<IG == 8 ? kXor7 : kXor2>(give);
   }
-  if constexpr (EO == 1) {
-    r[0] += dpp<kXor1>(r[0]);
-    return r[0] + dpp<kXor2>(r[0]);
-  } else {
-    float h[EO / 2];
-#pragma unroll
-    for (int e = 0; e < EO / 2; ++e) {
-      const float keep = b0 ? r[EO / 2 + e] : r[e], give = b0 ? r[e] : r[EO / 2 + e];
-      h[e] = keep + dpp<kXor1>(give);
-    }
-    if constexpr (EO == 2) return h[0] + dpp<kXor2>(h[0]);
-    if constexpr (EO == 4) {
-      const float keep = b1 ? h[1] : h[0], give = b1 ? h[0] : h[1];
-      return keep + dpp<kXor2>(give);
-    }
-  }
+  if constexpr (IG == 8) r[0] += dpp<kXor2>(r[0]);
+  if constexpr (EO == 1) return r[0] + dpp<kXor1>(r[0]);
+  const float keep = odd ? r[EO - 1] : r[0], give = odd ? r[0] : r[EO - 1];
+  return keep + dpp<kXor1>(give);
 }
 
 // Four consecutive values of a token's head row (zeros past D).
@@ -141,10 +129,12 @@ __device__ __forceinline__ float4 add4(float4 a, float4 b) {
 }
 
 // The scan of one (sequence, head, chunk), one block.
-template <int MODE, int DI, int EO, bool VEC>
+template <int MODE, int IP, int IG, int EO, bool VEC>
 __device__ __forceinline__ void scan(const Args& a, float4* lds, int64_t bid) {
-  constexpr int IP = 8 * DI;                  // padded head dimension
-  constexpr int NT = scan_threads(DI, EO);
+  // IP: the padded head dimension. A lane holds DI rows and EO columns of the state, IG lanes
+  // share a column, a wave takes CW columns
+  constexpr int DI = IP / IG, CW = EO * 64 / IG, NT = scan_threads(IP, IG, EO);
+  static_assert((IG == 4 && EO <= 2) || (IG == 8 && EO == 1), "layouts of group_sums");
   constexpr bool REV = MODE >= DK, TWO_STATES = MODE != DQ;
   constexpr int NI = n_ivec(MODE), NO = n_ovec(MODE);
   constexpr int C4 = IP / 4;                  // float4 chunks of a row
@@ -156,7 +146,7 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds, int64_t bid) {
   const int h = (int)(bh % a.H), D = a.D;
   const int64_t n = seq_len(a, b), t0 = ch * a.L, t1 = min(a.T, t0 + a.L), live = min(n, t1);
   const int cnt = live > t0 ? (int)(live - t0) : 0;  // live tokens of the chunk
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, ig = lane & 7, og = lane >> 3;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, ig = lane % IG, og = lane / IG;
 
   const float g = a.decay[h];
   const bool grouped = fabsf(g) >= kGroupMin;
@@ -236,10 +226,10 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds, int64_t bid) {
     }
   };
 
-  // state element (i, o): i = 32 (k / 4) + 4 ig + k % 4 (DI a multiple of 4), the o of this wave
+  // state element (i, o): rows in fours (DI a multiple of 4), the o of this wave
   constexpr int KN = DI % 4 == 0 ? 4 : DI;
-  auto idx_i = [&](int k) { return DI % 4 == 0 ? 32 * (k >> 2) + 4 * ig + (k & 3) : DI * ig + k; };
-  auto idx_o = [&](int e) { return 8 * EO * wave + EO * og + e; };
+  auto idx_i = [&](int k) { return KN * IG * (k / KN) + KN * ig + k % KN; };
+  auto idx_o = [&](int e) { return CW * wave + EO * og + e; };
   float X[DI][EO], Y[TWO_STATES ? DI : 1][EO];
 #pragma unroll
   for (int k = 0; k < DI; ++k)
@@ -273,7 +263,7 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds, int64_t bid) {
     float w[NO][EO];
 #pragma unroll
     for (int v = 0; v < NO; ++v) {
-      const float* p = reinterpret_cast<const float*>(&ov(v, j, 0)) + 8 * EO * wave + EO * og;
+      const float* p = reinterpret_cast<const float*>(&ov(v, j, 0)) + idx_o(0);
 #pragma unroll
       for (int e = 0; e < EO; ++e) w[v][e] = p[e];
     }
@@ -311,12 +301,12 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds, int64_t bid) {
           }
         }
     }
-    const float r = group_sums<EO>(pm, ps, lane);
-    const int o = idx_o(0) + (EO == 4 ? 2 * (lane & 1) + ((lane >> 1) & 1) : (EO == 2 ? lane & 1 : 0));
-    const bool mine = EO == 4 || (lane & (EO == 2 ? 2 : 3)) == 0;
+    const float r = group_sums<IG, EO>(pm, ps, lane);
+    const int o = idx_o(EO == 2 ? lane & 1 : 0);
+    const bool mine = EO == 2 || (lane & (IG / 2 - 1)) == 0;
     float* om = MODE == DK ? a.km : (MODE == DV ? a.vm : a.om);
     float* oS = MODE == DK ? a.kS : (MODE == DV ? a.vS : a.oS);
-    if (mine && o < D) ((lane & 4) ? oS : om)[ob + tok(s0 + j) * a.lo.st + o] = r;
+    if (mine && o < D) ((lane & (IG / 2)) ? oS : om)[ob + tok(s0 + j) * a.lo.st + o] = r;
   };
 
   for (int s0 = 0; s0 < cnt; s0 += kTok) {
@@ -374,25 +364,25 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds, int64_t bid) {
   }
 }
 
-template <int DI, int EO, bool VEC>
-__global__ void __launch_bounds__(scan_threads(DI, EO)) scan_fwd_kernel(Args a) {
-  __shared__ float4 lds[(n_ivec(FWD) + n_ovec(FWD)) * kTok * 2 * DI];
-  scan<FWD, DI, EO, VEC>(a, lds, blockIdx.x);
+template <int IP, int IG, int EO, bool VEC>
+__global__ void __launch_bounds__(scan_threads(IP, IG, EO)) scan_fwd_kernel(Args a) {
+  __shared__ float4 lds[(n_ivec(FWD) + n_ovec(FWD)) * kTok * IP / 4];
+  scan<FWD, IP, IG, EO, VEC>(a, lds, blockIdx.x);
 }
 // The three backward scans are independent and read the same tensors: one launch, the three
 // blocks of a chunk 8 block numbers apart, so that they run at about the same time on one of
 // the 8 XCDs and find each other's reads in its L2.
-template <int DI, int EO, bool VEC>
-__global__ void __launch_bounds__(scan_threads(DI, EO)) scan_bwd_kernel(Args a) {
-  __shared__ float4 lds[(n_ivec(DK) + n_ovec(DK)) * kTok * 2 * DI];
+template <int IP, int IG, int EO, bool VEC>
+__global__ void __launch_bounds__(scan_threads(IP, IG, EO)) scan_bwd_kernel(Args a) {
+  __shared__ float4 lds[(n_ivec(DK) + n_ovec(DK)) * kTok * IP / 4];
   const int64_t x = blockIdx.x, q = x >> 3, bid = (q / 3) * 8 + (x & 7);
   if (bid >= a.B * a.H * a.nch) return;
   if (q % 3 == 0)
-    scan<DK, DI, EO, VEC>(a, lds, bid);
+    scan<DK, IP, IG, EO, VEC>(a, lds, bid);
   else if (q % 3 == 1)
-    scan<DV, DI, EO, VEC>(a, lds, bid);
+    scan<DV, IP, IG, EO, VEC>(a, lds, bid);
   else
-    scan<DQ, DI, EO, VEC>(a, lds, bid);
+    scan<DQ, IP, IG, EO, VEC>(a, lds, bid);
 }
 
 // ------------------------------------------------------------------- chunk contributions
@@ -671,36 +661,36 @@ template <bool BWD, bool VEC>
 void launch_scan_v(const Args& a, int cols, hipStream_t s) {
   const int64_t n = a.B * a.H * a.nch;
   const dim3 grid((unsigned)(BWD ? cdiv(n, 8) * 24 : n));
-#define TAGI_SCAN(DI, EO)                                                                                   \
-  do {                                                                                                      \
-    if constexpr (BWD)                                                                                      \
-      hipLaunchKernelGGL((scan_bwd_kernel<DI, EO, VEC>), grid, dim3(scan_threads(DI, EO)), 0, s, a);        \
-    else                                                                                                    \
-      hipLaunchKernelGGL((scan_fwd_kernel<DI, EO, VEC>), grid, dim3(scan_threads(DI, EO)), 0, s, a);        \
-    return;                                                                                                 \
+#define TAGI_SCAN(IP, IG, EO)                                                                                     \
+  do {                                                                                                            \
+    if constexpr (BWD)                                                                                            \
+      hipLaunchKernelGGL((scan_bwd_kernel<IP, IG, EO, VEC>), grid, dim3(scan_threads(IP, IG, EO)), 0, s, a);      \
+    else                                                                                                          \
+      hipLaunchKernelGGL((scan_fwd_kernel<IP, IG, EO, VEC>), grid, dim3(scan_threads(IP, IG, EO)), 0, s, a);      \
+    return;                                                                                                       \
   } while (0)
-#define TAGI_SCAN_COLS(DI)     \
+#define TAGI_SCAN_COLS(IP)     \
   do {                         \
     if (cols == 8)             \
-      TAGI_SCAN(DI, 1);        \
+      TAGI_SCAN(IP, 8, 1);     \
     else if (cols == 16)       \
-      TAGI_SCAN(DI, 2);        \
+      TAGI_SCAN(IP, 4, 1);     \
     else                       \
-      TAGI_SCAN(DI, 4);        \
+      TAGI_SCAN(IP, 4, 2);     \
   } while (0)
   if (a.D <= 16) {
     if (cols == 8)
-      TAGI_SCAN(2, 1);
+      TAGI_SCAN(16, 8, 1);
     else
-      TAGI_SCAN(2, 2);
+      TAGI_SCAN(16, 4, 1);
   } else if (a.D <= 32) {
-    TAGI_SCAN_COLS(4);
+    TAGI_SCAN_COLS(32);
   } else if (a.D <= 64) {
-    TAGI_SCAN_COLS(8);
+    TAGI_SCAN_COLS(64);
   } else if (a.D <= 96) {
-    TAGI_SCAN_COLS(12);
+    TAGI_SCAN_COLS(96);
   } else {
-    TAGI_SCAN_COLS(16);
+    TAGI_SCAN_COLS(128);
   }
 #undef TAGI_SCAN
 #undef TAGI_SCAN_COLS
