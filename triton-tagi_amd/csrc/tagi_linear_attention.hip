@@ -109,14 +109,14 @@ __device__ __forceinline__ float group_sums(const float* pm, const float* ps, in
   return keep + dpp<kXor1>(give);
 }
 
-// Four consecutive values of a token's head row (zeros past D).
+// Four consecutive values of a token's head row, of which `left` are there (zeros for the others).
 template <bool VEC>
-__device__ __forceinline__ float4 load4(const float* p, int c, int D) {
-  if constexpr (VEC) return *reinterpret_cast<const float4*>(p + c);
-  float4 r = make_float4(p[c], 0.f, 0.f, 0.f);
-  if (c + 1 < D) r.y = p[c + 1];
-  if (c + 2 < D) r.z = p[c + 2];
-  if (c + 3 < D) r.w = p[c + 3];
+__device__ __forceinline__ float4 load4(const float* p, int left) {
+  if constexpr (VEC) return *reinterpret_cast<const float4*>(p);
+  float4 r = make_float4(p[0], 0.f, 0.f, 0.f);
+  if (left > 1) r.y = p[1];
+  if (left > 2) r.z = p[2];
+  if (left > 3) r.w = p[3];
   return r;
 }
 
@@ -167,32 +167,33 @@ __device__ __forceinline__ void scan(const Args& a, float4* lds, int64_t bid) {
   const double pj = grouped && stager ? ipow(gd, st) : 1.0, ij = 1.0 / pj;  // g^j, g^-j
   const float4 z4 = make_float4(0.f, 0.f, 0.f, 0.f);
 
-  const int64_t qb = b * a.lq.sb + h * a.lq.sh, kb = b * a.lk.sb + h * a.lk.sh, vb = b * a.lv.sb + h * a.lv.sh,
-                db = b * a.ld.sb + h * a.ld.sh, ob = b * a.lo.sb + h * a.lo.sh;
-
+  const int64_t ob = b * a.lo.sb + h * a.lo.sh;
   auto tok = [&](int r) -> int64_t { return REV ? live - 1 - r : t0 + r; };  // r-th token of the scan
 
+  // this thread's place in each operand, moved on by a stage at a time
+  const auto place = [&](const tagi_heads& l) { return b * l.sb + h * l.sh + tok(st) * l.st + 4 * sc; };
+  const auto stride = [&](const tagi_heads& l) { return (REV ? -kTok : kTok) * l.st; };
+  int64_t qo = place(a.lq), ko = place(a.lk), vo = place(a.lv), dO = place(a.ld);
   float4 x0 = z4, x1 = z4, x2 = z4, x3 = z4, x4 = z4, x5 = z4;
   auto fetch = [&](int s0) {
-    const int r = s0 + st;
-    if (stager && inside && r < cnt) {
-      const int64_t t = tok(r);
-      const int c = 4 * sc;
+    if (stager && inside && s0 + st < cnt) {
+      const int left = D - 4 * sc;
       if constexpr (MODE == FWD) {
-        x0 = load4<VEC>(a.mq + qb + t * a.lq.st, c, D), x1 = load4<VEC>(a.Sq + qb + t * a.lq.st, c, D);
-        x2 = load4<VEC>(a.mk + kb + t * a.lk.st, c, D), x3 = load4<VEC>(a.Sk + kb + t * a.lk.st, c, D);
-        x4 = load4<VEC>(a.mv + vb + t * a.lv.st, c, D), x5 = load4<VEC>(a.Sv + vb + t * a.lv.st, c, D);
+        x0 = load4<VEC>(a.mq + qo, left), x1 = load4<VEC>(a.Sq + qo, left);
+        x2 = load4<VEC>(a.mk + ko, left), x3 = load4<VEC>(a.Sk + ko, left);
+        x4 = load4<VEC>(a.mv + vo, left), x5 = load4<VEC>(a.Sv + vo, left);
       } else if constexpr (MODE == DQ) {
-        x0 = load4<VEC>(a.mv + vb + t * a.lv.st, c, D), x1 = load4<VEC>(a.mk + kb + t * a.lk.st, c, D);
-        x2 = load4<VEC>(a.dm + db + t * a.ld.st, c, D), x3 = load4<VEC>(a.dS + db + t * a.ld.st, c, D);
+        x0 = load4<VEC>(a.mv + vo, left), x1 = load4<VEC>(a.mk + ko, left);
+        x2 = load4<VEC>(a.dm + dO, left), x3 = load4<VEC>(a.dS + dO, left);
       } else {
-        x0 = load4<VEC>(a.mq + qb + t * a.lq.st, c, D);
-        x1 = load4<VEC>(a.dm + db + t * a.ld.st, c, D), x2 = load4<VEC>(a.dS + db + t * a.ld.st, c, D);
-        x3 = MODE == DK ? load4<VEC>(a.mv + vb + t * a.lv.st, c, D) : load4<VEC>(a.mk + kb + t * a.lk.st, c, D);
+        x0 = load4<VEC>(a.mq + qo, left);
+        x1 = load4<VEC>(a.dm + dO, left), x2 = load4<VEC>(a.dS + dO, left);
+        x3 = MODE == DK ? load4<VEC>(a.mv + vo, left) : load4<VEC>(a.mk + ko, left);
       }
     } else {
       x0 = x1 = x2 = x3 = x4 = x5 = z4;  // nothing to add, and a dead token's output is zero
     }
+    qo += stride(a.lq), ko += stride(a.lk), vo += stride(a.lv), dO += stride(a.ld);
   };
   auto stage = [&]() {
     if (!stager) return;
