@@ -517,6 +517,108 @@ def test_linear_attention_backward_against_jacobians_and_differences(dev):
               "qkv"[i] + " variance")
 
 
+# ============================================================================ large offsets
+def test_offsets_past_32_bits(dev):
+    """Tables, rows and strides whose element offsets pass 2^32."""
+    from triton_tagi_amd.kernels import (add_rms_norm, add_rms_norm_backward, embedding_lookup, embedding_param_deltas,
+                                         embedding_update, linear_attention, linear_attention_backward)
+
+    if torch.cuda.get_device_properties(dev).total_memory < 150 << 30:
+        pytest.skip("needs 150 GB of GPU memory")
+    r = g(1)
+    V, D = (1 << 21) + 3, 2052  # 4.3e9 elements
+    mw, Sw = torch.full((V, D), 0.5, device=dev), torch.full((V, D), 0.25, device=dev)
+    ids = torch.tensor([V - 1, 5, V - 1, 1 << 21, V], device=dev)
+    mw[V - 1] = torch.arange(D, device=dev, dtype=torch.float32)
+    mz, Sz = embedding_lookup(ids, mw, Sw, scale=2.0)
+    assert torch.equal(mz[0], 2.0 * mw[V - 1]) and torch.equal(mz[3], 2.0 * mw[1 << 21]) and (mz[4] == 0).all()
+    dm = torch.randn(5, D, generator=r).to(dev)
+    dmw, dSw = embedding_param_deltas(ids, dm, dm, Sw, scale=2.0)
+    close(dmw[V - 1], 0.5 * (d64(dm[0]) + d64(dm[2])), 70 * U * 0.5 * (d64(dm[0]).abs() + d64(dm[2]).abs()), "last row")
+    assert torch.equal(dmw[5], 0.5 * dm[1]) and (dmw[V - 2] == 0).all() and (dSw[V - 2] == 0).all()
+    assert int((dmw != 0).any(1).sum()) == 3
+    del dmw, dSw
+    before = mw[V - 1].clone()
+    embedding_update(ids, dm, dm, mw, Sw, 3.0, scale=2.0)
+    assert not torch.equal(mw[V - 1], before) and (mw[V - 2] == 0.5).all()
+    del mw, Sw
+    rows, D = (1 << 20) + 1, 2056  # 2.2e9 elements
+    m, S = torch.full((rows, D), 0.5, device=dev), torch.full((rows, D), 0.25, device=dev)
+    m[rows - 1] = torch.randn(D, generator=r).to(dev)
+    w, Sg = torch.ones(D, device=dev), torch.full((D,), 0.01, device=dev)
+    mz, Sz, ms, _, inv = add_rms_norm(m, S, m, S, w, Sg, need_sum_var=False)
+    want = add_rms_norm(m[-3:], S[-3:], m[-3:], S[-3:], w, Sg)
+    assert torch.equal(mz[-3:], want[0]) and torch.equal(Sz[-3:], want[1]) and torch.equal(inv[-3:], want[4])
+    del Sz
+    out = add_rms_norm_backward(mz, S, ms, inv, w, Sg)
+    tail = add_rms_norm_backward(mz[-3:], S[-3:], ms[-3:], inv[-3:], w, Sg)
+    assert torch.equal(out[0][-3:], tail[0]) and torch.equal(out[1][-3:], tail[1])
+    del m, S, mz, ms, inv, out
+    T, H, D = 20, 2, 24
+    buf = torch.empty((T - 1) * (1 << 28) + 2 * H * D, device=dev)  # 5.1e9 elements
+    x = [t.to(dev) for t in lin_inputs(1, T, H, D, 3)]
+    far = buf.as_strided((1, T, H, D), (0, 1 << 28, D, 1))
+    farS = buf.as_strided((1, T, H, D), (0, 1 << 28, D, 1), H * D)
+    far.copy_(x[2]), farS.copy_(x[3])
+    dec = decays(H).to(dev)
+    for a, b in zip(linear_attention(x[0], x[1], far, farS, x[4], x[5], dec), linear_attention(*x, dec)):
+        assert torch.equal(a, b)
+    for a, b in zip(linear_attention_backward(x[0], far, x[4], far, farS, dec),
+                    linear_attention_backward(x[0], x[2], x[4], x[2], x[3], dec)):
+        assert torch.equal(a, b)
+
+
+def test_float_ids_at_the_end_of_the_exact_range(dev):
+    """2^24 is the last float every id below which is exact: it is a row of a table of 2^24 + 1."""
+    from triton_tagi_amd.kernels import embedding_lookup
+
+    V = (1 << 24) + 1
+    mw = torch.arange(V, device=dev, dtype=torch.float32)[:, None].contiguous()
+    ids = torch.tensor([float(1 << 24), float((1 << 24) - 1), float((1 << 24) + 2)], device=dev)
+    mz, _ = embedding_lookup(ids, mw, torch.ones_like(mw))
+    assert mz[:, 0].tolist() == [float(1 << 24), float((1 << 24) - 1), 0.0]
+
+
+def test_calls_from_two_threads(dev):
+    """Calls at the same time on streams of their own give each its own answers."""
+    import threading
+
+    from triton_tagi_amd.kernels import embedding_param_deltas, linear_attention
+
+    r = g(4)
+    jobs = []
+    for s in range(2):
+        x = [t.to(dev) for t in lin_inputs(1, 400, 2, 40, s)]
+        ids, dm = torch.randint(0, 60, (9000,), generator=r).to(dev), torch.randn(9000, 36, generator=r).to(dev)
+        Sw = torch.rand(60, 36, generator=r).to(dev)
+        dec = decays(2).to(dev)
+
+        def work(x=x, dec=dec, ids=ids, dm=dm, Sw=Sw):
+            return (*linear_attention(*x, dec), *embedding_param_deltas(ids, dm, dm, Sw))
+
+        jobs.append((work, [t.clone() for t in work()], [], []))
+    torch.cuda.synchronize()
+
+    def thread(work, want, got, failed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[:] = work()
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001  (reported by the test's own thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=thread, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for _, want, got, failed in jobs:
+        assert not failed
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 # =============================================================================== refusals
 def test_refusals(dev):
     from triton_tagi_amd import kernels as K

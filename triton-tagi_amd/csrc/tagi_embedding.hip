@@ -70,7 +70,7 @@ __device__ __forceinline__ uint32_t category(const void* ids, int type, int64_t 
   int64_t id = -1;
   if (type == TAGI_IDS_F32) {
     const float f = static_cast<const float*>(ids)[t];
-    if (f > -1.f && f < (float)V) id = (int64_t)f;
+    if (f > -1.f && f < 9.2e18f) id = (int64_t)f;
   } else if (type == TAGI_IDS_I32) {
     id = static_cast<const int32_t*>(ids)[t];
   } else {

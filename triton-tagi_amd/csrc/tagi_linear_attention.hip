@@ -22,15 +22,15 @@
 //
 // Decay without a multiplication per token: inside a group of 8 tokens the state is kept
 // divided by g^j (token j), the powers go into the token's vectors when they are staged, and
-// the state is multiplied by g^8 between groups. |g| < 0.05 would overflow the powers and
-// decays token by token.
+// the state is multiplied by g^8 between groups. Below |g| = 1/4 the squared powers (4^14 at
+// most above it) would eat into the floats' range: such heads decay token by token.
 #include "tagi_common.h"
 
 namespace tagi {
 namespace {
 
 constexpr int kTok = 8;          // tokens per stage, and per decay group
-constexpr float kGroupMin = 0.05f;
+constexpr float kGroupMin = 0.25f;
 constexpr int kMaxHeadDim = 128;
 
 enum Mode { FWD = 0, DQ = 1, DK = 2, DV = 3 };
