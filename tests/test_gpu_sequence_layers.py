@@ -354,6 +354,27 @@ def test_checkpoint_round_trip(dev, tmp_path):
     assert torch.equal(a.forward(x.float().to(dev))[0], b.forward(x.float().to(dev))[0])
 
 
+@pytest.mark.parametrize("serve", ["prompt", "decode"])
+def test_backward_after_serving_needs_a_forward(dev, serve):
+    """A prompt or token between forward and backward replaces what the layers keep: refused,
+    and a forward of its own puts the backward right again."""
+    net, other = network(), network()
+    x, _ = batch(2, 6, 3)
+    x = x.to(dev).float()
+    delta = torch.ones(2, 6, V, device=dev)
+    _, _, states = net.prompt(x)
+    net.forward(x)
+    net.prompt(x.flip(1)) if serve == "prompt" else net.decode(x[:, :1], states)
+    # by the head's Linear where the token counts differ, else by the first layer that mixes tokens
+    with pytest.raises((RuntimeError, ValueError), match="without a forward|weight deltas"):
+        net.backward(delta, -delta)
+    other.forward(x), net.forward(x)
+    other.backward(delta, -delta), net.backward(delta, -delta)
+    for a, b in zip(net.layers, other.layers):
+        for (_, _, m, S), (_, _, om, oS) in zip(a._update_items(), b._update_items()):
+            assert torch.equal(m, om) and torch.equal(S, oS)
+
+
 def test_layers_refuse(dev):
     from triton_tagi_amd import (Embedding, Linear, LinearAttention, MultiheadAttentionV2, PositionalEncoding, ReLU,
                                  ResidualRMSNorm, Sequential)
