@@ -568,6 +568,52 @@ def test_offsets_past_32_bits(dev):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows,D", [((1 << 22) + 5, 3), ((1 << 26) + 3, 5)])
+def test_norm_of_more_rows_than_one_grid_dimension(dev, rows, D):
+    """The last rows of a batch whose blocks pass 2^32 threads: the same bits as by themselves."""
+    from triton_tagi_amd.kernels import add_rms_norm, add_rms_norm_backward
+
+    r = g(4)
+    m, S = torch.full((rows, D), 0.5, device=dev), torch.full((rows, D), 0.25, device=dev)
+    m[-3:], S[-3:] = torch.randn(3, D, generator=r).to(dev), torch.rand(3, D, generator=r).to(dev)
+    w, Sg = torch.randn(D, generator=r).to(dev), torch.rand(D, generator=r).to(dev)
+    got, want = add_rms_norm(m, S, m, S, w, Sg), add_rms_norm(m[-3:], S[-3:], m[-3:], S[-3:], w, Sg)
+    for a, b in zip(got, want):
+        assert torch.equal(a[-3:], b)
+    assert torch.equal(got[0][1], got[0][rows - 4]) and torch.equal(got[1][1], got[1][rows - 4])
+    out = add_rms_norm_backward(m, S, got[2], got[4], w, Sg)
+    tail = add_rms_norm_backward(m[-3:], S[-3:], got[2][-3:], got[4][-3:], w, Sg)
+    assert torch.equal(out[0][-3:], tail[0]) and torch.equal(out[1][-3:], tail[1])
+
+
+def test_lookup_of_more_tokens_than_one_grid(dev):
+    """2^23 + 9 tokens of rows that take a block each."""
+    from triton_tagi_amd.kernels import embedding_lookup
+
+    n, V, D = (1 << 23) + 9, 7, 516
+    if torch.cuda.get_device_properties(dev).total_memory < 60 << 30:
+        pytest.skip("needs 60 GB of GPU memory")
+    r = g(5)
+    mw, Sw = torch.randn(V, D, generator=r).to(dev), torch.rand(V, D, generator=r).to(dev)
+    ids = (torch.arange(n, device=dev) % V).to(torch.int32)
+    mz, Sz = embedding_lookup(ids, mw, Sw)
+    for t in (0, (1 << 23) - 1, 1 << 23, n - 1):
+        assert torch.equal(mz[t], mw[t % V]) and torch.equal(Sz[t], Sw[t % V])
+
+
+def test_overlapping_tensors_are_not_updated(dev):
+    from triton_tagi_amd.kernels import embedding_update, linear_attention_step
+
+    buf = torch.zeros(40, device=dev)
+    d = torch.zeros(2, 4, device=dev)
+    with pytest.raises(ValueError, match="share memory"):
+        embedding_update(torch.zeros(2, device=dev), d, d, buf[:20].view(5, 4), buf[16:36].view(5, 4), 2.0)
+    q = torch.zeros(1, 1, 4, device=dev)
+    with pytest.raises(ValueError, match="share memory"):
+        linear_attention_step(*([q] * 6), (buf[:16].view(1, 1, 4, 4), buf[12:28].view(1, 1, 4, 4)),
+                              torch.ones(1, device=dev))
+
+
 def test_float_ids_at_the_end_of_the_exact_range(dev):
     """2^24 is the last float every id below which is exact: it is a row of a table of 2^24 + 1."""
     from triton_tagi_amd.kernels import embedding_lookup

@@ -58,6 +58,10 @@ def test_library_argument_errors():
     err("tagi_linear_attention_fwd", *fwd(1, 4, 1, 8, i=1), match="state")
     err("tagi_linear_attention_fwd", *fwd(1, 4, 1, 8, e=(1, None)), match="state")
     err("tagi_linear_attention_fwd", *fwd(1 << 20, 4, 1 << 20, 8), match="too large")
+    err("tagi_linear_attention_fwd", *fwd(1 << 21, 4, 2, 8), match="too large")
+    err("tagi_linear_attention_step", *([None] * 6), h, h, h, *([None] * 6), h, 1 << 21, 2, 8, 1.0, None,
+        match="too large")
+    err("tagi_embedding_sorted_bwd", 1, 0, 1, 1, 1, 1, 1, 1 << 30, 50, 8, -1, 1.0, 1, 1 << 50, None, match="too large")
     assert lib.tagi_linear_attention_fwd(*fwd(0, 4, 1, 8)) == 0
     err("tagi_linear_attention_bwd", *([None] * 3), h, h, h, None, None, h, None, None, 0, *([None] * 6), h, 1, 4, 1, 8,
         1.0, None, 0, None, match="null pointer")

@@ -89,18 +89,19 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const void* __res
                                                                int chunks, int tok_per_block, int64_t pad, float c,
                                                                float c2) {
   const int t0 = (int)threadIdx.x / chunks, q0 = (int)threadIdx.x - t0 * chunks;
-  const int64_t t = (int64_t)blockIdx.x * tok_per_block + t0;
-  if (t0 >= tok_per_block || t >= n) return;
-  const uint32_t cat = category(ids, type, t, V, pad);
-  for (int q = q0; q < chunks; q += 256) {
-    const int at = columns(q, D).at;  // columns of two threads get the same values from both
-    f4 m = {0.f, 0.f, 0.f, 0.f}, s = m;
-    if (cat < V) {
-      const int64_t src = (int64_t)cat * D + at;
-      m = ldc<WIDE>(mw + src, D) * c, s = ldc<WIDE>(Sw + src, D) * c2;
+  if (t0 >= tok_per_block) return;
+  for (int64_t t = (int64_t)blockIdx.x * tok_per_block + t0; t < n; t += (int64_t)gridDim.x * tok_per_block) {
+    const uint32_t cat = category(ids, type, t, V, pad);
+    for (int q = q0; q < chunks; q += 256) {
+      const int at = columns(q, D).at;  // columns of two threads get the same values from both
+      f4 m = {0.f, 0.f, 0.f, 0.f}, s = m;
+      if (cat < V) {
+        const int64_t src = (int64_t)cat * D + at;
+        m = ldc<WIDE>(mw + src, D) * c, s = ldc<WIDE>(Sw + src, D) * c2;
+      }
+      stc<WIDE>(mz + t * D + at, m, D, 0);
+      stc<WIDE>(Sz + t * D + at, s, D, 0);
     }
-    stc<WIDE>(mz + t * D + at, m, D, 0);
-    stc<WIDE>(Sz + t * D + at, s, D, 0);
   }
 }
 
@@ -506,14 +507,14 @@ __global__ void __launch_bounds__(64 * kJoinWaves) embedding_join_kernel(SumArgs
     ahead = first_key(p + 1 + more + lane);
   }
   double s[8] = {};
-      const int64_t q0 = (more + 1) * wave / kJoinWaves, q1 = (more + 1) * (wave + 1) / kJoinWaves;
+  const int64_t q0 = (more + 1) * wave / kJoinWaves, q1 = (more + 1) * (wave + 1) / kJoinWaves;
 #pragma unroll 8
-      for (int64_t q = q0; q < q1; ++q) {
-        const float* x = a.part + ((p + q) * 2 + (q == 0 ? 1 : 0)) * 2 * a.D + c.at;
-        const f4 y = ldc<WIDE>(x, a.D), v = ldc<WIDE>(x + a.D, a.D);
-        s[0] += y.x, s[1] += y.y, s[2] += y.z, s[3] += y.w;
-        s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
-      }
+  for (int64_t q = q0; q < q1; ++q) {
+    const float* x = a.part + ((p + q) * 2 + (q == 0 ? 1 : 0)) * 2 * a.D + c.at;
+    const f4 y = ldc<WIDE>(x, a.D), v = ldc<WIDE>(x + a.D, a.D);
+    s[0] += y.x, s[1] += y.y, s[2] += y.z, s[3] += y.w;
+    s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) red[wave][e][lane] = s[e];
   __syncthreads();
@@ -564,7 +565,7 @@ int sorted_impl(const char* what, const void* ids, int type, const float* dmz, c
                 void* ws, int64_t ws_bytes, hipStream_t s) {
   TAGI_REQUIRE(type >= TAGI_IDS_F32 && type <= TAGI_IDS_I64, "%s: unknown id type %d", what, type);
   TAGI_REQUIRE(n >= 0 && V > 0 && D > 0, "%s: bad sizes", what);
-  TAGI_REQUIRE(n < (1ll << 31) && V < (1ll << 31) && D < (1ll << 21) && V * D < (1ll << 40), "%s: too large", what);
+  TAGI_REQUIRE(n < (1ll << 30) && V < (1ll << 31) && D < (1ll << 21) && V * D < (1ll << 40), "%s: too large", what);
   TAGI_REQUIRE(Sw && (n == 0 || (ids && dmz && dSz)), "%s: null pointer", what);
   TAGI_REQUIRE((dmw == nullptr) == (dSw == nullptr) && (upd || dmw), "%s: null pointer", what);
   const Layout l = layout(n, V, D);
@@ -642,13 +643,14 @@ extern "C" int tagi_embedding_scaled_fwd(const void* ids, int id_type, const flo
   const char* what = "tagi_embedding_scaled_fwd";
   TAGI_REQUIRE(id_type >= TAGI_IDS_F32 && id_type <= TAGI_IDS_I64, "%s: unknown id type %d", what, id_type);
   TAGI_REQUIRE(n >= 0 && V > 0 && D > 0, "%s: bad sizes", what);
-  TAGI_REQUIRE(n < (1ll << 31) && V < (1ll << 31) && D < (1ll << 21), "%s: too large", what);
+  TAGI_REQUIRE(n < (1ll << 30) && V < (1ll << 31) && D < (1ll << 21), "%s: too large", what);
   if (n == 0) return TAGI_OK;
   TAGI_REQUIRE(ids && mw && Sw && mz && Sz, "%s: null pointer", what);
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps(FAM_EMBEDDING, s, 0.0, 4.0 * n + 16.0 * n * D);
   const int chunks = (int)cdiv(D, 4), tpb = chunks < 256 ? 256 / chunks : 1;
-  const dim3 grid((unsigned)cdiv(n, tpb));
+  const int64_t blocks = cdiv(n, tpb);  // a launch has fewer than 2^32 threads
+  const dim3 grid((unsigned)(blocks < (1 << 23) ? blocks : (1 << 23)));
   const float c = (float)scale, c2 = (float)(scale * scale);
   const auto kernel = D < 4 ? embedding_lookup_kernel<false> : embedding_lookup_kernel<true>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, ids, id_type, mw, Sw, mz, Sz, n, V, (int)D, chunks, tpb,

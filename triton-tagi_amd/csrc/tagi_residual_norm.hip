@@ -59,10 +59,17 @@ __device__ __forceinline__ float row_sum(float x, float* red) {
   return x;
 }
 
+// Blocks in two dimensions: a launch has fewer than 2^32 threads in one.
+inline dim3 row_grid(int64_t blocks) {
+  const int64_t x = blocks < (1 << 20) ? blocks : (1 << 20);
+  return dim3((unsigned)x, (unsigned)cdiv(blocks, x));
+}
+__device__ __forceinline__ int64_t row_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // One pass: TPR threads hold a row's sums in registers (NV chunks of four each) between the
 // statistic and the output, so every input is read and every output written once. HBM bound:
-// 16384 x 4096 moves 2.15 GB in 380 us (5.65 TB/s;
-// a copy kernel reaches 6.26 here), 65536 x 256 537 MB in 93 us.
+// 16384 x 4096 moves 2.15 GB in 380 us (5.65 TB/s; a copy kernel reaches 6.26 here), 65536 x 256
+// 537 MB in 93 us.
 template <int TPR, int NV, bool NT>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(
     const float* __restrict__ ma, const float* __restrict__ Sa, const float* __restrict__ mr,
@@ -72,7 +79,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(
   __shared__ float red[TPR / 64];
   constexpr int RPB = TPR < 256 ? 256 / TPR : 1;  // rows of a block
   const int t = (int)threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * RPB + (int)threadIdx.x / TPR, o = row * D;
+  const int64_t row = row_block() * RPB + (int)threadIdx.x / TPR, o = row * D;
   if (row >= rows) return;  // TPR > 64 has one row a block: no thread of it leaves
   f4 m[NV], v[NV];
   float acc = 0.f;
@@ -103,28 +110,48 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) add_rms_norm_kernel(
   }
 }
 
-// Rows too long for registers, or shorter than four: the inputs are read twice.
-__global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(
-    const float* __restrict__ ma, const float* __restrict__ Sa, const float* __restrict__ mr,
-    const float* __restrict__ Sr, const float* __restrict__ mw, const float* __restrict__ Sw, float* __restrict__ mz,
-    float* __restrict__ Sz, float* __restrict__ ms, float* __restrict__ Ss, float* __restrict__ inv_rms, int D,
-    float eps) {
+struct FwdArgs {
+  const float *ma, *Sa, *mr, *Sr, *mw, *Sw;
+  float *mz, *Sz, *ms, *Ss, *inv;
+  int64_t rows;
+  int D;
+  float eps;
+};
+__device__ __forceinline__ void write_value(const FwdArgs& a, int64_t at, int c, float inv) {
+  const float m = a.ma[at] + a.mr[at], v = a.Sa[at] + a.Sr[at], g = a.mw[c], sg = a.Sw[c];
+  a.ms[at] = m;
+  if (a.Ss) a.Ss[at] = v;
+  a.mz[at] = m * inv * g;
+  a.Sz[at] = inv * inv * (v * (g * g + sg) + sg * (m * m));
+}
+
+// Rows too long for registers: the inputs are read twice.
+__global__ void __launch_bounds__(1024) add_rms_norm_long_kernel(FwdArgs a) {
   __shared__ float red[16];
-  const int64_t row = blockIdx.x, o = row * D;
+  const int64_t row = row_block(), o = row * a.D;
+  if (row >= a.rows) return;
   float acc = 0.f;
-  for (int c = threadIdx.x; c < D; c += 1024) {
-    const float m = ma[o + c] + mr[o + c], v = Sa[o + c] + Sr[o + c];
+  for (int c = threadIdx.x; c < a.D; c += 1024) {
+    const float m = a.ma[o + c] + a.mr[o + c], v = a.Sa[o + c] + a.Sr[o + c];
     acc += m * m + v;
   }
-  const float inv = 1.f / sqrtf(row_sum<1024>(acc, red) / (float)D + eps);
-  if (threadIdx.x == 0) inv_rms[row] = inv;
-  for (int c = threadIdx.x; c < D; c += 1024) {
-    const float m = ma[o + c] + mr[o + c], v = Sa[o + c] + Sr[o + c], g = mw[c], sg = Sw[c];
-    ms[o + c] = m;
-    if (Ss) Ss[o + c] = v;
-    mz[o + c] = m * inv * g;
-    Sz[o + c] = inv * inv * (v * (g * g + sg) + sg * (m * m));
+  const float inv = 1.f / sqrtf(row_sum<1024>(acc, red) / (float)a.D + a.eps);
+  if (threadIdx.x == 0) a.inv[row] = inv;
+  for (int c = threadIdx.x; c < a.D; c += 1024) write_value(a, o + c, c, inv);
+}
+
+// Rows shorter than four, a thread for each.
+__global__ void __launch_bounds__(256) add_rms_norm_short_kernel(FwdArgs a) {
+  const int64_t row = row_block() * 256 + threadIdx.x, o = row * a.D;
+  if (row >= a.rows) return;
+  float acc = 0.f;
+  for (int c = 0; c < a.D; ++c) {
+    const float m = a.ma[o + c] + a.mr[o + c], v = a.Sa[o + c] + a.Sr[o + c];
+    acc += m * m + v;
   }
+  const float inv = 1.f / sqrtf(acc / (float)a.D + a.eps);
+  a.inv[row] = inv;
+  for (int c = 0; c < a.D; ++c) write_value(a, o + c, c, inv);
 }
 
 // Blocks own a range of rows and 4 CT columns (CT threads across, 256 / CT rows at a time);
@@ -238,16 +265,9 @@ BwdPlan bwd_plan(int64_t rows, int64_t D) {
 // (16384 x 4096: forward 400 -> 380 us, backward 364 -> 342; 16384 x 1024: 120 -> 109, 105 -> 95).
 constexpr double kCacheBytes = 256e6;
 
-struct FwdArgs {
-  const float *ma, *Sa, *mr, *Sr, *mw, *Sw;
-  float *mz, *Sz, *ms, *Ss, *inv;
-  int64_t rows;
-  int D;
-  float eps;
-};
 template <int TPR, int NV>
 void launch_fwd(const FwdArgs& a, bool nt, hipStream_t s) {
-  const dim3 grid((unsigned)cdiv(a.rows, TPR < 256 ? 256 / TPR : 1)), block(TPR < 256 ? 256 : TPR);
+  const dim3 grid = row_grid(cdiv(a.rows, TPR < 256 ? 256 / TPR : 1)), block(TPR < 256 ? 256 : TPR);
   if (nt)
     hipLaunchKernelGGL((add_rms_norm_kernel<TPR, NV, true>), grid, block, 0, s, a.ma, a.Sa, a.mr, a.Sr, a.mw, a.Sw,
                        a.mz, a.Sz, a.ms, a.Ss, a.inv, a.rows, a.D, a.eps);
@@ -289,9 +309,10 @@ extern "C" int tagi_add_rmsnorm_fwd(const float* ma, const float* Sa, const floa
   // threads of a row: a wave for short rows, or for longer ones when there are rows enough to
   // fill the GPU; more where few rows would wait on each thread's loads
   const int64_t chunks = cdiv(D, 4);
-  if (chunks > 8 * 1024 || D < 4)
-    hipLaunchKernelGGL(add_rms_norm_long_kernel, dim3((unsigned)rows), dim3(1024), 0, s, ma, Sa, mr, Sr, mw, Sw, mz, Sz,
-                       ms, Ss, inv_rms, (int)D, eps);
+  if (D < 4)
+    hipLaunchKernelGGL(add_rms_norm_short_kernel, row_grid(cdiv(rows, 256)), dim3(256), 0, s, a);
+  else if (chunks > 8 * 1024)
+    hipLaunchKernelGGL(add_rms_norm_long_kernel, row_grid(rows), dim3(1024), 0, s, a);
   else if (chunks <= 64 || (chunks <= 4 * 64 && rows >= 4096))
     launch_fwd_nv<64>(a, nt, s);
   else if (chunks <= 256 || (chunks <= 8 * 256 && rows >= 512))

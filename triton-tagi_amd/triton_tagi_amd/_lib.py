@@ -317,6 +317,12 @@ def check_in_place(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    return (a.data_ptr() < b.data_ptr() + b.numel() * b.element_size()
+            and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size())
+
+
 def dense(t: torch.Tensor) -> torch.Tensor:
     """t itself when its storage is dense in its own dim order (row-major or channels-last)."""
     if t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)):

@@ -103,7 +103,7 @@ def embedding_update(ids: Tensor, delta_mz: Tensor, delta_Sz: Tensor, mw: Tensor
     _check_table(mw, "mw")
     _lib.check_with(Sw, "Sw", mw, mw.shape)
     _lib.check_in_place(mw, "mw"), _lib.check_in_place(Sw, "Sw")
-    if mw.data_ptr() == Sw.data_ptr():
+    if _lib.overlap(mw, Sw):
         raise ValueError("mw and Sw share memory")
     cap = float(cap_factor)
     if not 0.0 < cap <= 3.4e38:

@@ -14,7 +14,7 @@ operand at its mean, as the attention layer's backward does.
 
 Operands are (B, T, H, D) (a step's (B, H, D)) with any strides but the last dim's, which
 is 1: heads are read in place from a side-by-side projection buffer. A mean and its variance
-share strides; other layouts are copied. D is at most 128. ``decay`` (H,) is meant to lie
+share strides; other layouts are copied. D is at most 128, B H below 2^22. ``decay`` (H,) is meant to lie
 in [0, 1]; it is not checked, as that would wait for the GPU.
 """
 
@@ -169,7 +169,7 @@ def linear_attention_step(mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, mv: Te
     decay, scale = _decay(decay, mq, H), _scale(scale)
     M, P = _state(state, mq, (B, H, D, D))
     _lib.check_in_place(M, "state means"), _lib.check_in_place(P, "state variances")
-    if B and M.data_ptr() == P.data_ptr():
+    if _lib.overlap(M, P):
         raise ValueError("state: means and variances share memory")
     if active is not None:
         if not isinstance(active, torch.Tensor) or active.dtype not in (torch.bool, torch.uint8):
