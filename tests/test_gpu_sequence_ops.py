@@ -193,6 +193,12 @@ def test_add_rms_norm(dev, rows, D, stream):
     close(out[3], gS * gS * (dS * x * x).sum(0), 2 * kc * gS * gS * (dS * x * x).sum(0).abs(), "delta_Sw")
 
 
+@pytest.mark.parametrize("rows,D", [(3, 32768), (3, 32769), (2, 40003)])
+def test_add_rms_norm_of_the_longest_rows(dev, rows, D):
+    """The longest rows that stay in registers, and longer ones."""
+    test_add_rms_norm(dev, rows, D, True)
+
+
 def test_add_rms_norm_is_add_then_norm(dev):
     """The container layers' path equals Add followed by RMSNorm within both forms' roundings."""
     from triton_tagi_amd import Add, RMSNorm
