@@ -115,6 +115,12 @@ def test_embedding_lookup_deltas_update(dev, n, V, D, kind, dtype, pad, c):
         assert torch.equal(a, b) and torch.equal(a, x)
 
 
+@pytest.mark.parametrize("n,V", [((1 << 20) + 77, 1), (1 << 20, 7), (32769, 1), (32768, 500), (32700, 511), (20000, 70000)])
+def test_embedding_tables_and_batches_of_unlike_size(dev, n, V):
+    """Many tokens of few categories, and batches at the borders of the sort's forms."""
+    test_embedding_lookup_deltas_update(dev, n, V, 2, "uniform", torch.int32, -1, 1.5)
+
+
 def test_embedding_ids_outside_the_table(dev):
     from triton_tagi_amd.kernels import embedding_lookup, embedding_param_deltas
 

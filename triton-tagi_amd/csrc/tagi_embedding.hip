@@ -107,13 +107,17 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const void* __res
 
 // -------------------------------------------------------------------------------- sort
 // Least-significant-digit radix sort of (category, token index). Per digit: every block
-// counts its tile's digits; a wave per digit turns the blocks' counts into places; every
-// block writes its tile's pairs to them in order. Latency bound: 65536 tokens of 131071
-// categories take 2 digits of 9 bits, 18 us a digit. Up to kSmall tokens one block
-// does all of it in LDS: a launch instead of three per digit (4096 tokens x 64 over 50000 rows:
-// 25 us a call against 40, 16 tokens 16 against 30; 16384 tokens in one block took 24 us
-// against 15 for one digit).
+// counts its tile's digits; a wave per digit turns the blocks' counts into places (few blocks
+// add them up themselves); every block writes its tile's pairs to them in order. Latency bound:
+// 65536 tokens of 131071 categories take 2 digits of 9 bits, 18 us a digit. Up to kSmall tokens
+// one block does all of it in LDS: a launch instead of three per digit (4096 tokens x 64 over
+// 50000 rows: 25 us a call against 40, 16 tokens 16 against 30; 16384 tokens in one block took
+// 24 us against 15 for one digit).
 constexpr int kSmall = 4096, kSmallBits = 8;
+// Up to this many blocks and counts in all, every block adds the counts up itself, a launch less
+// per digit (us a call: 16 blocks of 7 bits 25 -> 23, 20 of 8 bits 69 -> 65; 32 of 10 bits
+// 43 -> 45, 64 of 9 67 -> 71).
+constexpr int kFewBlocks = 32, kFewCounts = 16384;
 
 struct SortPlan {
   int64_t nblk;
@@ -141,7 +145,7 @@ struct SortArgs {
   const uint32_t* vin;
   uint32_t* kout;
   uint32_t* vout;
-  uint32_t* hist;   // [digit][block]: counts, then places within the digit
+  uint32_t* hist;   // [digit][block]: counts, then places within the digit; few blocks: [block][digit], counts
   uint32_t* total;  // [digit]
   int64_t n, V, pad;
   int nblk, shift, bits;
@@ -182,7 +186,7 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, bool on, int bits) {
   return same;
 }
 
-template <int IT>
+template <int IT, bool FEW>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
   if (fills(a)) return;
   __shared__ uint32_t cnt[1 << kMaxRadixBits];
@@ -196,7 +200,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
     if (i < a.n) atomicAdd(&cnt[(sort_key(a, i) >> a.shift) & (radix - 1)], 1u);  // whole numbers: any order
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < radix; d += kSortThreads) a.hist[(int64_t)d * a.nblk + blockIdx.x] = cnt[d];
+  for (int d = threadIdx.x; d < radix; d += kSortThreads)
+    a.hist[FEW ? (int64_t)blockIdx.x * radix + d : (int64_t)d * a.nblk + blockIdx.x] = cnt[d];
 }
 
 // One wave per digit: the blocks' counts become places within the digit.
@@ -223,7 +228,7 @@ __global__ void __launch_bounds__(256) sort_places_kernel(SortArgs a) {
 // Each wave owns a contiguous strip of the tile, in order: a pair's place is its digit's
 // first place, the block's within the digit, the earlier strips' counts, and the digits met
 // before it in this strip (a counter per wave and digit, and a ballot match within 64 pairs).
-template <int IT>
+template <int IT, bool FEW>
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) {
   if (fills(a)) return;
   constexpr int W = kSortThreads / 64;
@@ -245,12 +250,26 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
     if (i0 + 64 * k < a.n) atomicAdd(&cnt[wave][(key[k] >> a.shift) & (radix - 1)], 1u);
   // digits' first places: a running sum over the digits, 256 at a time
   uint32_t first[(1 << kMaxRadixBits) / kSortThreads];
+  uint32_t inside[(1 << kMaxRadixBits) / kSortThreads];  // the block's first place within the digit
   uint32_t run = 0;
 #pragma unroll
   for (int r = 0; r < (1 << kMaxRadixBits) / kSortThreads; ++r) {
     if (r * kSortThreads >= radix) break;
     const int d = r * kSortThreads + (int)threadIdx.x;
-    const uint32_t c = d < radix ? a.total[d] : 0u;
+    uint32_t c = 0, in = 0;
+    if (d < radix) {
+      if constexpr (FEW) {
+#pragma unroll 8
+        for (int b = 0; b < a.nblk; ++b) {
+          const uint32_t h = a.hist[(int64_t)b * radix + d];
+          c += h;
+          in += b < (int)blockIdx.x ? h : 0u;
+        }
+      } else {
+        c = a.total[d], in = a.hist[(int64_t)d * a.nblk + blockIdx.x];
+      }
+    }
+    inside[r] = in;
     uint32_t x = c;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -273,7 +292,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
   for (int r = 0; r < (1 << kMaxRadixBits) / kSortThreads; ++r) {
     const int d = r * kSortThreads + (int)threadIdx.x;
     if (d >= radix) continue;
-    uint32_t at = first[r] + a.hist[(int64_t)d * a.nblk + blockIdx.x];
+    uint32_t at = first[r] + inside[r];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const uint32_t c = cnt[w][d];
@@ -293,7 +312,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(SortArgs a) 
       const uint32_t at = mine[d] + rank;
       a.kout[at] = key[k];
       a.vout[at] = val[k];
-      if (rank == 0) mine[d] = at + __popcll(same);  // after this round's reads: one wave, in order
+      if (rank == 0) mine[d] = at + __popcll(same);  // after these reads: one wave, in order
     }
   }
 }
@@ -582,7 +601,8 @@ int sorted_impl(const char* what, const void* ids, int type, const float* dmz, c
   a.total = reinterpret_cast<uint32_t*>(base + l.total);
   a.z0 = dmw, a.z1 = dSw;
   const bool small = n <= kSmall;
-  const int launches = small ? 1 : 3 * p.passes;
+  const bool few = p.nblk <= kFewBlocks && p.nblk << p.bits <= kFewCounts;
+  const int launches = small ? 1 : (few ? 2 : 3) * p.passes;
   const int64_t share = dmw ? cdiv(cdiv(V * D, launches), 4) * 4 : 0;
   int done = 0;
   // the next launch's grid: `work` blocks, and those for its share of the zeros
@@ -607,17 +627,23 @@ int sorted_impl(const char* what, const void* ids, int type, const float* dmz, c
       a.shift = k * p.bits;
       const dim3 block(kSortThreads);
       dim3 g = grid(p.nblk, kSortThreads);
-      if (p.items == 4)
-        hipLaunchKernelGGL(sort_count_kernel<4>, g, block, 0, s, a);
+      if (few)
+        hipLaunchKernelGGL((sort_count_kernel<4, true>), g, block, 0, s, a);
+      else if (p.items == 4)
+        hipLaunchKernelGGL((sort_count_kernel<4, false>), g, block, 0, s, a);
       else
-        hipLaunchKernelGGL(sort_count_kernel<16>, g, block, 0, s, a);
-      g = grid(cdiv(1 << p.bits, 4), kSortThreads);
-      hipLaunchKernelGGL(sort_places_kernel, g, block, 0, s, a);
+        hipLaunchKernelGGL((sort_count_kernel<16, false>), g, block, 0, s, a);
+      if (!few) {
+        g = grid(cdiv(1 << p.bits, 4), kSortThreads);
+        hipLaunchKernelGGL(sort_places_kernel, g, block, 0, s, a);
+      }
       g = grid(p.nblk, kSortThreads);
-      if (p.items == 4)
-        hipLaunchKernelGGL(sort_scatter_kernel<4>, g, block, 0, s, a);
+      if (few)
+        hipLaunchKernelGGL((sort_scatter_kernel<4, true>), g, block, 0, s, a);
+      else if (p.items == 4)
+        hipLaunchKernelGGL((sort_scatter_kernel<4, false>), g, block, 0, s, a);
       else
-        hipLaunchKernelGGL(sort_scatter_kernel<16>, g, block, 0, s, a);
+        hipLaunchKernelGGL((sort_scatter_kernel<16, false>), g, block, 0, s, a);
     }
   }
   SumArgs q{};
