@@ -375,6 +375,21 @@ def test_backward_after_serving_needs_a_forward(dev, serve):
             assert torch.equal(m, om) and torch.equal(S, oS)
 
 
+def test_prompts_without_tokens(dev):
+    """No sequence or no token is refused; sequences whose lengths are all zero leave zero states."""
+    net = network()
+    x = batch(3, 5, 1)[0].to(dev)
+    for empty in (x[:0], x[:, :0]):
+        with pytest.raises(ValueError, match="at least one"):
+            net.prompt(empty)
+    _, _, states = net.prompt(x, lengths=torch.zeros(3, dtype=torch.int64, device=dev))
+    M, P = states[1][0]
+    assert M.shape == (3, H, E // H, E // H) and not M.any() and not P.any()
+    m, S = net.decode(x[:, :1], states)
+    want, wS, _ = net.prompt(x[:, :1])
+    near(m, want, "first token"), near(S, wS, "its variances")
+
+
 def test_layers_refuse(dev):
     from triton_tagi_amd import (Embedding, Linear, LinearAttention, MultiheadAttentionV2, PositionalEncoding, ReLU,
                                  ResidualRMSNorm, Sequential)

@@ -80,6 +80,8 @@ class Sequential:
 
     def _serving_input(self, x: Tensor) -> tuple[Tensor, Tensor | None]:
         check_layers(self.layers)
+        if x.numel() == 0:
+            raise ValueError(f"expected at least one sequence of one token, got {tuple(x.shape)}")
         first = self.layers[0] if self.layers else None
         return x, (None if isinstance(first, (Linear, Embedding)) else torch.zeros_like(x))
 
