@@ -88,14 +88,14 @@ class LinearAttention(QkvProjections):
         for p in self._projections():
             p.ma_in, p._input_shape = cache["ma_in"], ma.shape
         mo, So = linear_attention(*ops, self._decay_on(ma.device), scale=self._scale, lengths=lengths)
-        self._cache = dict(cache, ops=ops, lengths=lengths)
+        self._cache = dict(cache, qkv=ops[::2], lengths=lengths)  # the means
         return mo.view(ma.shape), So.view(ma.shape)
 
     def backward(self, delta_mz: Tensor, delta_Sz: Tensor) -> tuple[Tensor, Tensor]:
         c = self._cache
         if c is None:
             raise RuntimeError("LinearAttention: backward without a forward")
-        q, k, v = c["ops"][0], c["ops"][2], c["ops"][4]
+        q, k, v = c["qkv"]
         B, S, E = *q.shape[:2], self.embed_dim
         dm, dS = linear_attention_backward_packed(q, k, v, delta_mz.reshape(q.shape), delta_Sz.reshape(q.shape),
                                                   self._decay_on(q.device), self._scale, c["lengths"])
