@@ -16,8 +16,8 @@
 // bound: 7 operations per state element and token forward. Every pass is one scan,
 //   X_t = g X_{t-1} + u_t w_t^T (one or two such states),  y_t[o] = sum_i r_t[i] f(X_t[i][o]),
 // whose columns o are independent: a wavefront keeps 32 columns of the state in registers
-// (4 lanes share a column and hold every fourth row of it; 8 in the backward scans of long
-// heads, 16 or 8 columns where waves are few), reads the token's vectors from LDS and adds the
+// (4 or 8 lanes share a column, each with as many of its rows; 16 or 8 columns where waves are
+// few), reads the token's vectors from LDS and adds the
 // partial sums over i in exchanges that halve the values each lane keeps. A fp32 MFMA has the
 // rate of the vector ALUs and does not run beside them: the rank-one update as 4 x 4 x 1 MFMAs
 // took 496 us where fmas take 474 (2 x 4096 tokens, 16 heads of 64, forward and backward).
@@ -660,15 +660,15 @@ inline bool al4(const tagi_heads& s) { return s.sb % 4 == 0 && s.st % 4 == 0 && 
 // columns) read the token's vectors more often; chunks cost a pass that sums each one's
 // contribution, the state traffic, and two launches. Measured (us, forward / backward; "n x c":
 // n chunks, c columns):
-//   64 x 256 tokens, 8 heads of 32:  1 x 8 64 / 116, 1 x 16 82 / 91, 1 x 32 101 / 93, 4 x 32 75 / 105
-//   32 x 128 tokens, 8 heads of 64:  1 x 8 48 / 79, 1 x 16 61 / 71, 2 x 16 81 / 113, 4 x 32 73 / 122
-//   2 x 4096 tokens, 16 heads of 64: 32 x 32 179 / 303, 16 x 32 280 / 285, 16 x 16 208 / 334
-//   1 x 512 tokens, 8 heads of 64:   16 x 8 34 / 37, 16 x 16 39 / 39, 16 x 32 48 / 47
-//   1 x 2048 tokens, 4 heads of 128: 64 x 16 79 / 130, 32 x 32 126 / 117, 64 x 32 94 / 137
-//   1 x 64 tokens, 8 heads of 32:    1 x 8 18 / 26, 1 x 16 21 / 27, 2 x 8 23 / 34
-//   3 x 339 tokens, 1 head of 128:   11 x 16 61 / 49, 6 x 16 - / 72
-//   32 x 2048 tokens, 8 heads of 64: 1 x 8 738 / 1216, 1 x 16 950 / 1079, 4 x 32 615 / 1056
-//   16 x 512 tokens, 8 heads of 128: 1 x 8 479 / -, 1 x 16 492 / 566, 4 x 32 326 / 556
+//   64 x 256 tokens, 8 heads of 32:  1 x 8 64 / 114, 1 x 16 81 / 91, 1 x 32 101 / 93, 4 x 32 75 / 105
+//   32 x 128 tokens, 8 heads of 64:  1 x 8 48 / 78, 1 x 16 56 / 65, 2 x 16 77 / 103, 4 x 32 73 / 122
+//   2 x 4096 tokens, 16 heads of 64: 32 x 32 181 / 301, 16 x 32 276 / 280, 16 x 16 191 / 303
+//   1 x 512 tokens, 8 heads of 64:   16 x 8 34 / 37, 16 x 16 37 / 39, 16 x 32 48 / 47
+//   1 x 2048 tokens, 4 heads of 128: 64 x 16 75 / 131, 32 x 32 126 / 115, 64 x 32 94 / 138
+//   1 x 64 tokens, 8 heads of 32:    1 x 8 18 / 24, 1 x 16 21 / 24, 2 x 8 22 / 31
+//   3 x 339 tokens, 1 head of 128:   11 x 16 56 / 49, 6 x 16 85 / 67
+//   32 x 2048 tokens, 8 heads of 64: 1 x 8 729 / 1218, 1 x 16 851 / 1012, 4 x 32 624 / 1055
+//   16 x 512 tokens, 8 heads of 128: 1 x 8 479 / -, 1 x 16 413 / 564, 4 x 32 326 / 554
 // So: no chunks where the widest waves that do reach 2048 (backward, whose three scans run side
 // by side: 1024); forward they may have 8 columns for few tokens, and long heads' have 16 at
 // least, since narrow waves spend their time reading LDS. No chunks below 128 tokens; else as
@@ -714,17 +714,20 @@ void launch_scan_v(const Args& a, int cols, hipStream_t s) {
       hipLaunchKernelGGL((scan_fwd_kernel<IP, IG, EO, VEC>), grid, dim3(scan_threads(IP, IG, EO)), 0, s, a);      \
     return;                                                                                                       \
   } while (0)
-  // lanes to a column: 4 leave the shorter sum, 8 read half as much from LDS, which bounds the
-  // backward scans of long heads (16 x 512 tokens, 8 heads of 128: 645 against 570 us)
-#define TAGI_SCAN_COLS(IP)                \
-  do {                                    \
-    constexpr int G = BWD && IP > 64 ? 8 : 4; \
-    if constexpr (IP <= 64)               \
-      if (cols == 8) TAGI_SCAN(IP, 8, 1); \
-    if (cols == 16)                       \
-      TAGI_SCAN(IP, G, G / 4);            \
-    else                                  \
-      TAGI_SCAN(IP, G, G / 2);            \
+  // Lanes to a column: 4 leave the shorter sum, 8 read half as much from LDS, which bounds 16
+  // columns of more than 32 features (backward 32 x 512 tokens, 8 heads of 64: 265 against 245
+  // us, forward 3 x 339, one head of 128: 69 and 63; 64 x 256, 8 heads of 32: 90 and 93) and the
+  // backward of 32 columns of more than 64 (16 x 512, 8 heads of 128: 645 and 570).
+#define TAGI_SCAN_COLS(IP)                        \
+  do {                                            \
+    constexpr int G16 = IP > 32 ? 8 : 4;          \
+    constexpr int G32 = BWD && IP > 64 ? 8 : 4;   \
+    if constexpr (IP <= 64)                       \
+      if (cols == 8) TAGI_SCAN(IP, 8, 1);         \
+    if (cols == 16)                               \
+      TAGI_SCAN(IP, G16, G16 / 4);                \
+    else                                          \
+      TAGI_SCAN(IP, G32, G32 / 2);                \
   } while (0)
   if (a.D <= 16) {
     if (cols == 8)
