@@ -17,10 +17,10 @@
 //   X_t = g X_{t-1} + u_t w_t^T (one or two such states),  y_t[o] = sum_i r_t[i] f(X_t[i][o]),
 // whose columns o are independent: a wavefront keeps 32 columns of the state in registers
 // (4 or 8 lanes share a column, each with as many of its rows; 16 or 8 columns where waves are
-// few), reads the token's vectors from LDS and adds the
-// partial sums over i in exchanges that halve the values each lane keeps. A fp32 MFMA has the
-// rate of the vector ALUs and does not run beside them: the rank-one update as 4 x 4 x 1 MFMAs
-// took 496 us where fmas take 474 (2 x 4096 tokens, 16 heads of 64, forward and backward).
+// few), reads the token's vectors from LDS and adds the partial sums over i in exchanges that
+// halve the values each lane keeps: 2 x 4096 tokens, 16 heads of 64, forward and backward 464 us.
+// A fp32 MFMA has the rate of the vector ALUs and does not run beside them: with the rank-one
+// update as 4 x 4 x 1 MFMAs the same took 496 us where fmas took 474.
 //
 // Decay without a multiplication per token: inside a group of 8 tokens the state is kept
 // divided by g^j (token j), the powers go into the token's vectors when they are staged, and
