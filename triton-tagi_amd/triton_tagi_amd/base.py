@@ -57,5 +57,10 @@ class LearnableLayer(Layer):
     def _update_groups(self):
         """The contiguous (m, S, delta_m, delta_S) groups the update applies: those of
         ``_update_items`` unless the layer keeps its parameters in larger buffers (the
-        attention layer's projections live side by side)."""
+        attention layer's projections live side by side). Asking changes nothing."""
         return self._update_items()
+
+    def _update_parts(self):
+        """The layers a container's update consists of, each updated as if it stood beside
+        the container; None for a layer that is updated as one."""
+        return None

@@ -13,6 +13,7 @@ from torch import Tensor
 
 from ..base import LearnableLayer
 from ..kernels.residual_norm import add_rms_norm, add_rms_norm_backward
+from ..update.parameters import update_layers
 from .resblock import delta_merge
 from .rms_norm import RMSNorm
 
@@ -96,26 +97,22 @@ class ResidualRMSNorm(LearnableLayer):
             items.extend(got)
         return items
 
+    def _update_parts(self):
+        return self._learnable_layers()
+
     def _update_groups(self):
-        """Groups of every layer inside, but those whose backward applied its update."""
-        layers = self._learnable_layers()
-        got = [None if layer._updated_in_backward else layer._update_groups() for layer in layers]
-        if any(g is None and not layer._updated_in_backward for g, layer in zip(got, layers)):
-            return None  # a layer with an update of its own: all through update()
+        """Groups of every layer inside; None (all through ``update``) where a layer has none or
+        its backward applied its update."""
         items = []
-        for g, layer in zip(got, layers):
-            if layer._updated_in_backward:
-                layer._updated_in_backward = False
-            else:
-                items.extend(g)
+        for layer in self._learnable_layers():
+            got = None if layer._updated_in_backward else layer._update_groups()
+            if got is None:
+                return None
+            items.extend(got)
         return items
 
     def update(self, cap_factor: float) -> None:
-        for layer in self._learnable_layers():
-            if layer._updated_in_backward:
-                layer._updated_in_backward = False
-            else:
-                layer.update(cap_factor)
+        update_layers(self._learnable_layers(), cap_factor)
 
     @property
     def num_parameters(self) -> int:

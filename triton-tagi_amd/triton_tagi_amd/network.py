@@ -24,7 +24,7 @@ from .layers.multihead_attention import MultiheadAttentionV2
 from .layers.serving import check_layers, run_prompt, run_step
 from .update.observation import compute_innovation, hrc_innovation
 from .update.in_backward import update_in_backward
-from .update.parameters import get_cap_factor, update_parameters_multi
+from .update.parameters import get_cap_factor, update_layers
 
 
 # Per-layer state that lives on the network's device: parameters, BatchNorm running
@@ -106,23 +106,7 @@ class Sequential:
 
     def update(self, cap_factor: float) -> None:
         """Capped update of every learnable layer (one launch for all exposed groups)."""
-        items = []
-        for layer in self.layers:
-            if not isinstance(layer, LearnableLayer):
-                continue
-            if layer._updated_in_backward:  # the backward pass applied it (update_in_backward)
-                layer._updated_in_backward = False
-                continue
-            got = layer._update_groups()
-            if got is None:
-                if items:
-                    update_parameters_multi(items, cap_factor)
-                    items = []
-                layer.update(cap_factor)
-            else:
-                items.extend(got)
-        if items:
-            update_parameters_multi(items, cap_factor)
+        update_layers([layer for layer in self.layers if isinstance(layer, LearnableLayer)], cap_factor)
 
     def step(self, x_batch: Tensor, y_batch: Tensor, sigma_v: float) -> tuple[Tensor, Tensor]:
         """forward -> innovation -> backward -> capped update (network.py:119-152).

@@ -55,3 +55,33 @@ def update_parameters_multi(items, cap_factor) -> None:
     pn = arr([it[0].numel() for it in items], ctypes.c_int64)
     _lib.call("tagi_capped_update_multi", ctypes.addressof(pm), ctypes.addressof(pS), ctypes.addressof(pdm),
               ctypes.addressof(pdS), ctypes.addressof(pn), k, float(cap_factor), _lib.stream_of(items[0][0]))
+
+
+def _single_layers(layers):
+    for layer in layers:
+        parts = layer._update_parts()
+        if parts is None:
+            yield layer
+        else:
+            yield from _single_layers(parts)
+
+
+def update_layers(layers, cap_factor) -> None:
+    """The capped update of learnable layers, containers opened: one launch for all exposed
+    groups, ``update`` for a layer that exposes none. A layer whose backward applied its update
+    (``update_in_backward``) is left out once."""
+    items = []
+    for layer in _single_layers(layers):
+        if layer._updated_in_backward:
+            layer._updated_in_backward = False
+            continue
+        got = layer._update_groups()
+        if got is None:
+            if items:
+                update_parameters_multi(items, cap_factor)
+                items = []
+            layer.update(cap_factor)
+        else:
+            items.extend(got)
+    if items:
+        update_parameters_multi(items, cap_factor)
