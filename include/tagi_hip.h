@@ -613,7 +613,8 @@ int64_t tagi_embedding_bwd_ws_bytes(int64_t n_tokens, int64_t V, int64_t D);
  * ids: n of the given type; float ids are cast toward zero. Ids equal to padding_idx or
  * outside [0, V) look up zeros and add nothing. dmw/dSw (V, D) are overwritten whole. The
  * sums' order is fixed by the ids (deterministic); the cost does not grow with V beyond
- * writing the deltas. n may be 0. n, V < 2^31, D < 2^21. */
+ * writing the deltas. n may be 0. Lookup: n < 2^30; sorted forms: n <= 2^30 - 64 and
+ * V D < 2^40; all: V < 2^31, D < 2^21. Larger sizes are refused before anything is launched. */
 enum { TAGI_IDS_F32 = 0, TAGI_IDS_I32 = 1, TAGI_IDS_I64 = 2 };
 int tagi_embedding_scaled_fwd(const void* ids, int id_type, const float* mw, const float* Sw,
                               float* mz, float* Sz, int64_t n, int64_t V, int64_t D,

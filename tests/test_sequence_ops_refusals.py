@@ -66,3 +66,17 @@ def test_library_argument_errors():
     err("tagi_linear_attention_bwd", *([None] * 3), h, h, h, None, None, h, None, None, 0, *([None] * 6), h, 1, 4, 1, 8,
         1.0, None, 0, None, match="null pointer")
     err("tagi_linear_attention_step", *([None] * 6), h, h, h, *([None] * 6), h, 1, 1, 8, 1.0, None, match="null pointer")
+
+
+def test_token_counts_at_the_limit_of_a_launch():
+    """2^30 - 64 tokens are the most whose joins (a block of 256 threads for every 64 tokens) stay
+    below 2^32 threads; more are refused before anything is launched, so that no row is updated
+    by a call that fails. The accepted count goes on to the next check (no workspace here)."""
+    from triton_tagi_amd import _lib
+
+    lib = _lib.load()
+    for n, match in (((1 << 30) - 64, "workspace"), ((1 << 30) - 63, "too large"), ((1 << 30) - 1, "too large")):
+        assert lib.tagi_embedding_sorted_bwd(1, 0, 1, 1, 1, 1, 1, n, 50, 1, -1, 1.0, None, 0, None) != 0
+        assert match in _lib.last_error(), (n, _lib.last_error())
+        assert lib.tagi_embedding_sorted_bwd_update(1, 0, 1, 1, 1, 1, None, None, 2.0, n, 50, 1, -1, 1.0, None, 0, None) != 0
+        assert match in _lib.last_error(), (n, _lib.last_error())

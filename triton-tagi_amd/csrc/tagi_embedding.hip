@@ -571,6 +571,11 @@ Layout layout(int64_t n, int64_t V, int64_t D) {
   return l;
 }
 
+// A launch has fewer than 2^32 threads: the joins' blocks for pieces of 64 tokens, which more
+// tokens than 2^17 always have.
+constexpr int64_t kMaxSorted = (1ll << 30) - 64;
+static_assert(kMaxSorted / 64 * 64 * kJoinWaves < (1ll << 32), "blocks of the joins");
+
 constexpr int kAhead = 4;
 template <bool UPD, bool WIDE>
 void launch_sums(const SumArgs& a, hipStream_t s) {
@@ -584,7 +589,7 @@ int sorted_impl(const char* what, const void* ids, int type, const float* dmz, c
                 void* ws, int64_t ws_bytes, hipStream_t s) {
   TAGI_REQUIRE(type >= TAGI_IDS_F32 && type <= TAGI_IDS_I64, "%s: unknown id type %d", what, type);
   TAGI_REQUIRE(n >= 0 && V > 0 && D > 0, "%s: bad sizes", what);
-  TAGI_REQUIRE(n < (1ll << 30) && V < (1ll << 31) && D < (1ll << 21) && V * D < (1ll << 40), "%s: too large", what);
+  TAGI_REQUIRE(n <= kMaxSorted && V < (1ll << 31) && D < (1ll << 21) && V * D < (1ll << 40), "%s: too large", what);
   TAGI_REQUIRE(Sw && (n == 0 || (ids && dmz && dSz)), "%s: null pointer", what);
   TAGI_REQUIRE((dmw == nullptr) == (dSw == nullptr) && (upd || dmw), "%s: null pointer", what);
   const Layout l = layout(n, V, D);
