@@ -155,10 +155,13 @@ __global__ void __launch_bounds__(256) add_rms_norm_short_kernel(FwdArgs a) {
 }
 
 // Blocks own a range of rows and 4 CT columns (CT threads across, 256 / CT rows at a time);
-// a thread keeps the weights and sums of its four columns in registers over the range, the
-// threads of a column are joined in float64 through LDS, and one partial sum per block,
-// column and moment goes to ws[moment][block][D]. HBM bound: 16384 x 4096 with deltas at the
-// sum moves 1.88 GB in 342 us (5.5 TB/s).
+// a thread keeps the weights and sums of its four columns in registers over the range, every
+// kFloatRows rows' floats added in float64 (wide rows leave few blocks, and the ranges grow
+// with the batch: 512 rows at 65536 x 8192), the threads of a column are joined in float64
+// through LDS, and one partial sum per block, column and moment goes to ws[moment][block][D].
+// HBM bound: 16384 x 4096 with deltas at the sum moves 1.88 GB in 343 us (5.5 TB/s); all floats
+// over the range took the same.
+constexpr int kFloatRows = 32;
 template <bool NT, bool WIDE>
 __global__ void __launch_bounds__(256) add_rms_norm_bwd_kernel(
     const float* __restrict__ dmz, const float* __restrict__ dSz, const float* __restrict__ dms,
@@ -168,38 +171,54 @@ __global__ void __launch_bounds__(256) add_rms_norm_bwd_kernel(
   __shared__ f4 red[2][256];
   const int RG = 256 / CT, ct = (int)threadIdx.x % CT, rg = (int)threadIdx.x / CT, nblk = (int)gridDim.x;
   const int64_t r0 = rows * blockIdx.x / nblk, r1 = rows * (blockIdx.x + 1) / nblk;
-  f4 am = {0.f, 0.f, 0.f, 0.f}, as = am;
+  double tm[4] = {}, ts[4] = {};
+  const auto fold = [&](const f4& m, const f4& s) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tm[e] += m[e], ts[e] += s[e];
+  };
   int skip = 4;
   if constexpr (WIDE) {
     const Cols c = columns((int)blockIdx.y * CT + ct, D);
     skip = rg < RG ? c.skip : 4;
     if (skip < 4) {
       const f4 g = *reinterpret_cast<const f4*>(mw + c.at);
+      for (int64_t p = r0 + rg; p < r1; p += (int64_t)kFloatRows * RG) {
+        const int64_t end = min(r1, p + (int64_t)kFloatRows * RG);
+        f4 am = {0.f, 0.f, 0.f, 0.f}, as = am;
 #pragma unroll 2
-      for (int64_t r = r0 + rg; r < r1; r += RG) {
-        const int64_t o = r * D + c.at;
-        const float inv = inv_rms[r];
-        const f4 a = ld<NT>(dmz + o), b = ld<NT>(dSz + o), x = ld<NT>(ms + o) * inv, k = g * inv;
-        f4 u = a * k, w = b * (k * k);
-        if (dms) u += ld<NT>(dms + o), w += ld<NT>(dSs + o);
-        st<NT>(dma + o, u);  // columns of two threads get the same values from both
-        st<NT>(dSa + o, w);
-        am += a * x;
-        as += b * (x * x);
+        for (int64_t r = p; r < end; r += RG) {
+          const int64_t o = r * D + c.at;
+          const float inv = inv_rms[r];
+          const f4 a = ld<NT>(dmz + o), b = ld<NT>(dSz + o), x = ld<NT>(ms + o) * inv, k = g * inv;
+          f4 u = a * k, w = b * (k * k);
+          if (dms) u += ld<NT>(dms + o), w += ld<NT>(dSs + o);
+          st<NT>(dma + o, u);  // columns of two threads get the same values from both
+          st<NT>(dSa + o, w);
+          am += a * x;
+          as += b * (x * x);
+        }
+        fold(am, as);
       }
     }
   } else if (rg < RG) {  // rows of one to three values, one thread across
     skip = 0;
-    for (int64_t r = r0 + rg; r < r1; r += RG)
-      for (int e = 0; e < D; ++e) {
-        const int64_t o = r * D + e;
-        const float inv = inv_rms[r], x = inv * ms[o], k = inv * mw[e], a = dmz[o], b = dSz[o];
-        dma[o] = a * k + (dms ? dms[o] : 0.f);
-        dSa[o] = b * (k * k) + (dSs ? dSs[o] : 0.f);
-        am[e] += a * x;
-        as[e] += b * (x * x);
-      }
+    for (int64_t p = r0 + rg; p < r1; p += (int64_t)kFloatRows * RG) {
+      const int64_t end = min(r1, p + (int64_t)kFloatRows * RG);
+      f4 am = {0.f, 0.f, 0.f, 0.f}, as = am;
+      for (int64_t r = p; r < end; r += RG)
+        for (int e = 0; e < D; ++e) {
+          const int64_t o = r * D + e;
+          const float inv = inv_rms[r], x = inv * ms[o], k = inv * mw[e], a = dmz[o], b = dSz[o];
+          dma[o] = a * k + (dms ? dms[o] : 0.f);
+          dSa[o] = b * (k * k) + (dSs ? dSs[o] : 0.f);
+          am[e] += a * x;
+          as[e] += b * (x * x);
+        }
+      fold(am, as);
+    }
   }
+  f4 am = {(float)tm[0], (float)tm[1], (float)tm[2], (float)tm[3]};
+  f4 as = {(float)ts[0], (float)ts[1], (float)ts[2], (float)ts[3]};
   // the thread's own columns first
   if (skip == 1) am = f4{am.y, am.z, am.w, 0.f}, as = f4{as.y, as.z, as.w, 0.f};
   if (skip == 2) am = f4{am.z, am.w, 0.f, 0.f}, as = f4{as.z, as.w, 0.f, 0.f};
