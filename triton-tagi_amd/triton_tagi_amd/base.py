@@ -28,6 +28,24 @@ class Layer(ABC):
         projections); containers walk them to place or visit every parameter tensor."""
         return ()
 
+    # The attribute that holds what ``backward`` reads (None before a forward), for layers that
+    # ``Sequential.prompt`` and ``decode`` run.
+    _backward_reads: str | None = None
+
+    def forget(self) -> None:
+        """Drops what the last forward left for a backward, here and in the layers inside."""
+        if self._backward_reads is not None:
+            setattr(self, self._backward_reads, None)
+        for layer in self.sublayers():
+            layer.forget()
+
+    def _kept(self):
+        """What the last forward left for the backward; refused where there is none."""
+        kept = getattr(self, self._backward_reads)
+        if kept is None:
+            raise RuntimeError(f"{type(self).__name__}: backward without a forward")
+        return kept
+
 
 class LearnableLayer(Layer):
     """Base class for layers with parameters updated by the capped TAGI rule."""

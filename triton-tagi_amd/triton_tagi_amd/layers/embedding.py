@@ -28,6 +28,8 @@ from ..update.parameters import update_parameters
 
 
 class Embedding(LearnableLayer):
+    _backward_reads = "cat_idx"
+
     def __init__(self, num_embeddings: int, embedding_dim: int, input_size: int = 0, scale: float = 1.0,
                  padding_idx: int = -1, device: str = "cuda", output_scale: float = 1.0,
                  sorted_deltas: bool | None = None) -> None:
@@ -78,7 +80,7 @@ class Embedding(LearnableLayer):
     def backward_param_deltas(self, delta_mz: Tensor, delta_Sz: Tensor):
         """The parameter deltas of ``backward`` without the (zero) deltas of the token ids;
         returns the ids."""
-        tokens = self.cat_idx
+        tokens = self._kept()
         if self.sorted_deltas:
             upd = in_backward.active()
             if upd is not None:

@@ -21,6 +21,8 @@ from ..update.parameters import update_parameters
 
 
 class LayerNorm(LearnableLayer):
+    _backward_reads = "ma_in"
+
     def __init__(self, normalized_shape: int, eps: float = 1e-5, bias: bool = True, device: str = "cuda",
                  gain_w: float = 1.0, gain_b: float = 1.0) -> None:
         self.normalized_shape = normalized_shape
@@ -63,7 +65,7 @@ class LayerNorm(LearnableLayer):
         dm = _lib.check(delta_mz.reshape(-1, D).contiguous(), "delta_mz")
         dS = _lib.check(delta_Sz.reshape(-1, D).contiguous(), "delta_Sz")
         rows = dm.shape[0]
-        if rows != self.ma_in.shape[0]:
+        if rows != self._kept().shape[0]:
             raise ValueError(f"LayerNorm: {rows} delta rows for {self.ma_in.shape[0]} forward rows")
         dev = dm.device
         dma, dSa = torch.empty_like(dm), torch.empty_like(dS)

@@ -37,6 +37,8 @@ def _dense(t):
 class Linear(LearnableLayer):
     """Fully connected layer with Gaussian weights; mw, Sw are (in, out), mb, Sb (1, out)."""
 
+    _backward_reads = "ma_in"
+
     def __init__(self, in_features: int, out_features: int, device: str = "cuda", init_method: str = "He",
                  gain_w: float = 1.0, gain_b: float = 1.0, bias: bool = True) -> None:
         self.in_features = in_features
@@ -94,6 +96,7 @@ class Linear(LearnableLayer):
         are multiplied by it (variances by its square). Within ``update_in_backward`` the kernel that forms the
         parameter deltas also applies the capped update (after the input deltas, which read
         the weight means, are queued), unless that kernel goes to the side stream."""
+        self._kept()
         dmz = delta_mz.reshape(-1, self.out_features).contiguous()
         dSz = delta_Sz.reshape(-1, self.out_features).contiguous()
         ctx = _overlap.active()

@@ -28,6 +28,8 @@ def default_decays(num_heads: int) -> list[float]:
 
 
 class LinearAttention(QkvProjections):
+    _backward_reads = "_cache"
+
     def __init__(self, embed_dim: int, num_heads: int, decay=None, bias: bool = False, gain_weight: float = 1.0,
                  gain_bias: float = 1.0, init_method: str = "He", device: str = "cuda") -> None:
         """``decay``: one number in [0, 1] for every head or a sequence of num_heads;
@@ -92,9 +94,7 @@ class LinearAttention(QkvProjections):
         return mo.view(ma.shape), So.view(ma.shape)
 
     def backward(self, delta_mz: Tensor, delta_Sz: Tensor) -> tuple[Tensor, Tensor]:
-        c = self._cache
-        if c is None:
-            raise RuntimeError("LinearAttention: backward without a forward")
+        c = self._kept()
         q, k, v = c["qkv"]
         B, S, E = *q.shape[:2], self.embed_dim
         dm, dS = linear_attention_backward_packed(q, k, v, delta_mz.reshape(q.shape), delta_Sz.reshape(q.shape),

@@ -43,6 +43,8 @@ def jacobian_backward(delta_m, delta_S, J):
 class ReLU(Layer):
     """Rectified-Gaussian activation; stores J for the backward pass."""
 
+    _backward_reads = "J"
+
     def __init__(self) -> None:
         self.J = None
 
@@ -52,7 +54,7 @@ class ReLU(Layer):
         return ma, Sa
 
     def backward(self, delta_mz: Tensor, delta_Sz: Tensor) -> tuple[Tensor, Tensor]:
-        return jacobian_backward(delta_mz, delta_Sz, self.J)
+        return jacobian_backward(delta_mz, delta_Sz, self._kept())
 
     def __repr__(self):
         return "ReLU()"

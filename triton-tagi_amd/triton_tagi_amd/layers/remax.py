@@ -39,6 +39,8 @@ triton_remax = remax
 class Remax(Layer):
     """Softmax alternative for Bayesian nets (sum of output means ~ 1)."""
 
+    _backward_reads = "J"
+
     def __init__(self) -> None:
         self.J: Tensor | None = None
 
@@ -48,7 +50,7 @@ class Remax(Layer):
         return mu_a, Sa
 
     def backward(self, delta_ma: Tensor, delta_Sa: Tensor) -> tuple[Tensor, Tensor]:
-        return jacobian_backward(delta_ma, delta_Sa, self.J)
+        return jacobian_backward(delta_ma, delta_Sa, self._kept())
 
     def __repr__(self) -> str:
         return "Remax()"

@@ -19,6 +19,8 @@ from .rms_norm import RMSNorm
 
 
 class ResidualRMSNorm(LearnableLayer):
+    _backward_reads = "_sum"
+
     def __init__(self, layers: list, normalized_shape, eps: float = 1e-6, gain_w: float = 1.0,
                  device: str = "cuda") -> None:
         self.layers = list(layers)
@@ -74,9 +76,7 @@ class ResidualRMSNorm(LearnableLayer):
     def backward(self, delta_mz: Tensor, delta_Sz: Tensor) -> tuple[Tensor, Tensor]:
         from .fused import backward_chain
 
-        if self._sum is None:
-            raise RuntimeError("ResidualRMSNorm: backward without a forward")
-        ms, inv = self._sum
+        ms, inv = self._kept()
         n = self.norm
         dm, dS, n.delta_mw, n.delta_Sw = add_rms_norm_backward(delta_mz.reshape(ms.shape), delta_Sz.reshape(ms.shape),
                                                                ms, inv, n.mw, n.Sw)

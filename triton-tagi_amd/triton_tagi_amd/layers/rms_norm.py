@@ -18,6 +18,8 @@ from ..update.parameters import update_parameters
 
 
 class RMSNorm(LearnableLayer):
+    _backward_reads = "ma_in"
+
     def __init__(self, normalized_shape, eps: float = 1e-6, gain_w: float = 1.0, device: str = "cuda") -> None:
         if isinstance(normalized_shape, int):
             normalized_shape = [normalized_shape]
@@ -51,6 +53,7 @@ class RMSNorm(LearnableLayer):
         return mz.reshape(self._input_shape), Sz.reshape(self._input_shape)
 
     def backward(self, delta_mz: Tensor, delta_Sz: Tensor) -> tuple[Tensor, Tensor]:
+        ma_in = self._kept()
         shape = delta_mz.shape
         dm = _lib.check(delta_mz.reshape(-1, self.ni).contiguous(), "delta_mz")
         dS = _lib.check(delta_Sz.reshape(-1, self.ni).contiguous(), "delta_Sz")
@@ -61,7 +64,7 @@ class RMSNorm(LearnableLayer):
         self.delta_Sw = torch.empty_like(self.delta_mw)
         ws = _lib.workspace(_lib.query("tagi_rmsnorm_bwd_ws_bytes", rows, self.ni), dev)
         wp, wb = _lib.ws_args(ws)
-        _lib.call("tagi_rmsnorm_bwd", dm.data_ptr(), dS.data_ptr(), self.ma_in.data_ptr(), self.inv_rms.data_ptr(),
+        _lib.call("tagi_rmsnorm_bwd", dm.data_ptr(), dS.data_ptr(), ma_in.data_ptr(), self.inv_rms.data_ptr(),
                   self.mw.data_ptr(), self.Sw.data_ptr(), dma.data_ptr(), dSa.data_ptr(), self.delta_mw.data_ptr(),
                   self.delta_Sw.data_ptr(), rows, self.ni, wp, wb, _lib.stream_of(dm))
         return dma.reshape(shape), dSa.reshape(shape)

@@ -5,8 +5,9 @@ branch); layers that act on each token by itself run as they are. Anything else 
 over a whole sequence, positional encodings, convolutions) is refused: fed token by token it
 would answer wrongly.
 
-The layers' forwards run here and replace what a backward reads, so the layers that mix tokens
-forget theirs: a backward after a prompt or a token needs a forward of its own, and says so.
+The layers' forwards run here and replace what a backward reads, so ``Sequential`` makes every
+layer forget it afterwards: a backward after a prompt or a token needs a forward of its own, and
+says so.
 """
 
 from __future__ import annotations
@@ -50,11 +51,9 @@ def run_prompt(layers, ma: Tensor, Sa: Tensor | None, lengths: Tensor | None, st
         state = None if states is None else states[i]
         if isinstance(layer, LinearAttention):
             ma, Sa, state = layer.prompt(ma, Sa, lengths, state)
-            layer._cache = None
         elif isinstance(layer, ResidualRMSNorm):
             bm, bS, state = run_prompt(layer.layers, ma, Sa, lengths, state)
             ma, Sa = layer._close(bm, bS, ma, Sa)[:2]
-            layer._sum = None
         else:
             ma, Sa = _tokenwise(layer, ma, Sa)
         out.append(state)
@@ -68,11 +67,9 @@ def run_step(layers, ma: Tensor, Sa: Tensor | None, states, active: Tensor | Non
     for layer, state in zip(layers, states):
         if isinstance(layer, LinearAttention):
             ma, Sa = layer.step(ma, Sa, state, active)
-            layer._cache = None
         elif isinstance(layer, ResidualRMSNorm):
             bm, bS = run_step(layer.layers, ma, Sa, state, active)
             ma, Sa = layer._close(bm, bS, ma, Sa)[:2]
-            layer._sum = None
         else:
             ma, Sa = _tokenwise(layer, ma, Sa)
     return ma, Sa

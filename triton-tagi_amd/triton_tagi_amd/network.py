@@ -78,12 +78,17 @@ class Sequential:
             Sa = torch.zeros_like(x)
         return forward_chain(self.layers, x, Sa)
 
-    def _serving_input(self, x: Tensor) -> tuple[Tensor, Tensor | None]:
+    def _serve(self, run, x: Tensor, *args):
         check_layers(self.layers)
         if x.numel() == 0:
             raise ValueError(f"expected at least one sequence of one token, got {tuple(x.shape)}")
         first = self.layers[0] if self.layers else None
-        return x, (None if isinstance(first, (Linear, Embedding)) else torch.zeros_like(x))
+        Sa = None if isinstance(first, (Linear, Embedding)) else torch.zeros_like(x)
+        try:
+            return run(self.layers, x, Sa, *args)
+        finally:  # the run replaced what the layers' last forward had left, also where it fails
+            for layer in self.layers:
+                layer.forget()
 
     def prompt(self, x: Tensor, lengths: Tensor | None = None, states: list | None = None):
         """Whole sequences through layers that carry states (LinearAttention, also inside
@@ -91,7 +96,7 @@ class Sequential:
         states after each sequence's last token). ``x`` (B, T) token ids or (B, T, features);
         ``lengths`` (B,) ends the sequences of a padded batch; ``states`` continues earlier
         ones (not written). Causal: the same moments as ``forward`` on whole sequences."""
-        return run_prompt(self.layers, *self._serving_input(x), lengths, states)
+        return self._serve(run_prompt, x, lengths, states)
 
     def decode(self, x: Tensor, states: list, active: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """The next token of every sequence, ``x`` (B, 1) ids or (B, 1, features): moments
@@ -99,7 +104,7 @@ class Sequential:
         sequences that are off keep theirs, and their outputs mean nothing."""
         if x.dim() < 2 or x.shape[1] != 1:
             raise ValueError(f"decode: expected one token of every sequence, (B, 1), got {tuple(x.shape)}")
-        return run_step(self.layers, *self._serving_input(x), states, active)
+        return self._serve(run_step, x, states, active)
 
     def backward(self, delta_mu: Tensor, delta_var: Tensor) -> tuple[Tensor, Tensor]:
         return backward_chain(self.layers, delta_mu, delta_var)
