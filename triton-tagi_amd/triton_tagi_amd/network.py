@@ -21,6 +21,7 @@ from .layers.embedding import Embedding
 from .layers.linear import Linear
 from .layers.fused import backward_chain, defer_bn_parameter_deltas, forward_chain
 from .layers.multihead_attention import MultiheadAttentionV2
+from .layers.residual_norm import ResidualRMSNorm
 from .layers.serving import check_layers, run_prompt, run_step
 from .update.observation import compute_innovation, hrc_innovation
 from .update.in_backward import update_in_backward
@@ -208,14 +209,22 @@ class Sequential:
     def num_parameters(self) -> int:
         return sum(layer.num_parameters for layer in self.layers if isinstance(layer, LearnableLayer))
 
-    def get_attention_scores(self) -> dict[int, tuple[Tensor, Tensor]]:
-        out: dict[int, tuple[Tensor, Tensor]] = {}
-        for i, layer in enumerate(self.layers):
-            if isinstance(layer, MultiheadAttentionV2):
-                out[i] = layer.get_attention_scores()
+    def get_attention_scores(self) -> dict[int | tuple[int, ...], tuple[Tensor, Tensor]]:
+        """Scores (means, variances) of every MultiheadAttentionV2, by its position in ``layers``;
+        one inside residual blocks by the positions on the way, outermost first."""
+        out = dict(_attention_scores(self.layers, ()))
         if not out:
             raise RuntimeError("No attention layers in this Sequential.")
         return out
+
+
+def _attention_scores(layers, path: tuple):
+    for i, layer in enumerate(layers):
+        at = (*path, i)
+        if isinstance(layer, MultiheadAttentionV2):
+            yield (at if path else i), layer.get_attention_scores()
+        elif isinstance(layer, ResidualRMSNorm):
+            yield from _attention_scores(layer.layers, at)
 
 
 class StepGraph:
