@@ -287,14 +287,16 @@ constexpr double kCacheBytes = 256e6;
 template <int TPR, int NV>
 void launch_fwd(const FwdArgs& a, bool nt, hipStream_t s) {
   const dim3 grid = row_grid(cdiv(a.rows, TPR < 256 ? 256 / TPR : 1)), block(TPR < 256 ? 256 : TPR);
-  if (nt)
-    hipLaunchKernelGGL((add_rms_norm_kernel<TPR, NV, true>), grid, block, 0, s, a.ma, a.Sa, a.mr, a.Sr, a.mw, a.Sw,
-                       a.mz, a.Sz, a.ms, a.Ss, a.inv, a.rows, a.D, a.eps);
-  else
-    hipLaunchKernelGGL((add_rms_norm_kernel<TPR, NV, false>), grid, block, 0, s, a.ma, a.Sa, a.mr, a.Sr, a.mw, a.Sw,
-                       a.mz, a.Sz, a.ms, a.Ss, a.inv, a.rows, a.D, a.eps);
+  // these take few rows only (below 4096 of 1024 values, 512 of 8192), which stay in the cache
+  constexpr bool kFew = (TPR == 256 && NV == 1) || (TPR == 1024 && NV <= 2);
+  auto kernel = add_rms_norm_kernel<TPR, NV, false>;
+  if constexpr (!kFew)
+    if (nt) kernel = add_rms_norm_kernel<TPR, NV, true>;
+  hipLaunchKernelGGL(kernel, grid, block, 0, s, a.ma, a.Sa, a.mr, a.Sr, a.mw, a.Sw, a.mz, a.Sz, a.ms, a.Ss, a.inv,
+                     a.rows, a.D, a.eps);
 }
-// Chunks of four per thread: rounded up to a kernel that holds them, TPR * 32 values at most.
+// Chunks of four per thread: rounded up to a kernel that holds them, TPR * 32 values at most
+// (a wave's rows are at most 1024 long).
 template <int TPR>
 void launch_fwd_nv(const FwdArgs& a, bool nt, hipStream_t s) {
   const int64_t nv = cdiv(cdiv(a.D, 4), TPR);
@@ -302,9 +304,9 @@ void launch_fwd_nv(const FwdArgs& a, bool nt, hipStream_t s) {
     launch_fwd<TPR, 1>(a, nt, s);
   else if (nv <= 2)
     launch_fwd<TPR, 2>(a, nt, s);
-  else if (nv <= 4)
+  else if (TPR == 64 || nv <= 4)
     launch_fwd<TPR, 4>(a, nt, s);
-  else
+  else if constexpr (TPR > 64)
     launch_fwd<TPR, 8>(a, nt, s);
 }
 
