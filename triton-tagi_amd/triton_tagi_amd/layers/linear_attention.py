@@ -55,13 +55,17 @@ class LinearAttention(QkvProjections):
         self.device = torch.device(device)
         self._make_projections(embed_dim)
         self._scale = 1.0 / math.sqrt(self.head_dim)
-        self._decays: dict[torch.device, Tensor] = {}  # the decays on each device they were used on
+        # on each device they were used on: the decays, and the numbers they were made from
+        self._decays: dict[torch.device, tuple[Tensor, tuple]] = {}
         self._cache: dict | None = None
 
     def _decay_on(self, device: torch.device) -> Tensor:
-        t = self._decays.get(device)
-        if t is None:
-            t = self._decays[device] = torch.tensor(self.decay, dtype=torch.float32, device=device)
+        t, made_from = self._decays.get(device, (None, None))
+        decay = tuple(self.decay)
+        if made_from != decay:
+            new = torch.tensor(decay, dtype=torch.float32, device=device)
+            t = new if t is None else t.copy_(new)  # in place: recorded graphs read it
+            self._decays[device] = t, decay
         return t
 
     def _project(self, ma: Tensor, Sa: Tensor) -> tuple[dict, list[Tensor]]:
