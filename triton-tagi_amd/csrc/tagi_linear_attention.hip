@@ -12,13 +12,19 @@
 //   dk = G_t v,  dSk = N_t (v^2);   dv = G_t^T k,  dSv = N_t^T (k^2)
 //
 // The squared state (M_t.M_t) is needed at every token and has no form as a matrix product
-// over a chunk, so the state advances token by token on the vector ALUs, and that is the
-// bound: 7 operations per state element and token forward. Every pass is one scan,
+// over a chunk, so the state advances token by token on the vector ALUs: 7 operations per state
+// element and token forward, 12 backward. Three of each serve the squared state; the others,
+// linear in their states, are taken along and not formed as matrix products over chunks. Every
+// pass is one scan,
 //   X_t = g X_{t-1} + u_t w_t^T (one or two such states),  y_t[o] = sum_i r_t[i] f(X_t[i][o]),
 // whose columns o are independent: a wavefront keeps 32 columns of the state in registers
 // (4 or 8 lanes share a column, each with as many of its rows; 16 or 8 columns where waves are
 // few), reads the token's vectors from LDS and adds the partial sums over i in exchanges that
-// halve the values each lane keeps: 2 x 4096 tokens, 16 heads of 64, forward and backward 464 us.
+// halve the values each lane keeps: 2 x 4096 tokens, 16 heads of 64, forward and backward 461 us.
+// Counters of that layout (forward, 64 features): 260 vector instructions a token and wave, 224
+// of them products; the vector ALUs are active in 1.07 of a CU's busy cycles (2 where two waves'
+// instructions run side by side all the time), LDS in 0.47, no bank conflicts. Backward: 1.12
+// and 0.49. Neither unit is full: two waves a SIMD wait for each other's LDS reads and sums.
 // A fp32 MFMA has the rate of the vector ALUs and does not run beside them: with the rank-one
 // update as 4 x 4 x 1 MFMAs the same took 496 us where fmas took 474.
 //
@@ -666,7 +672,7 @@ inline bool al4(const tagi_heads& s) { return s.sb % 4 == 0 && s.st % 4 == 0 && 
 //   1 x 512 tokens, 8 heads of 64:   16 x 8 34 / 37, 16 x 16 37 / 39, 16 x 32 48 / 47
 //   1 x 2048 tokens, 4 heads of 128: 64 x 16 75 / 131, 32 x 32 126 / 115, 64 x 32 94 / 138
 //   1 x 64 tokens, 8 heads of 32:    1 x 8 18 / 24, 1 x 16 21 / 24, 2 x 8 22 / 31
-//   3 x 339 tokens, 1 head of 128:   11 x 16 56 / 49, 6 x 16 85 / 67
+//   3 x 339 tokens, 1 head of 128:   11 x 16 56 / 49, 9 x 16 64 / 55, 6 x 16 85 / 67
 //   32 x 2048 tokens, 8 heads of 64: 1 x 8 729 / 1218, 1 x 16 851 / 1012, 4 x 32 624 / 1055
 //   16 x 512 tokens, 8 heads of 128: 1 x 8 479 / -, 1 x 16 413 / 564, 4 x 32 326 / 554
 // So: no chunks where the widest waves that do reach 2048 (backward, whose three scans run side
@@ -674,14 +680,16 @@ inline bool al4(const tagi_heads& s) { return s.sb % 4 == 0 && s.st % 4 == 0 && 
 // least, since narrow waves spend their time reading LDS. No chunks below 128 tokens; else as
 // many as bring 32-column waves there, of 32 tokens at least (backward: and of half a head's
 // features, its three states' traffic, where those are waves enough), with narrower waves
-// where that falls short.
+// where that falls short. Whole groups of kTok tokens make chunks longer than T / n: 3 x 339
+// tokens get 9 of 40, not 11 of 32.
 struct Chunks {
   int64_t L, nch;
   int cols;
 };
 Chunks chunks(int64_t B, int64_t T, int64_t H, int64_t D, bool bwd) {
-  // three-wave blocks (65 to 96 features) fit a CU twice, not 2 2/3 times: 512 of them at once
-  // (7 x 777 tokens, 6 heads of 80: 11 chunks 152, 14 chunks 181)
+  // three-wave blocks (65 to 96 features) fit a CU twice, not 2 2/3 times: 512 of them at once.
+  // Chunk counts are rounded up, so that a few more may be launched (7 x 777 tokens, 6 heads of
+  // 80: 11 chunks, 462 blocks, 152; 13, which this takes, 546 blocks, 152; 14, 588 blocks, 181)
   const int64_t heads = B * H, full = D > 64 && D <= 96 ? 1536 : 2048, target = bwd ? 1024 : full;
   const int64_t enough = bwd ? 512 : full;
   const int narrowest = D > 64 ? 16 : 8;

@@ -9,7 +9,8 @@ Two additions without a counterpart in the reference: ``output_scale`` c multipl
 moments looked up (means by c, variances by c^2; with it the deltas sum c delta_mu Sw and
 (c Sw)^2 delta_S), and ``sorted_deltas`` forms the deltas by sorting the tokens instead of
 scanning them once per category, which a large table needs. Within ``update_in_backward``
-the sorted form applies the capped update to the rows that occur as it forms their deltas.
+the sorted form applies the capped update to the rows that occur as it forms their deltas;
+the deltas of the whole table are stored as well unless its ``keep_deltas`` is false.
 """
 
 from __future__ import annotations

@@ -132,9 +132,10 @@ class Sequential:
     def _backward_scope(self, cap_factor: float):
         """One launch forms every BatchNorm2D's parameter deltas at the end of the backward
         pass; with ``overlap_param_deltas`` the Conv2D parameter-delta GEMMs run on a side
-        stream beside the input-delta chain (joined before the update); Linear layers apply
-        their capped update in the kernel that forms their parameter deltas
-        (``update_in_backward``), and the update after the backward pass does the rest."""
+        stream beside the input-delta chain (joined before the update); Linear layers and
+        Embeddings with ``sorted_deltas`` apply their capped update in the kernel that forms
+        their parameter deltas (``update_in_backward``; the deltas are stored as well), and the
+        update after the backward pass does the rest."""
         stack = contextlib.ExitStack()
         stack.enter_context(defer_bn_parameter_deltas())
         if self.overlap_param_deltas:  # exits first: the side stream is joined before the BN finalize

@@ -7,6 +7,7 @@ own parameters in one kernel: the epilogue that forms each delta also applies th
 update to that parameter in place, with the same arithmetic as the update kernel
 (``capped`` in the kernel library), so the result is the same to the bit. The deltas are
 still stored on the layer, as the reference's backward leaves them (linear.py:146-151).
+An Embedding with ``sorted_deltas`` does the same for the rows that occur in its tokens.
 What changes is the traffic: the parameters and their deltas cross HBM once instead of
 being written, read back and written again (the Linear layer of 4096 x 11008 moves 540 MB
 less per step). With ``keep_deltas=False`` the deltas are applied without being stored
@@ -37,7 +38,8 @@ def active():
 
 
 class update_in_backward:
-    """Context: Linear backward passes inside it also apply the capped update."""
+    """Context: backward passes of Linear layers and of Embeddings with ``sorted_deltas``
+    inside it also apply the capped update."""
 
     def __init__(self, cap_factor: float, keep_deltas: bool = True):
         if not cap_factor > 0.0:
