@@ -699,6 +699,108 @@ int tagi_linear_attention_step(const float* mq, const float* Sq, const float* mk
                                float* So, const tagi_heads* lo, int64_t B, int64_t H, int64_t D,
                                double scale, tagi_stream_t stream);
 
+/* RMSNorm of every query and key head (rms_norm.py:93-110 over head_dim) and its rotation by
+ * position, on Gaussian moments, in one pass (the rotation has no counterpart in the reference).
+ * Queries (B, T, H, D) and keys (B, T, G, D) with strides lq, lk (unit last stride; G may be 0);
+ * outputs dense. Weights wqm, wqS, wkm, wkS (D) each, or all NULL: no norm; inv (B, T, H + G):
+ * the norm's factors, which the backward reads. Pair u of a head, u < pairs, is features
+ * (u, u + pairs), or (2u, 2u + 1) if interleaved, and turns by position * freq[u] (radians); the
+ * features after the pairs stay. positions: (B, T, axes) int32 or int64 (pos_bytes 4 / 8); the
+ * first sections[0] pairs go by axis 0, the next sections[1] by axis 1, and so on (axes <= 4; the
+ * sections add up to pairs). freq is float64. pairs = 0: no rotation. D <= 256. */
+int tagi_qk_rotary_fwd(const float* mq, const float* Sq, const tagi_heads* lq, const float* mk,
+                       const float* Sk, const tagi_heads* lk, const float* wqm, const float* wqS,
+                       const float* wkm, const float* wkS, const void* positions, int pos_bytes,
+                       int64_t axes, const int64_t* sections, const double* freq, int64_t pairs,
+                       int interleaved, float eps, float* oqm, float* oqS, float* okm, float* okS,
+                       float* inv, int64_t B, int64_t T, int64_t H, int64_t G, int64_t D,
+                       tagi_stream_t stream);
+/* Its backward, inv held (rms_norm.py:115-134): deltas of the inputs (dense), and with weights
+ * their deltas (D each; queries' and keys', summed over tokens and heads, order fixed by the
+ * sizes). mq, mk: the forward's input means (not read without weights). */
+int tagi_qk_rotary_bwd(const float* dmq, const float* dSq, const tagi_heads* ldq, const float* dmk,
+                       const float* dSk, const tagi_heads* ldk, const float* mq,
+                       const tagi_heads* lq, const float* mk, const tagi_heads* lk,
+                       const float* inv, const float* wqm, const float* wqS, const float* wkm,
+                       const float* wkS, const void* positions, int pos_bytes, int64_t axes,
+                       const int64_t* sections, const double* freq, int64_t pairs, int interleaved,
+                       float* oqm, float* oqS, float* okm, float* okS, float* dwq, float* dSwq,
+                       float* dwk, float* dSwk, int64_t B, int64_t T, int64_t H, int64_t G,
+                       int64_t D, void* ws, int64_t ws_bytes, tagi_stream_t stream);
+int64_t tagi_qk_rotary_bwd_ws_bytes(int64_t B, int64_t T, int64_t H, int64_t G, int64_t D);
+
+/* A paged cache of keys and values (no counterpart in the reference). Four pools, means and
+ * variances of keys and values, each (pages, heads, page_size, head_dim), dense, of one type.
+ * TAGI_CACHE_FP8 (e4m3) holds codes and one power of two for each row of head_dim:
+ * value = code * 2^(e - 127), e from scales (pages, heads, page_size, 4) in the pools' order;
+ * scales is not read for the other types. table (B, width) int32: the pages of each sequence in
+ * order; token n of sequence b lies in page table[b][n / page_size]. Tokens whose page is not in
+ * the table or outside [0, pages) do not exist: they are not written, read as zeros, and are not
+ * seen by attention. head_dim <= 128. */
+enum { TAGI_CACHE_F32 = 0, TAGI_CACHE_BF16 = 1, TAGI_CACHE_FP8 = 2 };
+typedef struct {
+  void *km, *kS, *vm, *vS, *scales;
+  int64_t type, pages, heads, page_size, head_dim;
+} tagi_kv_cache;
+/* Tokens t < counts[b] (all T without counts) of keys and values (B, T, heads, head_dim) become
+ * tokens starts[b] + t (t without starts) of the cache, rounded to its type (nearest, ties to
+ * even). starts, counts: B int32 / int64 on the GPU. Tokens of one call that share a slot (a
+ * page twice among the tables' written pages) leave it with any mixture of them. */
+int tagi_kv_cache_write(const tagi_kv_cache* cache, const float* mk, const float* Sk,
+                        const tagi_heads* lk, const float* mv, const float* Sv,
+                        const tagi_heads* lv, const int32_t* table, int64_t width,
+                        const void* starts, int start_bytes, const void* counts, int count_bytes,
+                        int64_t B, int64_t T, tagi_stream_t stream);
+/* Tokens n < T of every sequence as dense (B, T, heads, head_dim), zeros from lengths[b] on. */
+int tagi_kv_cache_read(const tagi_kv_cache* cache, const int32_t* table, int64_t width,
+                       const void* lengths, int len_bytes, float* mk, float* Sk, float* mv,
+                       float* Sv, int64_t B, int64_t T, tagi_stream_t stream);
+
+/* Attention with Remax scores over sequences of any length (multihead_attention.py:154-267 with
+ * the Remax of remax.py:33-114), without storing the scores. Queries (B, T, H, D), keys and values
+ * (B, N, G, D), G dividing H: query head h reads key head h / (H / G). Query t stands at position
+ * starts[b] + t (t without starts); it sees the keys j < lengths[b] (N without lengths), and with
+ * causal those j <= its position; a query at or behind the length, or before 0, sees none. A query
+ * that sees nothing gets zeros and leaves no deltas. Keys that no query sees, and queries that see
+ * nothing, are not read into any sum whatever they hold. Score variances below 1e-20 count as
+ * 1e-20. rows: (3, B, H, T), written by the forward (sums of the rectified means and variances,
+ * and the weights' sum), read by the backward. lengths, starts: B int32 / int64 on the GPU.
+ * Outputs dense. D <= 128. */
+int tagi_remax_attention_fwd(const float* mq, const float* Sq, const tagi_heads* lq,
+                             const float* mk, const float* Sk, const tagi_heads* lk,
+                             const float* mv, const float* Sv, const tagi_heads* lv,
+                             const void* lengths, int len_bytes, const void* starts,
+                             int start_bytes, int causal, float* mo, float* So, float* rows,
+                             int64_t B, int64_t T, int64_t N, int64_t H, int64_t G, int64_t D,
+                             double scale, void* ws, int64_t ws_bytes, tagi_stream_t stream);
+int64_t tagi_remax_attention_fwd_ws_bytes(int64_t B, int64_t T, int64_t N, int64_t H, int64_t G,
+                                          int64_t D);
+/* Its backward (multihead_attention.py:209-267): the Remax and its Jacobian are formed again from
+ * the queries, keys and rows. Output deltas with strides ldq (queries) and ldkv (keys, values),
+ * so that they can lie side by side. */
+int tagi_remax_attention_bwd(const float* mq, const float* Sq, const tagi_heads* lq,
+                             const float* mk, const float* Sk, const tagi_heads* lk,
+                             const float* mv, const tagi_heads* lv, const float* dmo,
+                             const float* dSo, const tagi_heads* ldo, const float* rows,
+                             const void* lengths, int len_bytes, const void* starts,
+                             int start_bytes, int causal, float* dmq, float* dSq,
+                             const tagi_heads* ldq, float* dmk, float* dSk, float* dmv, float* dSv,
+                             const tagi_heads* ldkv, int64_t B, int64_t T, int64_t N, int64_t H,
+                             int64_t G, int64_t D, double scale, void* ws, int64_t ws_bytes,
+                             tagi_stream_t stream);
+int64_t tagi_remax_attention_bwd_ws_bytes(int64_t B, int64_t T, int64_t N, int64_t H, int64_t G,
+                                          int64_t D);
+/* One query of every sequence, (B, H, D), over its first lengths[b] tokens of a cache (those that
+ * exist); the outputs are dense. H is a multiple of the cache's heads. max_len: no length is
+ * above it (longer ones count as it). */
+int tagi_remax_attention_step(const float* mq, const float* Sq, const tagi_heads* lq,
+                              const tagi_kv_cache* cache, const int32_t* table, int64_t width,
+                              const void* lengths, int len_bytes, float* mo, float* So, int64_t B,
+                              int64_t H, int64_t max_len, double scale, void* ws, int64_t ws_bytes,
+                              tagi_stream_t stream);
+int64_t tagi_remax_attention_step_ws_bytes(int64_t B, int64_t H, int64_t G, int64_t D,
+                                           int64_t max_len);
+
 /* Sinusoidal positional encoding add (positional_encoding.py:62): out = ma + pe[:S]. */
 int tagi_pe_add(const float* ma, const float* pe, float* out, int64_t B, int64_t S, int64_t E,
                 tagi_stream_t stream);

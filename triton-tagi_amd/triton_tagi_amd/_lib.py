@@ -69,11 +69,21 @@ class Heads(ctypes.Structure):
     _fields_ = [(n, c_int64) for n in ("sb", "st", "sh")]
 
 
+class KvCache(ctypes.Structure):
+    """tagi_kv_cache: the pools of a paged cache."""
+
+    _fields_ = [(n, c_void_p) for n in ("km", "kS", "vm", "vS", "scales")] + [
+        (n, c_int64) for n in ("type", "pages", "heads", "page_size", "head_dim")
+    ]
+
+
 VP = POINTER(TagiView)
 GP = POINTER(ConvGeom)
 BP = POINTER(BnPending)
 PP = POINTER(Plan)
 HP = POINTER(Heads)
+CP = POINTER(KvCache)
+IP = POINTER(c_int64)
 OP_FWD, OP_FWD_FIXED, OP_BWD_DELTA, OP_WGRAD = range(4)  # TAGI_OP_*
 
 # name -> (restype, argtypes)
@@ -159,6 +169,21 @@ _SIGS = {
                                           I64, I64, DBL, P, I64, P]),
     "tagi_linear_attention_bwd_ws_bytes": (I64, [I64, I64, I64, I64]),
     "tagi_linear_attention_step": (c_int, [P, P, P, P, P, P, HP, HP, HP, P, P, P, P, P, P, HP, I64, I64, I64, DBL, P]),
+    "tagi_qk_rotary_fwd": (c_int, [P, P, HP, P, P, HP, P, P, P, P, P, c_int, I64, IP, P, I64, c_int, F, P, P, P, P, P,
+                                   I64, I64, I64, I64, I64, P]),
+    "tagi_qk_rotary_bwd": (c_int, [P, P, HP, P, P, HP, P, HP, P, HP, P, P, P, P, P, P, c_int, I64, IP, P, I64, c_int, P,
+                                   P, P, P, P, P, P, P, I64, I64, I64, I64, I64, P, I64, P]),
+    "tagi_qk_rotary_bwd_ws_bytes": (I64, [I64, I64, I64, I64, I64]),
+    "tagi_kv_cache_write": (c_int, [CP, P, P, HP, P, P, HP, P, I64, P, c_int, P, c_int, I64, I64, P]),
+    "tagi_kv_cache_read": (c_int, [CP, P, I64, P, c_int, P, P, P, P, I64, I64, P]),
+    "tagi_remax_attention_fwd": (c_int, [P, P, HP, P, P, HP, P, P, HP, P, c_int, P, c_int, c_int, P, P, P, I64, I64, I64,
+                                         I64, I64, I64, DBL, P, I64, P]),
+    "tagi_remax_attention_fwd_ws_bytes": (I64, [I64, I64, I64, I64, I64, I64]),
+    "tagi_remax_attention_bwd": (c_int, [P, P, HP, P, P, HP, P, HP, P, P, HP, P, P, c_int, P, c_int, c_int, P, P, HP, P,
+                                         P, P, P, HP, I64, I64, I64, I64, I64, I64, DBL, P, I64, P]),
+    "tagi_remax_attention_bwd_ws_bytes": (I64, [I64, I64, I64, I64, I64, I64]),
+    "tagi_remax_attention_step": (c_int, [P, P, HP, CP, P, I64, P, c_int, P, P, I64, I64, I64, DBL, P, I64, P]),
+    "tagi_remax_attention_step_ws_bytes": (I64, [I64, I64, I64, I64, I64]),
     "tagi_rmsnorm_bwd": (c_int, [P, P, P, P, P, P, P, P, P, P, I64, I64, P, I64, P]),
     "tagi_rmsnorm_bwd_ws_bytes": (I64, [I64, I64]),
     "tagi_embedding_fwd": (c_int, [P, P, P, P, P, I64, I64, I64, I64, P]),

@@ -1,0 +1,65 @@
+"""Checks and layouts of the attention operators' operands."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch import Tensor
+
+from .. import _lib
+
+
+def pair(m: Tensor, S: Tensor, name: str, ref: Tensor, shape) -> tuple[Tensor, Tensor]:
+    """A mean and its variance in one layout with a unit last stride."""
+    if (isinstance(m, Tensor) and isinstance(S, Tensor) and m.dtype is torch.float32 and S.dtype is torch.float32
+            and m.get_device() == ref.get_device() == S.get_device() and m.shape == shape == S.shape):
+        st = m.stride()
+        if st == S.stride() and (st[-1] == 1 or shape[-1] == 1):
+            return m, S
+    _lib.check_with(m, "m" + name, ref, shape)
+    _lib.check_with(S, "S" + name, ref, shape)
+    if m.stride() != S.stride() or (m.stride(-1) != 1 and m.shape[-1] != 1):
+        m, S = m.contiguous(), S.contiguous()
+    return m, S
+
+
+def mean(m: Tensor, name: str, ref: Tensor, shape) -> Tensor:
+    _lib.check_with(m, "m" + name, ref, shape)
+    return m if m.stride(-1) == 1 or m.shape[-1] == 1 else m.contiguous()
+
+
+def heads(t: Tensor) -> _lib.Heads:
+    st = t.stride()
+    return _lib.Heads(st[0], st[1], st[2]) if t.dim() == 4 else _lib.Heads(st[0], 0, st[1])
+
+
+def shape_of(t: Tensor, name: str, dims: int) -> torch.Size:
+    _lib.check(t, name, contiguous=False)
+    if t.dim() != dims or min(t.shape[-2:]) == 0:
+        what = "(B, T, H, D)" if dims == 4 else "(B, H, D)"
+        raise ValueError(f"{name}: expected {what} with heads and features, got {tuple(t.shape)}")
+    return t.shape
+
+
+def finite_scale(scale: float) -> float:
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    return scale
+
+
+def counts(t: Tensor | None, name: str, ref: Tensor, B: int) -> tuple[Tensor | None, int]:
+    """One integer a sequence, and its bytes (0 without a tensor)."""
+    if t is None:
+        return None, 0
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name}: expected an int32 or int64 tensor")
+    if t.device != ref.device or tuple(t.shape) != (B,):
+        raise ValueError(f"{name}: expected ({B},) on {ref.device}, got {tuple(t.shape)} on {t.device}")
+    return t.contiguous(), t.element_size()
+
+
+def key_heads(G: int, H: int) -> None:
+    if H % G:
+        raise ValueError(f"{H} query heads cannot share {G} key heads evenly")
