@@ -715,7 +715,7 @@ int tagi_qk_rotary_fwd(const float* mq, const float* Sq, const tagi_heads* lq, c
                        int interleaved, float eps, float* oqm, float* oqS, float* okm, float* okS,
                        float* inv, int64_t B, int64_t T, int64_t H, int64_t G, int64_t D,
                        tagi_stream_t stream);
-/* Its backward, inv held (rms_norm.py:115-134): deltas of the inputs (dense), and with weights
+/* Its backward, inv held (rms_norm.py:115-134): deltas of the inputs (strides loq, lok), and with weights
  * their deltas (D each; queries' and keys', summed over tokens and heads, order fixed by the
  * sizes). mq, mk: the forward's input means (not read without weights). */
 int tagi_qk_rotary_bwd(const float* dmq, const float* dSq, const tagi_heads* ldq, const float* dmk,
@@ -724,9 +724,10 @@ int tagi_qk_rotary_bwd(const float* dmq, const float* dSq, const tagi_heads* ldq
                        const float* inv, const float* wqm, const float* wqS, const float* wkm,
                        const float* wkS, const void* positions, int pos_bytes, int64_t axes,
                        const int64_t* sections, const double* freq, int64_t pairs, int interleaved,
-                       float* oqm, float* oqS, float* okm, float* okS, float* dwq, float* dSwq,
-                       float* dwk, float* dSwk, int64_t B, int64_t T, int64_t H, int64_t G,
-                       int64_t D, void* ws, int64_t ws_bytes, tagi_stream_t stream);
+                       float* oqm, float* oqS, const tagi_heads* loq, float* okm, float* okS,
+                       const tagi_heads* lok, float* dwq, float* dSwq, float* dwk, float* dSwk,
+                       int64_t B, int64_t T, int64_t H, int64_t G, int64_t D, void* ws,
+                       int64_t ws_bytes, tagi_stream_t stream);
 int64_t tagi_qk_rotary_bwd_ws_bytes(int64_t B, int64_t T, int64_t H, int64_t G, int64_t D);
 
 /* A paged cache of keys and values (no counterpart in the reference). Four pools, means and

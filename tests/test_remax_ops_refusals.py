@@ -68,8 +68,8 @@ def test_library_argument_errors():
     assert need > 0
 
     def bwd(ws, n, dw=(1,) * 4):
-        return (1, 1, h, 1, 1, h, 1, h, 1, h, 1, 1, 1, 1, 1, 1, 4, 1, sec(4), 1, 4, 0, 1, 1, 1, 1, *dw, 2, 300, 4, 2, 64, ws,
-                n, None)
+        return (1, 1, h, 1, 1, h, 1, h, 1, h, 1, 1, 1, 1, 1, 1, 4, 1, sec(4), 1, 4, 0, 1, 1, h, 1, 1, h, *dw, 2, 300, 4, 2, 64,
+                ws, n, None)
 
     err("tagi_qk_rotary_bwd", *bwd(1, need - 1), match="workspace")
     err("tagi_qk_rotary_bwd", *bwd(1, need, (1, None, 1, 1)), match="null pointer")

@@ -28,7 +28,7 @@ typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 struct Args {
   // forward: moments in, moments out. Backward: dq/dk deltas in, mq/mk the forward's means
   const float *mq, *Sq, *mk, *Sk, *dmq, *dSq, *dmk, *dSk;
-  tagi_heads lq, lk, ldq, ldk;
+  tagi_heads lq, lk, ldq, ldk, loq, lok;  // lo: the backward's outputs
   float *oqm, *oqS, *okm, *okS, *inv;
   const float *wqm, *wqS, *wkm, *wkS;  // NULL: no norm
   const void* positions;
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_bwd_kernel(const Args A) {
           da[j] *= wa, db[j] *= wb, ea[j] *= wa * wa, eb[j] *= wb * wb;
         }
       }
-      const int64_t o = q ? (token * A.H + h) * A.D : (token * A.G + h - A.H) * A.D;
+      const int64_t o = q ? head_at(A.loq, b, t, h) : head_at(A.lok, b, t, h - A.H);
       store_row<VEC>(A, (q ? A.oqm : A.okm) + o, lane, da, db);
       store_row<VEC>(A, (q ? A.oqS : A.okS) + o, lane, ea, eb);
     }
@@ -371,16 +371,16 @@ extern "C" int tagi_qk_rotary_bwd(const float* dmq, const float* dSq, const tagi
                                   const float* mk, const tagi_heads* lk, const float* inv, const float* wqm,
                                   const float* wqS, const float* wkm, const float* wkS, const void* positions,
                                   int pos_bytes, int64_t axes, const int64_t* sections, const double* freq,
-                                  int64_t pairs, int interleaved, float* oqm, float* oqS, float* okm, float* okS,
-                                  float* dwq, float* dSwq, float* dwk, float* dSwk, int64_t B, int64_t T, int64_t H,
+                                  int64_t pairs, int interleaved, float* oqm, float* oqS, const tagi_heads* loq,
+                                  float* okm, float* okS, const tagi_heads* lok, float* dwq, float* dSwq, float* dwk, float* dSwk, int64_t B, int64_t T, int64_t H,
                                   int64_t G, int64_t D, void* ws, int64_t ws_bytes, tagi_stream_t stream) {
   const char* what = "tagi_qk_rotary_bwd";
   Args a{};
   if (int rc = fill(what, a, B, T, H, G, D, positions, pos_bytes, axes, sections, freq, pairs, interleaved)) return rc;
   TAGI_REQUIRE(!!wqm == !!wqS && !!wqm == !!wkm && !!wqm == !!wkS, "%s: a norm has four weight moments", what);
   TAGI_REQUIRE(!wqm || (dwq && dSwq && dwk && dSwk), "%s: null pointer", what);
-  TAGI_REQUIRE(a.tokens == 0 || (dmq && dSq && ldq && oqm && oqS && (G == 0 || (dmk && dSk && ldk && okm && okS))),
-               "%s: null pointer", what);
+  TAGI_REQUIRE(a.tokens == 0 || (dmq && dSq && ldq && oqm && oqS && loq), "%s: null pointer", what);
+  TAGI_REQUIRE(a.tokens == 0 || G == 0 || (dmk && dSk && ldk && okm && okS && lok), "%s: null pointer", what);
   TAGI_REQUIRE(a.tokens == 0 || !wqm || (mq && lq && inv && (G == 0 || (mk && lk))), "%s: null pointer", what);
   const int64_t nblk = a.tokens ? bwd_blocks(a.tokens, H + G, D) : 0;
   TAGI_REQUIRE(!wqm || !nblk || (ws && ws_bytes >= tagi_qk_rotary_bwd_ws_bytes(B, T, H, G, D)),
@@ -388,8 +388,8 @@ extern "C" int tagi_qk_rotary_bwd(const float* dmq, const float* dSq, const tagi
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps(FAM_RMSNORM, s, 0.0, 20.0 * a.tokens * (H + G) * D);
   if (nblk) {
-    a.dmq = dmq, a.dSq = dSq, a.dmk = dmk, a.dSk = dSk, a.ldq = *ldq, a.mq = mq, a.mk = mk;
-    if (G) a.ldk = *ldk;
+    a.dmq = dmq, a.dSq = dSq, a.dmk = dmk, a.dSk = dSk, a.ldq = *ldq, a.loq = *loq, a.mq = mq, a.mk = mk;
+    if (G) a.ldk = *ldk, a.lok = *lok;
     if (lq) a.lq = *lq;
     if (lk) a.lk = *lk;
     a.wqm = wqm, a.wqS = wqS, a.wkm = wkm, a.wkS = wkS, a.inv = const_cast<float*>(inv);

@@ -22,6 +22,7 @@ from .layers import (
     PositionalEncoding,
     ReLU,
     Remax,
+    RemaxAttention,
     ResBlock,
     ResidualRMSNorm,
     RMSNorm,
@@ -53,5 +54,5 @@ __all__ = [
     "init_weight_bias_norm", "compute_innovation", "get_cap_factor", "update_parameters", "EvenSoftplus",
     "LayerNorm", "MaxPool2D", "RunDir", "load_model", "HierarchicalSoftmax", "class_to_obs", "labels_to_hrc",
     "obs_to_class_probs", "get_predicted_labels", "compute_innovation_with_indices", "hrc_innovation",
-    "LinearAttention", "ResidualRMSNorm",
+    "LinearAttention", "ResidualRMSNorm", "RemaxAttention",
 ]

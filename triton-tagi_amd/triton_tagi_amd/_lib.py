@@ -172,7 +172,7 @@ _SIGS = {
     "tagi_qk_rotary_fwd": (c_int, [P, P, HP, P, P, HP, P, P, P, P, P, c_int, I64, IP, P, I64, c_int, F, P, P, P, P, P,
                                    I64, I64, I64, I64, I64, P]),
     "tagi_qk_rotary_bwd": (c_int, [P, P, HP, P, P, HP, P, HP, P, HP, P, P, P, P, P, P, c_int, I64, IP, P, I64, c_int, P,
-                                   P, P, P, P, P, P, P, I64, I64, I64, I64, I64, P, I64, P]),
+                                   P, HP, P, P, HP, P, P, P, P, I64, I64, I64, I64, I64, P, I64, P]),
     "tagi_qk_rotary_bwd_ws_bytes": (I64, [I64, I64, I64, I64, I64]),
     "tagi_kv_cache_write": (c_int, [CP, P, P, HP, P, P, HP, P, I64, P, c_int, P, c_int, I64, I64, P]),
     "tagi_kv_cache_read": (c_int, [CP, P, I64, P, c_int, P, P, P, P, I64, I64, P]),

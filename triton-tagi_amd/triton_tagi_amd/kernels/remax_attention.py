@@ -75,6 +75,17 @@ def remax_attention_backward(mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, mv:
 
     ``rows``: of a ``remax_attention`` of the same operands. Keys' deltas are summed over the query
     heads that share them."""
+    dmq, dmk = (torch.empty(t.shape, device=t.device, dtype=torch.float32) for t in (mq, mk))
+    out = (dmq, torch.empty_like(dmq), dmk, *(torch.empty_like(dmk) for _ in range(3)))
+    remax_attention_backward_into(out, mq, Sq, mk, Sk, mv, delta_mo, delta_So, rows, scale, causal, lengths, starts)
+    return out
+
+
+def remax_attention_backward_into(out, mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, mv: Tensor, delta_mo: Tensor,
+                                  delta_So: Tensor, rows: Tensor, scale: float = 1.0, causal: bool = True,
+                                  lengths: Tensor | None = None, starts: Tensor | None = None) -> None:
+    """``remax_attention_backward`` into six tensors: the queries' two in one layout, the keys' and
+    values' four in one, unit last strides."""
     qs, ks = _sizes(mq, mk)
     B, T, H, D = qs
     N, G = ks[1:3]
@@ -86,17 +97,13 @@ def remax_attention_backward(mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, mv:
     scale = finite_scale(scale)
     lengths, len_bytes = counts(lengths, "lengths", mq, B)
     starts, start_bytes = counts(starts, "starts", mq, B)
-    dmq = torch.empty(qs, device=mq.device, dtype=torch.float32)
-    dmk = torch.empty(ks, device=mq.device, dtype=torch.float32)
-    out = (dmq, torch.empty_like(dmq), dmk, *(torch.empty_like(dmk) for _ in range(3)))
     ws = _lib.workspace(_lib.query("tagi_remax_attention_bwd_ws_bytes", B, T, N, H, G, D), mq.device)
     wp, wb = _lib.ws_args(ws)
     p = [t.data_ptr() for t in out]
     _lib.call_on(mq, "tagi_remax_attention_bwd", mq.data_ptr(), Sq.data_ptr(), heads(mq), mk.data_ptr(), Sk.data_ptr(),
                  heads(mk), mv.data_ptr(), heads(mv), dm.data_ptr(), dS.data_ptr(), heads(dm), rows.data_ptr(),
-                 _lib.ptr(lengths), len_bytes, _lib.ptr(starts), start_bytes, int(causal), p[0], p[1], heads(dmq),
-                 p[2], p[3], p[4], p[5], heads(dmk), B, T, N, H, G, D, scale, wp, wb, _lib.stream_of(mq))
-    return out
+                 _lib.ptr(lengths), len_bytes, _lib.ptr(starts), start_bytes, int(causal), p[0], p[1],
+                 heads(out[0]), p[2], p[3], p[4], p[5], heads(out[2]), B, T, N, H, G, D, scale, wp, wb, _lib.stream_of(mq))
 
 
 def remax_attention_step(mq: Tensor, Sq: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, scale: float = 1.0,

@@ -118,6 +118,18 @@ def qk_norm_rotary_backward(delta_mq: Tensor, delta_Sq: Tensor, delta_mk: Tensor
     dmwk, dSwk), each (D,). ``mq``, ``mk``: the forward's input means. The deltas turn back, then
 
         dm = d inv g, dS = D (inv g)^2;  dmw = Sg sum d inv m, dSw = Sg^2 sum D (inv m)^2."""
+    oqm, okm = (torch.empty(t.shape, device=t.device, dtype=torch.float32) for t in (mq, mk))
+    out = (oqm, torch.empty_like(oqm), okm, torch.empty_like(okm))
+    return (*out, *qk_norm_rotary_backward_into(out, delta_mq, delta_Sq, delta_mk, delta_Sk, mq, mk, inv, positions,
+                                                frequencies, weights, sections, interleaved))
+
+
+def qk_norm_rotary_backward_into(out, delta_mq: Tensor, delta_Sq: Tensor, delta_mk: Tensor, delta_Sk: Tensor,
+                                 mq: Tensor, mk: Tensor, inv: Tensor | None, positions: Tensor | None = None,
+                                 frequencies: Tensor | None = None, weights=None, sections=None,
+                                 interleaved: bool = False) -> tuple[Tensor, ...]:
+    """``qk_norm_rotary_backward`` into four tensors (a mean's and its variance's in one layout, unit
+    last stride); returns the weights' deltas."""
     qs, ks = _sizes(mq, mk)
     B, T, H, D = qs
     G = ks[2]
@@ -128,9 +140,7 @@ def qk_norm_rotary_backward(delta_mq: Tensor, delta_Sq: Tensor, delta_mk: Tensor
     if weights is not None:
         inv = _lib.dense_with(inv, "inv", mq, (B, T, H + G))
     pos, pos_bytes, axes, sec, freq, pairs = _turns(positions, frequencies, sections, mq, qs)
-    oqm = torch.empty(qs, device=mq.device, dtype=torch.float32)
-    okm = torch.empty(ks, device=mq.device, dtype=torch.float32)
-    oqS, okS = torch.empty_like(oqm), torch.empty_like(okm)
+    oqm, oqS, okm, okS = out
     dw = ()
     ws = None
     if weights is not None:
@@ -140,6 +150,7 @@ def qk_norm_rotary_backward(delta_mq: Tensor, delta_Sq: Tensor, delta_mk: Tensor
     _lib.call_on(mq, "tagi_qk_rotary_bwd", dmq.data_ptr(), dSq.data_ptr(), heads(dmq), dmk.data_ptr(), dSk.data_ptr(),
                  heads(dmk), mq.data_ptr(), heads(mq), mk.data_ptr(), heads(mk), _lib.ptr(inv),
                  *(_lib.ptr(x) for x in w), _lib.ptr(pos), pos_bytes, axes, sec, _lib.ptr(freq), pairs,
-                 int(interleaved), oqm.data_ptr(), oqS.data_ptr(), okm.data_ptr(), okS.data_ptr(),
-                 *((x.data_ptr() for x in dw) if dw else (None,) * 4), B, T, H, G, D, wp, wb, _lib.stream_of(mq))
-    return (oqm, oqS, okm, okS, *dw)
+                 int(interleaved), oqm.data_ptr(), oqS.data_ptr(), heads(oqm), okm.data_ptr(), okS.data_ptr(),
+                 heads(okm), *((x.data_ptr() for x in dw) if dw else (None,) * 4), B, T, H, G, D, wp, wb,
+                 _lib.stream_of(mq))
+    return dw

@@ -14,6 +14,7 @@ from .multihead_attention import MultiheadAttentionV2
 from .positional_encoding import PositionalEncoding
 from .relu import ReLU, bayesian_relu
 from .remax import Remax, remax, triton_remax
+from .remax_attention import AttentionState, RemaxAttention
 from .resblock import Add, ResBlock, add_shortcut, delta_merge, triton_add_shortcut, triton_delta_merge
 from .residual_norm import ResidualRMSNorm
 from .rms_norm import RMSNorm
@@ -22,6 +23,6 @@ __all__ = [
     "Add", "AvgPool2D", "BatchNorm2D", "Conv2D", "Embedding", "EvenSoftplus", "Flatten", "LayerNorm", "Linear",
     "MaxPool2D", "MultiheadAttentionV2", "even_softplus",
     "PositionalEncoding", "RMSNorm", "ReLU", "Remax", "ResBlock", "add_shortcut", "bayesian_relu", "delta_merge",
-    "LinearAttention", "ResidualRMSNorm",
+    "LinearAttention", "ResidualRMSNorm", "AttentionState", "RemaxAttention",
     "remax", "triton_add_shortcut", "triton_delta_merge", "triton_remax",
 ]

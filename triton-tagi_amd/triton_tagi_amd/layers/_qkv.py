@@ -23,21 +23,27 @@ class QkvProjections(LearnableLayer):
     """Base of the attention layers; expects embed_dim, has_bias, init_method, gain_weight,
     gain_bias and device to be set before ``_make_projections``."""
 
-    def _make_projections(self, width: int) -> None:
+    def _make_projections(self, width: int, kv_width: int | None = None) -> None:
+        """Queries ``width`` wide, keys and values ``kv_width`` (as the queries without)."""
+        kv_width = width if kv_width is None else kv_width
         kw = dict(device=self.device, init_method=self.init_method, gain_w=self.gain_weight, gain_b=self.gain_bias,
                   bias=self.has_bias)
         self.q_proj = Linear(self.embed_dim, width, **kw)
-        self.k_proj = Linear(self.embed_dim, width, **kw)
-        self.v_proj = Linear(self.embed_dim, width, **kw)
+        self.k_proj = Linear(self.embed_dim, kv_width, **kw)
+        self.v_proj = Linear(self.embed_dim, kv_width, **kw)
+        self._ends = (width, width + kv_width, width + 2 * kv_width)  # columns of q, k, v side by side
 
     def _projections(self):
         return (self.q_proj, self.k_proj, self.v_proj)
 
+    def _cols(self, i: int) -> slice:
+        return slice(self._ends[i - 1] if i else 0, self._ends[i])
+
     _QKV_ATTRS = ("mw", "Sw", "mb", "Sb")
 
     def _qkv_params(self) -> dict:
-        """The three projections' parameters side by side: (E, 3E) weights and (1, 3E)
-        biases, which the fused projection product and the update read directly. Each
+        """The three projections' parameters side by side: (E, L) weights and (1, L)
+        biases (L = 3E where keys and values are as wide as the queries), which the fused projection product and the update read directly. Each
         projection's mw, Sw, mb, Sb are column views of them, so in-place changes to either
         are seen by both (checkpoint restore copies in place). Built at the first forward;
         rebuilt from the projections' tensors if any of them was replaced since."""
@@ -51,21 +57,19 @@ class QkvProjections(LearnableLayer):
             if parts[0] is None:
                 continue
             buf = torch.cat(parts, 1)
-            n = parts[0].shape[1]
             for i, p in enumerate(projs):
-                setattr(p, attr, buf[:, i * n:(i + 1) * n])
+                setattr(p, attr, buf[:, self._cols(i)])
             bufs[attr] = buf
         self._qkv = bufs
         return bufs
 
     def _qkv_intact(self, bufs: dict) -> bool:
         for attr, buf in bufs.items():
-            n = buf.shape[1] // 3
             for i, p in enumerate(self._projections()):
-                t = getattr(p, attr, None)
+                t, cols = getattr(p, attr, None), self._cols(i)
                 if not (isinstance(t, Tensor) and t.device == buf.device and t.dtype == buf.dtype
-                        and tuple(t.shape) == (buf.shape[0], n) and t.stride() == buf.stride()
-                        and t.data_ptr() == buf.data_ptr() + i * n * buf.element_size()):
+                        and tuple(t.shape) == (buf.shape[0], cols.stop - cols.start) and t.stride() == buf.stride()
+                        and t.data_ptr() == buf.data_ptr() + cols.start * buf.element_size()):
                     return False
         return True
 
@@ -74,10 +78,9 @@ class QkvProjections(LearnableLayer):
 
     def _projection_param_deltas(self, c: dict, dqkv_m: Tensor, dqkv_S: Tensor) -> None:
         """Stores the three projections' parameter deltas, one product over the side-by-side
-        deltas (B*S, 3E) of their outputs (on the side stream within a step when large).
+        deltas (B*S, L) of their outputs (on the side stream within a step when large).
         ``c`` holds what the forward read: ma_in, w_S, b_S."""
-        E = self.embed_dim
-        L = 3 * E
+        E, L = self.embed_dim, self._ends[2]
         dev = dqkv_m.device
         projs = self._projections()
         ma_in = c["ma_in"]
@@ -86,11 +89,11 @@ class QkvProjections(LearnableLayer):
         side = ctx.fork(dev, ma_in, dqkv_m, dqkv_S, c["w_S"], c["b_S"]) if ctx is not None and big else None
         with torch.cuda.stream(side) if side is not None else contextlib.nullcontext():
             dmw, dSw, dmb, dSb = linear_param_deltas(ma_in, dqkv_m, dqkv_S, c["w_S"], c["b_S"])
-        # each projection's deltas are column views of the (E, 3E) ones, as its parameters
+        # each projection's deltas are column views of the (E, L) ones, as its parameters
         # are of the side-by-side buffers the update applies them to
         self._qkv_deltas = (dmw, dSw, dmb, dSb)
         for i, p in enumerate(projs):
-            cols = slice(i * E, (i + 1) * E)
+            cols = self._cols(i)
             p.delta_mw, p.delta_Sw = dmw[:, cols], dSw[:, cols]
             if self.has_bias:
                 p.delta_mb, p.delta_Sb = dmb[:, cols], dSb[:, cols]

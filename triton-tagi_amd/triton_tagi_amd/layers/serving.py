@@ -1,7 +1,7 @@
 """Prompts and single tokens through a list of layers with carried states.
 
-Layers that mix tokens keep a state (LinearAttention: its own; ResidualRMSNorm: those of its
-branch); layers that act on each token by itself run as they are. Anything else (attention
+Layers that mix tokens keep a state (LinearAttention and RemaxAttention: their own;
+ResidualRMSNorm: those of its branch); layers that act on each token by itself run as they are. Anything else (attention
 over a whole sequence, positional encodings, convolutions) is refused: fed token by token it
 would answer wrongly.
 
@@ -21,17 +21,19 @@ from .linear import Linear
 from .linear_attention import LinearAttention
 from .relu import ReLU
 from .remax import Remax
+from .remax_attention import RemaxAttention
 from .residual_norm import ResidualRMSNorm
 from .rms_norm import RMSNorm
 
 _TOKENWISE = (Embedding, Linear, ReLU, Remax, RMSNorm, LayerNorm)
+_STATEFUL = (LinearAttention, RemaxAttention)
 
 
 def check_layers(layers) -> None:
     for layer in layers:
         if isinstance(layer, ResidualRMSNorm):
             check_layers(layer.layers)
-        elif not isinstance(layer, (*_TOKENWISE, LinearAttention)):
+        elif not isinstance(layer, (*_TOKENWISE, *_STATEFUL)):
             raise TypeError(f"{type(layer).__name__} cannot run with a carried state")
 
 
@@ -49,7 +51,7 @@ def run_prompt(layers, ma: Tensor, Sa: Tensor | None, lengths: Tensor | None, st
         raise ValueError(f"states: {len(states)} entries for {len(layers)} layers")
     for i, layer in enumerate(layers):
         state = None if states is None else states[i]
-        if isinstance(layer, LinearAttention):
+        if isinstance(layer, _STATEFUL):
             ma, Sa, state = layer.prompt(ma, Sa, lengths, state)
         elif isinstance(layer, ResidualRMSNorm):
             bm, bS, state = run_prompt(layer.layers, ma, Sa, lengths, state)
@@ -65,7 +67,7 @@ def run_step(layers, ma: Tensor, Sa: Tensor | None, states, active: Tensor | Non
     if len(states) != len(layers):
         raise ValueError(f"states: {len(states)} entries for {len(layers)} layers")
     for layer, state in zip(layers, states):
-        if isinstance(layer, LinearAttention):
+        if isinstance(layer, _STATEFUL):
             ma, Sa = layer.step(ma, Sa, state, active)
         elif isinstance(layer, ResidualRMSNorm):
             bm, bS = run_step(layer.layers, ma, Sa, state, active)

@@ -92,7 +92,7 @@ class Sequential:
                 layer.forget()
 
     def prompt(self, x: Tensor, lengths: Tensor | None = None, states: list | None = None):
-        """Whole sequences through layers that carry states (LinearAttention, also inside
+        """Whole sequences through layers that carry states (LinearAttention, RemaxAttention, also inside
         ResidualRMSNorm) and layers that act on each token by itself: (means, variances,
         states after each sequence's last token). ``x`` (B, T) token ids or (B, T, features);
         ``lengths`` (B,) ends the sequences of a padded batch; ``states`` continues earlier
