@@ -14,22 +14,27 @@
 // Queries and keys are formed again from (mt, vt, s): one kernel walks keys for each query (dq),
 // one walks queries for each key (dk, dv); no atomics, every sum's order is fixed by the sizes.
 //
-// The queries of the H / G heads that share a key head are one list of rows, token by token.
-// Every product is 16 x 16 x 4 fp32 MFMAs with the walked side in the rows, so a lane holds the
-// scores of one row (or key) and its sums need no exchange until the end; and the tile's
-// registers are the next product's right operand as they are: lane group g holds rows 4 g + r,
-// and a sum over rows may take them in any order.
+// The queries of the H / G heads that share a key head are one list of rows, token by token. A wave
+// holds 16 rows (or keys) as right operands in registers; a block's waves walk tiles of 32 keys (or
+// rows) together, split into bf16 parts (tagi_split_bf16.h) as they go from HBM to LDS. The walked
+// side is in the rows of every product, so a lane holds the scores of one row (or key) and its sums
+// need no exchange until the end; and the registers of two products of 16 are the next product's
+// right operand as they are, whose left operand is the tile read transposed from LDS.
 #include "tagi_remax.h"
+#include "tagi_split_bf16.h"
 
 namespace tagi {
 namespace {
 
-typedef float v4 __attribute__((ext_vector_type(4)));
+typedef short h4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int kWaves = 4;
-constexpr int kRows = 16 * kWaves;  // rows (or keys) of a block
 constexpr int kTile = 32;           // keys (or rows) walked at a time
 constexpr int kMaxDim = 128;
+constexpr int kLdsBytes = 160 * 1024;
+// Walked by one block at most: the matrix cores cut sums off (they do not round them), about 1e-8
+// of the sum for every product added; the splits are added in fp32.
+constexpr int kMostWalked = 2048;
 
 struct Args {
   const float *mq, *Sq, *mk, *Sk, *mv, *Sv, *dm, *dS;
@@ -37,15 +42,12 @@ struct Args {
   const void *lengths, *starts;
   int len_bytes, start_bytes, causal;
   float *mo, *So, *rows, *dmk, *dSk, *dmv, *dSv;  // mo, So: dmq, dSq in the backward
-  float *sums, *parts;  // workspace: [split][2][BG][M], [split][BG][M][2 D + 1]
+  float *sums, *parts;  // workspace: [split][2][BG][M], [split][BG][M][2 D + 1] (or [..][N][4 D])
   int64_t B, M;         // M = T R rows of a key head
   int T, N, H, G, R, D, splits, chunk;
   float c, c2;
 };
 
-__device__ __forceinline__ v4 mfma(float a, float b, v4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
 __device__ __forceinline__ int64_t int_at(const void* p, int bytes, int64_t i) {
   return bytes == 8 ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
 }
@@ -70,55 +72,135 @@ __device__ __forceinline__ Seq sequence(const Args& A, int64_t b) {
 // Keys that row rho of its key head sees: those below this.
 __device__ __forceinline__ int row_limit(const Args& A, const Seq& s, int64_t rho) {
   if (rho >= A.M) return 0;
-  const int64_t pos = s.start + rho / A.R;
+  const int64_t pos = s.start + (int)rho / A.R;
   if (pos < 0 || pos >= s.len) return 0;
   return A.causal ? (int)pos + 1 : s.len;
 }
 // No row of [rho0, rho0 + n) sees a key from here on.
 __device__ __forceinline__ int block_limit(const Args& A, const Seq& s, int64_t rho0, int n) {
+  if (rho0 >= A.M) return 0;
   const int64_t last = (rho0 + n < A.M ? rho0 + n : A.M) - 1;
-  const int64_t first_pos = s.start + rho0 / A.R, pos = s.start + last / A.R;
+  const int64_t first_pos = s.start + (int)rho0 / A.R, pos = s.start + (int)last / A.R;
   if (first_pos >= s.len || pos < 0) return 0;
   return A.causal ? (int)(pos + 1 < s.len ? pos + 1 : s.len) : s.len;
 }
 
 __device__ __forceinline__ int64_t row_at(const Args& A, const tagi_heads& l, int64_t b, int g, int64_t rho) {
-  const int64_t t = rho / A.R;
-  return b * l.sb + t * l.st + (g * A.R + (rho - t * A.R)) * l.sh;
+  const int t = (int)rho / A.R;
+  return b * l.sb + (int64_t)t * l.st + (g * A.R + ((int)rho - t * A.R)) * l.sh;
+}
+__device__ __forceinline__ int64_t key_at(const tagi_heads& l, int64_t b, int g, int64_t key) {
+  return b * l.sb + key * l.st + g * l.sh;
+}
+__device__ __forceinline__ int64_t stat_at(const Args& A, int64_t b, int g, int64_t rho, int q) {
+  const int t = (int)rho / A.R, h = g * A.R + ((int)rho - t * A.R);
+  return ((q * A.B + b) * A.H + h) * A.T + t;
 }
 
-// kTile rows of an operand into LDS, zeros where there is none: nothing behind `end` is read.
-template <int DP>
-__device__ __forceinline__ void stage_keys(const Args& A, const float* p, const tagi_heads& l, int64_t b, int g, int key0,
-                                           int end, float (*to)[DP + 1]) {
-  for (int i = threadIdx.x; i < kTile * DP; i += 64 * kWaves) {
-    const int r = i / DP, d = i % DP;
-    to[r][d] = key0 + r < end && d < A.D ? p[b * l.sb + (int64_t)(key0 + r) * l.st + g * l.sh + d] : 0.f;
+// Eight neighbouring features from d on, zeros behind D. VEC: D is a multiple of eight.
+template <bool VEC>
+__device__ __forceinline__ void load8(const float* p, int d, int D, bool on, float (&x)[8]) {
+  if constexpr (VEC) {
+    f4 a = {0, 0, 0, 0}, b = a;
+    if (on && d < D) a = *reinterpret_cast<const f4*>(p + d), b = *reinterpret_cast<const f4*>(p + d + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = on && d + i < D ? p[d + i] : 0.f;
   }
 }
 
-// The right operand of a wave's 16 rows: lane group k4 of step s holds feature 4 s + k4.
+// ------------------------------------------------------------------------ walked tiles in LDS
+// A tile is kTile rows of operands in bf16 parts, [part][16 rows][32 features] in the order in
+// which a wave's lanes read a left operand: lane l the row l % 16, features 8 (l / 16) + 0..7.
+template <int DP, int PARTS>
+struct Tile {
+  static constexpr int S = DP / 32;
+  static constexpr int halves = PARTS * 2 * S * 512;  // 16-bit values
+  static constexpr int bytes = 2 * halves;
+};
 template <int DP>
-__device__ __forceinline__ void load_right(const Args& A, const float* p, int64_t at, bool on, float (&x)[DP / 4]) {
-  const int k4 = (threadIdx.x & 63) >> 4;
+__device__ __forceinline__ int piece(int part, int kt, int s) {
+  return ((part * 2 + kt) * (DP / 32) + s) * 512;
+}
+template <int DP, int P>
+__device__ __forceinline__ void put(short* tile, int first, int kt, int s, int lane, const Parts<P>& x) {
 #pragma unroll
-  for (int s = 0; s < DP / 4; ++s) x[s] = on && 4 * s + k4 < A.D ? p[at + 4 * s + k4] : 0.f;
+  for (int p = 0; p < P; ++p) *reinterpret_cast<bf8*>(tile + piece<DP>(first + p, kt, s) + 8 * lane) = x.p[p];
+}
+// 16 rows as a left operand.
+template <int DP>
+__device__ __forceinline__ Parts<3> left(const short* tile, int first, int kt, int s, int lane) {
+  Parts<3> x;
+#pragma unroll
+  for (int p = 0; p < 3; ++p) x.p[p] = *reinterpret_cast<const bf8*>(tile + piece<DP>(first + p, kt, s) + 8 * lane);
+  return x;
+}
+// The tile transposed, 16 features (16 dt + lane % 16) as rows of a left operand: lane group g
+// holds the tile's rows 4 g + 0..3 and 16 + 4 g + 0..3, as the registers of two products of 16
+// rows hold them. ds_read_b64_tr_b16: of the 64 bits that lane p of a group of 16 reads, lane q
+// gets element q % 4 of lanes q / 4 + 4 j, j = 0..3.
+template <int DP>
+__device__ __forceinline__ Parts<3> transposed(const short* tile, int first, int dt, int lane) {
+  typedef __attribute__((address_space(3))) h4 lds_h4;
+  const int p = lane & 15, g = lane >> 4;
+  const int at = (((dt & 1) * 2 + ((p & 3) >> 1)) * 16 + 4 * g + (p >> 2)) * 8 + 4 * (p & 1);
+  Parts<3> x;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    union {
+      bf8 v;
+      h4 h[2];
+    } u;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+      u.h[kt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4*)(tile + piece<DP>(first + k, kt, dt >> 1) + at));
+    x.p[k] = u.v;
+  }
+  return x;
 }
 
-// Score moments of 16 walked rows (LDS) against the wave's 16, queries on the right.
+// What a lane brings of the next tile: eight features of a row's mean and variance (or deltas).
+struct Unit {
+  float m[8], S[8];
+};
+// A tile takes 2 S units a lane and operand pair; wave w of W holds units w, w + W, ...
+template <int DP, int W>
+constexpr int units_of(int pairs) {
+  return (2 * (DP / 32) * pairs + W - 1) / W;
+}
+
+// The right operand of a wave's 16 rows: x in parts, eight features a lane and step.
 template <int DP>
-__device__ __forceinline__ void scores(const Args& A, const float (*km)[DP + 1], const float (*kS)[DP + 1], int r0,
-                                       const float (&qm)[DP / 4], const float (&qS)[DP / 4], v4& m, v4& v) {
-  const int i = r0 + (threadIdx.x & 15), k4 = (threadIdx.x & 63) >> 4;
-  m = v4{0, 0, 0, 0}, v = m;
+struct Right {
+  Parts<3> p[DP / 32];
+};
+
+// The wave's right operands of its rows of an (m, S) pair, by f(m, S) -> the operand's value.
+template <int DP, bool VEC, typename F>
+__device__ __forceinline__ void load_right(const float* pm, const float* pS, int64_t at, int D, bool on, int k8, F&& f) {
 #pragma unroll
-  for (int s = 0; s < DP / 4; ++s) {
-    const float a = km[i][4 * s + k4], b = kS[i][4 * s + k4];
-    m = mfma(a, qm[s], m);
-    v = mfma(fmaf(a, a, b), qS[s], v);
-    v = mfma(b, qm[s] * qm[s], v);
+  for (int s = 0; s < DP / 32; ++s) {
+    float m[8], S[8];
+    load8<VEC>(pm + at, 32 * s + 8 * k8, D, on, m);
+    load8<VEC>(pS + at, 32 * s + 8 * k8, D, on, S);
+    f(s, m, S);
   }
-  m *= A.c, v *= A.c2;
+}
+
+// Moments of the scores of 16 walked rows: m = a0 b0, v = a1 b1 + a2 b2 with a0, a1, a2 the parts
+// 0, 3, 6 of the tile.
+template <int DP>
+__device__ __forceinline__ void scores(const short* tile, int kt, int lane, const Right<DP>& b0, const Right<DP>& b1,
+                                       const Right<DP>& b2, acc4& m, acc4& v) {
+  m = acc4{0, 0, 0, 0}, v = m;
+#pragma unroll
+  for (int s = 0; s < DP / 32; ++s) {
+    m = mma(left<DP>(tile, 0, kt, s, lane), b0.p[s], m);
+    v = mma(left<DP>(tile, 3, kt, s, lane), b1.p[s], v);
+    v = mma(left<DP>(tile, 6, kt, s, lane), b2.p[s], v);
+  }
 }
 
 // The sum over the four lane groups that share a column.
@@ -127,337 +209,613 @@ __device__ __forceinline__ float group_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
+// Blocks in one dimension: (split, key head, rows), the rows of one key head on one XCD where the
+// key heads divide evenly, so that their keys stay in its L2.
 struct Place {
-  int64_t b, bg, rho0;
+  int64_t b, bg, block;
   int g, split;
 };
-// Rows of late tokens first where they are the longest.
-__device__ __forceinline__ Place place(const Args& A) {
+__device__ __forceinline__ Place place(const Args& A, int64_t blocks) {
+  const int64_t BG = A.B * A.G;
+  int64_t i = blockIdx.x;
   Place p;
-  const int64_t blocks = (A.M + kRows - 1) / kRows;
-  const int64_t i = A.causal ? blocks - 1 - blockIdx.x : blockIdx.x;
-  p.rho0 = i * kRows;
-  p.bg = (int64_t)blockIdx.y;
-  p.split = blockIdx.z;
+  if (BG % 8 == 0) {
+    const int64_t x = i & 7, k = i >> 3, per = blocks * A.splits;
+    p.bg = x + 8 * (k / per);
+    i = k % per;
+  } else {
+    p.bg = i / (blocks * A.splits);
+    i -= p.bg * blocks * A.splits;
+  }
+  p.split = (int)(i / blocks);
+  p.block = i - p.split * blocks;
   p.b = p.bg / A.G;
   p.g = (int)(p.bg - p.b * A.G);
   return p;
 }
 
-template <int DP>
-__global__ void __launch_bounds__(64 * kWaves) stats_kernel(const Args A) {
-  __shared__ float km[kTile][DP + 1], kS[kTile][DP + 1];
-  const Place p = place(A);
+// ---------------------------------------------------------------------------------- forward
+// Keys (and values) of the tile from key0 on into units, and units into the tile.
+template <int DP, bool VEC, int W, int U>
+__device__ __forceinline__ void fetch_keys(const Args& A, const Place& p, int key0, int to, int pairs, int wave, int lane,
+                                           bool value_variances, Unit (&u)[U]) {
+  constexpr int S = DP / 32;
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    const int i = wave + j * W;
+    if (i >= 2 * S * pairs) continue;
+    const bool value = i >= 2 * S;
+    const int k = value ? i - 2 * S : i, kt = k / S, s = k % S, key = key0 + 16 * kt + (lane & 15);
+    const bool on = key < to;
+    const int64_t at = on ? key_at(value ? A.lv : A.lk, p.b, p.g, key) : 0;
+    const int d = 32 * s + 8 * (lane >> 4);
+    load8<VEC>((value ? A.mv : A.mk) + at, d, A.D, on, u[j].m);
+    if (!value || value_variances) load8<VEC>((value ? A.Sv : A.Sk) + at, d, A.D, on, u[j].S);
+  }
+}
+// Parts: keys k 0, k^2 3, Sk 6; values v 9, v^2 12 (, Sv 15).
+template <int DP, int W, int U>
+__device__ __forceinline__ void put_keys(short* tile, int pairs, int wave, int lane, bool value_variances,
+                                         const Unit (&u)[U]) {
+  constexpr int S = DP / 32;
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    const int i = wave + j * W;
+    if (i >= 2 * S * pairs) continue;
+    const bool value = i >= 2 * S;
+    const int k = value ? i - 2 * S : i, kt = k / S, s = k % S, first = value ? 9 : 0;
+    float x[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) x[q] = u[j].m[q] * u[j].m[q];
+    put<DP>(tile, first, kt, s, lane, split<3>(u[j].m));
+    put<DP>(tile, first + 3, kt, s, lane, split<3>(x));
+    if (!value || value_variances) put<DP>(tile, first + 6, kt, s, lane, split<3>(u[j].S));
+  }
+}
+
+// Queries on the right: q, Sq, Sq + q^2 (against k, k^2, Sk).
+template <int DP, bool VEC>
+__device__ __forceinline__ void load_queries(const Args& A, int64_t at, bool on, int k8, Right<DP>& q, Right<DP>& Q,
+                                             Right<DP>& P) {
+  load_right<DP, VEC>(A.mq, A.Sq, at, A.D, on, k8, [&](int s, float (&m)[8], float (&S)[8]) {
+    q.p[s] = split<3>(m), Q.p[s] = split<3>(S);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) S[i] = fmaf(m[i], m[i], S[i]);
+    P.p[s] = split<3>(S);
+  });
+}
+
+// Sums of the rectified moments. NC x 16 rows a wave.
+template <int DP, bool VEC, int W, int NC>
+__global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
+  constexpr int U = units_of<DP, W>(1), kRows = 16 * W;
+  typedef Tile<DP, 9> Keys;
+  extern __shared__ __align__(16) short lds[];
+  const int64_t blocks = (A.M + NC * kRows - 1) / (NC * kRows);
+  Place p = place(A, blocks);
+  if (A.causal) p.block = blocks - 1 - p.block;  // the longest rows first
   const Seq s = sequence(A, p.b);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g4 = lane >> 4;
-  const int64_t rho = p.rho0 + wave * 16 + (lane & 15);
-  const int lim = row_limit(A, s, rho);
-  float qm[DP / 4], qS[DP / 4];
-  const int64_t at = lim ? row_at(A, A.lq, p.b, p.g, rho) : 0;
-  load_right<DP>(A, A.mq, at, lim > 0, qm);
-  load_right<DP>(A, A.Sq, at, lim > 0, qS);
-  const int from = p.split * A.chunk, all = block_limit(A, s, p.rho0, kRows);
-  const int to = all < from + A.chunk ? all : from + A.chunk;
-  float mt = 0.f, vt = 0.f;
-  for (int key0 = from; key0 < to; key0 += kTile) {
-    __syncthreads();
-    stage_keys<DP>(A, A.mk, A.lk, p.b, p.g, key0, to, km);
-    stage_keys<DP>(A, A.Sk, A.lk, p.b, p.g, key0, to, kS);
-    __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k8 = lane >> 4;
+  const int64_t block0 = p.block * NC * kRows, wave0 = block0 + wave * NC * 16;
+  const int from = p.split * A.chunk;
+  auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
+  const int to = end(block_limit(A, s, block0, NC * kRows)), wave_to = end(block_limit(A, s, wave0, NC * 16));
+  if (from >= to) return;
+  Right<DP> q[NC], Q[NC], P[NC];
+  int lim[NC];
+  float mt[NC] = {}, vt[NC] = {};
 #pragma unroll
-    for (int r0 = 0; r0 < kTile; r0 += 16) {
-      v4 m, v;
-      scores<DP>(A, km, kS, r0, qm, qS, m, v);
+  for (int c = 0; c < NC; ++c) {
+    const int64_t rho = wave0 + 16 * c + (lane & 15);
+    lim[c] = row_limit(A, s, rho);
+    load_queries<DP, VEC>(A, lim[c] ? row_at(A, A.lq, p.b, p.g, rho) : 0, lim[c] > 0, k8, q[c], Q[c], P[c]);
+  }
+  Unit u[U];
+  fetch_keys<DP, VEC, W>(A, p, from, to, 1, wave, lane, false, u);
+  put_keys<DP, W>(lds, 1, wave, lane, false, u);
+  __syncthreads();
+  int buf = 0;
+  for (int key0 = from; key0 < to; key0 += kTile, buf ^= 1) {
+    const short* tile = lds + buf * Keys::halves;
+    const bool more = key0 + kTile < to;
+    if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 1, wave, lane, false, u);
+    if (key0 < wave_to) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float mm, vm, cdf;
-        rectify(m[r], v[r], mm, vm, cdf);
-        const bool seen = key0 + r0 + 4 * g4 + r < lim;
-        mt += seen ? mm : 0.f, vt += seen ? vm : 0.f;
+      for (int kt = 0; kt < 2; ++kt) {
+        acc4 m[NC], v[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) m[c] = v[c] = acc4{0, 0, 0, 0};
+#pragma unroll
+        for (int st = 0; st < DP / 32; ++st) {
+          const Parts<3> a = left<DP>(tile, 0, kt, st, lane);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) m[c] = mma(a, q[c].p[st], m[c]);
+          const Parts<3> b = left<DP>(tile, 3, kt, st, lane);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) v[c] = mma(b, Q[c].p[st], v[c]);
+          const Parts<3> d = left<DP>(tile, 6, kt, st, lane);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) v[c] = mma(d, P[c].p[st], v[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float mm, vm, cdf;
+            rectify(m[c][r] * A.c, v[c][r] * A.c2, mm, vm, cdf);
+            const bool seen = key0 + 16 * kt + 4 * k8 + r < lim[c];
+            mt[c] += seen ? mm : 0.f, vt[c] += seen ? vm : 0.f;
+          }
       }
     }
+    if (more) put_keys<DP, W>(lds + (buf ^ 1) * Keys::halves, 1, wave, lane, false, u);
+    __syncthreads();
   }
-  mt = group_sum(mt), vt = group_sum(vt);
-  if (g4 == 0 && rho < A.M) {
-    float* o = A.sums + ((int64_t)p.split * 2 * A.B * A.G + p.bg) * A.M + rho;
-    o[0] = mt, o[A.B * A.G * A.M] = vt;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const float x = group_sum(mt[c]), y = group_sum(vt[c]);
+    const int64_t rho = wave0 + 16 * c + lane;
+    if (k8 == 0 && rho < A.M) {
+      float* o = A.sums + ((int64_t)p.split * 2 * A.B * A.G + p.bg) * A.M + rho;
+      o[0] = x, o[A.B * A.G * A.M] = y;
+    }
   }
 }
 
-__device__ __forceinline__ void store_rows(const Args& A, int64_t b, int g, int64_t rho, int q, float x) {
-  const int64_t t = rho / A.R, h = g * A.R + (rho - t * A.R);
-  A.rows[((q * A.B + b) * A.H + h) * A.T + t] = x;
-}
-__device__ __forceinline__ float load_rows(const Args& A, int64_t b, int g, int64_t rho, int q) {
-  const int64_t t = rho / A.R, h = g * A.R + (rho - t * A.R);
-  return A.rows[((q * A.B + b) * A.H + h) * A.T + t];
+// The splits that reach a row, and their sums in order.
+__device__ __forceinline__ int splits_to(const Args& A, int lim) { return (lim + A.chunk - 1) / A.chunk; }
+__device__ __forceinline__ void add_sums(const Args& A, const Place& p, int64_t rho, int lim, float& mt, float& vt) {
+  const float* o = A.sums + p.bg * A.M + rho;
+  const int64_t step = A.B * A.G * A.M;
+  for (int i = 0; i < splits_to(A, lim); ++i, o += 2 * step) mt += o[0], vt += o[step];
 }
 
-template <int DP>
-__global__ void __launch_bounds__(64 * kWaves) outputs_kernel(const Args A) {
-  __shared__ float km[kTile][DP + 1], kS[kTile][DP + 1], vm_[kTile][DP + 1], vS_[kTile][DP + 1];
-  const Place p = place(A);
+template <int DP, bool VEC, int W>
+__global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
+  constexpr int U = units_of<DP, W>(2), DT = DP / 16, kRows = 16 * W;
+  typedef Tile<DP, 18> KeysValues;
+  constexpr int bufs = 2 * KeysValues::bytes <= kLdsBytes ? 2 : 1;
+  extern __shared__ __align__(16) short lds[];
+  const int64_t blocks = (A.M + kRows - 1) / kRows;
+  Place p = place(A, blocks);
+  if (A.causal) p.block = blocks - 1 - p.block;
   const Seq s = sequence(A, p.b);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g4 = lane >> 4, col = lane & 15;
-  const int64_t rho = p.rho0 + wave * 16 + col;
-  const int lim = row_limit(A, s, rho);
-  float qm[DP / 4], qS[DP / 4];
-  const int64_t at = lim ? row_at(A, A.lq, p.b, p.g, rho) : 0;
-  load_right<DP>(A, A.mq, at, lim > 0, qm);
-  load_right<DP>(A, A.Sq, at, lim > 0, qS);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k8 = lane >> 4;
+  const int64_t block0 = p.block * kRows, wave0 = block0 + wave * 16, rho = wave0 + (lane & 15);
+  const int lim = row_limit(A, s, rho), from = p.split * A.chunk;
+  auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
+  const int to = end(block_limit(A, s, block0, kRows)), wave_to = end(block_limit(A, s, wave0, 16));
+  if (from >= to && p.split > 0) return;
   float mt = 0.f, vt = 0.f;
-  if (rho < A.M) {
-    const float* o = A.sums + p.bg * A.M + rho;
-    const int64_t step = A.B * A.G * A.M;
-    for (int i = 0; i < A.splits; ++i, o += 2 * step) mt += o[0], vt += o[step];
-    if (p.split == 0 && g4 == 0) store_rows(A, p.b, p.g, rho, 0, mt), store_rows(A, p.b, p.g, rho, 1, vt);
-  }
+  if (lim) add_sums(A, p, rho, lim, mt, vt);
+  if (p.split == 0 && k8 == 0 && rho < A.M)
+    A.rows[stat_at(A, p.b, p.g, rho, 0)] = mt, A.rows[stat_at(A, p.b, p.g, rho, 1)] = vt;
   const RowSums rs = row_sums(mt, vt);
-  const int from = p.split * A.chunk, all = block_limit(A, s, p.rho0, kRows);
-  const int to = all < from + A.chunk ? all : from + A.chunk;
+  Right<DP> q, Q, P;
+  load_queries<DP, VEC>(A, lim ? row_at(A, A.lq, p.b, p.g, rho) : 0, lim > 0, k8, q, Q, P);
   float sum = 0.f;
-  v4 om[DP / 16], oS[DP / 16];
+  acc4 om[DT], oS[DT];
 #pragma unroll
-  for (int d = 0; d < DP / 16; ++d) om[d] = oS[d] = v4{0, 0, 0, 0};
+  for (int d = 0; d < DT; ++d) om[d] = oS[d] = acc4{0, 0, 0, 0};
+  Unit u[U];
+  if (from < to) {
+    fetch_keys<DP, VEC, W>(A, p, from, to, 2, wave, lane, true, u);
+    put_keys<DP, W>(lds, 2, wave, lane, true, u);
+  }
+  __syncthreads();
+  int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile) {
-    __syncthreads();
-    stage_keys<DP>(A, A.mk, A.lk, p.b, p.g, key0, to, km);
-    stage_keys<DP>(A, A.Sk, A.lk, p.b, p.g, key0, to, kS);
-    stage_keys<DP>(A, A.mv, A.lv, p.b, p.g, key0, to, vm_);
-    stage_keys<DP>(A, A.Sv, A.lv, p.b, p.g, key0, to, vS_);
-    __syncthreads();
+    const short* tile = lds + buf * KeysValues::halves;
+    const bool more = key0 + kTile < to;
+    if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, lane, true, u);
+    if (key0 < wave_to) {
+      float w[8], kw[8];
 #pragma unroll
-    for (int r0 = 0; r0 < kTile; r0 += 16) {
-      v4 m, v;
-      scores<DP>(A, km, kS, r0, qm, qS, m, v);
+      for (int kt = 0; kt < 2; ++kt) {
+        acc4 m, v;
+        scores<DP>(tile, kt, lane, q, Q, P, m, v);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float mm, vm, cdf, w, k, xw, rw;
-        rectify(m[r], v[r], mm, vm, cdf);
-        weigh(mm, vm, rs, w, k, xw, rw);
-        const int j = r0 + 4 * g4 + r;
-        w = key0 + j < lim ? w : 0.f;
-        sum += w;
-        const float w2 = w * w, kw = k * w2;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-          const float a = vm_[j][16 * d + col], b = vS_[j][16 * d + col];
-          om[d] = mfma(a, w, om[d]);
-          oS[d] = mfma(fmaf(a, a, b), kw, oS[d]);
-          oS[d] = mfma(b, w2, oS[d]);
+        for (int r = 0; r < 4; ++r) {
+          float mm, vm, cdf, x, k, xw, rw;
+          rectify(m[r] * A.c, v[r] * A.c2, mm, vm, cdf);
+          weigh(mm, vm, rs, x, k, xw, rw);
+          x = key0 + 16 * kt + 4 * k8 + r < lim ? x : 0.f;
+          sum += x;
+          w[4 * kt + r] = x, kw[4 * kt + r] = k * x * x;
         }
       }
+      {
+        const Parts<3> b = split<3>(w);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) om[d] = mma(transposed<DP>(tile, 9, d, lane), b, om[d]);
+      }
+      {
+        const Parts<3> b = split<3>(kw);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) oS[d] = mma(transposed<DP>(tile, 12, d, lane), b, oS[d]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) kw[i] = fmaf(w[i], w[i], kw[i]);
+      {
+        const Parts<3> b = split<3>(kw);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) oS[d] = mma(transposed<DP>(tile, 15, d, lane), b, oS[d]);
+      }
     }
+    if (bufs == 2) buf ^= 1;
+    if (bufs == 1) __syncthreads();
+    if (more) put_keys<DP, W>(lds + buf * KeysValues::halves, 2, wave, lane, true, u);
+    __syncthreads();
   }
   sum = group_sum(sum);
   if (rho >= A.M) return;
   if (A.splits > 1) {
     float* o = A.parts + (((int64_t)p.split * A.B * A.G + p.bg) * A.M + rho) * (2 * A.D + 1);
-    if (g4 == 0) o[2 * A.D] = sum;
+    if (k8 == 0) o[2 * A.D] = sum;
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d)
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int f = 16 * d + 4 * g4 + r;
+        const int f = 16 * d + 4 * k8 + r;
         if (f < A.D) o[f] = om[d][r], o[A.D + f] = oS[d][r];
       }
     return;
   }
-  if (g4 == 0) store_rows(A, p.b, p.g, rho, 2, sum);
+  if (k8 == 0) A.rows[stat_at(A, p.b, p.g, rho, 2)] = sum;
   const float inv = fast_rcp(fmaxf(sum, kRemaxFloor)), inv2 = inv * inv;
   const int64_t o = row_at(A, A.loq, p.b, p.g, rho);
 #pragma unroll
-  for (int d = 0; d < DP / 16; ++d)
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int f = 16 * d + 4 * g4 + r;
+      const int f = 16 * d + 4 * k8 + r;
       if (f < A.D) A.mo[o + f] = om[d][r] * inv, A.So[o + f] = oS[d][r] * inv2;
     }
 }
 
-// The splits of a row added in order; a wave to a row.
+// The splits that reach a row added in order; a wave to a row. NORM: divided by the weights' sum.
+template <bool NORM>
 __global__ void __launch_bounds__(256) join_kernel(const Args A) {
   const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (i >= A.B * A.G * A.M) return;
-  const int64_t bg = i / A.M, rho = i - bg * A.M, b = bg / A.G, step = A.B * A.G * A.M * (2 * A.D + 1);
-  const int g = (int)(bg - b * A.G), lane = threadIdx.x & 63;
-  const float* p = A.parts + i * (2 * A.D + 1);
-  float sum = 0.f;
-  for (int k = 0; k < A.splits; ++k) sum += p[k * step + 2 * A.D];
-  if (lane == 0) store_rows(A, b, g, rho, 2, sum);
-  const float inv = fast_rcp(fmaxf(sum, kRemaxFloor)), inv2 = inv * inv;
+  const int width = 2 * A.D + (NORM ? 1 : 0);
+  const int64_t bg = i / A.M, rho = i - bg * A.M, b = bg / A.G, step = A.B * A.G * A.M * width;
+  const int g = (int)(bg - b * A.G), lane = threadIdx.x & 63, n = splits_to(A, row_limit(A, sequence(A, b), rho));
+  const float* p = A.parts + i * width;
+  float inv = 1.f;
+  if constexpr (NORM) {
+    float sum = 0.f;
+    for (int k = 0; k < n; ++k) sum += p[k * step + 2 * A.D];
+    if (lane == 0) A.rows[stat_at(A, b, g, rho, 2)] = sum;
+    inv = fast_rcp(fmaxf(sum, kRemaxFloor));
+  }
   const int64_t o = row_at(A, A.loq, b, g, rho);
   for (int f = lane; f < A.D; f += 64) {
     float x = 0.f, y = 0.f;
-    for (int k = 0; k < A.splits; ++k) x += p[k * step + f], y += p[k * step + A.D + f];
-    A.mo[o + f] = x * inv, A.So[o + f] = y * inv2;
+    for (int k = 0; k < n; ++k) x += p[k * step + f], y += p[k * step + A.D + f];
+    A.mo[o + f] = x * inv, A.So[o + f] = y * (inv * inv);
   }
 }
 
+// --------------------------------------------------------------------------------- backward
 // Deltas of the queries.
-template <int DP>
-__global__ void __launch_bounds__(64 * kWaves) dq_kernel(const Args A) {
-  __shared__ float km[kTile][DP + 1], kS[kTile][DP + 1], vm_[kTile][DP + 1];
-  const Place p = place(A);
+template <int DP, bool VEC, int W>
+__global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
+  constexpr int U = units_of<DP, W>(2), DT = DP / 16, kRows = 16 * W;
+  typedef Tile<DP, 15> KeysValues;
+  constexpr int bufs = 2 * KeysValues::bytes <= kLdsBytes ? 2 : 1;
+  extern __shared__ __align__(16) short lds[];
+  const int64_t blocks = (A.M + kRows - 1) / kRows;
+  Place p = place(A, blocks);
+  if (A.causal) p.block = blocks - 1 - p.block;
   const Seq s = sequence(A, p.b);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g4 = lane >> 4, col = lane & 15;
-  const int64_t rho = p.rho0 + wave * 16 + col;
-  const int lim = row_limit(A, s, rho);
-  float qm[DP / 4], qS[DP / 4], dm[DP / 4], dS[DP / 4];
-  const int64_t at = lim ? row_at(A, A.lq, p.b, p.g, rho) : 0, dat = lim ? row_at(A, A.ld, p.b, p.g, rho) : 0;
-  load_right<DP>(A, A.mq, at, lim > 0, qm);
-  load_right<DP>(A, A.Sq, at, lim > 0, qS);
-  load_right<DP>(A, A.dm, dat, lim > 0, dm);
-  load_right<DP>(A, A.dS, dat, lim > 0, dS);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k8 = lane >> 4;
+  const int64_t block0 = p.block * kRows, wave0 = block0 + wave * 16, rho = wave0 + (lane & 15);
+  const int lim = row_limit(A, s, rho), from = p.split * A.chunk;
+  auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
+  const int to = end(block_limit(A, s, block0, kRows)), wave_to = end(block_limit(A, s, wave0, 16));
+  if (from >= to && p.split > 0) return;
   float mt = 0.f, vt = 0.f, sum = 0.f;
-  if (lim) mt = load_rows(A, p.b, p.g, rho, 0), vt = load_rows(A, p.b, p.g, rho, 1), sum = load_rows(A, p.b, p.g, rho, 2);
+  if (lim)
+    mt = A.rows[stat_at(A, p.b, p.g, rho, 0)], vt = A.rows[stat_at(A, p.b, p.g, rho, 1)],
+    sum = A.rows[stat_at(A, p.b, p.g, rho, 2)];
   const RowSums rs = row_sums(mt, vt);
   const float inv = fast_rcp(fmaxf(sum, kRemaxFloor));
-  const int to = block_limit(A, s, p.rho0, kRows);
-  v4 om[DP / 16], oS[DP / 16];
+  Right<DP> q, Q, P, dm, dS;
+  load_queries<DP, VEC>(A, lim ? row_at(A, A.lq, p.b, p.g, rho) : 0, lim > 0, k8, q, Q, P);
+  load_right<DP, VEC>(A.dm, A.dS, lim ? row_at(A, A.ld, p.b, p.g, rho) : 0, A.D, lim > 0, k8,
+                      [&](int st, float (&m)[8], float (&S)[8]) { dm.p[st] = split<3>(m), dS.p[st] = split<3>(S); });
+  acc4 om[DT], oS[DT];
 #pragma unroll
-  for (int d = 0; d < DP / 16; ++d) om[d] = oS[d] = v4{0, 0, 0, 0};
-  for (int key0 = 0; key0 < to; key0 += kTile) {
-    __syncthreads();
-    stage_keys<DP>(A, A.mk, A.lk, p.b, p.g, key0, to, km);
-    stage_keys<DP>(A, A.Sk, A.lk, p.b, p.g, key0, to, kS);
-    stage_keys<DP>(A, A.mv, A.lv, p.b, p.g, key0, to, vm_);
-    __syncthreads();
+  for (int d = 0; d < DT; ++d) om[d] = oS[d] = acc4{0, 0, 0, 0};
+  Unit u[U];
+  if (from < to) {
+    fetch_keys<DP, VEC, W>(A, p, from, to, 2, wave, lane, false, u);
+    put_keys<DP, W>(lds, 2, wave, lane, false, u);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int key0 = from; key0 < to; key0 += kTile) {
+    const short* tile = lds + buf * KeysValues::halves;
+    const bool more = key0 + kTile < to;
+    if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, lane, false, u);
+    if (key0 < wave_to) {
+      float x[8], X[8];
 #pragma unroll
-    for (int r0 = 0; r0 < kTile; r0 += 16) {
-      v4 m, v, e = {0, 0, 0, 0}, E = e;
-      scores<DP>(A, km, kS, r0, qm, qS, m, v);
+      for (int kt = 0; kt < 2; ++kt) {
+        acc4 m, v, e = {0, 0, 0, 0}, E = e;
+        scores<DP>(tile, kt, lane, q, Q, P, m, v);
 #pragma unroll
-      for (int i = 0; i < DP / 4; ++i) {
-        const float a = vm_[r0 + col][4 * i + g4];
-        e = mfma(a, dm[i], e);
-        E = mfma(a * a, dS[i], E);
-      }
+        for (int st = 0; st < DP / 32; ++st) {
+          e = mma(left<DP>(tile, 9, kt, st, lane), dm.p[st], e);
+          E = mma(left<DP>(tile, 12, kt, st, lane), dS.p[st], E);
+        }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float mm, vm, cdf, w, k, xw, rw;
-        rectify(m[r], v[r], mm, vm, cdf);
-        weigh(mm, vm, rs, w, k, xw, rw);
-        const int j = r0 + 4 * g4 + r;
-        const float J = remax_jacobian(v[r], mm, cdf, w * inv, k, xw, rw) * A.c;
-        const float x = key0 + j < lim ? e[r] * J : 0.f, X = key0 + j < lim ? E[r] * J * J : 0.f;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-          const float a = km[j][16 * d + col];
-          om[d] = mfma(a, x, om[d]);
-          oS[d] = mfma(a * a, X, oS[d]);
+        for (int r = 0; r < 4; ++r) {
+          float mm, vm, cdf, w, k, xw, rw;
+          const float var = v[r] * A.c2;
+          rectify(m[r] * A.c, var, mm, vm, cdf);
+          weigh(mm, vm, rs, w, k, xw, rw);
+          float J = remax_jacobian(var, mm, cdf, w * inv, k, xw, rw) * A.c;
+          J = key0 + 16 * kt + 4 * k8 + r < lim ? J : 0.f;
+          x[4 * kt + r] = e[r] * J, X[4 * kt + r] = E[r] * (J * J);
         }
       }
+      {
+        const Parts<3> b = split<3>(x);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) om[d] = mma(transposed<DP>(tile, 0, d, lane), b, om[d]);
+      }
+      {
+        const Parts<3> b = split<3>(X);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) oS[d] = mma(transposed<DP>(tile, 3, d, lane), b, oS[d]);
+      }
     }
+    if (bufs == 2) buf ^= 1;
+    if (bufs == 1) __syncthreads();
+    if (more) put_keys<DP, W>(lds + buf * KeysValues::halves, 2, wave, lane, false, u);
+    __syncthreads();
   }
   if (rho >= A.M) return;
-  const int64_t o = row_at(A, A.loq, p.b, p.g, rho);
+  const bool whole = A.splits == 1;
+  float* const to_m = whole ? A.mo + row_at(A, A.loq, p.b, p.g, rho)
+                            : A.parts + (((int64_t)p.split * A.B * A.G + p.bg) * A.M + rho) * (2 * A.D);
+  float* const to_S = whole ? A.So + row_at(A, A.loq, p.b, p.g, rho) : to_m + A.D;
 #pragma unroll
-  for (int d = 0; d < DP / 16; ++d)
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int f = 16 * d + 4 * g4 + r;
-      if (f < A.D) A.mo[o + f] = om[d][r], A.So[o + f] = oS[d][r];
+      const int f = 16 * d + 4 * k8 + r;
+      if (f < A.D) to_m[f] = om[d][r], to_S[f] = oS[d][r];
     }
 }
 
-// Deltas of the keys and values: a wave holds 16 keys and walks the rows that see them.
-template <int DP>
-__global__ void __launch_bounds__(64 * kWaves) dkv_kernel(const Args A) {
-  __shared__ float qm[kTile][DP + 1], qS[kTile][DP + 1], dm[kTile][DP + 1], dS[kTile][DP + 1];
-  __shared__ float stat[5][kTile];  // inv_mt, y, c_mt, 1 / s; limit
-  const int64_t bg = blockIdx.y, b = bg / A.G;
-  const int g = (int)(bg - b * A.G);
-  const Seq s = sequence(A, b);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g4 = lane >> 4, col = lane & 15;
-  const int key0 = blockIdx.x * kRows, key = key0 + wave * 16 + col;
-  float km[DP / 4], kS[DP / 4], vm_[DP / 4];
-  const bool on = key < s.len;
-  load_right<DP>(A, A.mk, b * A.lk.sb + (int64_t)key * A.lk.st + g * A.lk.sh, on, km);
-  load_right<DP>(A, A.Sk, b * A.lk.sb + (int64_t)key * A.lk.st + g * A.lk.sh, on, kS);
-  load_right<DP>(A, A.mv, b * A.lv.sb + (int64_t)key * A.lv.st + g * A.lv.sh, on, vm_);
-  v4 okm[DP / 16], okS[DP / 16], ovm[DP / 16], ovS[DP / 16];
-#pragma unroll
-  for (int d = 0; d < DP / 16; ++d) okm[d] = okS[d] = ovm[d] = ovS[d] = v4{0, 0, 0, 0};
-  // rows of positions [max(0, first key's if causal), len)
+// Rows that see a key of a block from key0 on: [first, end).
+struct RowRange {
+  int64_t first, end;
+};
+__device__ __forceinline__ RowRange rows_of(const Args& A, const Seq& s, int key0) {
+  if (key0 >= s.len) return {0, 0};
+  // positions from 0, and with causal from the first key, to the length
   int64_t first = (A.causal ? key0 : 0) - s.start, last = s.len - s.start;
   if (first < 0) first = 0;
-  if (first < -s.start) first = -s.start;
   if (last > A.T) last = A.T;
-  const int64_t end = key0 < s.len ? last * A.R : 0;
-  for (int64_t rho0 = first * A.R; rho0 < end; rho0 += kTile) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTile * DP; i += 64 * kWaves) {
-      const int r = i / DP, d = i % DP;
-      const int64_t rho = rho0 + r;
-      const bool in = rho < end && d < A.D;
-      const int64_t qa = in ? row_at(A, A.lq, b, g, rho) + d : 0, da = in ? row_at(A, A.ld, b, g, rho) + d : 0;
-      qm[r][d] = in ? A.mq[qa] : 0.f, qS[r][d] = in ? A.Sq[qa] : 0.f;
-      dm[r][d] = in ? A.dm[da] : 0.f, dS[r][d] = in ? A.dS[da] : 0.f;
+  return first < last ? RowRange{first * A.R, last * A.R} : RowRange{0, 0};
+}
+
+// Deltas of the keys and values: a wave holds 16 keys, the block walks the rows that see them.
+// Parts of a row: q 0, Sq 3, q^2 6 (against k, k^2 + Sk, Sk); dm 9, dS 12.
+template <int DP, bool VEC, int W>
+__global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
+  constexpr int S = DP / 32, U = units_of<DP, W>(2), DT = DP / 16, kKeys = 16 * W;
+  typedef Tile<DP, 15> Queries;
+  constexpr int bufs = 2 * Queries::bytes + 2 * 5 * kTile * 4 <= kLdsBytes ? 2 : 1;
+  extern __shared__ __align__(16) short lds[];
+  float* const stats = reinterpret_cast<float*>(lds + bufs * Queries::halves);  // [buffer][5][kTile]
+  const Place p = place(A, (A.N + kKeys - 1) / kKeys);
+  const Seq s = sequence(A, p.b);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k8 = lane >> 4;
+  const int key0 = (int)p.block * kKeys, wave_key = key0 + wave * 16, key = wave_key + (lane & 15);
+  const RowRange all = rows_of(A, s, key0), mine = rows_of(A, s, wave_key);
+  const int64_t chunk0 = (int64_t)p.split * A.chunk, chunk1 = chunk0 + A.chunk;
+  const int64_t from = all.first > chunk0 ? all.first : chunk0, to = all.end < chunk1 ? all.end : chunk1;
+  if (from >= to && A.splits > 1) return;
+  const bool on = key < s.len;
+  Right<DP> k, K, Sk, vm, vv;
+  load_right<DP, VEC>(A.mk, A.Sk, on ? key_at(A.lk, p.b, p.g, key) : 0, A.D, on, k8,
+                      [&](int st, float (&m)[8], float (&x)[8]) {
+                        k.p[st] = split<3>(m), Sk.p[st] = split<3>(x);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = fmaf(m[i], m[i], x[i]);
+                        K.p[st] = split<3>(x);
+                      });
+  load_right<DP, VEC>(A.mv, A.mv, on ? key_at(A.lv, p.b, p.g, key) : 0, A.D, on, k8,
+                      [&](int st, float (&m)[8], float (&x)[8]) {
+                        vm.p[st] = split<3>(m);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] *= x[i];
+                        vv.p[st] = split<3>(x);
+                      });
+  acc4 okm[DT], okS[DT], ovm[DT], ovS[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) okm[d] = okS[d] = ovm[d] = ovS[d] = acc4{0, 0, 0, 0};
+  Unit u[U];
+  float st3[3];
+  int st_lim = 0;
+  auto fetch = [&](int64_t rho0) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = wave + j * W;
+      if (i >= 4 * S) continue;
+      const bool delta = i >= 2 * S;
+      const int n = delta ? i - 2 * S : i, kt = n / S, st = n % S;
+      const int64_t rho = rho0 + 16 * kt + (lane & 15);
+      const bool in = rho < to;
+      const int64_t at = in ? row_at(A, delta ? A.ld : A.lq, p.b, p.g, rho) : 0;
+      load8<VEC>((delta ? A.dm : A.mq) + at, 32 * st + 8 * k8, A.D, in, u[j].m);
+      load8<VEC>((delta ? A.dS : A.Sq) + at, 32 * st + 8 * k8, A.D, in, u[j].S);
     }
     if (threadIdx.x < kTile) {
       const int64_t rho = rho0 + threadIdx.x;
-      const int lim = rho < end ? row_limit(A, s, rho) : 0;
-      float mt = 0.f, vt = 0.f, sum = 0.f;
-      if (lim) mt = load_rows(A, b, g, rho, 0), vt = load_rows(A, b, g, rho, 1), sum = load_rows(A, b, g, rho, 2);
-      const RowSums rs = row_sums(mt, vt);
-      stat[0][threadIdx.x] = rs.inv_mt, stat[1][threadIdx.x] = rs.y, stat[2][threadIdx.x] = rs.c_mt;
-      stat[3][threadIdx.x] = fast_rcp(fmaxf(sum, kRemaxFloor));
-      stat[4][threadIdx.x] = __int_as_float(lim);
+      st_lim = rho < to ? row_limit(A, s, rho) : 0;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) st3[i] = st_lim ? A.rows[stat_at(A, p.b, p.g, rho, i)] : 0.f;
     }
-    __syncthreads();
+  };
+  auto store = [&](int buf) {
+    short* tile = lds + buf * Queries::halves;
 #pragma unroll
-    for (int r0 = 0; r0 < kTile; r0 += 16) {
-      v4 m = {0, 0, 0, 0}, v = m, e = m, E = m;
+    for (int j = 0; j < U; ++j) {
+      const int i = wave + j * W;
+      if (i >= 4 * S) continue;
+      const bool delta = i >= 2 * S;
+      const int n = delta ? i - 2 * S : i, kt = n / S, st = n % S, first = delta ? 9 : 0;
+      put<DP>(tile, first, kt, st, lane, split<3>(u[j].m));
+      put<DP>(tile, first + 3, kt, st, lane, split<3>(u[j].S));
+      if (!delta) {
+        float x[8];
 #pragma unroll
-      for (int i = 0; i < DP / 4; ++i) {
-        const float a = qm[r0 + col][4 * i + g4], c = qS[r0 + col][4 * i + g4];
-        m = mfma(a, km[i], m);
-        v = mfma(c, fmaf(km[i], km[i], kS[i]), v);
-        v = mfma(a * a, kS[i], v);
-        e = mfma(dm[r0 + col][4 * i + g4], vm_[i], e);
-        E = mfma(dS[r0 + col][4 * i + g4], vm_[i] * vm_[i], E);
+        for (int e = 0; e < 8; ++e) x[e] = u[j].m[e] * u[j].m[e];
+        put<DP>(tile, 6, kt, st, lane, split<3>(x));
       }
-      m *= A.c, v *= A.c2;
+    }
+    if (threadIdx.x < kTile) {
+      const RowSums r = row_sums(st3[0], st3[1]);
+      float* o = stats + buf * 5 * kTile + threadIdx.x;
+      o[0] = r.inv_mt, o[kTile] = r.y, o[2 * kTile] = r.c_mt;
+      o[3 * kTile] = fast_rcp(fmaxf(st3[2], kRemaxFloor));
+      o[4 * kTile] = __int_as_float(st_lim);
+    }
+  };
+  if (from < to) fetch(from), store(0);
+  __syncthreads();
+  int buf = 0;
+  for (int64_t rho0 = from; rho0 < to; rho0 += kTile) {
+    const short* tile = lds + buf * Queries::halves;
+    const float* st = stats + buf * 5 * kTile;
+    const bool more = rho0 + kTile < to;
+    if (more) fetch(rho0 + kTile);
+    if (wave_key < s.len && rho0 + kTile > mine.first) {
+      float a[8], x[8], X[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = r0 + 4 * g4 + r;
-        const RowSums rs{stat[0][j], stat[1][j], stat[2][j]};
-        float mm, vm, cdf, w, k, xw, rw;
-        rectify(m[r], v[r], mm, vm, cdf);
-        weigh(mm, vm, rs, w, k, xw, rw);
-        const bool seen = key < __float_as_int(stat[4][j]);
-        const float a = seen ? w * stat[3][j] : 0.f, a2 = a * a;
-        const float J = remax_jacobian(v[r], mm, cdf, w * stat[3][j], k, xw, rw) * A.c;
-        const float x = seen ? e[r] * J : 0.f, X = seen ? E[r] * J * J : 0.f;
+      for (int kt = 0; kt < 2; ++kt) {
+        acc4 m, v, e = {0, 0, 0, 0}, E = e;
+        scores<DP>(tile, kt, lane, k, K, Sk, m, v);
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-          const float q = qm[j][16 * d + col];
-          okm[d] = mfma(q, x, okm[d]);
-          okS[d] = mfma(q * q, X, okS[d]);
-          ovm[d] = mfma(dm[j][16 * d + col], a, ovm[d]);
-          ovS[d] = mfma(dS[j][16 * d + col], a2, ovS[d]);
+        for (int i = 0; i < S; ++i) {
+          e = mma(left<DP>(tile, 9, kt, i, lane), vm.p[i], e);
+          E = mma(left<DP>(tile, 12, kt, i, lane), vv.p[i], E);
+        }
+        const int j = 16 * kt + 4 * k8;
+        const acc4 inv_mt = *reinterpret_cast<const acc4*>(st + j), y = *reinterpret_cast<const acc4*>(st + kTile + j),
+                   c_mt = *reinterpret_cast<const acc4*>(st + 2 * kTile + j),
+                   inv = *reinterpret_cast<const acc4*>(st + 3 * kTile + j),
+                   lims = *reinterpret_cast<const acc4*>(st + 4 * kTile + j);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const RowSums rs{inv_mt[r], y[r], c_mt[r]};
+          float mm, vmo, cdf, w, kk, xw, rw;
+          const float var = v[r] * A.c2;
+          rectify(m[r] * A.c, var, mm, vmo, cdf);
+          weigh(mm, vmo, rs, w, kk, xw, rw);
+          w *= inv[r];
+          float J = remax_jacobian(var, mm, cdf, w, kk, xw, rw) * A.c;
+          const bool seen = key < __float_as_int(lims[r]);
+          J = seen ? J : 0.f;
+          a[4 * kt + r] = seen ? w : 0.f;
+          x[4 * kt + r] = e[r] * J, X[4 * kt + r] = E[r] * (J * J);
         }
       }
+      {
+        const Parts<3> b = split<3>(x);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) okm[d] = mma(transposed<DP>(tile, 0, d, lane), b, okm[d]);
+      }
+      {
+        const Parts<3> b = split<3>(X);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) okS[d] = mma(transposed<DP>(tile, 6, d, lane), b, okS[d]);
+      }
+      {
+        const Parts<3> b = split<3>(a);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) ovm[d] = mma(transposed<DP>(tile, 9, d, lane), b, ovm[d]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] *= a[i];
+      {
+        const Parts<3> b = split<3>(a);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) ovS[d] = mma(transposed<DP>(tile, 12, d, lane), b, ovS[d]);
+      }
     }
+    if (bufs == 2) buf ^= 1;
+    if (bufs == 1) __syncthreads();
+    if (more) store(buf);
+    __syncthreads();
   }
   if (key >= A.N) return;
-  const int64_t o = b * A.lokv.sb + (int64_t)key * A.lokv.st + g * A.lokv.sh;
+  const bool whole = A.splits == 1;
+  float* out[4] = {A.dmk, A.dSk, A.dmv, A.dSv};
+  const int64_t at = whole ? key_at(A.lokv, p.b, p.g, key) : (((int64_t)p.split * A.B * A.G + p.bg) * A.N + key) * (4 * A.D);
 #pragma unroll
-  for (int d = 0; d < DP / 16; ++d)
+  for (int i = 0; i < 4; ++i) {
+    float* const o = (whole ? out[i] : A.parts + i * A.D) + at;
+    const acc4* x = i == 0 ? okm : (i == 1 ? okS : (i == 2 ? ovm : ovS));
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int f = 16 * d + 4 * g4 + r;
-      if (f < A.D)
-        A.dmk[o + f] = okm[d][r], A.dSk[o + f] = okS[d][r], A.dmv[o + f] = ovm[d][r], A.dSv[o + f] = ovS[d][r];
-    }
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int f = 16 * d + 4 * k8 + r;
+        if (f < A.D) o[f] = x[d][r];
+      }
+  }
 }
 
-int splits_of(int64_t B, int64_t T, int64_t N, int64_t H, int64_t G) {
-  const int64_t blocks = cdiv(T * (H / G), kRows) * B * G;
-  int64_t s = cdiv(1024, blocks);
-  if (s > cdiv(N, 256)) s = cdiv(N, 256);
-  return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+// The splits of rows that reach a key, in order; a wave to a key. kv_keys: keys of a dkv block.
+__global__ void __launch_bounds__(256) join_keys_kernel(const Args A, int kv_keys) {
+  const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (i >= A.B * A.G * A.N) return;
+  const int64_t bg = i / A.N, b = bg / A.G, step = A.B * A.G * A.N * (4 * A.D);
+  const int key = (int)(i - bg * A.N), g = (int)(bg - b * A.G);
+  const RowRange r = rows_of(A, sequence(A, b), key / kv_keys * kv_keys);
+  const int k0 = (int)(r.first / A.chunk), k1 = (int)((r.end + A.chunk - 1) / A.chunk);
+  const float* p = A.parts + i * (4 * A.D);
+  const int64_t o = key_at(A.lokv, b, g, key);
+  for (int f = threadIdx.x & 63; f < 4 * A.D; f += 64) {
+    float x = 0.f;
+    if (r.first < r.end)
+      for (int k = k0; k < k1; ++k) x += p[k * step + f];
+    const int q = f / A.D;
+    float* out = q == 0 ? A.dmk : (q == 1 ? A.dSk : (q == 2 ? A.dmv : A.dSv));
+    out[o + f - q * A.D] = x;
+  }
+}
+
+// ------------------------------------------------------------------------------------ plans
+constexpr int kStatsWaves = 8, kOutWaves = 8;
+// Waves of a backward block. Five right operands of 128 features take 240 registers: one wave a SIMD.
+template <int DP>
+constexpr int back_waves() {
+  return DP == 128 ? 4 : 8;
+}
+int padded(int64_t D) { return D <= 32 ? 32 : (D <= 64 ? 64 : 128); }
+int back_rows(int64_t D) { return 16 * (padded(D) == 128 ? 4 : 8); }
+
+// Splits of `walked` for blocks of `rows` of `own` on each of BG key heads: as many as fill the
+// GPU three times over, at least 256 walked each and at most kMostWalked.
+struct Splits {
+  int n, chunk;
+};
+Splits splits_of(int64_t own, int64_t rows, int64_t BG, int64_t walked) {
+  const int64_t blocks = cdiv(own, rows) * BG;
+  int64_t n = cdiv(768, blocks < 1 ? 1 : blocks);
+  if (n > cdiv(walked, 256)) n = cdiv(walked, 256);
+  if (n < cdiv(walked, kMostWalked)) n = cdiv(walked, kMostWalked);
+  if (n < 1) n = 1;
+  const int64_t chunk = cdiv(cdiv(walked, n), kTile) * kTile;
+  return {(int)n, (int)(chunk < kTile ? kTile : chunk)};
 }
 
 int check_sizes(const char* what, int64_t B, int64_t T, int64_t N, int64_t H, int64_t G, int64_t D) {
@@ -467,20 +825,69 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t N, int64_t H, in
                    T * (H / G) < (1ll << 30), "%s: too large", what);
   return TAGI_OK;
 }
-int64_t part_floats(int64_t B, int64_t G, int64_t M, int64_t D, int splits) {
-  return splits > 1 ? splits * B * G * M * (2 * D + 1) : 0;
+
+// 1-D launches of blocks * splits on every key head: fewer than 2^32 threads.
+int grid_of(const char* what, int64_t own, int64_t rows, int64_t BG, int splits, int threads, dim3* grid) {
+  const int64_t n = cdiv(own, rows) * BG * splits;
+  TAGI_REQUIRE(n * threads < (1ll << 32), "%s: too large", what);
+  *grid = dim3((unsigned)n);
+  return TAGI_OK;
+}
+dim3 join_grid(int64_t rows) {
+  const int64_t blocks = cdiv(rows, 4), x = blocks < (1 << 20) ? blocks : (1 << 20);
+  return dim3((unsigned)x, (unsigned)cdiv(blocks, x));
+}
+template <typename K>
+void go(K kernel, dim3 grid, int threads, int lds, hipStream_t s, const Args& a) {
+  if (lds > 64 * 1024)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, s, a);
+}
+constexpr int two_or_one(int bytes, int more) { return (2 * (bytes + more) <= kLdsBytes ? 2 : 1) * (bytes + more); }
+
+template <int DP, bool VEC>
+int forward(const char* what, Args a, hipStream_t s) {
+  const int64_t BG = a.B * a.G;
+  constexpr int NC = DP == 128 ? 1 : 2;
+  dim3 grid;
+  if (int rc = grid_of(what, a.M, 16 * kStatsWaves * NC, BG, a.splits, 64 * kStatsWaves, &grid)) return rc;
+  dim3 out;
+  if (int rc = grid_of(what, a.M, 16 * kOutWaves, BG, a.splits, 64 * kOutWaves, &out)) return rc;
+  go(stats_kernel<DP, VEC, kStatsWaves, NC>, grid, 64 * kStatsWaves, 2 * Tile<DP, 9>::bytes, s, a);
+  go(outputs_kernel<DP, VEC, kOutWaves>, out, 64 * kOutWaves, two_or_one(Tile<DP, 18>::bytes, 0), s, a);
+  if (a.splits > 1) hipLaunchKernelGGL(join_kernel<true>, join_grid(BG * a.M), dim3(256), 0, s, a);
+  return TAGI_OK;
+}
+template <int DP, bool VEC>
+int backward(const char* what, Args a, float* ws, hipStream_t s) {
+  const int64_t BG = a.B * a.G;
+  constexpr int W = back_waves<DP>(), rows = 16 * W;
+  if (a.T) {
+    const Splits sp = splits_of(a.M, rows, BG, a.N);
+    a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;
+    dim3 grid;
+    if (int rc = grid_of(what, a.M, rows, BG, sp.n, 64 * W, &grid)) return rc;
+    go(dq_kernel<DP, VEC, W>, grid, 64 * W, two_or_one(Tile<DP, 15>::bytes, 0), s, a);
+    if (sp.n > 1) hipLaunchKernelGGL(join_kernel<false>, join_grid(BG * a.M), dim3(256), 0, s, a);
+  }
+  if (a.N) {
+    const Splits sp = splits_of(a.N, rows, BG, a.M);
+    a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;  // the stream's order keeps the joins apart
+    dim3 grid;
+    if (int rc = grid_of(what, a.N, rows, BG, sp.n, 64 * W, &grid)) return rc;
+    go(dkv_kernel<DP, VEC, W>, grid, 64 * W, two_or_one(Tile<DP, 15>::bytes, 5 * kTile * 4), s, a);
+    if (sp.n > 1) hipLaunchKernelGGL(join_keys_kernel, join_grid(BG * a.N), dim3(256), 0, s, a, rows);
+  }
+  return TAGI_OK;
 }
 
-#define BY_DIM(kernel, grid)                                                       \
-  do {                                                                             \
-    const dim3 threads(64 * kWaves);                                               \
-    if (D <= 32)                                                                   \
-      hipLaunchKernelGGL(kernel<32>, grid, threads, 0, s, a);                      \
-    else if (D <= 64)                                                              \
-      hipLaunchKernelGGL(kernel<64>, grid, threads, 0, s, a);                      \
-    else                                                                           \
-      hipLaunchKernelGGL(kernel<128>, grid, threads, 0, s, a);                     \
-  } while (0)
+// rows of whole groups of eight features
+bool vec8(int64_t D) { return D % 8 == 0; }
+#define BY_DIM(run, ...)                                                                   \
+  (vec8(D) ? (D <= 32 ? run<32, true>(__VA_ARGS__) : (D <= 64 ? run<64, true>(__VA_ARGS__)    \
+                                                              : run<128, true>(__VA_ARGS__))) \
+           : (D <= 32 ? run<32, false>(__VA_ARGS__) : (D <= 64 ? run<64, false>(__VA_ARGS__)  \
+                                                               : run<128, false>(__VA_ARGS__))))
 
 }  // namespace
 }  // namespace tagi
@@ -490,8 +897,8 @@ using namespace tagi;
 extern "C" int64_t tagi_remax_attention_fwd_ws_bytes(int64_t B, int64_t T, int64_t N, int64_t H, int64_t G,
                                                      int64_t D) {
   if (B <= 0 || T <= 0 || N < 0 || H <= 0 || G <= 0 || D <= 0 || H % G) return 0;
-  const int splits = splits_of(B, T, N, H, G);
-  return 4 * (2 * splits * B * H * T + part_floats(B, G, T * (H / G), D, splits));
+  const Splits sp = splits_of(T * (H / G), 16 * kOutWaves, B * G, N);
+  return 4 * B * H * T * sp.n * (2 + (sp.n > 1 ? 2 * D + 1 : 0));
 }
 
 extern "C" int tagi_remax_attention_fwd(const float* mq, const float* Sq, const tagi_heads* lq, const float* mk,
@@ -518,20 +925,21 @@ extern "C" int tagi_remax_attention_fwd(const float* mq, const float* Sq, const 
   a.mo = mo, a.So = So, a.rows = rows, a.loq = tagi_heads{T * H * D, H * D, D};
   a.B = B, a.T = (int)T, a.N = (int)N, a.H = (int)H, a.G = (int)G, a.R = (int)(H / G), a.D = (int)D, a.M = T * (H / G);
   a.c = (float)scale, a.c2 = (float)(scale * scale);
-  a.splits = splits_of(B, T, N, H, G);
-  a.chunk = (int)(cdiv(cdiv(N, a.splits), kTile) * kTile);
+  const Splits sp = splits_of(a.M, 16 * kOutWaves, B * G, N);
+  a.splits = sp.n, a.chunk = sp.chunk;
   a.sums = static_cast<float*>(ws), a.parts = a.sums + 2 * a.splits * B * H * T;
-  const dim3 grid((unsigned)cdiv(a.M, kRows), (unsigned)(B * G), (unsigned)a.splits);
-  BY_DIM(stats_kernel, grid);
-  BY_DIM(outputs_kernel, grid);
-  if (a.splits > 1) {
-    const int64_t blocks = cdiv(B * G * a.M, 4), x = blocks < (1 << 20) ? blocks : (1 << 20);
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)x, (unsigned)cdiv(blocks, x)), dim3(256), 0, s, a);
-  }
+  if (int rc = BY_DIM(forward, what, a, s)) return rc;
   return check_launch(what);
 }
 
-extern "C" int64_t tagi_remax_attention_bwd_ws_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+extern "C" int64_t tagi_remax_attention_bwd_ws_bytes(int64_t B, int64_t T, int64_t N, int64_t H, int64_t G,
+                                                     int64_t D) {
+  if (B <= 0 || T < 0 || N < 0 || H <= 0 || G <= 0 || D <= 0 || H % G) return 0;
+  const int64_t M = T * (H / G), rows = back_rows(D);
+  const int q = splits_of(M, rows, B * G, N).n, kv = splits_of(N, rows, B * G, M).n;
+  const int64_t a = q > 1 ? q * B * G * M * 2 * D : 0, b = kv > 1 ? kv * B * G * N * 4 * D : 0;
+  return 4 * (a > b ? a : b);
+}
 
 extern "C" int tagi_remax_attention_bwd(const float* mq, const float* Sq, const tagi_heads* lq, const float* mk,
                                         const float* Sk, const tagi_heads* lk, const float* mv, const tagi_heads* lv,
@@ -548,7 +956,8 @@ extern "C" int tagi_remax_attention_bwd(const float* mq, const float* Sq, const 
   TAGI_REQUIRE(N == 0 || (mk && Sk && lk && mv && lv && dmk && dSk && dmv && dSv && ldkv), "%s: null pointer", what);
   TAGI_REQUIRE(!lengths || len_bytes == 4 || len_bytes == 8, "%s: lengths are int32 or int64", what);
   TAGI_REQUIRE(!starts || start_bytes == 4 || start_bytes == 8, "%s: starts are int32 or int64", what);
-  (void)ws, (void)ws_bytes;
+  const int64_t need = tagi_remax_attention_bwd_ws_bytes(B, T, N, H, G, D);
+  TAGI_REQUIRE(need == 0 || (ws && ws_bytes >= need), "%s: workspace too small", what);
   hipStream_t s = (hipStream_t)stream;
   ProfScope ps(FAM_ATTN_SCORES, s, 28.0 * B * H * T * N * D * (causal && T == N ? 0.5 : 1.0),
                D * B * (24.0 * T * H + 28.0 * N * G));
@@ -560,14 +969,6 @@ extern "C" int tagi_remax_attention_bwd(const float* mq, const float* Sq, const 
   a.mo = dmq, a.So = dSq, a.rows = const_cast<float*>(rows), a.dmk = dmk, a.dSk = dSk, a.dmv = dmv, a.dSv = dSv;
   a.B = B, a.T = (int)T, a.N = (int)N, a.H = (int)H, a.G = (int)G, a.R = (int)(H / G), a.D = (int)D, a.M = T * (H / G);
   a.c = (float)scale, a.c2 = (float)(scale * scale);
-  a.splits = 1;
-  if (T) {
-    const dim3 grid((unsigned)cdiv(a.M, kRows), (unsigned)(B * G));
-    BY_DIM(dq_kernel, grid);
-  }
-  if (N) {
-    const dim3 grid((unsigned)cdiv(N, kRows), (unsigned)(B * G));
-    BY_DIM(dkv_kernel, grid);
-  }
+  if (int rc = BY_DIM(backward, what, a, static_cast<float*>(ws), s)) return rc;
   return check_launch(what);
 }
