@@ -1,4 +1,4 @@
-"""Coefficients of the lower tail's Mills ratio R(a) and of 1 - a R(a) in tagi_remax.h.
+"""Coefficients of the lower tail's Mills ratio R(a) and of 1 - a R(a) in tagi_remax.h, both over sqrt(2 pi).
 
 Both are fitted as t p(t) and t^2 q(t) in t = 1 / (1 + a / 4) over 0 <= a <= 9 by least squares
 whose weights are raised where the relative error is largest (Lawson's iteration, towards the
@@ -37,7 +37,9 @@ def fit(fn, power):
 
 
 if __name__ == "__main__":
-    for name, fn, power in (("R / t", mills, 1), ("(1 - a R) / t^2", lambda a: 1 - a * mills(a), 2)):
+    density = 1 / np.sqrt(2 * np.pi)
+    for name, fn, power in (("R / t", lambda a: density * mills(a), 1),
+                            ("(1 - a R) / t^2", lambda a: density * (1 - a * mills(a)), 2)):
         c, error = fit(fn, power)
         print(f"{name}: relative error {error:.1e}")
         print("  " + ", ".join(f"{a:.9e}f" for a in c[::-1]))

@@ -8,79 +8,93 @@
 // (the second line from the first by z = m + ...: no side subtracts near values but R - x(1 - xR),
 // which loses x^2 / 2 of R's rounding; 3e-6 of the variance at x = 4, where the weight is 1e-5 of
 // its row). R and 1 - x R are polynomials in t = 1 / (1 + x / 4) (gen_tail_fit.py: relative error
-// 1.3e-8 and 2.3e-8, in fp32 4e-7 and 7e-7), so the two tails and both signs run without a branch.
+// 1.3e-8 and 2.3e-8, in fp32 4e-7 and 7e-7), so the two tails and both signs run without a branch:
+// the vector ALUs bound the attention kernels, and this is half of their work.
 #pragma once
 #include "tagi_moments.h"
 
 namespace tagi {
 
 constexpr float kRemaxFloor = 1e-6f;  // of means, variances, weights and their sums
-constexpr float kVarFloor = 1e-20f;   // of a score's variance
+constexpr float kVarFloor = 1e-20f;   // of a score's variance: a stays finite for means up to 1e28
 
-// In: a score's moments. Out: floored moments of max(z, 0) and Phi.
-__device__ __forceinline__ void rectify(float m, float v, float& mm, float& vm, float& cdf) {
+struct Rectified {
+  float mm, vm;   // moments of max(z, 0), floored
+  float cdf, rs;  // Phi(a), 1 / sqrt(v)
+};
+__device__ __forceinline__ Rectified rectify(float m, float v) {
+  Rectified o;
   v = fmaxf(v, kVarFloor);
-  const float rs = fast_rsqrt(v), sd = v * rs, a = m * rs;
-  const float x = fminf(fabsf(a), 1e4f);  // its square stays finite
+  o.rs = fast_rsqrt(v);
+  const float sd = v * o.rs, a = m * o.rs, x = fabsf(a);
   const float t = fast_rcp(fmaf(0.25f, x, 1.0f));
-  float p = 8.162231129e-02f;
-  p = fmaf(p, t, -4.702841742e-01f);
-  p = fmaf(p, t, 9.322739078e-01f);
-  p = fmaf(p, t, -7.467720368e-01f);
-  p = fmaf(p, t, 6.768747605e-01f);
-  p = fmaf(p, t, 3.456174901e-03f);
-  p = fmaf(p, t, 2.822860731e-01f);
-  p = fmaf(p, t, 2.434708960e-01f);
-  p = fmaf(p, t, 2.503862088e-01f);
-  float u = 2.179881536e-01f;
-  u = fmaf(u, t, -1.113959958e+00f);
-  u = fmaf(u, t, 2.007446407e+00f);
-  u = fmaf(u, t, -1.577014472e+00f);
-  u = fmaf(u, t, 1.186129971e+00f);
-  u = fmaf(u, t, -1.551880686e-01f);
-  u = fmaf(u, t, 2.570016636e-01f);
-  u = fmaf(u, t, 1.145055705e-01f);
-  u = fmaf(u, t, 6.309070943e-02f);
-  const float R = p * t, u1 = u * t * t;
-  // exp(-x^2 / 2): the exponent's rounding is x^2 2^-25 of the value, as that of x itself
-  const float pdf = INV_SQRT_2PI * __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
-  const float f = pdf * u1, q = pdf * fmaf(-x, u1, R), tail = pdf * R;
+  float p = 3.256259095e-02f;  // R / (t sqrt(2 pi))
+  p = fmaf(p, t, -1.876162406e-01f);
+  p = fmaf(p, t, 3.719234782e-01f);
+  p = fmaf(p, t, -2.979189386e-01f);
+  p = fmaf(p, t, 2.700339600e-01f);
+  p = fmaf(p, t, 1.378814559e-03f);
+  p = fmaf(p, t, 1.126158497e-01f);
+  p = fmaf(p, t, 9.713083447e-02f);
+  p = fmaf(p, t, 9.988964513e-02f);
+  float u = 8.696469113e-02f;  // (1 - x R) / (t^2 sqrt(2 pi))
+  u = fmaf(u, t, -4.444057261e-01f);
+  u = fmaf(u, t, 8.008552477e-01f);
+  u = fmaf(u, t, -6.291377500e-01f);
+  u = fmaf(u, t, 4.731973958e-01f);
+  u = fmaf(u, t, -6.191108207e-02f);
+  u = fmaf(u, t, 1.025288298e-01f);
+  u = fmaf(u, t, 4.568111342e-02f);
+  u = fmaf(u, t, 2.516955149e-02f);
+  // exp(-x^2 / 2) t: the exponent's rounding is x^2 2^-25 of the value, as that of x itself
+  const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f) * t, ut = u * t;
+  const float f = e * ut, q = e * fmaf(-x, ut, p), tail = e * p;
   const bool up = a >= 0.0f;
   const float mean = fmaf(sd, f, fmaxf(m, 0.0f));
-  const float var = fmaf(-f, f, up ? fmaf(-2.0f * x, f, 1.0f - q) : q);
-  cdf = up ? 1.0f - tail : tail;
-  mm = fmaxf(mean, kRemaxFloor);
-  // where the floor lifts the mean, the variance is taken about the lifted one (as rect_moments)
-  vm = fmaxf(fmaf(mean - mm, fmaf(-2.0f, m, mean + mm), v * var), kRemaxFloor);
+  const float var = fmaf(-f, f, up ? 1.0f - fmaf(2.0f * x, f, q) : q);
+  o.cdf = up ? 1.0f - tail : tail;
+  o.mm = fmaxf(mean, kRemaxFloor);
+  // where the floor lifts the mean by d, the variance is taken about the lifted one: less 2 d (mm -
+  // m) and d^2, of which 2 d mm and d^2 are below 2e-6 of the variance's own floor
+  o.vm = fmaxf(fmaf(-2.0f * m, mean - o.mm, v * var), kRemaxFloor);
+  return o;
 }
 
 // A row's sums of mm and vm, as the weights use them.
 struct RowSums {
-  float inv_mt, y, c_mt;
+  float inv_mt, y, y1, c_mt;  // 1 / mt, vt / mt^2, 1 + y, y1 / mt
 };
 __device__ __forceinline__ RowSums row_sums(float mt, float vt) {
   RowSums r;
   r.inv_mt = fast_rcp(fmaxf(mt, kRemaxFloor));
   r.y = fmaxf(vt, kRemaxFloor) * r.inv_mt * r.inv_mt;
-  r.c_mt = r.inv_mt * (1.0f + r.y);
+  r.y1 = 1.0f + r.y;
+  r.c_mt = r.inv_mt * r.y1;
   return r;
 }
 
-// A score's weight before its row's normalisation, w, and its variance over w^2 (k = num rw^2);
-// xw, rw feed the Jacobian (the log-normal stage in closed form, as remax_row).
-__device__ __forceinline__ void weigh(float mm, float vm, const RowSums& r, float& w, float& k, float& xw, float& rw) {
-  const float rm = fast_rcp(mm), vr = vm * rm, x = vr * rm, ww = vr * r.inv_mt;
-  rw = fast_rcp(1.0f + ww);
-  w = fmaxf(mm * r.c_mt * rw, kRemaxFloor);
-  xw = x - ww;
-  k = fmaxf((xw + (r.y - ww)) + fmaf(x, r.y, -(ww * ww)), 0.0f) * rw * rw;
+// A score's weight before its row's normalisation and the weight's relative variance: the
+// log-normal stage in closed form (remax_row) with x = vm / mm^2 and w = vm / (mm mt) multiplied out,
+//   weight = mm c_mt / (1 + w) = mm^2 c_mt / d,  d = mm + s,  s = vm / mt
+//   k = [(1 + x)(1 + y) - (1 + w)^2] / (1 + w)^2 = [vm (1 + y) + y mm^2 - s (mm + d)] / d^2
+struct Weight {
+  float w, k, rd;  // rd = 1 / d
+};
+__device__ __forceinline__ Weight weigh(const Rectified& z, const RowSums& r) {
+  Weight o;
+  const float s = z.vm * r.inv_mt, d = z.mm + s;
+  o.rd = fast_rcp(d);
+  o.w = fmaxf(z.mm * o.rd * z.mm * r.c_mt, kRemaxFloor);
+  const float num = fmaf(-s, z.mm + d, fmaf(r.y, z.mm * z.mm, z.vm * r.y1));
+  o.k = fmaxf(num, 0.0f) * o.rd * o.rd;
+  return o;
 }
 
-// J = cov(weight, z) / v of the normalised weight mua.
-__device__ __forceinline__ float remax_jacobian(float v, float mm, float cdf, float mua, float k, float xw, float rw) {
-  v = fmaxf(v, kVarFloor);
-  const float cov = fmaxf(xw, 0.0f) * rw * mua * mm * fast_rcp(fmaxf(cdf, kRemaxFloor));
-  return fminf(__builtin_amdgcn_sqrtf(k * mua * mua * v), cov) * fast_rcp(v);
+// J = cov(weight, z) / v of the normalised weight a: a times the lesser of sqrt(k / v) and
+// (x - w) / (1 + w) mm / (Phi v), (x - w) / (1 + w) mm = vm (1 - mm / mt) / d.
+__device__ __forceinline__ float remax_jacobian(const Rectified& z, const Weight& w, float a, const RowSums& r) {
+  const float cov = fmaxf(fmaf(-z.mm, r.inv_mt, 1.0f), 0.0f) * (z.vm * w.rd) * fast_rcp(fmaxf(z.cdf, kRemaxFloor));
+  return a * z.rs * fminf(__builtin_amdgcn_sqrtf(w.k), cov * z.rs);
 }
 
 }  // namespace tagi

@@ -111,6 +111,15 @@ __device__ __forceinline__ void load8(const float* p, int d, int D, bool on, flo
   }
 }
 
+// The block's wave, in a scalar register.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+// x, of which the compiler knows nothing: what a tile's addresses need of it is formed in every
+// tile and not kept in registers across them.
+__device__ __forceinline__ int hidden(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // ------------------------------------------------------------------------ walked tiles in LDS
 // A tile is kTile rows of operands in bf16 parts, [part][16 rows][32 features] in the order in
 // which a wave's lanes read a left operand: lane l the row l % 16, features 8 (l / 16) + 0..7.
@@ -129,36 +138,40 @@ __device__ __forceinline__ void put(short* tile, int first, int kt, int s, int l
 #pragma unroll
   for (int p = 0; p < P; ++p) *reinterpret_cast<bf8*>(tile + piece<DP>(first + p, kt, s) + 8 * lane) = x.p[p];
 }
-// 16 rows as a left operand.
+// c += a b, a 16 rows of the tile: part by part, so that four registers hold the left operand.
 template <int DP>
-__device__ __forceinline__ Parts<3> left(const short* tile, int first, int kt, int s, int lane) {
-  Parts<3> x;
+__device__ __forceinline__ acc4 mma_left(const short* tile, int first, int kt, int s, int lane, const Parts<3>& b, acc4 c) {
+  const short* at = tile + hidden(piece<DP>(first, 0, 0)) + 8 * lane;
 #pragma unroll
-  for (int p = 0; p < 3; ++p) x.p[p] = *reinterpret_cast<const bf8*>(tile + piece<DP>(first + p, kt, s) + 8 * lane);
-  return x;
+  for (int i = 2; i >= 0; --i) {
+    const bf8 a = *reinterpret_cast<const bf8*>(at + piece<DP>(i, kt, s));
+#pragma unroll
+    for (int j = 2 - i; j >= 0; --j) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b.p[j], c, 0, 0, 0);
+  }
+  return c;
 }
 // The tile transposed, 16 features (16 dt + lane % 16) as rows of a left operand: lane group g
 // holds the tile's rows 4 g + 0..3 and 16 + 4 g + 0..3, as the registers of two products of 16
 // rows hold them. ds_read_b64_tr_b16: of the 64 bits that lane p of a group of 16 reads, lane q
 // gets element q % 4 of lanes q / 4 + 4 j, j = 0..3.
 template <int DP>
-__device__ __forceinline__ Parts<3> transposed(const short* tile, int first, int dt, int lane) {
+__device__ __forceinline__ acc4 mma_transposed(const short* tile, int first, int dt, int lane, const Parts<3>& b, acc4 c) {
   typedef __attribute__((address_space(3))) h4 lds_h4;
   const int p = lane & 15, g = lane >> 4;
-  const int at = (((dt & 1) * 2 + ((p & 3) >> 1)) * 16 + 4 * g + (p >> 2)) * 8 + 4 * (p & 1);
-  Parts<3> x;
+  const short* at = tile + hidden(piece<DP>(first, 0, 0)) + ((((p & 3) >> 1) * 16 + 4 * g + (p >> 2)) * 8 + 4 * (p & 1));
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
+  for (int i = 2; i >= 0; --i) {
     union {
       bf8 v;
       h4 h[2];
     } u;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
-      u.h[kt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4*)(tile + piece<DP>(first + k, kt, dt >> 1) + at));
-    x.p[k] = u.v;
+      u.h[kt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4*)(at + piece<DP>(i, kt, dt >> 1) + (dt & 1) * 256));
+#pragma unroll
+    for (int j = 2 - i; j >= 0; --j) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u.v, b.p[j], c, 0, 0, 0);
   }
-  return x;
+  return c;
 }
 
 // What a lane brings of the next tile: eight features of a row's mean and variance (or deltas).
@@ -177,7 +190,7 @@ struct Right {
   Parts<3> p[DP / 32];
 };
 
-// The wave's right operands of its rows of an (m, S) pair, by f(m, S) -> the operand's value.
+// The wave's right operands of its rows of an (m, S) pair, formed by f.
 template <int DP, bool VEC, typename F>
 __device__ __forceinline__ void load_right(const float* pm, const float* pS, int64_t at, int D, bool on, int k8, F&& f) {
 #pragma unroll
@@ -197,16 +210,30 @@ __device__ __forceinline__ void scores(const short* tile, int kt, int lane, cons
   m = acc4{0, 0, 0, 0}, v = m;
 #pragma unroll
   for (int s = 0; s < DP / 32; ++s) {
-    m = mma(left<DP>(tile, 0, kt, s, lane), b0.p[s], m);
-    v = mma(left<DP>(tile, 3, kt, s, lane), b1.p[s], v);
-    v = mma(left<DP>(tile, 6, kt, s, lane), b2.p[s], v);
+    m = mma_left<DP>(tile, 0, kt, s, lane, b0.p[s], m);
+    v = mma_left<DP>(tile, 3, kt, s, lane, b1.p[s], v);
+    v = mma_left<DP>(tile, 6, kt, s, lane, b2.p[s], v);
   }
 }
+
+// Nothing is scheduled across: operands of later products loaded early would take the registers
+// of those in use.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
 // The sum over the four lane groups that share a column.
 __device__ __forceinline__ float group_sum(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
+}
+
+// The least of a wave's lanes, in a scalar register.
+__device__ __forceinline__ int least(int x) {
+#pragma unroll
+  for (int w = 32; w > 0; w >>= 1) {
+    const int y = __shfl_xor(x, w);
+    x = x < y ? x : y;
+  }
+  return __builtin_amdgcn_readfirstlane(x);
 }
 
 // Blocks in one dimension: (split, key head, rows), the rows of one key head on one XCD where the
@@ -235,49 +262,66 @@ __device__ __forceinline__ Place place(const Args& A, int64_t blocks) {
 }
 
 // ---------------------------------------------------------------------------------- forward
-// Keys (and values) of the tile from key0 on into units, and units into the tile.
+// Unit i of the tile of keys (and values) from key0 on, and the unit's place in the tile. Parts:
+// keys k 0, k^2 3, Sk 6; values v 9, v^2 12 (, Sv 15).
+template <int DP, bool VEC>
+__device__ __forceinline__ void fetch_key(const Args& A, const Place& p, int key0, int to, int i, int lane,
+                                          bool value_variances, Unit& u) {
+  constexpr int S = DP / 32;
+  const bool value = i >= 2 * S;
+  const int k = value ? i - 2 * S : i, kt = k / S, s = k % S, key = key0 + 16 * kt + (lane & 15);
+  const bool on = key < to;
+  const int64_t at = on ? key_at(value ? A.lv : A.lk, p.b, p.g, key) : 0;
+  const int d = 32 * s + 8 * (lane >> 4);
+  load8<VEC>((value ? A.mv : A.mk) + at, d, A.D, on, u.m);
+  if (!value || value_variances) load8<VEC>((value ? A.Sv : A.Sk) + at, d, A.D, on, u.S);
+}
+template <int DP>
+__device__ __forceinline__ void put_key(short* tile, int i, int lane, bool value_variances, const Unit& u) {
+  constexpr int S = DP / 32;
+  const bool value = i >= 2 * S;
+  const int k = value ? i - 2 * S : i, kt = k / S, s = k % S, first = value ? 9 : 0;
+  float x[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) x[q] = u.m[q] * u.m[q];
+  put<DP>(tile, first, kt, s, lane, split<3>(u.m));
+  put<DP>(tile, first + 3, kt, s, lane, split<3>(x));
+  if (!value || value_variances) put<DP>(tile, first + 6, kt, s, lane, split<3>(u.S));
+}
 template <int DP, bool VEC, int W, int U>
 __device__ __forceinline__ void fetch_keys(const Args& A, const Place& p, int key0, int to, int pairs, int wave, int lane,
                                            bool value_variances, Unit (&u)[U]) {
-  constexpr int S = DP / 32;
 #pragma unroll
-  for (int j = 0; j < U; ++j) {
-    const int i = wave + j * W;
-    if (i >= 2 * S * pairs) continue;
-    const bool value = i >= 2 * S;
-    const int k = value ? i - 2 * S : i, kt = k / S, s = k % S, key = key0 + 16 * kt + (lane & 15);
-    const bool on = key < to;
-    const int64_t at = on ? key_at(value ? A.lv : A.lk, p.b, p.g, key) : 0;
-    const int d = 32 * s + 8 * (lane >> 4);
-    load8<VEC>((value ? A.mv : A.mk) + at, d, A.D, on, u[j].m);
-    if (!value || value_variances) load8<VEC>((value ? A.Sv : A.Sk) + at, d, A.D, on, u[j].S);
-  }
+  for (int j = 0; j < U; ++j)
+    if (wave + j * W < 2 * (DP / 32) * pairs)
+      fetch_key<DP, VEC>(A, p, key0, to, wave + j * W, lane, value_variances, u[j]);
 }
-// Parts: keys k 0, k^2 3, Sk 6; values v 9, v^2 12 (, Sv 15).
 template <int DP, int W, int U>
 __device__ __forceinline__ void put_keys(short* tile, int pairs, int wave, int lane, bool value_variances,
                                          const Unit (&u)[U]) {
-  constexpr int S = DP / 32;
 #pragma unroll
-  for (int j = 0; j < U; ++j) {
-    const int i = wave + j * W;
-    if (i >= 2 * S * pairs) continue;
-    const bool value = i >= 2 * S;
-    const int k = value ? i - 2 * S : i, kt = k / S, s = k % S, first = value ? 9 : 0;
-    float x[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) x[q] = u[j].m[q] * u[j].m[q];
-    put<DP>(tile, first, kt, s, lane, split<3>(u[j].m));
-    put<DP>(tile, first + 3, kt, s, lane, split<3>(x));
-    if (!value || value_variances) put<DP>(tile, first + 6, kt, s, lane, split<3>(u[j].S));
+  for (int j = 0; j < U; ++j)
+    if (wave + j * W < 2 * (DP / 32) * pairs) put_key<DP>(tile, wave + j * W, lane, value_variances, u[j]);
+}
+// Unit by unit, where registers do not hold more.
+template <int DP, bool VEC, int W>
+__device__ __forceinline__ void pass_keys(const Args& A, const Place& p, int key0, int to, short* tile, int pairs, int wave,
+                                          int lane, bool value_variances) {
+  Unit u;
+#pragma unroll 1
+  for (int i = wave; i < 2 * (DP / 32) * pairs; i += W) {
+    fetch_key<DP, VEC>(A, p, key0, to, i, hidden(lane), value_variances, u);
+    put_key<DP>(tile, i, hidden(lane), value_variances, u);
   }
 }
 
-// Queries on the right: q, Sq, Sq + q^2 (against k, k^2, Sk).
+// Queries on the right: q, Sq, Sq + q^2 (against k, k^2, Sk), scaled.
 template <int DP, bool VEC>
 __device__ __forceinline__ void load_queries(const Args& A, int64_t at, bool on, int k8, Right<DP>& q, Right<DP>& Q,
                                              Right<DP>& P) {
   load_right<DP, VEC>(A.mq, A.Sq, at, A.D, on, k8, [&](int s, float (&m)[8], float (&S)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[i] *= A.c, S[i] *= A.c2;
     q.p[s] = split<3>(m), Q.p[s] = split<3>(S);
 #pragma unroll
     for (int i = 0; i < 8; ++i) S[i] = fmaf(m[i], m[i], S[i]);
@@ -295,7 +339,7 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
   Place p = place(A, blocks);
   if (A.causal) p.block = blocks - 1 - p.block;  // the longest rows first
   const Seq s = sequence(A, p.b);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k8 = lane >> 4;
+  const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
   const int64_t block0 = p.block * NC * kRows, wave0 = block0 + wave * NC * 16;
   const int from = p.split * A.chunk;
   auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
@@ -310,15 +354,19 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
     lim[c] = row_limit(A, s, rho);
     load_queries<DP, VEC>(A, lim[c] ? row_at(A, A.lq, p.b, p.g, rho) : 0, lim[c] > 0, k8, q[c], Q[c], P[c]);
   }
+  int whole = lim[0];  // tiles up to here are seen by all of the wave's rows
+#pragma unroll
+  for (int c = 1; c < NC; ++c) whole = whole < lim[c] ? whole : lim[c];
+  whole = least(whole);
   Unit u[U];
   fetch_keys<DP, VEC, W>(A, p, from, to, 1, wave, lane, false, u);
   put_keys<DP, W>(lds, 1, wave, lane, false, u);
   __syncthreads();
   int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile, buf ^= 1) {
-    const short* tile = lds + buf * Keys::halves;
+    const short* tile = lds + hidden(buf * Keys::halves);
     const bool more = key0 + kTile < to;
-    if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 1, wave, lane, false, u);
+    if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 1, wave, hidden(lane), false, u);
     if (key0 < wave_to) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -327,25 +375,39 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
         for (int c = 0; c < NC; ++c) m[c] = v[c] = acc4{0, 0, 0, 0};
 #pragma unroll
         for (int st = 0; st < DP / 32; ++st) {
-          const Parts<3> a = left<DP>(tile, 0, kt, st, lane);
+          const short* at = tile + piece<DP>(0, kt, st) + 8 * lane;
 #pragma unroll
-          for (int c = 0; c < NC; ++c) m[c] = mma(a, q[c].p[st], m[c]);
-          const Parts<3> b = left<DP>(tile, 3, kt, st, lane);
+          for (int i = 2; i >= 0; --i) {
+            const bf8 k = *reinterpret_cast<const bf8*>(at + piece<DP>(i, 0, 0)),
+                      k2 = *reinterpret_cast<const bf8*>(at + piece<DP>(3 + i, 0, 0)),
+                      Sk = *reinterpret_cast<const bf8*>(at + piece<DP>(6 + i, 0, 0));
 #pragma unroll
-          for (int c = 0; c < NC; ++c) v[c] = mma(b, Q[c].p[st], v[c]);
-          const Parts<3> d = left<DP>(tile, 6, kt, st, lane);
+            for (int j = 2 - i; j >= 0; --j)
 #pragma unroll
-          for (int c = 0; c < NC; ++c) v[c] = mma(d, P[c].p[st], v[c]);
+              for (int c = 0; c < NC; ++c) {
+                m[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[c].p[st].p[j], m[c], 0, 0, 0);
+                v[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k2, Q[c].p[st].p[j], v[c], 0, 0, 0);
+                v[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Sk, P[c].p[st].p[j], v[c], 0, 0, 0);
+              }
+          }
         }
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float mm, vm, cdf;
-            rectify(m[c][r] * A.c, v[c][r] * A.c2, mm, vm, cdf);
-            const bool seen = key0 + 16 * kt + 4 * k8 + r < lim[c];
-            mt[c] += seen ? mm : 0.f, vt[c] += seen ? vm : 0.f;
+            const Rectified z = rectify(m[c][r], v[c][r]);
+            m[c][r] = z.mm, v[c][r] = z.vm;
           }
+          if (key0 + kTile > whole) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool seen = key0 + 16 * kt + 4 * k8 + r < lim[c];
+              m[c][r] = seen ? m[c][r] : 0.f, v[c][r] = seen ? v[c][r] : 0.f;
+            }
+          }
+          mt[c] += (m[c][0] + m[c][1]) + (m[c][2] + m[c][3]);
+          vt[c] += (v[c][0] + v[c][1]) + (v[c][2] + v[c][3]);
+        }
       }
     }
     if (more) put_keys<DP, W>(lds + (buf ^ 1) * Keys::halves, 1, wave, lane, false, u);
@@ -372,15 +434,16 @@ __device__ __forceinline__ void add_sums(const Args& A, const Place& p, int64_t 
 
 template <int DP, bool VEC, int W>
 __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
-  constexpr int U = units_of<DP, W>(2), DT = DP / 16, kRows = 16 * W;
+  constexpr int DT = DP / 16, kRows = 16 * W;
   typedef Tile<DP, 18> KeysValues;
   constexpr int bufs = 2 * KeysValues::bytes <= kLdsBytes ? 2 : 1;
+  constexpr bool ahead = units_of<DP, W>(2) == 1;  // the next tile waits in registers where they suffice
   extern __shared__ __align__(16) short lds[];
   const int64_t blocks = (A.M + kRows - 1) / kRows;
   Place p = place(A, blocks);
   if (A.causal) p.block = blocks - 1 - p.block;
   const Seq s = sequence(A, p.b);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k8 = lane >> 4;
+  const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
   const int64_t block0 = p.block * kRows, wave0 = block0 + wave * 16, rho = wave0 + (lane & 15);
   const int lim = row_limit(A, s, rho), from = p.split * A.chunk;
   auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
@@ -393,58 +456,65 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
   const RowSums rs = row_sums(mt, vt);
   Right<DP> q, Q, P;
   load_queries<DP, VEC>(A, lim ? row_at(A, A.lq, p.b, p.g, rho) : 0, lim > 0, k8, q, Q, P);
+  const int whole = least(lim);
   float sum = 0.f;
   acc4 om[DT], oS[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) om[d] = oS[d] = acc4{0, 0, 0, 0};
-  Unit u[U];
-  if (from < to) {
-    fetch_keys<DP, VEC, W>(A, p, from, to, 2, wave, lane, true, u);
-    put_keys<DP, W>(lds, 2, wave, lane, true, u);
-  }
+  Unit u[1];
+  if (from < to) pass_keys<DP, VEC, W>(A, p, from, to, lds, 2, wave, lane, true);
   __syncthreads();
   int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile) {
-    const short* tile = lds + buf * KeysValues::halves;
+    const short* tile = lds + hidden(buf * KeysValues::halves);
     const bool more = key0 + kTile < to;
-    if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, lane, true, u);
+    if (ahead && more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), true, u);
     if (key0 < wave_to) {
       float w[8], kw[8];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
+        fence();
         acc4 m, v;
         scores<DP>(tile, kt, lane, q, Q, P, m, v);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float mm, vm, cdf, x, k, xw, rw;
-          rectify(m[r] * A.c, v[r] * A.c2, mm, vm, cdf);
-          weigh(mm, vm, rs, x, k, xw, rw);
-          x = key0 + 16 * kt + 4 * k8 + r < lim ? x : 0.f;
-          sum += x;
-          w[4 * kt + r] = x, kw[4 * kt + r] = k * x * x;
+          const Weight x = weigh(rectify(m[r], v[r]), rs);
+          w[4 * kt + r] = x.w, kw[4 * kt + r] = x.k;
         }
       }
+      if (key0 + kTile > whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = key0 + 16 * (i >> 2) + 4 * k8 + (i & 3) < lim ? w[i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) kw[i] *= w[i] * w[i], sum += w[i];
+      fence();
       {
         const Parts<3> b = split<3>(w);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) om[d] = mma(transposed<DP>(tile, 9, d, lane), b, om[d]);
+        for (int d = 0; d < DT; ++d) om[d] = mma_transposed<DP>(tile, 9, d, lane, b, om[d]);
       }
+      fence();
       {
         const Parts<3> b = split<3>(kw);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) oS[d] = mma(transposed<DP>(tile, 12, d, lane), b, oS[d]);
+        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(tile, 12, d, lane, b, oS[d]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) kw[i] = fmaf(w[i], w[i], kw[i]);
+      fence();
       {
         const Parts<3> b = split<3>(kw);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) oS[d] = mma(transposed<DP>(tile, 15, d, lane), b, oS[d]);
+        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(tile, 15, d, lane, b, oS[d]);
       }
     }
     if (bufs == 2) buf ^= 1;
     if (bufs == 1) __syncthreads();
-    if (more) put_keys<DP, W>(lds + buf * KeysValues::halves, 2, wave, lane, true, u);
+    if (!ahead && more)
+      pass_keys<DP, VEC, W>(A, p, key0 + kTile, to, lds, 2, wave, lane, true);
+    else if (more)
+      put_keys<DP, W>(lds + buf * KeysValues::halves, 2, wave, lane, true, u);
     __syncthreads();
   }
   sum = group_sum(sum);
@@ -501,15 +571,16 @@ __global__ void __launch_bounds__(256) join_kernel(const Args A) {
 // Deltas of the queries.
 template <int DP, bool VEC, int W>
 __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
-  constexpr int U = units_of<DP, W>(2), DT = DP / 16, kRows = 16 * W;
+  constexpr int DT = DP / 16, kRows = 16 * W;
   typedef Tile<DP, 15> KeysValues;
   constexpr int bufs = 2 * KeysValues::bytes <= kLdsBytes ? 2 : 1;
+  constexpr bool ahead = units_of<DP, W>(2) == 1;
   extern __shared__ __align__(16) short lds[];
   const int64_t blocks = (A.M + kRows - 1) / kRows;
   Place p = place(A, blocks);
   if (A.causal) p.block = blocks - 1 - p.block;
   const Seq s = sequence(A, p.b);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k8 = lane >> 4;
+  const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
   const int64_t block0 = p.block * kRows, wave0 = block0 + wave * 16, rho = wave0 + (lane & 15);
   const int lim = row_limit(A, s, rho), from = p.split * A.chunk;
   auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
@@ -524,57 +595,71 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
   Right<DP> q, Q, P, dm, dS;
   load_queries<DP, VEC>(A, lim ? row_at(A, A.lq, p.b, p.g, rho) : 0, lim > 0, k8, q, Q, P);
   load_right<DP, VEC>(A.dm, A.dS, lim ? row_at(A, A.ld, p.b, p.g, rho) : 0, A.D, lim > 0, k8,
-                      [&](int st, float (&m)[8], float (&S)[8]) { dm.p[st] = split<3>(m), dS.p[st] = split<3>(S); });
+                      [&](int st, float (&m)[8], float (&S)[8]) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) m[i] *= A.c, S[i] *= A.c2;
+                        dm.p[st] = split<3>(m), dS.p[st] = split<3>(S);
+                      });
+  const int whole_tiles = least(lim);
   acc4 om[DT], oS[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) om[d] = oS[d] = acc4{0, 0, 0, 0};
-  Unit u[U];
-  if (from < to) {
-    fetch_keys<DP, VEC, W>(A, p, from, to, 2, wave, lane, false, u);
-    put_keys<DP, W>(lds, 2, wave, lane, false, u);
-  }
+  Unit u[1];
+  if (from < to) pass_keys<DP, VEC, W>(A, p, from, to, lds, 2, wave, lane, false);
   __syncthreads();
   int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile) {
-    const short* tile = lds + buf * KeysValues::halves;
+    const short* tile = lds + hidden(buf * KeysValues::halves);
     const bool more = key0 + kTile < to;
-    if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, lane, false, u);
+    if (ahead && more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), false, u);
     if (key0 < wave_to) {
       float x[8], X[8];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        acc4 m, v, e = {0, 0, 0, 0}, E = e;
+        fence();
+        acc4 m, v;
         scores<DP>(tile, kt, lane, q, Q, P, m, v);
 #pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const Rectified z = rectify(m[r], v[r]);
+          const Weight w = weigh(z, rs);
+          m[r] = remax_jacobian(z, w, w.w * inv, rs);
+        }
+        acc4 e = {0, 0, 0, 0}, E = e;
+#pragma unroll
         for (int st = 0; st < DP / 32; ++st) {
-          e = mma(left<DP>(tile, 9, kt, st, lane), dm.p[st], e);
-          E = mma(left<DP>(tile, 12, kt, st, lane), dS.p[st], E);
+          e = mma_left<DP>(tile, 9, kt, st, lane, dm.p[st], e);
+          E = mma_left<DP>(tile, 12, kt, st, lane, dS.p[st], E);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float mm, vm, cdf, w, k, xw, rw;
-          const float var = v[r] * A.c2;
-          rectify(m[r] * A.c, var, mm, vm, cdf);
-          weigh(mm, vm, rs, w, k, xw, rw);
-          float J = remax_jacobian(var, mm, cdf, w * inv, k, xw, rw) * A.c;
-          J = key0 + 16 * kt + 4 * k8 + r < lim ? J : 0.f;
-          x[4 * kt + r] = e[r] * J, X[4 * kt + r] = E[r] * (J * J);
+        for (int r = 0; r < 4; ++r) x[4 * kt + r] = e[r] * m[r], X[4 * kt + r] = E[r] * (m[r] * m[r]);
+      }
+      if (key0 + kTile > whole_tiles) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool seen = key0 + 16 * (i >> 2) + 4 * k8 + (i & 3) < lim;
+          x[i] = seen ? x[i] : 0.f, X[i] = seen ? X[i] : 0.f;
         }
       }
+      fence();
       {
         const Parts<3> b = split<3>(x);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) om[d] = mma(transposed<DP>(tile, 0, d, lane), b, om[d]);
+        for (int d = 0; d < DT; ++d) om[d] = mma_transposed<DP>(tile, 0, d, lane, b, om[d]);
       }
+      fence();
       {
         const Parts<3> b = split<3>(X);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) oS[d] = mma(transposed<DP>(tile, 3, d, lane), b, oS[d]);
+        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(tile, 3, d, lane, b, oS[d]);
       }
     }
     if (bufs == 2) buf ^= 1;
     if (bufs == 1) __syncthreads();
-    if (more) put_keys<DP, W>(lds + buf * KeysValues::halves, 2, wave, lane, false, u);
+    if (!ahead && more)
+      pass_keys<DP, VEC, W>(A, p, key0 + kTile, to, lds, 2, wave, lane, false);
+    else if (more)
+      put_keys<DP, W>(lds + buf * KeysValues::halves, 2, wave, lane, false, u);
     __syncthreads();
   }
   if (rho >= A.M) return;
@@ -605,23 +690,28 @@ __device__ __forceinline__ RowRange rows_of(const Args& A, const Seq& s, int key
 }
 
 // Deltas of the keys and values: a wave holds 16 keys, the block walks the rows that see them.
-// Parts of a row: q 0, Sq 3, q^2 6 (against k, k^2 + Sk, Sk); dm 9, dS 12.
-template <int DP, bool VEC, int W>
+// Parts of a row: c q 0, c^2 Sq 3, (c q)^2 6 (against k, k^2 + Sk, Sk); dm 9, dS 12. The scale of the
+// scores' deltas is that of the queries they multiply.
+// KEYS, VALUES: which of the two: both where registers hold four sums of a head, else one after the
+// other, with the scores formed once more.
+template <int DP, bool VEC, int W, bool KEYS, bool VALUES>
 __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
-  constexpr int S = DP / 32, U = units_of<DP, W>(2), DT = DP / 16, kKeys = 16 * W;
+  constexpr int S = DP / 32, DT = DP / 16, kKeys = 16 * W;
   typedef Tile<DP, 15> Queries;
   constexpr int bufs = 2 * Queries::bytes + 2 * 5 * kTile * 4 <= kLdsBytes ? 2 : 1;
   extern __shared__ __align__(16) short lds[];
+  constexpr bool ahead = units_of<DP, W>(2) == 1;
   float* const stats = reinterpret_cast<float*>(lds + bufs * Queries::halves);  // [buffer][5][kTile]
   const Place p = place(A, (A.N + kKeys - 1) / kKeys);
   const Seq s = sequence(A, p.b);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, k8 = lane >> 4;
+  const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
   const int key0 = (int)p.block * kKeys, wave_key = key0 + wave * 16, key = wave_key + (lane & 15);
   const RowRange all = rows_of(A, s, key0), mine = rows_of(A, s, wave_key);
   const int64_t chunk0 = (int64_t)p.split * A.chunk, chunk1 = chunk0 + A.chunk;
   const int64_t from = all.first > chunk0 ? all.first : chunk0, to = all.end < chunk1 ? all.end : chunk1;
   if (from >= to && A.splits > 1) return;
   const bool on = key < s.len;
+  constexpr int DK = KEYS ? DT : 1, DV = VALUES ? DT : 1;
   Right<DP> k, K, Sk, vm, vv;
   load_right<DP, VEC>(A.mk, A.Sk, on ? key_at(A.lk, p.b, p.g, key) : 0, A.D, on, k8,
                       [&](int st, float (&m)[8], float (&x)[8]) {
@@ -630,83 +720,83 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
                         for (int i = 0; i < 8; ++i) x[i] = fmaf(m[i], m[i], x[i]);
                         K.p[st] = split<3>(x);
                       });
-  load_right<DP, VEC>(A.mv, A.mv, on ? key_at(A.lv, p.b, p.g, key) : 0, A.D, on, k8,
+  if constexpr (KEYS)
+    load_right<DP, VEC>(A.mv, A.mv, on ? key_at(A.lv, p.b, p.g, key) : 0, A.D, on, k8,
                       [&](int st, float (&m)[8], float (&x)[8]) {
                         vm.p[st] = split<3>(m);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) x[i] *= x[i];
                         vv.p[st] = split<3>(x);
                       });
-  acc4 okm[DT], okS[DT], ovm[DT], ovS[DT];
+  acc4 okm[DK], okS[DK], ovm[DV], ovS[DV];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) okm[d] = okS[d] = ovm[d] = ovS[d] = acc4{0, 0, 0, 0};
-  Unit u[U];
-  float st3[3];
-  int st_lim = 0;
-  auto fetch = [&](int64_t rho0) {
+  for (int d = 0; d < DK; ++d) okm[d] = okS[d] = acc4{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int i = wave + j * W;
-      if (i >= 4 * S) continue;
-      const bool delta = i >= 2 * S;
-      const int n = delta ? i - 2 * S : i, kt = n / S, st = n % S;
-      const int64_t rho = rho0 + 16 * kt + (lane & 15);
-      const bool in = rho < to;
-      const int64_t at = in ? row_at(A, delta ? A.ld : A.lq, p.b, p.g, rho) : 0;
-      load8<VEC>((delta ? A.dm : A.mq) + at, 32 * st + 8 * k8, A.D, in, u[j].m);
-      load8<VEC>((delta ? A.dS : A.Sq) + at, 32 * st + 8 * k8, A.D, in, u[j].S);
-    }
-    if (threadIdx.x < kTile) {
-      const int64_t rho = rho0 + threadIdx.x;
-      st_lim = rho < to ? row_limit(A, s, rho) : 0;
+  for (int d = 0; d < DV; ++d) ovm[d] = ovS[d] = acc4{0, 0, 0, 0};
+  auto fetch_unit = [&](int64_t rho0, int i, int ln, Unit& u) {
+    const bool delta = i >= 2 * S;
+    const int n = delta ? i - 2 * S : i, kt = n / S, st = n % S;
+    const int64_t rho = rho0 + 16 * kt + (ln & 15);
+    const bool in = rho < to;
+    const int64_t at = in ? row_at(A, delta ? A.ld : A.lq, p.b, p.g, rho) : 0;
+    load8<VEC>((delta ? A.dm : A.mq) + at, 32 * st + 8 * (ln >> 4), A.D, in, u.m);
+    load8<VEC>((delta ? A.dS : A.Sq) + at, 32 * st + 8 * (ln >> 4), A.D, in, u.S);
+  };
+  auto store_unit = [&](short* tile, int i, int ln, Unit& u) {
+    const bool delta = i >= 2 * S;
+    const int n = delta ? i - 2 * S : i, kt = n / S, st = n % S, first = delta ? 9 : 0;
+    const float c = delta ? 1.f : A.c, c2 = delta ? 1.f : A.c2;
 #pragma unroll
-      for (int i = 0; i < 3; ++i) st3[i] = st_lim ? A.rows[stat_at(A, p.b, p.g, rho, i)] : 0.f;
+    for (int e = 0; e < 8; ++e) u.m[e] *= c, u.S[e] *= c2;
+    put<DP>(tile, first, kt, st, ln, split<3>(u.m));
+    put<DP>(tile, first + 3, kt, st, ln, split<3>(u.S));
+    if (!delta) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u.m[e] *= u.m[e];
+      put<DP>(tile, 6, kt, st, ln, split<3>(u.m));
     }
   };
-  auto store = [&](int buf) {
-    short* tile = lds + buf * Queries::halves;
+  // a row of the tile for each of the first threads
+  auto row_stats = [&](int64_t rho0, int buf) {
+    const int tid = wave * 64 + hidden(lane);
+    if (tid >= kTile) return;
+    const int64_t rho = rho0 + tid;
+    const int lim = rho < to ? row_limit(A, s, rho) : 0;
+    float x[3];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int i = wave + j * W;
-      if (i >= 4 * S) continue;
-      const bool delta = i >= 2 * S;
-      const int n = delta ? i - 2 * S : i, kt = n / S, st = n % S, first = delta ? 9 : 0;
-      put<DP>(tile, first, kt, st, lane, split<3>(u[j].m));
-      put<DP>(tile, first + 3, kt, st, lane, split<3>(u[j].S));
-      if (!delta) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = u[j].m[e] * u[j].m[e];
-        put<DP>(tile, 6, kt, st, lane, split<3>(x));
-      }
-    }
-    if (threadIdx.x < kTile) {
-      const RowSums r = row_sums(st3[0], st3[1]);
-      float* o = stats + buf * 5 * kTile + threadIdx.x;
-      o[0] = r.inv_mt, o[kTile] = r.y, o[2 * kTile] = r.c_mt;
-      o[3 * kTile] = fast_rcp(fmaxf(st3[2], kRemaxFloor));
-      o[4 * kTile] = __int_as_float(st_lim);
-    }
+    for (int i = 0; i < 3; ++i) x[i] = lim ? A.rows[stat_at(A, p.b, p.g, rho, i)] : 0.f;
+    const RowSums r = row_sums(x[0], x[1]);
+    float* o = stats + buf * 5 * kTile + tid;
+    o[0] = r.inv_mt, o[kTile] = r.y, o[2 * kTile] = r.c_mt;
+    o[3 * kTile] = fast_rcp(fmaxf(x[2], kRemaxFloor));
+    o[4 * kTile] = __int_as_float(lim);
   };
-  if (from < to) fetch(from), store(0);
+  auto pass_rows = [&](int64_t rho0, int buf) {
+    Unit u;
+#pragma unroll 1
+    for (int i = wave; i < 4 * S; i += W) {
+      fetch_unit(rho0, i, hidden(lane), u);
+      store_unit(lds + buf * Queries::halves, i, hidden(lane), u);
+    }
+    row_stats(rho0, buf);
+  };
+  Unit u;
+  if (from < to) pass_rows(from, 0);
   __syncthreads();
   int buf = 0;
   for (int64_t rho0 = from; rho0 < to; rho0 += kTile) {
-    const short* tile = lds + buf * Queries::halves;
+    const short* tile = lds + hidden(buf * Queries::halves);
     const float* st = stats + buf * 5 * kTile;
     const bool more = rho0 + kTile < to;
-    if (more) fetch(rho0 + kTile);
-    if (wave_key < s.len && rho0 + kTile > mine.first) {
+    const bool busy = wave_key < s.len && rho0 + kTile > mine.first;
+    if (busy) {
       float a[8], x[8], X[8];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        acc4 m, v, e = {0, 0, 0, 0}, E = e;
+        fence();
+        acc4 m, v;
         scores<DP>(tile, kt, lane, k, K, Sk, m, v);
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          e = mma(left<DP>(tile, 9, kt, i, lane), vm.p[i], e);
-          E = mma(left<DP>(tile, 12, kt, i, lane), vv.p[i], E);
-        }
+        fence();
         const int j = 16 * kt + 4 * k8;
         const acc4 inv_mt = *reinterpret_cast<const acc4*>(st + j), y = *reinterpret_cast<const acc4*>(st + kTile + j),
                    c_mt = *reinterpret_cast<const acc4*>(st + 2 * kTile + j),
@@ -714,55 +804,74 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
                    lims = *reinterpret_cast<const acc4*>(st + 4 * kTile + j);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const RowSums rs{inv_mt[r], y[r], c_mt[r]};
-          float mm, vmo, cdf, w, kk, xw, rw;
-          const float var = v[r] * A.c2;
-          rectify(m[r] * A.c, var, mm, vmo, cdf);
-          weigh(mm, vmo, rs, w, kk, xw, rw);
-          w *= inv[r];
-          float J = remax_jacobian(var, mm, cdf, w, kk, xw, rw) * A.c;
-          const bool seen = key < __float_as_int(lims[r]);
-          J = seen ? J : 0.f;
-          a[4 * kt + r] = seen ? w : 0.f;
-          x[4 * kt + r] = e[r] * J, X[4 * kt + r] = E[r] * (J * J);
+          const RowSums rs{inv_mt[r], y[r], 1.f + y[r], c_mt[r]};
+          const Rectified z = rectify(m[r], v[r]);
+          const Weight w = weigh(z, rs);
+          const float n = key < __float_as_int(lims[r]) ? w.w * inv[r] : 0.f;
+          if constexpr (KEYS) m[r] = remax_jacobian(z, w, n, rs);
+          a[4 * kt + r] = n;
+        }
+        if constexpr (KEYS) {
+          fence();
+          acc4 e = {0, 0, 0, 0}, E = e;
+#pragma unroll
+          for (int i = 0; i < S; ++i) {
+            e = mma_left<DP>(tile, 9, kt, i, lane, vm.p[i], e);
+            E = mma_left<DP>(tile, 12, kt, i, lane, vv.p[i], E);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[4 * kt + r] = e[r] * m[r], X[4 * kt + r] = E[r] * (m[r] * m[r]);
         }
       }
-      {
-        const Parts<3> b = split<3>(x);
+      if constexpr (KEYS) {
+        fence();
+        {
+          const Parts<3> b = split<3>(x);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) okm[d] = mma(transposed<DP>(tile, 0, d, lane), b, okm[d]);
+          for (int d = 0; d < DT; ++d) okm[d] = mma_transposed<DP>(tile, 0, d, lane, b, okm[d]);
+        }
+        fence();
+        {
+          const Parts<3> b = split<3>(X);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) okS[d] = mma_transposed<DP>(tile, 6, d, lane, b, okS[d]);
+        }
       }
-      {
-        const Parts<3> b = split<3>(X);
+      fence();
+      if (ahead && more && wave < 4 * S) fetch_unit(rho0 + kTile, wave, hidden(lane), u);  // here its registers are free
+      if constexpr (VALUES) {
+        fence();
+        {
+          const Parts<3> b = split<3>(a);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) okS[d] = mma(transposed<DP>(tile, 6, d, lane), b, okS[d]);
-      }
-      {
-        const Parts<3> b = split<3>(a);
+          for (int d = 0; d < DT; ++d) ovm[d] = mma_transposed<DP>(tile, 9, d, lane, b, ovm[d]);
+        }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) ovm[d] = mma(transposed<DP>(tile, 9, d, lane), b, ovm[d]);
-      }
+        for (int i = 0; i < 8; ++i) a[i] *= a[i];
+        fence();
+        {
+          const Parts<3> b = split<3>(a);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] *= a[i];
-      {
-        const Parts<3> b = split<3>(a);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) ovS[d] = mma(transposed<DP>(tile, 12, d, lane), b, ovS[d]);
+          for (int d = 0; d < DT; ++d) ovS[d] = mma_transposed<DP>(tile, 12, d, lane, b, ovS[d]);
+        }
       }
     }
+    if (ahead && more && !busy && wave < 4 * S) fetch_unit(rho0 + kTile, wave, hidden(lane), u);
     if (bufs == 2) buf ^= 1;
     if (bufs == 1) __syncthreads();
-    if (more) store(buf);
+    if (ahead && more) {
+      if (wave < 4 * S) store_unit(lds + buf * Queries::halves, wave, hidden(lane), u);
+      row_stats(rho0 + kTile, buf);
+    } else if (more) {
+      pass_rows(rho0 + kTile, buf);
+    }
     __syncthreads();
   }
   if (key >= A.N) return;
   const bool whole = A.splits == 1;
-  float* out[4] = {A.dmk, A.dSk, A.dmv, A.dSv};
   const int64_t at = whole ? key_at(A.lokv, p.b, p.g, key) : (((int64_t)p.split * A.B * A.G + p.bg) * A.N + key) * (4 * A.D);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float* const o = (whole ? out[i] : A.parts + i * A.D) + at;
-    const acc4* x = i == 0 ? okm : (i == 1 ? okS : (i == 2 ? ovm : ovS));
+  auto put_out = [&](float* out, int i, const auto& x) {
+    float* const o = (whole ? out : A.parts + i * A.D) + at;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -770,7 +879,9 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
         const int f = 16 * d + 4 * k8 + r;
         if (f < A.D) o[f] = x[d][r];
       }
-  }
+  };
+  if constexpr (KEYS) put_out(A.dmk, 0, okm), put_out(A.dSk, 1, okS);
+  if constexpr (VALUES) put_out(A.dmv, 2, ovm), put_out(A.dSv, 3, ovS);
 }
 
 // The splits of rows that reach a key, in order; a wave to a key. kv_keys: keys of a dkv block.
@@ -875,7 +986,13 @@ int backward(const char* what, Args a, float* ws, hipStream_t s) {
     a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;  // the stream's order keeps the joins apart
     dim3 grid;
     if (int rc = grid_of(what, a.N, rows, BG, sp.n, 64 * W, &grid)) return rc;
-    go(dkv_kernel<DP, VEC, W>, grid, 64 * W, two_or_one(Tile<DP, 15>::bytes, 5 * kTile * 4), s, a);
+    const int lds = two_or_one(Tile<DP, 15>::bytes, 5 * kTile * 4);
+    if constexpr (DP == 128) {
+      go(dkv_kernel<DP, VEC, W, true, false>, grid, 64 * W, lds, s, a);
+      go(dkv_kernel<DP, VEC, W, false, true>, grid, 64 * W, lds, s, a);
+    } else {
+      go(dkv_kernel<DP, VEC, W, true, true>, grid, 64 * W, lds, s, a);
+    }
     if (sp.n > 1) hipLaunchKernelGGL(join_keys_kernel, join_grid(BG * a.N), dim3(256), 0, s, a, rows);
   }
   return TAGI_OK;

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC>())) scores
     const int64_t h = b * A.H + g * A.R + r0;
     float mt[HT] = {}, vt[HT] = {};
     if (from < to) {
-      Parts<3> q[S], Q[S], P[S];  // q, Sq, Sq + q^2
+      Parts<3> q[S], Q[S], P[S];  // q, Sq, Sq + q^2, scaled
       const int64_t qa = b * A.lq.sb + (int64_t)(g * A.R + r0 + (col < n ? col : n - 1)) * A.lq.sh;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC>())) scores
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int d = feature<Cell, DP>(s, k8) + i;
-          x[i] = d < D ? A.mq[qa + d] : 0.f, X[i] = d < D ? A.Sq[qa + d] : 0.f;
+          x[i] = d < D ? A.mq[qa + d] * A.c1 : 0.f, X[i] = d < D ? A.Sq[qa + d] * A.c2 : 0.f;
           y[i] = fmaf(x[i], x[i], X[i]);
         }
         q[s] = split<3>(x), Q[s] = split<3>(X), P[s] = split<3>(y);
@@ -245,19 +245,18 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC>())) scores
         const bool on = from + key < to, there = on && slot[key < A.wave_keys ? key : 0] >= 0;
 #pragma unroll
         for (int r = 0; r < HT; ++r) {
-          if (r >= n) break;
-          float mm, vm, cdf;
-          rectify(tile[wave][0][r * kRow + lane] * A.c1, tile[wave][1][r * kRow + lane] * A.c2, mm, vm, cdf);
-          if (!there) mm = vm = 0.f;
-          if (on) A.scores[(h + r) * A.max_len + from + key] = make_float2(mm, vm);
-          mt[r] += mm, vt[r] += vm;
+          if (r >= n) continue;
+          Rectified z = rectify(tile[wave][0][r * kRow + lane], tile[wave][1][r * kRow + lane]);
+          if (!there) z.mm = z.vm = 0.f;
+          if (on) A.scores[(h + r) * A.max_len + from + key] = make_float2(z.mm, z.vm);
+          mt[r] += z.mm, vt[r] += z.vm;
         }
         wave_sync();
       }
     }
 #pragma unroll
     for (int r = 0; r < HT; ++r) {
-      if (r >= n) break;
+      if (r >= n) continue;
       const float x = wave_sum(mt[r]), y = wave_sum(vt[r]);
       if (lane == 0) {
         float* o = A.sums + ((h + r) * A.splits * kWaves + (int)blockIdx.x * kWaves + wave) * 2;
@@ -317,10 +316,13 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
         if constexpr (scaled_rows) a = pm[i0 + lane], s = pS[i0 + lane];
 #pragma unroll
         for (int r = 0; r < HT; ++r) {
-          if (r >= n) break;
-          float w = 0.f, k = 0.f, xw, rw;
+          if (r >= n) continue;
+          float w = 0.f, k = 0.f;
           const float2 x = on ? A.scores[(h + r) * A.max_len + key0 + lane] : make_float2(0.f, 0.f);
-          if (x.x > 0.f) weigh(x.x, x.y, row[r], w, k, xw, rw);
+          if (x.x > 0.f) {
+            const Weight o = weigh(Rectified{x.x, x.y, 0.f, 0.f}, row[r]);
+            w = o.w, k = o.k;
+          }
           total[r] += w;
           // the powers of two of the rows go into their weights
           const float w2 = w * w, kw = k * w2;
@@ -380,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
     }
 #pragma unroll
     for (int r = 0; r < HT; ++r) {
-      if (r >= n) break;
+      if (r >= n) continue;
       const float x = wave_sum(total[r]);
       if (lane == 0) totals[wave][r] = x;
     }
