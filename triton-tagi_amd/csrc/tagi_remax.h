@@ -16,7 +16,9 @@
 namespace tagi {
 
 constexpr float kRemaxFloor = 1e-6f;  // of means, variances, weights and their sums
-constexpr float kVarFloor = 1e-20f;   // of a score's variance: a stays finite for means up to 1e28
+// Added to a score's variance: a stays finite for means up to 1e28, and a variance above 1e-13 does
+// not change.
+constexpr float kVarFloor = 1e-20f;
 
 struct Rectified {
   float mm, vm;   // moments of max(z, 0), floored
@@ -24,7 +26,7 @@ struct Rectified {
 };
 __device__ __forceinline__ Rectified rectify(float m, float v) {
   Rectified o;
-  v = fmaxf(v, kVarFloor);
+  v += kVarFloor;
   o.rs = fast_rsqrt(v);
   const float sd = v * o.rs, a = m * o.rs, x = fabsf(a);
   const float t = fast_rcp(fmaf(0.25f, x, 1.0f));
@@ -50,7 +52,7 @@ __device__ __forceinline__ Rectified rectify(float m, float v) {
   const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f) * t, ut = u * t;
   const float f = e * ut, q = e * fmaf(-x, ut, p), tail = e * p;
   const bool up = a >= 0.0f;
-  const float mean = fmaf(sd, f, fmaxf(m, 0.0f));
+  const float mean = fmaf(sd, f, up ? m : 0.0f);
   const float var = fmaf(-f, f, up ? 1.0f - fmaf(2.0f * x, f, q) : q);
   o.cdf = up ? 1.0f - tail : tail;
   o.mm = fmaxf(mean, kRemaxFloor);

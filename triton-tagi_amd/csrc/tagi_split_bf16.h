@@ -18,6 +18,19 @@ struct Parts {
   bf8 p[P];
 };
 
+// What a part leaves: x0 - p.x and x1 - p.y, each one product-sum of the packed pair with (-1, 0) or
+// (0, -1) that takes no unpacking (exact: the difference is a float). The two constants come from
+// scalar registers: written out, (-1, 0) becomes the inline constant -1.0, which the hardware reads
+// as (0, -1).
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void rest_of(bf2 p, float& x0, float& x1) {
+  uint32_t c0 = 0x0000bf80u, c1 = 0xbf800000u;
+  asm("" : "+s"(c0));
+  asm("" : "+s"(c1));
+  x0 = __builtin_amdgcn_fdot2_f32_bf16(p, __builtin_bit_cast(bf2, c0), x0, false);
+  x1 = __builtin_amdgcn_fdot2_f32_bf16(p, __builtin_bit_cast(bf2, c1), x1, false);
+}
+
 template <int P>
 __device__ __forceinline__ Parts<P> split(const float (&x)[8]) {
   Parts<P> out;
@@ -25,14 +38,13 @@ __device__ __forceinline__ Parts<P> split(const float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) rest[i] = x[i];
 #pragma unroll
-  for (int k = 0; k < P; ++k) {
+  for (int k = 0; k < P; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out.p[k][i] = (__bf16)rest[i];
-    if (k + 1 < P) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) rest[i] -= (float)out.p[k][i];
+    for (int i = 0; i < 8; i += 2) {
+      const bf2 p = {(__bf16)rest[i], (__bf16)rest[i + 1]};
+      out.p[k][i] = p.x, out.p[k][i + 1] = p.y;
+      if (k + 1 < P) rest_of(p, rest[i], rest[i + 1]);
     }
-  }
   return out;
 }
 
