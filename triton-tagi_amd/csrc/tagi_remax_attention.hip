@@ -113,6 +113,8 @@ __device__ __forceinline__ void load8(const float* p, int d, int D, bool on, flo
 
 // The block's wave, in a scalar register.
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+// x is formed here, and not where it is used: what it is formed from would wait in registers.
+__device__ __forceinline__ void formed(float& x) { asm volatile("" : "+v"(x)); }
 // x, of which the compiler knows nothing: what a tile's addresses need of it is formed in every
 // tile and not kept in registers across them.
 __device__ __forceinline__ int hidden(int x) {
@@ -480,6 +482,7 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
         for (int r = 0; r < 4; ++r) {
           const Weight x = weigh(rectify(m[r], v[r]), rs);
           w[4 * kt + r] = x.w, kw[4 * kt + r] = x.k;
+          formed(w[4 * kt + r]), formed(kw[4 * kt + r]);
         }
       }
       if (key0 + kTile > whole) {
@@ -623,7 +626,9 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
         for (int r = 0; r < 4; ++r) {
           const Rectified z = rectify(m[r], v[r]);
           const Weight w = weigh(z, rs);
-          m[r] = remax_jacobian(z, w, w.w * inv, rs);
+          float J = remax_jacobian(z, w, w.w * inv, rs);
+          formed(J);
+          m[r] = J;
         }
         acc4 e = {0, 0, 0, 0}, E = e;
 #pragma unroll
@@ -698,10 +703,10 @@ template <int DP, bool VEC, int W, bool KEYS, bool VALUES>
 __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   constexpr int S = DP / 32, DT = DP / 16, kKeys = 16 * W;
   typedef Tile<DP, 15> Queries;
-  constexpr int bufs = 2 * Queries::bytes + 2 * 5 * kTile * 4 <= kLdsBytes ? 2 : 1;
+  constexpr int bufs = 2 * Queries::bytes + 2 * 4 * kTile * 4 <= kLdsBytes ? 2 : 1;
   extern __shared__ __align__(16) short lds[];
   constexpr bool ahead = units_of<DP, W>(2) == 1;
-  float* const stats = reinterpret_cast<float*>(lds + bufs * Queries::halves);  // [buffer][5][kTile]
+  float* const stats = reinterpret_cast<float*>(lds + bufs * Queries::halves);  // [buffer][4][kTile]: 1 / mt, y, 1 / s, limit
   const Place p = place(A, (A.N + kKeys - 1) / kKeys);
   const Seq s = sequence(A, p.b);
   const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
@@ -766,10 +771,9 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
 #pragma unroll
     for (int i = 0; i < 3; ++i) x[i] = lim ? A.rows[stat_at(A, p.b, p.g, rho, i)] : 0.f;
     const RowSums r = row_sums(x[0], x[1]);
-    float* o = stats + buf * 5 * kTile + tid;
-    o[0] = r.inv_mt, o[kTile] = r.y, o[2 * kTile] = r.c_mt;
-    o[3 * kTile] = fast_rcp(fmaxf(x[2], kRemaxFloor));
-    o[4 * kTile] = __int_as_float(lim);
+    float* o = stats + buf * 4 * kTile + tid;
+    o[0] = r.inv_mt, o[kTile] = r.y, o[2 * kTile] = fast_rcp(fmaxf(x[2], kRemaxFloor));
+    o[3 * kTile] = __int_as_float(lim);
   };
   auto pass_rows = [&](int64_t rho0, int buf) {
     Unit u;
@@ -786,53 +790,62 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   int buf = 0;
   for (int64_t rho0 = from; rho0 < to; rho0 += kTile) {
     const short* tile = lds + hidden(buf * Queries::halves);
-    const float* st = stats + buf * 5 * kTile;
+    const float* st = stats + buf * 4 * kTile;
     const bool more = rho0 + kTile < to;
     const bool busy = wave_key < s.len && rho0 + kTile > mine.first;
     if (busy) {
-      float a[8], x[8], X[8];
+      float a[8], J[8];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         fence();
         acc4 m, v;
         scores<DP>(tile, kt, lane, k, K, Sk, m, v);
-        fence();
-        const int j = 16 * kt + 4 * k8;
-        const acc4 inv_mt = *reinterpret_cast<const acc4*>(st + j), y = *reinterpret_cast<const acc4*>(st + kTile + j),
-                   c_mt = *reinterpret_cast<const acc4*>(st + 2 * kTile + j),
-                   inv = *reinterpret_cast<const acc4*>(st + 3 * kTile + j),
-                   lims = *reinterpret_cast<const acc4*>(st + 4 * kTile + j);
+        const float* const row = st + 16 * kt + 4 * k8;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const RowSums rs{inv_mt[r], y[r], 1.f + y[r], c_mt[r]};
+          if ((r & 1) == 0) fence();  // two scores at a time: the registers of four are not there
+          RowSums rs;
+          rs.inv_mt = row[r], rs.y = row[kTile + r], rs.y1 = 1.f + rs.y, rs.c_mt = rs.inv_mt * rs.y1;
           const Rectified z = rectify(m[r], v[r]);
           const Weight w = weigh(z, rs);
-          const float n = key < __float_as_int(lims[r]) ? w.w * inv[r] : 0.f;
-          if constexpr (KEYS) m[r] = remax_jacobian(z, w, n, rs);
+          const float n = key < __float_as_int(row[3 * kTile + r]) ? w.w * row[2 * kTile + r] : 0.f;
           a[4 * kt + r] = n;
-        }
-        if constexpr (KEYS) {
-          fence();
-          acc4 e = {0, 0, 0, 0}, E = e;
-#pragma unroll
-          for (int i = 0; i < S; ++i) {
-            e = mma_left<DP>(tile, 9, kt, i, lane, vm.p[i], e);
-            E = mma_left<DP>(tile, 12, kt, i, lane, vv.p[i], E);
+          formed(a[4 * kt + r]);
+          if constexpr (KEYS) {
+            J[4 * kt + r] = remax_jacobian(z, w, a[4 * kt + r], rs);
+            formed(J[4 * kt + r]);
           }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[4 * kt + r] = e[r] * m[r], X[4 * kt + r] = E[r] * (m[r] * m[r]);
         }
       }
       if constexpr (KEYS) {
+        float x[8];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          fence();
+          acc4 e = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < S; ++i) e = mma_left<DP>(tile, 9, kt, i, lane, vm.p[i], e);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[4 * kt + r] = e[r] * J[4 * kt + r];
+        }
         fence();
         {
           const Parts<3> b = split<3>(x);
 #pragma unroll
           for (int d = 0; d < DT; ++d) okm[d] = mma_transposed<DP>(tile, 0, d, lane, b, okm[d]);
         }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          fence();
+          acc4 E = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < S; ++i) E = mma_left<DP>(tile, 12, kt, i, lane, vv.p[i], E);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[4 * kt + r] = E[r] * (J[4 * kt + r] * J[4 * kt + r]);
+        }
         fence();
         {
-          const Parts<3> b = split<3>(X);
+          const Parts<3> b = split<3>(x);
 #pragma unroll
           for (int d = 0; d < DT; ++d) okS[d] = mma_transposed<DP>(tile, 6, d, lane, b, okS[d]);
         }
@@ -986,7 +999,7 @@ int backward(const char* what, Args a, float* ws, hipStream_t s) {
     a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;  // the stream's order keeps the joins apart
     dim3 grid;
     if (int rc = grid_of(what, a.N, rows, BG, sp.n, 64 * W, &grid)) return rc;
-    const int lds = two_or_one(Tile<DP, 15>::bytes, 5 * kTile * 4);
+    const int lds = two_or_one(Tile<DP, 15>::bytes, 4 * kTile * 4);
     if constexpr (DP == 128) {
       go(dkv_kernel<DP, VEC, W, true, false>, grid, 64 * W, lds, s, a);
       go(dkv_kernel<DP, VEC, W, false, true>, grid, 64 * W, lds, s, a);
