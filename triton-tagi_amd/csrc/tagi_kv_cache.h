@@ -28,8 +28,10 @@ struct CacheView {
 // Row (page slot) of token `at` of sequence b for key head g: -1 where the table or the pool
 // has no such page.
 __device__ __forceinline__ int64_t cache_row(const CacheView& c, int64_t b, int64_t at, int g) {
-  const int64_t i = at / c.page;
-  if (at < 0 || i >= c.width) return -1;
+  if (at < 0) return -1;
+  // a division of 64 bits takes the time of the row's loads
+  const int64_t i = at >> 31 ? at / c.page : (int64_t)((uint32_t)at / (uint32_t)c.page);
+  if (i >= c.width) return -1;
   const int64_t p = c.table[b * c.width + i];
   if (p < 0 || p >= c.pages) return -1;
   return (p * c.G + g) * c.page + (at - i * c.page);

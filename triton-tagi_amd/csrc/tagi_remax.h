@@ -64,38 +64,42 @@ __device__ __forceinline__ Rectified rectify(float m, float v) {
 
 // A row's sums of mm and vm, as the weights use them.
 struct RowSums {
-  float inv_mt, y, y1, c_mt;  // 1 / mt, vt / mt^2, 1 + y, y1 / mt
+  float inv_mt, vt, c_mt;  // 1 / mt, vt, (1 + vt / mt^2) / mt
 };
 __device__ __forceinline__ RowSums row_sums(float mt, float vt) {
   RowSums r;
   r.inv_mt = fast_rcp(fmaxf(mt, kRemaxFloor));
-  r.y = fmaxf(vt, kRemaxFloor) * r.inv_mt * r.inv_mt;
-  r.y1 = 1.0f + r.y;
-  r.c_mt = r.inv_mt * r.y1;
+  r.vt = fmaxf(vt, kRemaxFloor);
+  r.c_mt = fmaf(r.vt * r.inv_mt, r.inv_mt, 1.0f) * r.inv_mt;
   return r;
 }
 
 // A score's weight before its row's normalisation and the weight's relative variance: the
 // log-normal stage in closed form (remax_row) with x = vm / mm^2 and w = vm / (mm mt) multiplied out,
 //   weight = mm c_mt / (1 + w) = mm^2 c_mt / d,  d = mm + s,  s = vm / mt
-//   k = [(1 + x)(1 + y) - (1 + w)^2] / (1 + w)^2 = [vm (1 + y) + y mm^2 - s (mm + d)] / d^2
+//   k = [(1 + x)(1 + vt / mt^2) - (1 + w)^2] / (1 + w)^2 = [vm u^2 + (vt - vm) (p^2 + s / mt)] / d^2,
+//       p = mm / mt, u = 1 - p
+// (what cancels is taken out by hand: a row of one key has u = 0, vt = vm and no variance, and with
+// few keys a difference of the products would lose what their roundings are of it).
 struct Weight {
-  float w, k, rd;  // rd = 1 / d
+  float w, k, rd, u;  // rd = 1 / d
 };
 __device__ __forceinline__ Weight weigh(const Rectified& z, const RowSums& r) {
   Weight o;
   const float s = z.vm * r.inv_mt, d = z.mm + s;
   o.rd = fast_rcp(d);
   o.w = fmaxf(z.mm * o.rd * z.mm * r.c_mt, kRemaxFloor);
-  const float num = fmaf(-s, z.mm + d, fmaf(r.y, z.mm * z.mm, z.vm * r.y1));
+  const float p = z.mm * r.inv_mt;
+  o.u = 1.0f - p;
+  const float num = fmaf(r.vt - z.vm, fmaf(p, p, s * r.inv_mt), z.vm * (o.u * o.u));
   o.k = fmaxf(num, 0.0f) * o.rd * o.rd;
   return o;
 }
 
 // J = cov(weight, z) / v of the normalised weight a: a times the lesser of sqrt(k / v) and
 // (x - w) / (1 + w) mm / (Phi v), (x - w) / (1 + w) mm = vm (1 - mm / mt) / d.
-__device__ __forceinline__ float remax_jacobian(const Rectified& z, const Weight& w, float a, const RowSums& r) {
-  const float cov = fmaxf(fmaf(-z.mm, r.inv_mt, 1.0f), 0.0f) * (z.vm * w.rd) * fast_rcp(fmaxf(z.cdf, kRemaxFloor));
+__device__ __forceinline__ float remax_jacobian(const Rectified& z, const Weight& w, float a) {
+  const float cov = fmaxf(w.u, 0.0f) * (z.vm * w.rd) * fast_rcp(fmaxf(z.cdf, kRemaxFloor));
   return a * z.rs * fminf(__builtin_amdgcn_sqrtf(w.k), cov * z.rs);
 }
 

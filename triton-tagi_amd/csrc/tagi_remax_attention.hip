@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
         for (int r = 0; r < 4; ++r) {
           const Rectified z = rectify(m[r], v[r]);
           const Weight w = weigh(z, rs);
-          float J = remax_jacobian(z, w, w.w * inv, rs);
+          float J = remax_jacobian(z, w, w.w * inv);
           formed(J);
           m[r] = J;
         }
@@ -703,10 +703,10 @@ template <int DP, bool VEC, int W, bool KEYS, bool VALUES>
 __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   constexpr int S = DP / 32, DT = DP / 16, kKeys = 16 * W;
   typedef Tile<DP, 15> Queries;
-  constexpr int bufs = 2 * Queries::bytes + 2 * 4 * kTile * 4 <= kLdsBytes ? 2 : 1;
+  constexpr int bufs = 2 * Queries::bytes + 2 * 5 * kTile * 4 <= kLdsBytes ? 2 : 1;
   extern __shared__ __align__(16) short lds[];
   constexpr bool ahead = units_of<DP, W>(2) == 1;
-  float* const stats = reinterpret_cast<float*>(lds + bufs * Queries::halves);  // [buffer][4][kTile]: 1 / mt, y, 1 / s, limit
+  float* const stats = reinterpret_cast<float*>(lds + bufs * Queries::halves);  // [buffer][5][kTile]: 1 / mt, vt, c_mt, 1 / s, limit
   const Place p = place(A, (A.N + kKeys - 1) / kKeys);
   const Seq s = sequence(A, p.b);
   const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
@@ -771,9 +771,9 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
 #pragma unroll
     for (int i = 0; i < 3; ++i) x[i] = lim ? A.rows[stat_at(A, p.b, p.g, rho, i)] : 0.f;
     const RowSums r = row_sums(x[0], x[1]);
-    float* o = stats + buf * 4 * kTile + tid;
-    o[0] = r.inv_mt, o[kTile] = r.y, o[2 * kTile] = fast_rcp(fmaxf(x[2], kRemaxFloor));
-    o[3 * kTile] = __int_as_float(lim);
+    float* o = stats + buf * 5 * kTile + tid;
+    o[0] = r.inv_mt, o[kTile] = r.vt, o[2 * kTile] = r.c_mt, o[3 * kTile] = fast_rcp(fmaxf(x[2], kRemaxFloor));
+    o[4 * kTile] = __int_as_float(lim);
   };
   auto pass_rows = [&](int64_t rho0, int buf) {
     Unit u;
@@ -790,7 +790,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   int buf = 0;
   for (int64_t rho0 = from; rho0 < to; rho0 += kTile) {
     const short* tile = lds + hidden(buf * Queries::halves);
-    const float* st = stats + buf * 4 * kTile;
+    const float* st = stats + buf * 5 * kTile;
     const bool more = rho0 + kTile < to;
     const bool busy = wave_key < s.len && rho0 + kTile > mine.first;
     if (busy) {
@@ -804,15 +804,14 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           if ((r & 1) == 0) fence();  // two scores at a time: the registers of four are not there
-          RowSums rs;
-          rs.inv_mt = row[r], rs.y = row[kTile + r], rs.y1 = 1.f + rs.y, rs.c_mt = rs.inv_mt * rs.y1;
+          const RowSums rs{row[r], row[kTile + r], row[2 * kTile + r]};
           const Rectified z = rectify(m[r], v[r]);
           const Weight w = weigh(z, rs);
-          const float n = key < __float_as_int(row[3 * kTile + r]) ? w.w * row[2 * kTile + r] : 0.f;
+          const float n = key < __float_as_int(row[4 * kTile + r]) ? w.w * row[3 * kTile + r] : 0.f;
           a[4 * kt + r] = n;
           formed(a[4 * kt + r]);
           if constexpr (KEYS) {
-            J[4 * kt + r] = remax_jacobian(z, w, a[4 * kt + r], rs);
+            J[4 * kt + r] = remax_jacobian(z, w, a[4 * kt + r]);
             formed(J[4 * kt + r]);
           }
         }
@@ -999,7 +998,7 @@ int backward(const char* what, Args a, float* ws, hipStream_t s) {
     a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;  // the stream's order keeps the joins apart
     dim3 grid;
     if (int rc = grid_of(what, a.N, rows, BG, sp.n, 64 * W, &grid)) return rc;
-    const int lds = two_or_one(Tile<DP, 15>::bytes, 4 * kTile * 4);
+    const int lds = two_or_one(Tile<DP, 15>::bytes, 5 * kTile * 4);
     if constexpr (DP == 128) {
       go(dkv_kernel<DP, VEC, W, true, false>, grid, 64 * W, lds, s, a);
       go(dkv_kernel<DP, VEC, W, false, true>, grid, 64 * W, lds, s, a);

@@ -8,10 +8,11 @@
 //   join:   the splits' sums added in order and normalised
 // HBM bound: the cache is read once, straight into the registers that feed the matrix cores, and
 // the scores between the launches are 16 bytes a token and head beside 4 D cells a token and key
-// head. The query heads that share a key head are the columns of the products, 16 at a time (a
-// column that no head has is computed and dropped: 9 to 18 MFMAs for 32 features of 16 tokens take
-// less time than the cells' way from HBM). Products: tagi_split_bf16.h; cells of 8 and 16 bits are
-// one part, so only the queries and weights are split.
+// head. Cells of 8 and 16 bits are one bf16 part (tagi_split_bf16.h; their squares one and two),
+// so only the queries and weights are split. The query heads that share a key head are the columns
+// of the products. Four of them at a time take all 16 columns with their three parts, four for each
+// (the last four are zeros), and a product of all parts is one MFMA instead of three; more than four
+// take 16 columns at a time, part after part.
 #include "tagi_kv_cache.h"
 #include "tagi_remax.h"
 #include "tagi_split_bf16.h"
@@ -70,56 +71,179 @@ __device__ __forceinline__ void wave_sync() {
 // N neighbouring cells of a row as they lie in memory.
 template <typename T, int N>
 struct Raw {
-  T x[N];
+  static constexpr int words = (N * (int)sizeof(T) + 3) / 4;
+  uint32_t w[words];
 };
-// Features from d on, zeros behind D. VEC: rows are whole groups of N, aligned to them.
+// A GPU's memory, said so: of two pointers to choose from the compiler would not know it.
+template <typename T>
+__device__ __forceinline__ T load_global(const void* p) {
+  return *(const __attribute__((address_space(1))) T*)(p);
+}
+// Features from d on. VEC: rows are whole groups of N, aligned to them, and behind D the row's first
+// stand: they meet a query's zeros (a row with a NaN there has NaN scores as it is) or go to sums
+// that nobody reads. Else zeros.
 template <bool VEC, typename T, int N>
 __device__ __forceinline__ Raw<T, N> load_raw(const T* row, int d, int D) {
   Raw<T, N> r;
-  if constexpr (VEC) {
-    constexpr int bytes = N * sizeof(T);
-    typedef uint32_t words __attribute__((ext_vector_type(bytes >= 4 ? bytes / 4 : 1)));
-    if constexpr (bytes >= 4) {
-      words w = {};
-      if (d < D) w = *reinterpret_cast<const words*>(row + d);
-      __builtin_memcpy(&r, &w, bytes);
-    } else {
-      uint16_t w = 0;
-      if (d < D) w = *reinterpret_cast<const uint16_t*>(row + d);
-      __builtin_memcpy(&r, &w, bytes);
-    }
+  if constexpr (VEC && N * sizeof(T) >= 4) {
+    typedef uint32_t words __attribute__((ext_vector_type(Raw<T, N>::words)));
+    const words w = load_global<words>(row + (d < D ? d : 0));
+#pragma unroll
+    for (int i = 0; i < Raw<T, N>::words; ++i) r.w[i] = w[i];
+  } else if constexpr (VEC) {
+    r.w[0] = load_global<uint16_t>(row + (d < D ? d : 0));
   } else {
 #pragma unroll
+    for (int i = 0; i < Raw<T, N>::words; ++i) r.w[i] = 0;
+#pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (d + i < D)
-        r.x[i] = row[d + i];
-      else
-        r.x[i] = T{};
+      uint32_t x = 0;
+      if (d + i < D) {
+        if constexpr (sizeof(T) == 4) x = load_global<uint32_t>(row + d + i);
+        if constexpr (sizeof(T) == 2) x = load_global<uint16_t>(row + d + i);
+        if constexpr (sizeof(T) == 1) x = load_global<uint8_t>(row + d + i);
+      }
+      constexpr int per = 4 / sizeof(T);
+      r.w[i / per] |= x << (32 / per * (i % per));
     }
   }
   return r;
 }
-template <int N>
-__device__ __forceinline__ void floats(const Raw<float, N>& r, float (&x)[N]) {
+// Eight of them.
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, 8> eight(const Raw<T, N>& r, int first) {
+  Raw<T, 8> o;
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = r.x[i];
+  for (int i = 0; i < Raw<T, 8>::words; ++i) o.w[i] = r.w[first * (int)sizeof(T) / 4 + i];
+  return o;
+}
+
+// Eight cells as bf16 parts, and their squares.
+__device__ __forceinline__ Parts<3> parts_of(const Raw<float, 8>& r) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r.w[i]);
+  return split<3>(x);
+}
+__device__ __forceinline__ Parts<3> squares_of(const Raw<float, 8>& r) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r.w[i]) * __uint_as_float(r.w[i]);
+  return split<3>(x);
+}
+__device__ __forceinline__ Parts<1> parts_of(const Raw<__bf16, 8>& r) {
+  Parts<1> o;
+  __builtin_memcpy(&o.p[0], r.w, 16);
+  return o;
+}
+__device__ __forceinline__ Parts<2> squares_of(const Raw<__bf16, 8>& r) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float lo = __uint_as_float(r.w[i] << 16), hi = __uint_as_float(r.w[i] & 0xffff0000u);
+    x[2 * i] = lo * lo, x[2 * i + 1] = hi * hi;
+  }
+  return split<2>(x);
+}
+__device__ __forceinline__ Parts<1> parts_of(const Raw<uint8_t, 8>& r) {
+  bf2 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[i] = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.w[i / 2], 1.0f, true)
+                   : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.w[i / 2], 1.0f, false);
+  Parts<1> o;
+  __builtin_memcpy(&o.p[0], x, 16);
+  return o;
+}
+__device__ __forceinline__ Parts<1> squares_of(const Raw<uint8_t, 8>& r) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto p = (i & 1) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)r.w[i / 2], true)
+                           : __builtin_amdgcn_cvt_pk_f32_fp8((int)r.w[i / 2], false);
+    x[2 * i] = p[0] * p[0], x[2 * i + 1] = p[1] * p[1];
+  }
+  return split<1>(x);
+}
+
+// Eight rows of N cells as N columns of eight.
+template <int N>
+__device__ __forceinline__ void turn(const Raw<float, N> (&a)[8], Raw<float, 8> (&o)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[j].w[i] = a[i].w[j];
 }
 template <int N>
-__device__ __forceinline__ void floats(const Raw<__bf16, N>& r, float (&x)[N]) {
+__device__ __forceinline__ void turn(const Raw<__bf16, N> (&a)[8], Raw<__bf16, 8> (&o)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = (float)r.x[i];
+  for (int j = 0; j < N; j += 2)
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const uint32_t x = a[i].w[j / 2], y = a[i + 1].w[j / 2];
+      o[j].w[i / 2] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+      o[j + 1].w[i / 2] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+    }
 }
 template <int N>
-__device__ __forceinline__ void floats(const Raw<uint8_t, N>& r, float (&x)[N]) {
-  uint32_t w[(N + 3) / 4] = {};
-  __builtin_memcpy(w, &r, N);
+__device__ __forceinline__ void turn(const Raw<uint8_t, N> (&a)[8], Raw<uint8_t, 8> (&o)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const auto p = (i & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i / 4], true)
-                           : __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i / 4], false);
-    x[i] = p[0], x[i + 1] = p[1];
+  for (int j = 0; j < N; j += 4)
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const uint32_t x0 = a[i].w[j / 4], x1 = a[i + 1].w[j / 4], x2 = a[i + 2].w[j / 4], x3 = a[i + 3].w[j / 4];
+      const uint32_t l0 = __builtin_amdgcn_perm(x1, x0, 0x05010400u), l1 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
+      o[j].w[i / 4] = __builtin_amdgcn_perm(l1, l0, 0x05040100u);
+      o[j + 1].w[i / 4] = __builtin_amdgcn_perm(l1, l0, 0x07060302u);
+      if (j + 2 < N) {
+        const uint32_t h0 = __builtin_amdgcn_perm(x1, x0, 0x07030602u), h1 = __builtin_amdgcn_perm(x3, x2, 0x07030602u);
+        o[j + 2].w[i / 4] = __builtin_amdgcn_perm(h1, h0, 0x05040100u);
+        o[j + 3].w[i / 4] = __builtin_amdgcn_perm(h1, h0, 0x07060302u);
+      }
+    }
+}
+
+// The right operand of HT heads: column 4 p + r is part p of head r, or column r of each part.
+template <int HT>
+struct Right {
+  bf8 p[HT == 4 ? 1 : 3];
+};
+template <int HT, int PA>
+__device__ __forceinline__ acc4 mul(const Parts<PA>& a, const Right<HT>& b, acc4 c) {
+  if constexpr (HT == 4) {
+#pragma unroll
+    for (int i = PA - 1; i >= 0; --i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[0], c, 0, 0, 0);
+    return c;
+  } else {
+    Parts<3> x;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) x.p[i] = b.p[i];
+    return mma(a, x, c);
   }
 }
+// This lane's column of it.
+template <int HT>
+__device__ __forceinline__ Right<HT> right_of(const float (&x)[8], int col) {
+  const Parts<3> s = split<3>(x);
+  Right<HT> o;
+  if constexpr (HT == 4)
+    o.p[0] = col < 4 ? s.p[0] : (col < 8 ? s.p[1] : (col < 12 ? s.p[2] : bf8{}));
+  else
+    o.p[0] = s.p[0], o.p[1] = s.p[1], o.p[2] = s.p[2];
+  return o;
+}
+// A row's sum over the columns of a head's parts, in every one of them.
+template <int HT>
+__device__ __forceinline__ float over_parts(float x) {
+  if constexpr (HT == 4) {
+    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));  // 8 columns on
+    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x124, 0xf, 0xf, true));  // 4 columns on
+  }
+  return x;
+}
+
+// What a row holds that is not there.
+__device__ const uint4 kNothing[32] = {};
 
 // 2^(e - 127), e the biased exponent a row was written with
 __device__ __forceinline__ float power(uint32_t e) { return __builtin_ldexpf(1.0f, (int)e - 127); }
@@ -140,27 +264,32 @@ __device__ __forceinline__ void wave_slots(const Args& A, int64_t b, int g, int 
   wave_sync();
 }
 
-// First of the eight features that lane group k8 brings to step s. Where 64 features are 64
-// bytes, two steps share a lane's 16 bytes.
-template <typename Cell, int DP>
+// Eight features of every 32 to a lane group; where 64 features are 64 bytes, two steps share a
+// lane's 16 bytes.
+template <typename T, int DP>
+constexpr int group_of() {
+  return sizeof(T) == 1 && DP >= 64 ? 16 : 8;
+}
+template <typename T, int DP>
 __device__ __forceinline__ int feature(int s, int k8) {
-  if constexpr (sizeof(typename Cell::type) == 1 && DP >= 64) return 64 * (s >> 1) + 16 * k8 + 8 * (s & 1);
-  return 32 * s + 8 * k8;
+  constexpr int N = group_of<T, DP>(), per = N / 8;
+  return 4 * N * (s / per) + N * k8 + 8 * (s % per);
 }
 
-// Blocks of a CU: the operands of long heads in several parts, or gathered cell by cell, take a
-// SIMD's registers for one wave.
-template <typename Cell, int DP, bool VEC>
-constexpr int blocks_of() {
-  return DP == 128 && !(VEC && sizeof(typename Cell::type) == 1) ? 1 : 2;
-}
-
-// HT query heads at a time: 4 of the 16 columns where a key head has no more (a wave's tables in
-// LDS are a quarter, so a CU holds two blocks).
+// Blocks of a CU: fp32 cells of long heads, and 16 columns of three parts, take a SIMD's registers
+// for one wave; so do cells gathered one by one.
 template <typename Cell, int DP, bool VEC, int HT>
-__global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC>())) scores_kernel(const Args A) {
+constexpr int blocks_of() {
+  if (DP < 128) return VEC || HT == 4 ? 2 : 1;
+  return VEC && HT == 4 && sizeof(typename Cell::type) < 4 ? 2 : 1;
+}
+
+// HT query heads at a time.
+template <typename Cell, int DP, bool VEC, int HT>
+__global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) scores_kernel(const Args A) {
   typedef typename Cell::type T;
-  constexpr int S = DP / 32, P1 = CellParts<Cell>::one, P2 = CellParts<Cell>::two;
+  constexpr int S = DP / 32, N = group_of<T, DP>(), L = DP / (4 * N);  // L loads of N features
+  constexpr int F = 4 / sizeof(T);                                     // tiles in flight
   constexpr bool scaled_rows = sizeof(T) == 1;
   constexpr int kRow = 64 + 4;  // floats of a head's 64 scores, banks apart
   __shared__ int64_t slots[kWaves][kWaveKeys];
@@ -173,76 +302,75 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC>())) scores
   int64_t* slot = slots[wave];
   float *pm = powers[wave], *pS = pm + (scaled_rows ? kWaveKeys : 0);
   if (from < to) wave_slots<Cell>(A, b, g, from, to, lane, 0, slot, pm, pS);
+  const int head = HT == 4 ? col & 3 : col;
   for (int r0 = 0; r0 < A.R; r0 += HT) {
     const int n = A.R - r0 < HT ? A.R - r0 : HT;
     const int64_t h = b * A.H + g * A.R + r0;
     float mt[HT] = {}, vt[HT] = {};
     if (from < to) {
-      Parts<3> q[S], Q[S], P[S];  // q, Sq, Sq + q^2, scaled
-      const int64_t qa = b * A.lq.sb + (int64_t)(g * A.R + r0 + (col < n ? col : n - 1)) * A.lq.sh;
+      Right<HT> q[S], Q[S], P[S];  // q, Sq, Sq + q^2, scaled
+      const int64_t qa = b * A.lq.sb + (int64_t)(g * A.R + r0 + (head < n ? head : n - 1)) * A.lq.sh;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         float x[8], X[8], y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int d = feature<Cell, DP>(s, k8) + i;
+          const int d = feature<T, DP>(s, k8) + i;
           x[i] = d < D ? A.mq[qa + d] * A.c1 : 0.f, X[i] = d < D ? A.Sq[qa + d] * A.c2 : 0.f;
           y[i] = fmaf(x[i], x[i], X[i]);
         }
-        q[s] = split<3>(x), Q[s] = split<3>(X), P[s] = split<3>(y);
+        q[s] = right_of<HT>(x, col), Q[s] = right_of<HT>(X, col), P[s] = right_of<HT>(y, col);
       }
       const int tiles = (to - from + 15) / 16;
-      Raw<T, 8> km[S], kS[S];
-      auto fetch = [&](int t) {
+      Raw<T, N> km[F][L], kS[F][L];
+      auto fetch = [&](int t, int f) {
         const int64_t row = slot[16 * t + col], at = (row < 0 ? 0 : row) * D;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const int d = feature<Cell, DP>(s, k8);
-          km[s] = load_raw<VEC, T, 8>(static_cast<const T*>(A.c.km) + at, d, D);
-          kS[s] = load_raw<VEC, T, 8>(static_cast<const T*>(A.c.kS) + at, d, D);
+        for (int l = 0; l < L; ++l) {
+          const int d = 4 * N * l + N * k8;
+          km[f][l] = load_raw<VEC, T, N>(static_cast<const T*>(A.c.km) + at, d, D);
+          kS[f][l] = load_raw<VEC, T, N>(static_cast<const T*>(A.c.kS) + at, d, D);
         }
       };
-      fetch(0);
-      for (int t = 0; t < tiles; ++t) {
-        acc4 m = {0, 0, 0, 0}, v = m, w = m;
-        Raw<T, 8> am[S], aS[S];
 #pragma unroll
-        for (int s = 0; s < S; ++s) am[s] = km[s], aS[s] = kS[s];
-        if (t + 1 < tiles) fetch(t + 1);
+      for (int f = 0; f < F; ++f)
+        if (f < tiles) fetch(f, f);
+      for (int t0 = 0; t0 < tiles; t0 += 4) {  // 64 keys
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          float x[8], y[8];
-          floats(am[s], x);
-          m = mma(split<P1>(x), q[s], m);
+        for (int u = 0; u < 4; ++u) {
+          const int t = t0 + u, f = u % F;
+          if (t >= tiles) continue;
+          acc4 m = {0, 0, 0, 0}, v = m, w = m;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= x[i];
-          floats(aS[s], y);
+          for (int s = 0; s < S; ++s) {
+            const Raw<T, 8> x = eight(km[f][8 * s / N], 8 * s % N), y = eight(kS[f][8 * s / N], 8 * s % N);
+            m = mul<HT>(parts_of(x), q[s], m);
+            v = mul<HT>(squares_of(x), Q[s], v);
+            if constexpr (scaled_rows)
+              w = mul<HT>(parts_of(y), P[s], w);
+            else
+              v = mul<HT>(parts_of(y), P[s], v);
+          }
+          if (t + F < tiles) fetch(t + F, f);
           if constexpr (scaled_rows) {
-            v = mma(split<P2>(x), Q[s], v);
-            w = mma(split<P1>(y), P[s], w);
-          } else {
-            v = mma(split<P2>(x), Q[s], v);
-            v = mma(split<P1>(y), P[s], v);
-          }
-        }
-        const int at = 16 * (t & 3) + 4 * k8;  // of the 64 keys under way
-        if constexpr (scaled_rows) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float a = pm[16 * t + 4 * k8 + r], s = pS[16 * t + 4 * k8 + r];
-            m[r] *= a;
-            v[r] = fmaf(v[r] * a, a, w[r] * s);
+            for (int r = 0; r < 4; ++r) {
+              const float a = pm[16 * t + 4 * k8 + r], s = pS[16 * t + 4 * k8 + r];
+              m[r] *= a;
+              v[r] = fmaf(v[r] * a, a, w[r] * s);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) m[r] = over_parts<HT>(m[r]), v[r] = over_parts<HT>(v[r]);
+          if (col < n) {
+            *reinterpret_cast<acc4*>(&tile[wave][0][col * kRow + 16 * u + 4 * k8]) = m;
+            *reinterpret_cast<acc4*>(&tile[wave][1][col * kRow + 16 * u + 4 * k8]) = v;
           }
         }
-        if (col < n) {
-          *reinterpret_cast<acc4*>(&tile[wave][0][col * kRow + at]) = m;
-          *reinterpret_cast<acc4*>(&tile[wave][1][col * kRow + at]) = v;
-        }
-        if ((t & 3) != 3 && t + 1 < tiles) continue;
-        // 64 keys: a lane to a key, the heads one after another
+        // a lane to a key, the heads one after another
         wave_sync();
-        const int key = (t & ~3) * 16 + lane;
-        const bool on = from + key < to, there = on && slot[key < A.wave_keys ? key : 0] >= 0;
+        const int key = 16 * t0 + lane;
+        const bool on = from + key < to, there = on && slot[key] >= 0;
 #pragma unroll
         for (int r = 0; r < HT; ++r) {
           if (r >= n) continue;
@@ -270,15 +398,15 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC>())) scores
 // 8 k8 + 7 of every 32: the j-th of them, over the eight keys, is its share of a product whose rows
 // are the features ND r + j. So a load covers whole rows and no value moves between lanes.
 template <typename Cell, int DP, bool VEC, int HT>
-__global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, VEC>())) values_kernel(const Args A) {
+__global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, VEC, HT>())) values_kernel(const Args A) {
   typedef typename Cell::type T;
-  constexpr int ND = DP / 16, P1 = CellParts<Cell>::one, P2 = CellParts<Cell>::two;
-  constexpr bool scaled_rows = sizeof(T) == 1;
-  constexpr int kRow = 64 + 8;  // keys of a head's weights, banks apart
-  constexpr int kPart = HT * kRow;
+  constexpr int ND = DP / 16;
+  constexpr bool scaled_rows = sizeof(T) == 1, ahead = sizeof(T) < 4;  // the next 32 keys' cells are in flight
+  constexpr int kRow = 64 + 8;                // keys of a column's weights, banks apart
+  constexpr int kCols = HT == 4 ? 16 : 3 * HT;  // columns: part p of head r is HT p + r
   __shared__ int64_t slots[kWaves][kWaveKeys];
   __shared__ float powers[kWaves][scaled_rows ? 2 * kWaveKeys : 1];
-  __shared__ __align__(16) __bf16 weights[kWaves][9 * kPart];  // [w, kw, kw + w^2][part][head][key]
+  __shared__ __align__(16) __bf16 weights[kWaves][3 * kCols * kRow];  // [w, kw, kw + w^2][column][key]
   __shared__ RowSums row[HT];
   __shared__ float totals[kWaves][HT];
   const int64_t b = blockIdx.z;
@@ -290,10 +418,23 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
   int64_t* slot = slots[wave];
   float *pm = powers[wave], *pS = pm + (scaled_rows ? kWaveKeys : 0);
   if (from < to) wave_slots<Cell>(A, b, g, from, to, lane, 2, slot, pm, pS);
+  __bf16* W = weights[wave];
+  Raw<T, ND> am[8], aS[8];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // what is not there weighs nothing, whatever its slot holds
+      const int64_t at = slot[i0 + 8 * k8 + i];
+      const T* const none = reinterpret_cast<const T*>(kNothing);
+      am[i] = load_raw<VEC, T, ND>(at < 0 ? none : static_cast<const T*>(A.c.vm) + at * D, ND * col, D);
+      aS[i] = load_raw<VEC, T, ND>(at < 0 ? none : static_cast<const T*>(A.c.vS) + at * D, ND * col, D);
+    }
+  };
   for (int r0 = 0; r0 < A.R; r0 += HT) {
     const int n = A.R - r0 < HT ? A.R - r0 : HT;
     const int64_t h = b * A.H + g * A.R + r0;
     __syncthreads();  // the heads before are done with the sums and weights
+    if (ahead && from < to) fetch(0);
     for (int r = wave; r < n; r += kWaves) {
       const float* p = A.sums + (h + r) * A.splits * kWaves * 2;
       float mt = 0.f, vt = 0.f;
@@ -301,12 +442,13 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
       mt = wave_sum(mt), vt = wave_sum(vt);
       if (lane == 0) row[r] = row_sums(mt, vt);
     }
+    // columns that no head writes
+    for (int i = lane; i < 3 * kCols * kRow / 8; i += 64) reinterpret_cast<bf8*>(W)[i] = bf8{};
     __syncthreads();
     acc4 om[ND], oS[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) om[j] = oS[j] = acc4{0, 0, 0, 0};
     float total[HT] = {};
-    __bf16* W = weights[wave];
     for (int key0 = from; key0 < to; key0 += 64) {
       const int i0 = key0 - from;
       {
@@ -314,15 +456,15 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
         const bool on = key0 + lane < to;
         float a = 1.f, s = 1.f;
         if constexpr (scaled_rows) a = pm[i0 + lane], s = pS[i0 + lane];
+        float2 z[HT];
+#pragma unroll
+        for (int r = 0; r < HT; ++r)
+          z[r] = on && r < n ? A.scores[(h + r) * A.max_len + key0 + lane] : make_float2(0.f, 0.f);
 #pragma unroll
         for (int r = 0; r < HT; ++r) {
           if (r >= n) continue;
-          float w = 0.f, k = 0.f;
-          const float2 x = on ? A.scores[(h + r) * A.max_len + key0 + lane] : make_float2(0.f, 0.f);
-          if (x.x > 0.f) {
-            const Weight o = weigh(Rectified{x.x, x.y, 0.f, 0.f}, row[r]);
-            w = o.w, k = o.k;
-          }
+          const Weight o = weigh(Rectified{z[r].x, z[r].y, 0.f, 0.f}, row[r]);
+          const float w = z[r].x > 0.f ? o.w : 0.f, k = z[r].x > 0.f ? o.k : 0.f;
           total[r] += w;
           // the powers of two of the rows go into their weights
           const float w2 = w * w, kw = k * w2;
@@ -333,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
 #pragma unroll
             for (int p = 0; p < 3; ++p) {
               const __bf16 part = (__bf16)rest;
-              W[(3 * q + p) * kPart + r * kRow + lane] = part;
+              W[(kCols * q + HT * p + r) * kRow + lane] = part;
               rest -= (float)part;
             }
           }
@@ -343,39 +485,21 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         if (key0 + 32 * half >= to) break;
-        Raw<T, ND> am[8], aS[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int64_t at = slot[i0 + 32 * half + 8 * k8 + i], o = (at < 0 ? 0 : at) * D;
-          am[i] = load_raw<VEC, T, ND>(static_cast<const T*>(A.c.vm) + o, ND * col, D);
-          aS[i] = load_raw<VEC, T, ND>(static_cast<const T*>(A.c.vS) + o, ND * col, D);
-        }
-        Parts<3> w[3];
+        if (!ahead) fetch(i0 + 32 * half);
+        Raw<T, 8> x[ND], y[ND];
+        turn(am, x), turn(aS, y);
+        if (ahead && key0 + 32 * half + 32 < to) fetch(i0 + 32 * half + 32);
+        Right<HT> w[3];
 #pragma unroll
         for (int q = 0; q < 3; ++q)
 #pragma unroll
-          for (int p = 0; p < 3; ++p)
-            w[q].p[p] = *reinterpret_cast<const bf8*>(W + (3 * q + p) * kPart + (col < n ? col : n - 1) * kRow + 32 * half + 8 * k8);
-        float x[8][ND], y[8][ND];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          floats(am[i], x[i]), floats(aS[i], y[i]);
-          // what is not there weighs nothing, whatever its slot holds
-          if (slot[i0 + 32 * half + 8 * k8 + i] < 0) {
-#pragma unroll
-            for (int j = 0; j < ND; ++j) x[i][j] = y[i][j] = 0.f;
-          }
-        }
+          for (int p = 0; p < (HT == 4 ? 1 : 3); ++p)
+            w[q].p[p] = *reinterpret_cast<const bf8*>(W + (kCols * q + HT * p + col) * kRow + 32 * half + 8 * k8);
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
-          float e[8], f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = x[i][j], f[i] = y[i][j];
-          om[j] = mma(split<P1>(e), w[0], om[j]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] *= e[i];
-          oS[j] = mma(split<P2>(e), w[1], oS[j]);
-          oS[j] = mma(split<P1>(f), w[2], oS[j]);
+          om[j] = mul<HT>(parts_of(x[j]), w[0], om[j]);
+          oS[j] = mul<HT>(squares_of(x[j]), w[1], oS[j]);
+          oS[j] = mul<HT>(parts_of(y[j]), w[2], oS[j]);
         }
       }
       wave_sync();
@@ -397,8 +521,10 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
 #pragma unroll
       for (int j = 0; j < ND; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (col < HT) red[(wave * DP + ND * (4 * k8 + r) + j) * HT + col] = k == 0 ? om[j][r] : oS[j][r];
+        for (int r = 0; r < 4; ++r) {
+          const float x = over_parts<HT>(k == 0 ? om[j][r] : oS[j][r]);
+          if (col < HT) red[(wave * DP + ND * (4 * k8 + r) + j) * HT + col] = x;
+        }
       __syncthreads();
       for (int i = threadIdx.x; i < n * D; i += kThreads) {
         const int r = i / D, f = i - r * D;
@@ -417,21 +543,27 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
   }
 }
 
-// A wave to a query head: the splits that its sequence's length reaches, in order.
+// A block to a query head, a thread to a sum: the splits that its sequence's length reaches, in order.
 __global__ void __launch_bounds__(kThreads) join_kernel(const Args A) {
-  const int64_t h = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (h >= A.B * A.H) return;
+  __shared__ float totals[kWaves];
+  const int64_t h = blockIdx.x;
   const int D = A.c.D, step = 2 * D + 1, block_keys = kWaves * A.wave_keys;
   const int len = length_of(A, h / A.H), n = len <= block_keys ? 1 : (len + block_keys - 1) / block_keys;
   const float* p = A.parts + h * A.splits * step;
-  float sum = 0.f;
-  for (int k = 0; k < n; ++k) sum += p[k * step + 2 * D];
-  const float inv = fast_rcp(fmaxf(sum, kRemaxFloor)), inv2 = inv * inv;
-  for (int f = threadIdx.x & 63; f < D; f += 64) {
-    float x = 0.f, y = 0.f;
-    for (int k = 0; k < n; ++k) x += p[k * step + f], y += p[k * step + D + f];
-    A.mo[h * D + f] = x * inv, A.So[h * D + f] = y * inv2;
+  float sum = 0.f, x = 0.f;
+  for (int k = threadIdx.x; k < n; k += kThreads) sum += p[(int64_t)k * step + 2 * D];
+  const int f = threadIdx.x;  // 2 D <= kThreads
+  if (f < 2 * D) {
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) x += p[(int64_t)k * step + f];
   }
+  sum = wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) totals[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+  const float inv = fast_rcp(fmaxf(sum, kRemaxFloor));
+  if (f < D) A.mo[h * D + f] = x * inv;
+  else if (f < 2 * D) A.So[h * D + f - D] = x * inv * inv;
 }
 
 // Keys of a wave: as many as leave a few blocks for each of the 256 CUs.
@@ -513,6 +645,6 @@ extern "C" int tagi_remax_attention_step(const float* mq, const float* Sq, const
     launch_dim<Bf16Cell>(a, vec, grid, s);
   else
     launch_dim<Fp8Cell>(a, vec, grid, s);
-  hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv(B * H, kWaves)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(B * H)), dim3(kThreads), 0, s, a);
   return check_launch(what);
 }
