@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kWaveKeys = 256;  // most keys of a wave: their slots and scales stay in LDS
+constexpr int kWaveKeys = 512;  // most keys of a wave: their slots and scales stay in LDS
 
 // Parts of a cell's value and of its square.
 template <typename Cell>
@@ -242,20 +242,34 @@ __device__ __forceinline__ float over_parts(float x) {
   return x;
 }
 
+// Eight features of a query from d on, any behind D. Loads without a branch between them: all are in
+// flight at once.
+__device__ __forceinline__ void load_query(const float* p, int d, int D, float (&x)[8]) {
+  const bool whole = D % 8 == 0;
+  if (whole) {
+    const f4u a = load4(p + (d < D ? d : 0)), b = load4(p + (d < D ? d : 0) + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < 4 ? a[i & 3] : b[i & 3];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[d + i < D ? d + i : 0];
+  }
+}
+
 // What a row holds that is not there.
 __device__ const uint4 kNothing[32] = {};
 
 // 2^(e - 127), e the biased exponent a row was written with
 __device__ __forceinline__ float power(uint32_t e) { return __builtin_ldexpf(1.0f, (int)e - 127); }
 
-// Slots of a wave's keys (a page lookup each), -1 where there is no token; for 8-bit cells also
+// Where a wave's keys begin in the pools (a page lookup each), -1 where there is no token; for 8-bit cells also
 // the powers of two of their means and variances.
 template <typename Cell>
 __device__ __forceinline__ void wave_slots(const Args& A, int64_t b, int g, int from, int to, int lane, int first_scale,
                                            int64_t* slot, float* pm, float* pS) {
   for (int i = lane; i < A.wave_keys; i += 64) {
     const int64_t row = from + i < to ? cache_row(A.c, b, from + i, g) : -1;
-    slot[i] = row;
+    slot[i] = row < 0 ? -1 : row * A.c.D;
     if constexpr (sizeof(typename Cell::type) == 1) {
       const uint32_t e = row < 0 ? 0x7f7f7f7fu : reinterpret_cast<const uint32_t*>(A.c.scales)[row];
       pm[i] = power((e >> (8 * first_scale)) & 255), pS[i] = power((e >> (8 * first_scale + 8)) & 255);
@@ -289,7 +303,7 @@ template <typename Cell, int DP, bool VEC, int HT>
 __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) scores_kernel(const Args A) {
   typedef typename Cell::type T;
   constexpr int S = DP / 32, N = group_of<T, DP>(), L = DP / (4 * N);  // L loads of N features
-  constexpr int F = 4 / sizeof(T);                                     // tiles in flight
+  constexpr int F = VEC && HT == 4 ? 4 / sizeof(T) : 1;                // tiles in flight
   constexpr bool scaled_rows = sizeof(T) == 1;
   constexpr int kRow = 64 + 4;  // floats of a head's 64 scores, banks apart
   __shared__ int64_t slots[kWaves][kWaveKeys];
@@ -301,7 +315,6 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) sc
   const int to = from + A.wave_keys < len ? from + A.wave_keys : len;
   int64_t* slot = slots[wave];
   float *pm = powers[wave], *pS = pm + (scaled_rows ? kWaveKeys : 0);
-  if (from < to) wave_slots<Cell>(A, b, g, from, to, lane, 0, slot, pm, pS);
   const int head = HT == 4 ? col & 3 : col;
   for (int r0 = 0; r0 < A.R; r0 += HT) {
     const int n = A.R - r0 < HT ? A.R - r0 : HT;
@@ -310,21 +323,31 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) sc
     if (from < to) {
       Right<HT> q[S], Q[S], P[S];  // q, Sq, Sq + q^2, scaled
       const int64_t qa = b * A.lq.sb + (int64_t)(g * A.R + r0 + (head < n ? head : n - 1)) * A.lq.sh;
+      float x[S][8], X[S][8];
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        float x[8], X[8], y[8];
+        load_query(A.mq + qa, feature<T, DP>(s, k8), D, x[s]);
+        load_query(A.Sq + qa, feature<T, DP>(s, k8), D, X[s]);
+      }
+      // while the queries are on their way
+      if (r0 == 0) wave_slots<Cell>(A, b, g, from, to, lane, 0, slot, pm, pS);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int d = feature<T, DP>(s, k8) + i;
-          x[i] = d < D ? A.mq[qa + d] * A.c1 : 0.f, X[i] = d < D ? A.Sq[qa + d] * A.c2 : 0.f;
-          y[i] = fmaf(x[i], x[i], X[i]);
+          const bool on = feature<T, DP>(s, k8) + i < D;
+          x[s][i] = on ? x[s][i] * A.c1 : 0.f, X[s][i] = on ? X[s][i] * A.c2 : 0.f;
+          y[i] = fmaf(x[s][i], x[s][i], X[s][i]);
         }
-        q[s] = right_of<HT>(x, col), Q[s] = right_of<HT>(X, col), P[s] = right_of<HT>(y, col);
+        q[s] = right_of<HT>(x[s], col), Q[s] = right_of<HT>(X[s], col), P[s] = right_of<HT>(y, col);
       }
-      const int tiles = (to - from + 15) / 16;
+      // whole groups of four tiles, and every fetch is made (the last ones again): what waits for a
+      // load counts those behind it, and behind a branch it would have to wait for all
+      const int tiles = (to - from + 63) / 64 * 4;
       Raw<T, N> km[F][L], kS[F][L];
       auto fetch = [&](int t, int f) {
-        const int64_t row = slot[16 * t + col], at = (row < 0 ? 0 : row) * D;
+        const int64_t row = slot[16 * t + col], at = row < 0 ? 0 : row;
 #pragma unroll
         for (int l = 0; l < L; ++l) {
           const int d = 4 * N * l + N * k8;
@@ -333,13 +356,14 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) sc
         }
       };
 #pragma unroll
-      for (int f = 0; f < F; ++f)
-        if (f < tiles) fetch(f, f);
+      for (int f = 0; f < F; ++f) {
+        fetch(f, f);
+        __builtin_amdgcn_sched_barrier(0);  // in this order: it is what the waits count
+      }
       for (int t0 = 0; t0 < tiles; t0 += 4) {  // 64 keys
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int t = t0 + u, f = u % F;
-          if (t >= tiles) continue;
           acc4 m = {0, 0, 0, 0}, v = m, w = m;
 #pragma unroll
           for (int s = 0; s < S; ++s) {
@@ -351,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) sc
             else
               v = mul<HT>(parts_of(y), P[s], v);
           }
-          if (t + F < tiles) fetch(t + F, f);
+          fetch(t + F < tiles ? t + F : t, f);
           if constexpr (scaled_rows) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -373,10 +397,10 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) sc
         const bool on = from + key < to, there = on && slot[key] >= 0;
 #pragma unroll
         for (int r = 0; r < HT; ++r) {
-          if (r >= n) continue;
+          if (HT > 4 && r >= n) continue;
           Rectified z = rectify(tile[wave][0][r * kRow + lane], tile[wave][1][r * kRow + lane]);
-          if (!there) z.mm = z.vm = 0.f;
-          if (on) A.scores[(h + r) * A.max_len + from + key] = make_float2(z.mm, z.vm);
+          z.mm = there ? z.mm : 0.f, z.vm = there ? z.vm : 0.f;
+          if (on && r < n) A.scores[(h + r) * A.max_len + from + key] = make_float2(z.mm, z.vm);
           mt[r] += z.mm, vt[r] += z.vm;
         }
         wave_sync();
@@ -384,9 +408,9 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) sc
     }
 #pragma unroll
     for (int r = 0; r < HT; ++r) {
-      if (r >= n) continue;
+      if (HT > 4 && r >= n) continue;
       const float x = wave_sum(mt[r]), y = wave_sum(vt[r]);
-      if (lane == 0) {
+      if (lane == 0 && r < n) {
         float* o = A.sums + ((h + r) * A.splits * kWaves + (int)blockIdx.x * kWaves + wave) * 2;
         o[0] = x, o[1] = y;
       }
@@ -401,7 +425,7 @@ template <typename Cell, int DP, bool VEC, int HT>
 __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, VEC, HT>())) values_kernel(const Args A) {
   typedef typename Cell::type T;
   constexpr int ND = DP / 16;
-  constexpr bool scaled_rows = sizeof(T) == 1, ahead = sizeof(T) < 4;  // the next 32 keys' cells are in flight
+  constexpr bool scaled_rows = sizeof(T) == 1, ahead = DP * sizeof(T) <= 128;  // the next 32 keys' cells are in flight
   constexpr int kRow = 64 + 8;                // keys of a column's weights, banks apart
   constexpr int kCols = HT == 4 ? 16 : 3 * HT;  // columns: part p of head r is HT p + r
   __shared__ int64_t slots[kWaves][kWaveKeys];
@@ -420,14 +444,17 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
   if (from < to) wave_slots<Cell>(A, b, g, from, to, lane, 2, slot, pm, pS);
   __bf16* W = weights[wave];
   Raw<T, ND> am[8], aS[8];
+  const T* none = reinterpret_cast<const T*>(kNothing);
+  asm volatile("" : "+v"(none));  // its address is kept, not formed again
   auto fetch = [&](int i0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       // what is not there weighs nothing, whatever its slot holds
       const int64_t at = slot[i0 + 8 * k8 + i];
-      const T* const none = reinterpret_cast<const T*>(kNothing);
-      am[i] = load_raw<VEC, T, ND>(at < 0 ? none : static_cast<const T*>(A.c.vm) + at * D, ND * col, D);
-      aS[i] = load_raw<VEC, T, ND>(at < 0 ? none : static_cast<const T*>(A.c.vS) + at * D, ND * col, D);
+      const T *m = static_cast<const T*>(A.c.vm) + at, *S = static_cast<const T*>(A.c.vS) + at;
+      asm("" : "+v"(m), "+v"(S));  // formed before the choice, which then is no branch
+      am[i] = load_raw<VEC, T, ND>(at < 0 ? none : m, ND * col, D);
+      aS[i] = load_raw<VEC, T, ND>(at < 0 ? none : S, ND * col, D);
     }
   };
   for (int r0 = 0; r0 < A.R; r0 += HT) {
@@ -449,22 +476,25 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
 #pragma unroll
     for (int j = 0; j < ND; ++j) om[j] = oS[j] = acc4{0, 0, 0, 0};
     float total[HT] = {};
+    float2 z[HT];
+    auto fetch_scores = [&](int key0) {
+      const int key = key0 + lane < to ? key0 + lane : from;
+#pragma unroll
+      for (int r = 0; r < HT; ++r) z[r] = A.scores[(h + (r < n ? r : 0)) * A.max_len + key];
+    };
+    if (from < to) fetch_scores(from);
     for (int key0 = from; key0 < to; key0 += 64) {
       const int i0 = key0 - from;
       {
         // a lane to a key
-        const bool on = key0 + lane < to;
         float a = 1.f, s = 1.f;
         if constexpr (scaled_rows) a = pm[i0 + lane], s = pS[i0 + lane];
-        float2 z[HT];
-#pragma unroll
-        for (int r = 0; r < HT; ++r)
-          z[r] = on && r < n ? A.scores[(h + r) * A.max_len + key0 + lane] : make_float2(0.f, 0.f);
 #pragma unroll
         for (int r = 0; r < HT; ++r) {
-          if (r >= n) continue;
+          if (HT > 4 && r >= n) continue;
           const Weight o = weigh(Rectified{z[r].x, z[r].y, 0.f, 0.f}, row[r]);
-          const float w = z[r].x > 0.f ? o.w : 0.f, k = z[r].x > 0.f ? o.k : 0.f;
+          const bool there = key0 + lane < to && r < n && z[r].x > 0.f;
+          const float w = there ? o.w : 0.f, k = there ? o.k : 0.f;
           total[r] += w;
           // the powers of two of the rows go into their weights
           const float w2 = w * w, kw = k * w2;
@@ -482,13 +512,13 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
         }
       }
       wave_sync();
-#pragma unroll 1
+      fetch_scores(key0 + 64 < to ? key0 + 64 : key0);
+#pragma unroll
       for (int half = 0; half < 2; ++half) {
-        if (key0 + 32 * half >= to) break;
         if (!ahead) fetch(i0 + 32 * half);
         Raw<T, 8> x[ND], y[ND];
         turn(am, x), turn(aS, y);
-        if (ahead && key0 + 32 * half + 32 < to) fetch(i0 + 32 * half + 32);
+        if (ahead) fetch(half == 0 || key0 + 64 < to ? i0 + 32 * half + 32 : i0);
         Right<HT> w[3];
 #pragma unroll
         for (int q = 0; q < 3; ++q)
@@ -506,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
     }
 #pragma unroll
     for (int r = 0; r < HT; ++r) {
-      if (r >= n) continue;
+      if (HT > 4 && r >= n) continue;
       const float x = wave_sum(total[r]);
       if (lane == 0) totals[wave][r] = x;
     }
