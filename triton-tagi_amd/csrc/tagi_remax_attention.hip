@@ -32,9 +32,11 @@ typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kTile = 32;           // keys (or rows) walked at a time
 constexpr int kMaxDim = 128;
 constexpr int kLdsBytes = 160 * 1024;
-// Walked by one block at most: the matrix cores cut sums off (they do not round them), about 1e-8
-// of the sum for every product added; the splits are added in fp32.
-constexpr int kMostWalked = 2048;
+// Walked by one block at most: the matrix cores cut sums off (they do not round them), and what is
+// lost of a sum of positive terms grows with their number (late rows' variances: 1.6e-6 after 2048
+// keys, 1e-6 after 1024; the join takes 23 us more of 6.2 ms at 4096 tokens). The gradients' terms have
+// both signs: 1e-6 after 2048. The splits are added in fp32.
+constexpr int kMostWalked = 1024, kMostWalkedBack = 2048;
 
 struct Args {
   const float *mq, *Sq, *mk, *Sk, *mv, *Sv, *dm, *dS;
@@ -204,23 +206,67 @@ __device__ __forceinline__ void load_right(const float* pm, const float* pS, int
   }
 }
 
-// Moments of the scores of 16 walked rows: m = a0 b0, v = a1 b1 + a2 b2 with a0, a1, a2 the parts
-// 0, 3, 6 of the tile.
+// The same in two halves: the products of the first parts, and the others. The matrix cores cut
+// sums off: a score's mean, on which its tail's weight depends as exp(-m^2 / 2 v), takes the others
+// while the sum is small, and then is cut once a step instead of six times (rows of few keys: 1.6e-6
+// of the variances wrong before, 6e-7 so).
 template <int DP>
-__device__ __forceinline__ void scores(const short* tile, int kt, int lane, const Right<DP>& b0, const Right<DP>& b1,
-                                       const Right<DP>& b2, acc4& m, acc4& v) {
-  m = acc4{0, 0, 0, 0}, v = m;
+__device__ __forceinline__ acc4 mma_first(const short* tile, int first, int kt, int s, int lane, const Parts<3>& b, acc4 c) {
+  const bf8 a = *reinterpret_cast<const bf8*>(tile + hidden(piece<DP>(first, 0, 0)) + 8 * lane + piece<DP>(0, kt, s));
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b.p[0], c, 0, 0, 0);
+}
+template <int DP, bool FIRST>
+__device__ __forceinline__ void mma_left(const short* tile, int first, int kt, int s, int lane, const Parts<3>& b, acc4& c,
+                                         acc4& rest) {
+  const short* at = tile + hidden(piece<DP>(first, 0, 0)) + 8 * lane;
 #pragma unroll
-  for (int s = 0; s < DP / 32; ++s) {
-    m = mma_left<DP>(tile, 0, kt, s, lane, b0.p[s], m);
-    v = mma_left<DP>(tile, 3, kt, s, lane, b1.p[s], v);
-    v = mma_left<DP>(tile, 6, kt, s, lane, b2.p[s], v);
+  for (int i = 2; i >= 0; --i) {
+    const bf8 a = *reinterpret_cast<const bf8*>(at + piece<DP>(i, kt, s));
+#pragma unroll
+    for (int j = 2 - i; j >= 0; --j) {
+      if (i + j > 0)
+        rest = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b.p[j], rest, 0, 0, 0);
+      else if (FIRST)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b.p[j], c, 0, 0, 0);
+    }
   }
 }
 
 // Nothing is scheduled across: operands of later products loaded early would take the registers
 // of those in use.
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// Moments of the scores of 16 walked rows: m = a0 b0, v = a1 b1 + a2 b2 with a0, a1, a2 the parts
+// 0, 3, 6 of the tile.
+template <int DP>
+__device__ __forceinline__ void scores(const short* tile, int kt, int lane, const Right<DP>& b0, const Right<DP>& b1,
+                                       const Right<DP>& b2, acc4& m, acc4& v) {
+  acc4 dm = {0, 0, 0, 0}, dv = dm;
+  if constexpr (DP < 128) {
+    m = v = dm;
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) {
+      mma_left<DP, true>(tile, 0, kt, s, lane, b0.p[s], m, dm);
+      mma_left<DP, true>(tile, 3, kt, s, lane, b1.p[s], v, dv);
+      mma_left<DP, true>(tile, 6, kt, s, lane, b2.p[s], v, dv);
+    }
+    m += dm, v += dv;
+  } else {  // the registers of two more sums are not there: the keys' first parts are read again
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) {
+      mma_left<DP, false>(tile, 0, kt, s, lane, b0.p[s], m, dm);
+      mma_left<DP, false>(tile, 3, kt, s, lane, b1.p[s], v, dv);
+      mma_left<DP, false>(tile, 6, kt, s, lane, b2.p[s], v, dv);
+    }
+    m = dm, v = dv;
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) {
+      m = mma_first<DP>(tile, 0, kt, s, lane, b0.p[s], m);
+      v = mma_first<DP>(tile, 3, kt, s, lane, b1.p[s], v);
+      v = mma_first<DP>(tile, 6, kt, s, lane, b2.p[s], v);
+    }
+  }
+}
 
 // The sum over the four lane groups that share a column.
 __device__ __forceinline__ float group_sum(float x) {
@@ -372,26 +418,36 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
     if (key0 < wave_to) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
+        // the sums that scores() makes, to the last bit: where a row has few keys, its weights depend on
+        // their differences from the row's sums
         acc4 m[NC], v[NC];
+        if constexpr (DP == 128) {
+          scores<DP>(tile, kt, lane, q[0], Q[0], P[0], m[0], v[0]);
+        } else {
+          acc4 dm[NC], dv[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) m[c] = v[c] = acc4{0, 0, 0, 0};
+          for (int c = 0; c < NC; ++c) m[c] = v[c] = dm[c] = dv[c] = acc4{0, 0, 0, 0};
 #pragma unroll
-        for (int st = 0; st < DP / 32; ++st) {
-          const short* at = tile + piece<DP>(0, kt, st) + 8 * lane;
+          for (int st = 0; st < DP / 32; ++st) {
+            const short* at = tile + piece<DP>(0, kt, st) + 8 * lane;
 #pragma unroll
-          for (int i = 2; i >= 0; --i) {
-            const bf8 k = *reinterpret_cast<const bf8*>(at + piece<DP>(i, 0, 0)),
-                      k2 = *reinterpret_cast<const bf8*>(at + piece<DP>(3 + i, 0, 0)),
-                      Sk = *reinterpret_cast<const bf8*>(at + piece<DP>(6 + i, 0, 0));
+            for (int i = 2; i >= 0; --i) {
+              const bf8 k = *reinterpret_cast<const bf8*>(at + piece<DP>(i, 0, 0)),
+                        k2 = *reinterpret_cast<const bf8*>(at + piece<DP>(3 + i, 0, 0)),
+                        Sk = *reinterpret_cast<const bf8*>(at + piece<DP>(6 + i, 0, 0));
 #pragma unroll
-            for (int j = 2 - i; j >= 0; --j)
+              for (int j = 2 - i; j >= 0; --j)
 #pragma unroll
-              for (int c = 0; c < NC; ++c) {
-                m[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[c].p[st].p[j], m[c], 0, 0, 0);
-                v[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k2, Q[c].p[st].p[j], v[c], 0, 0, 0);
-                v[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Sk, P[c].p[st].p[j], v[c], 0, 0, 0);
-              }
+                for (int c = 0; c < NC; ++c) {
+                  acc4 &x = i + j ? dm[c] : m[c], &y = i + j ? dv[c] : v[c];
+                  x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[c].p[st].p[j], x, 0, 0, 0);
+                  y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k2, Q[c].p[st].p[j], y, 0, 0, 0);
+                  y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Sk, P[c].p[st].p[j], y, 0, 0, 0);
+                }
+            }
           }
+#pragma unroll
+          for (int c = 0; c < NC; ++c) m[c] += dm[c], v[c] += dv[c];
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -927,15 +983,15 @@ int padded(int64_t D) { return D <= 32 ? 32 : (D <= 64 ? 64 : 128); }
 int back_rows(int64_t D) { return 16 * (padded(D) == 128 ? 4 : 8); }
 
 // Splits of `walked` for blocks of `rows` of `own` on each of BG key heads: as many as fill the
-// GPU three times over, at least 256 walked each and at most kMostWalked.
+// GPU three times over, at least 256 walked each and at most `most`.
 struct Splits {
   int n, chunk;
 };
-Splits splits_of(int64_t own, int64_t rows, int64_t BG, int64_t walked) {
+Splits splits_of(int64_t own, int64_t rows, int64_t BG, int64_t walked, int64_t most) {
   const int64_t blocks = cdiv(own, rows) * BG;
   int64_t n = cdiv(768, blocks < 1 ? 1 : blocks);
   if (n > cdiv(walked, 256)) n = cdiv(walked, 256);
-  if (n < cdiv(walked, kMostWalked)) n = cdiv(walked, kMostWalked);
+  if (n < cdiv(walked, most)) n = cdiv(walked, most);
   if (n < 1) n = 1;
   const int64_t chunk = cdiv(cdiv(walked, n), kTile) * kTile;
   return {(int)n, (int)(chunk < kTile ? kTile : chunk)};
@@ -986,7 +1042,7 @@ int backward(const char* what, Args a, float* ws, hipStream_t s) {
   const int64_t BG = a.B * a.G;
   constexpr int W = back_waves<DP>(), rows = 16 * W;
   if (a.T) {
-    const Splits sp = splits_of(a.M, rows, BG, a.N);
+    const Splits sp = splits_of(a.M, rows, BG, a.N, kMostWalkedBack);
     a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;
     dim3 grid;
     if (int rc = grid_of(what, a.M, rows, BG, sp.n, 64 * W, &grid)) return rc;
@@ -994,7 +1050,7 @@ int backward(const char* what, Args a, float* ws, hipStream_t s) {
     if (sp.n > 1) hipLaunchKernelGGL(join_kernel<false>, join_grid(BG * a.M), dim3(256), 0, s, a);
   }
   if (a.N) {
-    const Splits sp = splits_of(a.N, rows, BG, a.M);
+    const Splits sp = splits_of(a.N, rows, BG, a.M, kMostWalkedBack);
     a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;  // the stream's order keeps the joins apart
     dim3 grid;
     if (int rc = grid_of(what, a.N, rows, BG, sp.n, 64 * W, &grid)) return rc;
@@ -1026,7 +1082,7 @@ using namespace tagi;
 extern "C" int64_t tagi_remax_attention_fwd_ws_bytes(int64_t B, int64_t T, int64_t N, int64_t H, int64_t G,
                                                      int64_t D) {
   if (B <= 0 || T <= 0 || N < 0 || H <= 0 || G <= 0 || D <= 0 || H % G) return 0;
-  const Splits sp = splits_of(T * (H / G), 16 * kOutWaves, B * G, N);
+  const Splits sp = splits_of(T * (H / G), 16 * kOutWaves, B * G, N, kMostWalked);
   return 4 * B * H * T * sp.n * (2 + (sp.n > 1 ? 2 * D + 1 : 0));
 }
 
@@ -1054,7 +1110,7 @@ extern "C" int tagi_remax_attention_fwd(const float* mq, const float* Sq, const 
   a.mo = mo, a.So = So, a.rows = rows, a.loq = tagi_heads{T * H * D, H * D, D};
   a.B = B, a.T = (int)T, a.N = (int)N, a.H = (int)H, a.G = (int)G, a.R = (int)(H / G), a.D = (int)D, a.M = T * (H / G);
   a.c = (float)scale, a.c2 = (float)(scale * scale);
-  const Splits sp = splits_of(a.M, 16 * kOutWaves, B * G, N);
+  const Splits sp = splits_of(a.M, 16 * kOutWaves, B * G, N, kMostWalked);
   a.splits = sp.n, a.chunk = sp.chunk;
   a.sums = static_cast<float*>(ws), a.parts = a.sums + 2 * a.splits * B * H * T;
   if (int rc = BY_DIM(forward, what, a, s)) return rc;
@@ -1065,7 +1121,8 @@ extern "C" int64_t tagi_remax_attention_bwd_ws_bytes(int64_t B, int64_t T, int64
                                                      int64_t D) {
   if (B <= 0 || T < 0 || N < 0 || H <= 0 || G <= 0 || D <= 0 || H % G) return 0;
   const int64_t M = T * (H / G), rows = back_rows(D);
-  const int q = splits_of(M, rows, B * G, N).n, kv = splits_of(N, rows, B * G, M).n;
+  const int q = splits_of(M, rows, B * G, N, kMostWalkedBack).n,
+            kv = splits_of(N, rows, B * G, M, kMostWalkedBack).n;
   const int64_t a = q > 1 ? q * B * G * M * 2 * D : 0, b = kv > 1 ? kv * B * G * N * 4 * D : 0;
   return 4 * (a > b ? a : b);
 }
