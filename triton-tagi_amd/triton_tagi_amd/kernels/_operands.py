@@ -34,6 +34,11 @@ def heads(t: Tensor) -> _lib.Heads:
     return _lib.Heads(st[0], st[1], st[2]) if t.dim() == 4 else _lib.Heads(st[0], 0, st[1])
 
 
+def dense_like(t: Tensor, shape) -> Tensor:
+    """An output of t's shape, dense (the shorter way to it where t is)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(shape)
+
+
 def shape_of(t: Tensor, name: str, dims: int) -> torch.Size:
     _lib.check(t, name, contiguous=False)
     if t.dim() != dims or min(t.shape[-2:]) == 0:

@@ -24,7 +24,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._operands import counts, finite_scale, heads, key_heads, mean, pair, shape_of
+from ._operands import counts, dense_like, finite_scale, heads, key_heads, mean, pair, shape_of
 from .kv_cache import KVCache, cache_struct, check_table
 
 
@@ -53,9 +53,9 @@ def remax_attention(mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, mv: Tensor, 
     scale = finite_scale(scale)
     lengths, len_bytes = counts(lengths, "lengths", mq, B)
     starts, start_bytes = counts(starts, "starts", mq, B)
-    mo = torch.empty(qs, device=mq.device, dtype=torch.float32)
+    mo = dense_like(mq, qs)
     So = torch.empty_like(mo)
-    rows = torch.empty((3, B, H, T), device=mq.device, dtype=torch.float32)
+    rows = mq.new_empty((3, B, H, T))
     ws = _lib.workspace(_lib.query("tagi_remax_attention_fwd_ws_bytes", B, T, N, H, G, D), mq.device)
     wp, wb = _lib.ws_args(ws)
     _lib.call_on(mq, "tagi_remax_attention_fwd", mq.data_ptr(), Sq.data_ptr(), heads(mq), mk.data_ptr(), Sk.data_ptr(),
@@ -128,7 +128,7 @@ def remax_attention_step(mq: Tensor, Sq: Tensor, cache: KVCache, table: Tensor, 
     most = room if max_len is None else min(int(max_len), room)
     if most < 0:
         raise ValueError(f"max_len must not be negative, got {max_len}")
-    mo = torch.empty(shape, device=mq.device, dtype=torch.float32)
+    mo = dense_like(mq, shape)
     So = torch.empty_like(mo)
     ws = _lib.workspace(_lib.query("tagi_remax_attention_step_ws_bytes", B, H, c.heads, D, most), mq.device)
     wp, wb = _lib.ws_args(ws)

@@ -20,7 +20,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._operands import heads, mean, pair, shape_of
+from ._operands import dense_like, heads, mean, pair, shape_of
 
 
 def rotary_frequencies(pairs: int, base: float = 10000.0, device="cuda") -> Tensor:
@@ -99,10 +99,9 @@ def qk_norm_rotary(mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, positions: Te
     pos, pos_bytes, axes, sec, freq, pairs = _turns(positions, frequencies, sections, mq, qs)
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    oqm = torch.empty(qs, device=mq.device, dtype=torch.float32)
-    okm = torch.empty(ks, device=mq.device, dtype=torch.float32)
+    oqm, okm = dense_like(mq, qs), dense_like(mk, ks)
     oqS, okS = torch.empty_like(oqm), torch.empty_like(okm)
-    inv = None if weights is None else torch.empty((B, T, H + G), device=mq.device, dtype=torch.float32)
+    inv = None if weights is None else mq.new_empty((B, T, H + G))
     _lib.call_on(mq, "tagi_qk_rotary_fwd", mq.data_ptr(), Sq.data_ptr(), heads(mq), mk.data_ptr(), Sk.data_ptr(),
                  heads(mk), *(_lib.ptr(x) for x in w), _lib.ptr(pos), pos_bytes, axes, sec, _lib.ptr(freq), pairs,
                  int(interleaved), float(eps), oqm.data_ptr(), oqS.data_ptr(), okm.data_ptr(), okS.data_ptr(),
@@ -144,7 +143,7 @@ def qk_norm_rotary_backward_into(out, delta_mq: Tensor, delta_Sq: Tensor, delta_
     dw = ()
     ws = None
     if weights is not None:
-        dw = tuple(torch.empty(D, device=mq.device, dtype=torch.float32) for _ in range(4))
+        dw = tuple(mq.new_empty(D) for _ in range(4))
         ws = _lib.workspace(_lib.query("tagi_qk_rotary_bwd_ws_bytes", B, T, H, G, D), mq.device)
     wp, wb = _lib.ws_args(ws)
     _lib.call_on(mq, "tagi_qk_rotary_bwd", dmq.data_ptr(), dSq.data_ptr(), heads(dmq), dmk.data_ptr(), dSk.data_ptr(),
