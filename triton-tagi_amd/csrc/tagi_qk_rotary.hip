@@ -59,8 +59,8 @@ __device__ __forceinline__ Unit unit(const Args& A, int u) {
   return x;
 }
 
-// A lane's eight features of one row, a[4] and b[4]. VEC: four neighbouring pairs, all turning
-// or none, in two 16-byte accesses; otherwise pairs lane, lane + L, ... one feature at a time.
+// A lane's eight features of one row, a[4] and b[4]. VEC: four neighbouring pairs (all turning or
+// none, where a pair's features lie apart) in two 16-byte accesses; otherwise pairs lane, lane + L, ... one feature at a time.
 template <bool VEC>
 __device__ __forceinline__ void load_row(const Args& A, const float* p, int lane, float (&a)[4], float (&b)[4]) {
   if constexpr (VEC) {
@@ -151,6 +151,11 @@ __device__ __forceinline__ int64_t head_at(const tagi_heads& l, int64_t b, int64
   return b * l.sb + t * l.st + h * l.sh;
 }
 
+// The token's batch element: a division of 64 bits takes as long as a row's products.
+__device__ __forceinline__ int64_t batch_of(const Args& A, int64_t token) {
+  return A.tokens >> 31 ? token / A.T : (int64_t)((uint32_t)token / (uint32_t)A.T);
+}
+
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) qk_rotary_fwd_kernel(const Args A) {
   extern __shared__ float2 cs[];
@@ -164,7 +169,7 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_fwd_kernel(const Args A) {
     const int r = base + (int)threadIdx.x / A.L;
     const bool on = r < n * heads;
     const int tok = on ? r / heads : 0, h = on ? r % heads : 0;
-    const int64_t token = token0 + tok, b = token / A.T, t = token - b * A.T;
+    const int64_t token = token0 + tok, b = batch_of(A, token), t = token - b * A.T;
     const bool q = h < A.H;
     const int64_t at = q ? head_at(A.lq, b, t, h) : head_at(A.lk, b, t, h - A.H);
     float ma[4], mb[4], Sa[4], Sb[4];
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_bwd_kernel(const Args A) {
     __syncthreads();
     for (int r = (int)threadIdx.x / A.L; r < n * heads; r += groups) {
       const int tok = r / heads, h = r % heads;
-      const int64_t token = token0 + tok, b = token / A.T, t = token - b * A.T;
+      const int64_t token = token0 + tok, b = batch_of(A, token), t = token - b * A.T;
       const bool q = h < A.H;
       const int64_t at = q ? head_at(A.ldq, b, t, h) : head_at(A.ldk, b, t, h - A.H);
       float da[4], db[4], ea[4], eb[4], c[4], s[4];
@@ -324,7 +329,7 @@ int fill(const char* what, Args& a, int64_t B, int64_t T, int64_t H, int64_t G, 
   return TAGI_OK;
 }
 // four neighbouring pairs turn together or not at all, and rows end with a lane
-bool vec_rows(const Args& a) { return a.pairs % 4 == 0 && a.D % 8 == 0; }
+bool vec_rows(const Args& a) { return a.D % 8 == 0 && (a.interleaved || a.pairs % 4 == 0); }
 
 }  // namespace
 }  // namespace tagi

@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
         // the sums that scores() makes, to the last bit: where a row has few keys, its weights depend on
         // their differences from the row's sums
         acc4 m[NC], v[NC];
-        if constexpr (DP == 128) {
+        if constexpr (NC == 1) {
           scores<DP>(tile, kt, lane, q[0], Q[0], P[0], m[0], v[0]);
         } else {
           acc4 dm[NC], dv[NC];
@@ -974,13 +974,13 @@ __global__ void __launch_bounds__(256) join_keys_kernel(const Args A, int kv_key
 
 // ------------------------------------------------------------------------------------ plans
 constexpr int kStatsWaves = 8, kOutWaves = 8;
-// Waves of a backward block. Five right operands of 128 features take 240 registers: one wave a SIMD.
+// Waves of a backward block. Five right operands of 96 (128) features take 180 (240) registers: one
+// wave a SIMD.
 template <int DP>
 constexpr int back_waves() {
-  return DP == 128 ? 4 : 8;
+  return DP > 64 ? 4 : 8;
 }
-int padded(int64_t D) { return D <= 32 ? 32 : (D <= 64 ? 64 : 128); }
-int back_rows(int64_t D) { return 16 * (padded(D) == 128 ? 4 : 8); }
+int back_rows(int64_t D) { return 16 * (D > 64 ? 4 : 8); }
 
 // Splits of `walked` for blocks of `rows` of `own` on each of BG key heads: as many as fill the
 // GPU three times over, at least 256 walked each and at most `most`.
@@ -1027,7 +1027,7 @@ constexpr int two_or_one(int bytes, int more) { return (2 * (bytes + more) <= kL
 template <int DP, bool VEC>
 int forward(const char* what, Args a, hipStream_t s) {
   const int64_t BG = a.B * a.G;
-  constexpr int NC = DP == 128 ? 1 : 2;
+  constexpr int NC = DP > 64 ? 1 : 2;
   dim3 grid;
   if (int rc = grid_of(what, a.M, 16 * kStatsWaves * NC, BG, a.splits, 64 * kStatsWaves, &grid)) return rc;
   dim3 out;
@@ -1068,11 +1068,11 @@ int backward(const char* what, Args a, float* ws, hipStream_t s) {
 
 // rows of whole groups of eight features
 bool vec8(int64_t D) { return D % 8 == 0; }
-#define BY_DIM(run, ...)                                                                   \
-  (vec8(D) ? (D <= 32 ? run<32, true>(__VA_ARGS__) : (D <= 64 ? run<64, true>(__VA_ARGS__)    \
-                                                              : run<128, true>(__VA_ARGS__))) \
-           : (D <= 32 ? run<32, false>(__VA_ARGS__) : (D <= 64 ? run<64, false>(__VA_ARGS__)  \
-                                                               : run<128, false>(__VA_ARGS__))))
+#define BY_DIM_OF(run, vec, ...)                                                       \
+  (D <= 32 ? run<32, vec>(__VA_ARGS__)                                                  \
+           : (D <= 64 ? run<64, vec>(__VA_ARGS__)                                       \
+                      : (D <= 96 ? run<96, vec>(__VA_ARGS__) : run<128, vec>(__VA_ARGS__))))
+#define BY_DIM(run, ...) (vec8(D) ? BY_DIM_OF(run, true, __VA_ARGS__) : BY_DIM_OF(run, false, __VA_ARGS__))
 
 }  // namespace
 }  // namespace tagi

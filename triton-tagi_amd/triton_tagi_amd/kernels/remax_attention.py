@@ -75,7 +75,7 @@ def remax_attention_backward(mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, mv:
 
     ``rows``: of a ``remax_attention`` of the same operands. Keys' deltas are summed over the query
     heads that share them."""
-    dmq, dmk = (torch.empty(t.shape, device=t.device, dtype=torch.float32) for t in (mq, mk))
+    dmq, dmk = (dense_like(t, t.shape) for t in (mq, mk))
     out = (dmq, torch.empty_like(dmq), dmk, *(torch.empty_like(dmk) for _ in range(3)))
     remax_attention_backward_into(out, mq, Sq, mk, Sk, mv, delta_mo, delta_So, rows, scale, causal, lengths, starts)
     return out

@@ -117,7 +117,7 @@ def qk_norm_rotary_backward(delta_mq: Tensor, delta_Sq: Tensor, delta_mk: Tensor
     dmwk, dSwk), each (D,). ``mq``, ``mk``: the forward's input means. The deltas turn back, then
 
         dm = d inv g, dS = D (inv g)^2;  dmw = Sg sum d inv m, dSw = Sg^2 sum D (inv m)^2."""
-    oqm, okm = (torch.empty(t.shape, device=t.device, dtype=torch.float32) for t in (mq, mk))
+    oqm, okm = (dense_like(t, t.shape) for t in (mq, mk))
     out = (oqm, torch.empty_like(oqm), okm, torch.empty_like(okm))
     return (*out, *qk_norm_rotary_backward_into(out, delta_mq, delta_Sq, delta_mk, delta_Sk, mq, mk, inv, positions,
                                                 frequencies, weights, sections, interleaved))
@@ -143,7 +143,7 @@ def qk_norm_rotary_backward_into(out, delta_mq: Tensor, delta_Sq: Tensor, delta_
     dw = ()
     ws = None
     if weights is not None:
-        dw = tuple(mq.new_empty(D) for _ in range(4))
+        dw = mq.new_empty((4, D)).unbind()
         ws = _lib.workspace(_lib.query("tagi_qk_rotary_bwd_ws_bytes", B, T, H, G, D), mq.device)
     wp, wb = _lib.ws_args(ws)
     _lib.call_on(mq, "tagi_qk_rotary_bwd", dmq.data_ptr(), dSq.data_ptr(), heads(dmq), dmk.data_ptr(), dSk.data_ptr(),
