@@ -418,8 +418,8 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
     if (key0 < wave_to) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        // the sums that scores() makes, to the last bit: where a row has few keys, its weights depend on
-        // their differences from the row's sums
+        // the sums that scores() makes, in its order to the last bit: where a row has few keys, its weights
+        // depend on their differences from the row's sums
         acc4 m[NC], v[NC];
         if constexpr (NC == 1) {
           scores<DP>(tile, kt, lane, q[0], Q[0], P[0], m[0], v[0]);
@@ -431,20 +431,19 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
           for (int st = 0; st < DP / 32; ++st) {
             const short* at = tile + piece<DP>(0, kt, st) + 8 * lane;
 #pragma unroll
-            for (int i = 2; i >= 0; --i) {
-              const bf8 k = *reinterpret_cast<const bf8*>(at + piece<DP>(i, 0, 0)),
-                        k2 = *reinterpret_cast<const bf8*>(at + piece<DP>(3 + i, 0, 0)),
-                        Sk = *reinterpret_cast<const bf8*>(at + piece<DP>(6 + i, 0, 0));
+            for (int x = 0; x < 3; ++x)  // k q, k^2 Q, Sk P
 #pragma unroll
-              for (int j = 2 - i; j >= 0; --j)
+              for (int i = 2; i >= 0; --i) {
+                const bf8 k = *reinterpret_cast<const bf8*>(at + piece<DP>(3 * x + i, 0, 0));
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                  acc4 &x = i + j ? dm[c] : m[c], &y = i + j ? dv[c] : v[c];
-                  x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[c].p[st].p[j], x, 0, 0, 0);
-                  y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k2, Q[c].p[st].p[j], y, 0, 0, 0);
-                  y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Sk, P[c].p[st].p[j], y, 0, 0, 0);
-                }
-            }
+                for (int j = 2 - i; j >= 0; --j)
+#pragma unroll
+                  for (int c = 0; c < NC; ++c) {
+                    const bf8 b = x == 0 ? q[c].p[st].p[j] : (x == 1 ? Q[c].p[st].p[j] : P[c].p[st].p[j]);
+                    acc4& to = x == 0 ? (i + j ? dm[c] : m[c]) : (i + j ? dv[c] : v[c]);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, b, to, 0, 0, 0);
+                  }
+              }
           }
 #pragma unroll
           for (int c = 0; c < NC; ++c) m[c] += dm[c], v[c] += dv[c];
