@@ -734,7 +734,7 @@ int64_t tagi_qk_rotary_bwd_ws_bytes(int64_t B, int64_t T, int64_t H, int64_t G, 
  * variances of keys and values, each (pages, heads, page_size, head_dim), dense, of one type.
  * TAGI_CACHE_FP8 (e4m3) holds codes and one power of two for each row of head_dim:
  * value = code * 2^(e - 127), e from scales (pages, heads, page_size, 4) in the pools' order;
- * scales is not read for the other types. table (B, width) int32: the pages of each sequence in
+ * scales is aligned to 4 bytes and not read for the other types. table (B, width) int32: the pages of each sequence in
  * order; token n of sequence b lies in page table[b][n / page_size]. Tokens whose page is not in
  * the table or outside [0, pages) do not exist: they are not written, read as zeros, and are not
  * seen by attention. head_dim <= 128. */
@@ -763,8 +763,8 @@ int tagi_kv_cache_read(const tagi_kv_cache* cache, const int32_t* table, int64_t
  * starts[b] + t (t without starts); it sees the keys j < lengths[b] (N without lengths), and with
  * causal those j <= its position; a query at or behind the length, or before 0, sees none. A query
  * that sees nothing gets zeros and leaves no deltas. Keys that no query sees, and queries that see
- * nothing, are not read into any sum whatever they hold. Score variances below 1e-20 count as
- * 1e-20. rows: (3, B, H, T), written by the forward (sums of the rectified means and variances,
+ * nothing, are not read into any sum whatever they hold. 1e-20 is added to every score's
+ * variance. rows: (3, B, H, T), written by the forward (sums of the rectified means and variances,
  * and the weights' sum), read by the backward. lengths, starts: B int32 / int64 on the GPU.
  * Outputs dense. D <= 128. */
 int tagi_remax_attention_fwd(const float* mq, const float* Sq, const tagi_heads* lq,

@@ -20,6 +20,18 @@
 // side is in the rows of every product, so a lane holds the scores of one row (or key) and its sums
 // need no exchange until the end; and the registers of two products of 16 are the next product's
 // right operand as they are, whose left operand is the tile read transposed from LDS.
+//
+// What bounds it: instruction issue. A score of 64 features takes 18 MFMAs' 16th parts forward for
+// its moments (twice: statistics and weights) and 9 for the outputs, beside 66 vector instructions
+// for its moments and weight; a matrix instruction of this shape holds back a SIMD's vector
+// instructions for most of its 16 cycles (16 of them and 64 multiply-adds: 221 ns in turn, 117 and 144
+// alone; two waves, one each: 215), so the two add up: 3270 + 510 + 2300 cycles of a wave's tile of 32
+// keys, 6240 measured. Neither more waves, nor the two kinds interleaved instruction by instruction,
+// nor priorities between the waves changed that. (The shape of 32 rows and columns would run beside
+// vector work, 155 ns, but its right operands and sums of 64 features take more than the 256
+// registers of two waves a SIMD.) Measured: 2 x 4096 tokens, 16 heads of 64 over 4, causal: statistics
+// 0.73 ms, outputs 1.61, dq 1.65, dk and dv 2.47, joins 0.17: 97 TFLOP/s of fp32 products; on the fp32
+// matrix cores, whose peak is 154, the same kernels took twice as long.
 #include "tagi_remax.h"
 #include "tagi_split_bf16.h"
 
@@ -377,7 +389,8 @@ __device__ __forceinline__ void load_queries(const Args& A, int64_t at, bool on,
   });
 }
 
-// Sums of the rectified moments. NC x 16 rows a wave.
+// Sums of the rectified moments. NC x 16 rows a wave: two where the right operands fit (heads of up
+// to 64), so that a left operand read from LDS serves both.
 template <int DP, bool VEC, int W, int NC>
 __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
   constexpr int U = units_of<DP, W>(1), kRows = 16 * W;
@@ -752,8 +765,8 @@ __device__ __forceinline__ RowRange rows_of(const Args& A, const Seq& s, int key
 // Deltas of the keys and values: a wave holds 16 keys, the block walks the rows that see them.
 // Parts of a row: c q 0, c^2 Sq 3, (c q)^2 6 (against k, k^2 + Sk, Sk); dm 9, dS 12. The scale of the
 // scores' deltas is that of the queries they multiply.
-// KEYS, VALUES: which of the two: both where registers hold four sums of a head, else one after the
-// other, with the scores formed once more.
+// KEYS, VALUES: which of the two: both where registers hold four sums of a head (up to 96 features),
+// else one after the other, with the scores formed once more.
 template <int DP, bool VEC, int W, bool KEYS, bool VALUES>
 __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   constexpr int S = DP / 32, DT = DP / 16, kKeys = 16 * W;
@@ -974,7 +987,7 @@ __global__ void __launch_bounds__(256) join_keys_kernel(const Args A, int kv_key
 // ------------------------------------------------------------------------------------ plans
 constexpr int kStatsWaves = 8, kOutWaves = 8;
 // Waves of a backward block. Five right operands of 96 (128) features take 180 (240) registers: one
-// wave a SIMD.
+// wave a SIMD has 512; eight waves would keep them in scratch memory.
 template <int DP>
 constexpr int back_waves() {
   return DP > 64 ? 4 : 8;
@@ -982,7 +995,8 @@ constexpr int back_waves() {
 int back_rows(int64_t D) { return 16 * (D > 64 ? 4 : 8); }
 
 // Splits of `walked` for blocks of `rows` of `own` on each of BG key heads: as many as fill the
-// GPU three times over, at least 256 walked each and at most `most`.
+// GPU three times over, at least 256 walked each (a block's own operands are loaded and split again
+// for each) and at most `most`.
 struct Splits {
   int n, chunk;
 };

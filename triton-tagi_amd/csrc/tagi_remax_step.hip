@@ -10,9 +10,15 @@
 // the scores between the launches are 16 bytes a token and head beside 4 D cells a token and key
 // head. Cells of 8 and 16 bits are one bf16 part (tagi_split_bf16.h; their squares one and two),
 // so only the queries and weights are split. The query heads that share a key head are the columns
-// of the products. Four of them at a time take all 16 columns with their three parts, four for each
-// (the last four are zeros), and a product of all parts is one MFMA instead of three; more than four
-// take 16 columns at a time, part after part.
+// of the products. Up to four of them take all 16 columns with their three parts, four for each (the
+// last four are zeros), and a product of all parts is one MFMA instead of three; more than four take
+// 16 columns at a time, part after part (16 sequences of 16384 tokens, 8 key heads of 128 in e4m3,
+// four query heads to each: 288 us, 395 as 16 columns; five: 404, 441 as four and one).
+//
+// Measured: the same in bf16, one query head to a key head, 407 us for 2.15 GB, 5.3 TB/s; in e4m3
+// 265 us for 1.08 GB, 4.1 TB/s: there a cell's way to bf16, its square and the scores' moments (800
+// vector instructions for a wave's 64 keys) are as long as its way from HBM. Loads are counted:
+// behind a branch each tile waited for all of them (611 us of 16 x 28672 tokens, 492 without).
 #include "tagi_kv_cache.h"
 #include "tagi_remax.h"
 #include "tagi_split_bf16.h"
@@ -22,23 +28,9 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kWaveKeys = 512;  // most keys of a wave: their slots and scales stay in LDS
-
-// Parts of a cell's value and of its square.
-template <typename Cell>
-struct CellParts;
-template <>
-struct CellParts<F32Cell> {
-  static constexpr int one = 3, two = 3;
-};
-template <>
-struct CellParts<Bf16Cell> {
-  static constexpr int one = 1, two = 2;
-};
-template <>
-struct CellParts<Fp8Cell> {
-  static constexpr int one = 1, two = 1;
-};
+// Most keys of a wave: their slots and scales stay in LDS. A block's way to its first tile (lengths,
+// pages, queries) is shared by more of them: 16 x 28672 tokens 511 us at 256, 492 at 512.
+constexpr int kWaveKeys = 512;
 
 struct Args {
   const float *mq, *Sq;
@@ -596,7 +588,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Args A) {
   else if (f < 2 * D) A.So[h * D + f - D] = x * inv * inv;
 }
 
-// Keys of a wave: as many as leave a few blocks for each of the 256 CUs.
+// Keys of a wave: as many as leave four blocks for each of the 256 CUs.
 int wave_keys_of(int64_t B, int64_t G, int64_t max_len) {
   int keys = kWaveKeys;
   while (keys > 64 && B * G * cdiv(max_len, kWaves * keys) < 1024) keys /= 2;

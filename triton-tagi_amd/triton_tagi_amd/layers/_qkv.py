@@ -42,10 +42,10 @@ class QkvProjections(LearnableLayer):
     _QKV_ATTRS = ("mw", "Sw", "mb", "Sb")
 
     def _qkv_params(self) -> dict:
-        """The three projections' parameters side by side: (E, L) weights and (1, L)
-        biases (L = 3E where keys and values are as wide as the queries), which the fused projection product and the update read directly. Each
-        projection's mw, Sw, mb, Sb are column views of them, so in-place changes to either
-        are seen by both (checkpoint restore copies in place). Built at the first forward;
+        """The three projections' parameters side by side: (E, L) weights and (1, L) biases (L = 3E
+        where keys and values are as wide as the queries), which the fused projection product and
+        the update read directly. Each projection's mw, Sw, mb, Sb are column views of them, so
+        in-place changes to either are seen by both (checkpoint restore copies in place). Built at the first forward;
         rebuilt from the projections' tensors if any of them was replaced since."""
         projs = self._projections()
         bufs = getattr(self, "_qkv", None)

@@ -1,9 +1,9 @@
 """Prompts and single tokens through a list of layers with carried states.
 
 Layers that mix tokens keep a state (LinearAttention and RemaxAttention: their own;
-ResidualRMSNorm: those of its branch); layers that act on each token by itself run as they are. Anything else (attention
-over a whole sequence, positional encodings, convolutions) is refused: fed token by token it
-would answer wrongly.
+ResidualRMSNorm: those of its branch); layers that act on each token by itself run as they are.
+Anything else (attention over a whole sequence, positional encodings, convolutions) is refused: fed
+token by token it would answer wrongly.
 
 The layers' forwards run here and replace what a backward reads, so ``Sequential`` makes every
 layer forget it afterwards: a backward after a prompt or a token needs a forward of its own, and
