@@ -360,8 +360,10 @@ template <int DP, int W, int U>
 __device__ __forceinline__ void put_keys(short* tile, int pairs, int wave, int lane, bool value_variances,
                                          const Unit (&u)[U]) {
 #pragma unroll
-  for (int j = 0; j < U; ++j)
+  for (int j = 0; j < U; ++j) {
+    if (U > 1) fence();
     if (wave + j * W < 2 * (DP / 32) * pairs) put_key<DP>(tile, wave + j * W, lane, value_variances, u[j]);
+  }
 }
 // Unit by unit, where registers do not hold more.
 template <int DP, bool VEC, int W>
@@ -538,7 +540,9 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
   for (int key0 = from; key0 < to; key0 += kTile) {
     const short* tile = lds + hidden(buf * KeysValues::halves);
     const bool more = key0 + kTile < to;
-    if (ahead && more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), true, u);
+    if constexpr (ahead) {
+      if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), true, u);
+    }
     if (key0 < wave_to) {
       float w[8], kw[8];
 #pragma unroll
@@ -581,11 +585,31 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
       }
     }
     if (bufs == 2) buf ^= 1;
-    if (bufs == 1) __syncthreads();
-    if (!ahead && more)
-      pass_keys<DP, VEC, W>(A, p, key0 + kTile, to, lds, 2, wave, lane, true);
-    else if (more)
-      put_keys<DP, W>(lds + buf * KeysValues::halves, 2, wave, lane, true, u);
+    short* const next = lds + buf * KeysValues::halves;
+    if constexpr (ahead) {
+      if (bufs == 1) __syncthreads();
+      if (more) put_keys<DP, W>(next, 2, wave, lane, true, u);
+    } else {
+      const int key1 = more ? key0 + kTile : to;
+      fence();
+      if constexpr (DP < 128) {
+        Unit v[units_of<DP, W>(2)];  // only here: it would take the products' registers
+        fetch_keys<DP, VEC, W>(A, p, key1, to, 2, wave, hidden(lane), true, v);
+        if (bufs == 1) __syncthreads();
+        fence();
+        put_keys<DP, W>(next, 2, wave, hidden(lane), true, v);
+      } else {  // one after the other: two take 130 registers of the products' to scratch memory
+        Unit v;
+        fetch_key<DP, VEC>(A, p, key1, to, wave, hidden(lane), true, v);
+        if (bufs == 1) __syncthreads();
+        put_key<DP>(next, wave, hidden(lane), true, v);
+#pragma unroll 1
+        for (int i = wave + W; i < 4 * (DP / 32); i += W) {
+          fetch_key<DP, VEC>(A, p, key1, to, i, hidden(lane), true, v);
+          put_key<DP>(next, i, hidden(lane), true, v);
+        }
+      }
+    }
     __syncthreads();
   }
   sum = group_sum(sum);
@@ -682,7 +706,9 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
   for (int key0 = from; key0 < to; key0 += kTile) {
     const short* tile = lds + hidden(buf * KeysValues::halves);
     const bool more = key0 + kTile < to;
-    if (ahead && more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), false, u);
+    if constexpr (ahead) {
+      if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), false, u);
+    }
     if (key0 < wave_to) {
       float x[8], X[8];
 #pragma unroll
@@ -728,11 +754,19 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
       }
     }
     if (bufs == 2) buf ^= 1;
-    if (bufs == 1) __syncthreads();
-    if (!ahead && more)
-      pass_keys<DP, VEC, W>(A, p, key0 + kTile, to, lds, 2, wave, lane, false);
-    else if (more)
-      put_keys<DP, W>(lds + buf * KeysValues::halves, 2, wave, lane, false, u);
+    short* const next = lds + buf * KeysValues::halves;
+    if constexpr (ahead) {
+      if (bufs == 1) __syncthreads();
+      if (more) put_keys<DP, W>(next, 2, wave, lane, false, u);
+    } else {
+      const int key1 = more ? key0 + kTile : to;
+      Unit v[units_of<DP, W>(2)];  // only here: it would take the products' registers
+      fence();
+      fetch_keys<DP, VEC, W>(A, p, key1, to, 2, wave, hidden(lane), false, v);
+      if (bufs == 1) __syncthreads();
+      fence();
+      put_keys<DP, W>(next, 2, wave, hidden(lane), false, v);
+    }
     __syncthreads();
   }
   if (rho >= A.M) return;
@@ -938,13 +972,26 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
     }
     if (ahead && more && !busy && wave < 4 * S) fetch_unit(rho0 + kTile, wave, hidden(lane), u);
     if (bufs == 2) buf ^= 1;
-    if (bufs == 1) __syncthreads();
-    if (ahead && more) {
-      if (wave < 4 * S) store_unit(lds + buf * Queries::halves, wave, hidden(lane), u);
-      row_stats(rho0 + kTile, buf);
-    } else if (more) {
-      pass_rows(rho0 + kTile, buf);
+    short* const next = lds + buf * Queries::halves;
+    if constexpr (ahead) {
+      if (bufs == 1) __syncthreads();
+      if (more && wave < 4 * S) store_unit(next, wave, hidden(lane), u);
+    } else {
+      constexpr int n = 4 * S / W;
+      static_assert(n * W == 4 * S, "whole units for each wave");
+      const int64_t rho1 = more ? rho0 + kTile : to;
+      Unit v[n];  // only here: it would take the products' registers
+      fence();
+#pragma unroll
+      for (int j = 0; j < n; ++j) fetch_unit(rho1, wave + j * W, hidden(lane), v[j]);
+      if (bufs == 1) __syncthreads();
+#pragma unroll
+      for (int j = 0; j < n; ++j) {
+        fence();
+        store_unit(next, wave + j * W, hidden(lane), v[j]);
+      }
     }
+    if (more) row_stats(rho0 + kTile, buf);
     __syncthreads();
   }
   if (key >= A.N) return;
