@@ -377,6 +377,32 @@ __device__ __forceinline__ void pass_keys(const Args& A, const Place& p, int key
   }
 }
 
+// The next tile of keys and values behind the products: a wave's loads are in flight together, across
+// the barrier (BARRIER) behind which the tile's place is free. Of 128 features one after the other: two
+// at once take 130 registers of the outputs' products to scratch memory (1.69 -> 2.75 ms).
+template <int DP, bool VEC, int W, bool BARRIER>
+__device__ __forceinline__ void next_keys(const Args& A, const Place& p, int key0, int to, short* tile, int wave, int lane,
+                                          bool value_variances) {
+  fence();
+  if constexpr (DP < 128) {
+    Unit u[units_of<DP, W>(2)];
+    fetch_keys<DP, VEC, W>(A, p, key0, to, 2, wave, hidden(lane), value_variances, u);
+    if (BARRIER) __syncthreads();
+    fence();
+    put_keys<DP, W>(tile, 2, wave, hidden(lane), value_variances, u);
+  } else {
+    Unit u;
+    fetch_key<DP, VEC>(A, p, key0, to, wave, hidden(lane), value_variances, u);
+    if (BARRIER) __syncthreads();
+    put_key<DP>(tile, wave, hidden(lane), value_variances, u);
+#pragma unroll 1
+    for (int i = wave + W; i < 4 * (DP / 32); i += W) {
+      fetch_key<DP, VEC>(A, p, key0, to, i, hidden(lane), value_variances, u);
+      put_key<DP>(tile, i, hidden(lane), value_variances, u);
+    }
+  }
+}
+
 // Queries on the right: q, Sq, Sq + q^2 (against k, k^2, Sk), scaled.
 template <int DP, bool VEC>
 __device__ __forceinline__ void load_queries(const Args& A, int64_t at, bool on, int k8, Right<DP>& q, Right<DP>& Q,
@@ -590,25 +616,7 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
       if (bufs == 1) __syncthreads();
       if (more) put_keys<DP, W>(next, 2, wave, lane, true, u);
     } else {
-      const int key1 = more ? key0 + kTile : to;
-      fence();
-      if constexpr (DP < 128) {
-        Unit v[units_of<DP, W>(2)];  // only here: it would take the products' registers
-        fetch_keys<DP, VEC, W>(A, p, key1, to, 2, wave, hidden(lane), true, v);
-        if (bufs == 1) __syncthreads();
-        fence();
-        put_keys<DP, W>(next, 2, wave, hidden(lane), true, v);
-      } else {  // one after the other: two take 130 registers of the products' to scratch memory
-        Unit v;
-        fetch_key<DP, VEC>(A, p, key1, to, wave, hidden(lane), true, v);
-        if (bufs == 1) __syncthreads();
-        put_key<DP>(next, wave, hidden(lane), true, v);
-#pragma unroll 1
-        for (int i = wave + W; i < 4 * (DP / 32); i += W) {
-          fetch_key<DP, VEC>(A, p, key1, to, i, hidden(lane), true, v);
-          put_key<DP>(next, i, hidden(lane), true, v);
-        }
-      }
+      next_keys<DP, VEC, W, bufs == 1>(A, p, more ? key0 + kTile : to, to, next, wave, lane, true);
     }
     __syncthreads();
   }
@@ -759,13 +767,7 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
       if (bufs == 1) __syncthreads();
       if (more) put_keys<DP, W>(next, 2, wave, lane, false, u);
     } else {
-      const int key1 = more ? key0 + kTile : to;
-      Unit v[units_of<DP, W>(2)];  // only here: it would take the products' registers
-      fence();
-      fetch_keys<DP, VEC, W>(A, p, key1, to, 2, wave, hidden(lane), false, v);
-      if (bufs == 1) __syncthreads();
-      fence();
-      put_keys<DP, W>(next, 2, wave, hidden(lane), false, v);
+      next_keys<DP, VEC, W, bufs == 1>(A, p, more ? key0 + kTile : to, to, next, wave, lane, false);
     }
     __syncthreads();
   }
@@ -1033,6 +1035,9 @@ __global__ void __launch_bounds__(256) join_keys_kernel(const Args A, int kv_key
 
 // ------------------------------------------------------------------------------------ plans
 constexpr int kStatsWaves = 8, kOutWaves = 8;
+// Kernels of four waves keep what they have in 512 registers and nothing in scratch memory: operands of
+// four registers that the compiler had put there, beside accumulation registers, came back wrong.
+//
 // Waves of a backward block. Five right operands of 96 (128) features take 180 (240) registers: one
 // wave a SIMD has 512; eight waves would keep them in scratch memory.
 template <int DP>
