@@ -88,6 +88,32 @@ def test_step_heads(dtype, R, D, dev):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, FP8])
+@pytest.mark.parametrize("R,D", [(4, 128), (3, 96), (4, 64), (1, 32), (2, 40)])
+def test_step_in_one_launch_and_in_three(dtype, R, D, dev):
+    """The same lengths under a bound that one block holds and under one that it does not."""
+    from triton_tagi_amd import kernels as K
+
+    B, G, page, longest = 3, 2, 32, 256
+    cache = cache_of(dev, 30, G, page, D, dtype)
+    table = torch.randperm(30, generator=torch.Generator().manual_seed(R))[:27].view(B, 9).int().to(dev)
+    K.cache_write(cache, *rows_of(B, longest, G, D, 7 * R + D, dev), table)
+    ln = torch.tensor([longest, 0, 201], device=dev)
+    r = torch.Generator().manual_seed(D)
+    mq, Sq = torch.randn(B, R * G, D, generator=r).to(dev), (0.05 * torch.rand(B, R * G, D, generator=r)).to(dev)
+    pools = values(cache)
+    at = torch.arange(longest)
+    for most in (256, 257):
+        mo, So = K.remax_attention_step(mq, Sq, cache, table, ln, scale=1 / math.sqrt(D), max_len=most)
+        assert not mo[1].any() and not So[1].any()
+        for b in (0, 2):
+            n = int(ln[b])
+            pg = table[b].cpu().long()[at[:n] // page]
+            keys = [p[pg, :, at[:n] % page][None] for p in pools]
+            ref = attention(mq[b, None, None], Sq[b, None, None], *keys, 1 / math.sqrt(D), causal=False, starts=[n - 1])
+            within(mo[b, None, None], ref[0], f"mo {b} {most}"), within(So[b, None, None], ref[1], f"So {b} {most}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, FP8])
 def test_step_of_many_long_sequences(dtype, dev):
     """Enough sequences for the longest stretch of keys to a wave; all read the same few pages."""
     from triton_tagi_amd import kernels as K

@@ -1,7 +1,8 @@
 // Remax attention of one query of every sequence over the pages of its cache.
 //
 // The formulas of tagi_remax_attention.hip with one row per head. A sequence's tokens are split
-// over blocks; a weight needs the sums over all of them first, so there are three launches:
+// over blocks; a weight needs the sums over all of them first, so there are three launches (one where
+// a block holds a sequence and every block a CU):
 //   scores: the keys' pages once; moments of the rectified scores (mm, vm) to the workspace, and
 //           each wave's sums of them
 //   values: those sums added in order, weights, the values' pages once; each split's sums
@@ -292,7 +293,7 @@ constexpr int blocks_of() {
 
 // HT query heads at a time.
 template <typename Cell, int DP, bool VEC, int HT>
-__global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) scores_kernel(const Args A) {
+__device__ __forceinline__ void scores_of(const Args& A) {
   typedef typename Cell::type T;
   constexpr int S = DP / 32, N = group_of<T, DP>(), L = DP / (4 * N);  // L loads of N features
   constexpr int F = VEC && HT == 4 ? 4 / sizeof(T) : 1;                // tiles in flight
@@ -410,11 +411,17 @@ __global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) sc
   }
 }
 
+template <typename Cell, int DP, bool VEC, int HT>
+__global__ void __launch_bounds__(kThreads, (blocks_of<Cell, DP, VEC, HT>())) scores_kernel(const Args A) {
+  scores_of<Cell, DP, VEC, HT>(A);
+}
+
 // Lane (r, k8) of a wave brings the features ND r .. ND r + ND - 1 (ND = DP / 16) of keys 8 k8 ..
 // 8 k8 + 7 of every 32: the j-th of them, over the eight keys, is its share of a product whose rows
 // are the features ND r + j. So a load covers whole rows and no value moves between lanes.
-template <typename Cell, int DP, bool VEC, int HT>
-__global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, VEC, HT>())) values_kernel(const Args A) {
+// WHOLE: the block has all of its sequence's tokens and writes the outputs.
+template <typename Cell, int DP, bool VEC, int HT, bool WHOLE>
+__device__ __forceinline__ void values_of(const Args& A) {
   typedef typename Cell::type T;
   constexpr int ND = DP / 16;
   constexpr bool scaled_rows = sizeof(T) == 1, ahead = DP * sizeof(T) <= 128;  // the next 32 keys' cells are in flight
@@ -553,16 +560,40 @@ __global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, 
         float x = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) x += red[(w * DP + f) * HT + r];
-        part[r * step + k * D + f] = x;
+        if constexpr (WHOLE) {
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) sum += totals[w][r];
+          const float inv = fast_rcp(fmaxf(sum, kRemaxFloor));
+          if (k == 0)
+            A.mo[(h + r) * D + f] = x * inv;
+          else
+            A.So[(h + r) * D + f] = x * inv * inv;
+        } else {
+          part[r * step + k * D + f] = x;
+        }
       }
     }
-    if ((int)threadIdx.x < n) {
+    if (!WHOLE && (int)threadIdx.x < n) {
       float x = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) x += totals[w][threadIdx.x];
       part[threadIdx.x * step + 2 * D] = x;
     }
   }
+}
+
+template <typename Cell, int DP, bool VEC, int HT>
+__global__ void __launch_bounds__(kThreads, (HT == 16 ? 1 : blocks_of<Cell, DP, VEC, HT>())) values_kernel(const Args A) {
+  values_of<Cell, DP, VEC, HT, false>(A);
+}
+// Sequences that one block holds: no launch waits for another. A lane reads the scores that it wrote
+// itself.
+template <typename Cell, int DP>
+__global__ void __launch_bounds__(kThreads, 1) whole_kernel(const Args A) {
+  scores_of<Cell, DP, true, 4>(A);
+  __syncthreads();  // the waves' sums
+  values_of<Cell, DP, true, 4, true>(A);
 }
 
 // A block to a query head, a thread to a sum: the splits that its sequence's length reaches, in order.
@@ -604,9 +635,16 @@ template <typename Cell, int DP, bool VEC, int HT>
 void launch(const Args& a, dim3 grid, hipStream_t s) {
   hipLaunchKernelGGL((scores_kernel<Cell, DP, VEC, HT>), grid, dim3(kThreads), 0, s, a);
   hipLaunchKernelGGL((values_kernel<Cell, DP, VEC, HT>), grid, dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(a.B * a.H)), dim3(kThreads), 0, s, a);
 }
 template <typename Cell, int DP>
 void launch_heads(const Args& a, bool vec, dim3 grid, hipStream_t s) {
+  // One launch where no CU has two blocks (8 sequences of 256 tokens, 8 key heads of 32 in fp32: 16.4
+  // us, 21.6 as three; 64 of 128 in bf16: 42.8, 39.3, since a CU holds one block of it and two of theirs).
+  if (vec && a.R <= 4 && a.splits == 1 && a.B * a.c.G <= 256) {
+    hipLaunchKernelGGL((whole_kernel<Cell, DP>), grid, dim3(kThreads), 0, s, a);
+    return;
+  }
   if (a.R <= 4)
     vec ? launch<Cell, DP, true, 4>(a, grid, s) : launch<Cell, DP, false, 4>(a, grid, s);
   else
@@ -667,6 +705,5 @@ extern "C" int tagi_remax_attention_step(const float* mq, const float* Sq, const
     launch_dim<Bf16Cell>(a, vec, grid, s);
   else
     launch_dim<Fp8Cell>(a, vec, grid, s);
-  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(B * H)), dim3(kThreads), 0, s, a);
   return check_launch(what);
 }

@@ -116,8 +116,8 @@ def cache_read(cache: KVCache, table: Tensor, lengths: Tensor, tokens: int) -> t
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError(f"tokens must not be negative, got {tokens}")
-    out = tuple(torch.empty((B, tokens, c.heads, c.head_dim), device=table.device, dtype=torch.float32)
-                for _ in range(4))
+    mk = torch.empty((B, tokens, c.heads, c.head_dim), device=table.device, dtype=torch.float32)
+    out = (mk, *(torch.empty_like(mk) for _ in range(3)))
     _lib.call_on(table, "tagi_kv_cache_read", c, table.data_ptr(), table.shape[1], lengths.data_ptr(), len_bytes,
                  *(t.data_ptr() for t in out), B, tokens, _lib.stream_of(table))
     return out
