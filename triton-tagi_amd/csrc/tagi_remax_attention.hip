@@ -149,6 +149,12 @@ template <int DP>
 __device__ __forceinline__ int piece(int part, int kt, int s) {
   return ((part * 2 + kt) * (DP / 32) + s) * 512;
 }
+// An operand's place: in the instruction where a tile is within its reach of 64 KB; where it is not
+// (heads of 128), formed where it is used, since the sums would wait in registers.
+template <int DP>
+__device__ __forceinline__ int offset(int x) {
+  return DP == 128 ? hidden(x) : x;
+}
 template <int DP, int P>
 __device__ __forceinline__ void put(short* tile, int first, int kt, int s, int lane, const Parts<P>& x) {
 #pragma unroll
@@ -156,8 +162,8 @@ __device__ __forceinline__ void put(short* tile, int first, int kt, int s, int l
 }
 // c += a b, a 16 rows of the tile: part by part, so that four registers hold the left operand.
 template <int DP>
-__device__ __forceinline__ acc4 mma_left(const short* tile, int first, int kt, int s, int lane, const Parts<3>& b, acc4 c) {
-  const short* at = tile + hidden(piece<DP>(first, 0, 0)) + 8 * lane;
+__device__ __forceinline__ acc4 mma_left(const short* left, int first, int kt, int s, const Parts<3>& b, acc4 c) {
+  const short* at = left + offset<DP>(piece<DP>(first, 0, 0));
 #pragma unroll
   for (int i = 2; i >= 0; --i) {
     const bf8 a = *reinterpret_cast<const bf8*>(at + piece<DP>(i, kt, s));
@@ -170,11 +176,14 @@ __device__ __forceinline__ acc4 mma_left(const short* tile, int first, int kt, i
 // holds the tile's rows 4 g + 0..3 and 16 + 4 g + 0..3, as the registers of two products of 16
 // rows hold them. ds_read_b64_tr_b16: of the 64 bits that lane p of a group of 16 reads, lane q
 // gets element q % 4 of lanes q / 4 + 4 j, j = 0..3.
-template <int DP>
-__device__ __forceinline__ acc4 mma_transposed(const short* tile, int first, int dt, int lane, const Parts<3>& b, acc4 c) {
-  typedef __attribute__((address_space(3))) h4 lds_h4;
+__device__ __forceinline__ int turned_at(int lane) {
   const int p = lane & 15, g = lane >> 4;
-  const short* at = tile + hidden(piece<DP>(first, 0, 0)) + ((((p & 3) >> 1) * 16 + 4 * g + (p >> 2)) * 8 + 4 * (p & 1));
+  return (((p & 3) >> 1) * 16 + 4 * g + (p >> 2)) * 8 + 4 * (p & 1);
+}
+template <int DP>
+__device__ __forceinline__ acc4 mma_transposed(const short* turned, int first, int dt, const Parts<3>& b, acc4 c) {
+  typedef __attribute__((address_space(3))) h4 lds_h4;
+  const short* at = turned + offset<DP>(piece<DP>(first, 0, 0));
 #pragma unroll
   for (int i = 2; i >= 0; --i) {
     union {
@@ -223,14 +232,14 @@ __device__ __forceinline__ void load_right(const float* pm, const float* pS, int
 // while the sum is small, and then is cut once a step instead of six times (rows of few keys: 1.6e-6
 // of the variances wrong before, 6e-7 so).
 template <int DP>
-__device__ __forceinline__ acc4 mma_first(const short* tile, int first, int kt, int s, int lane, const Parts<3>& b, acc4 c) {
-  const bf8 a = *reinterpret_cast<const bf8*>(tile + hidden(piece<DP>(first, 0, 0)) + 8 * lane + piece<DP>(0, kt, s));
+__device__ __forceinline__ acc4 mma_first(const short* left, int first, int kt, int s, const Parts<3>& b, acc4 c) {
+  const bf8 a = *reinterpret_cast<const bf8*>(left + offset<DP>(piece<DP>(first, kt, s)));
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b.p[0], c, 0, 0, 0);
 }
 template <int DP, bool FIRST>
-__device__ __forceinline__ void mma_left(const short* tile, int first, int kt, int s, int lane, const Parts<3>& b, acc4& c,
+__device__ __forceinline__ void mma_left(const short* left, int first, int kt, int s, const Parts<3>& b, acc4& c,
                                          acc4& rest) {
-  const short* at = tile + hidden(piece<DP>(first, 0, 0)) + 8 * lane;
+  const short* at = left + offset<DP>(piece<DP>(first, 0, 0));
 #pragma unroll
   for (int i = 2; i >= 0; --i) {
     const bf8 a = *reinterpret_cast<const bf8*>(at + piece<DP>(i, kt, s));
@@ -251,31 +260,31 @@ __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 // Moments of the scores of 16 walked rows: m = a0 b0, v = a1 b1 + a2 b2 with a0, a1, a2 the parts
 // 0, 3, 6 of the tile.
 template <int DP>
-__device__ __forceinline__ void scores(const short* tile, int kt, int lane, const Right<DP>& b0, const Right<DP>& b1,
+__device__ __forceinline__ void scores(const short* left, int kt, const Right<DP>& b0, const Right<DP>& b1,
                                        const Right<DP>& b2, acc4& m, acc4& v) {
   acc4 dm = {0, 0, 0, 0}, dv = dm;
   if constexpr (DP < 128) {
     m = v = dm;
 #pragma unroll
     for (int s = 0; s < DP / 32; ++s) {
-      mma_left<DP, true>(tile, 0, kt, s, lane, b0.p[s], m, dm);
-      mma_left<DP, true>(tile, 3, kt, s, lane, b1.p[s], v, dv);
-      mma_left<DP, true>(tile, 6, kt, s, lane, b2.p[s], v, dv);
+      mma_left<DP, true>(left, 0, kt, s, b0.p[s], m, dm);
+      mma_left<DP, true>(left, 3, kt, s, b1.p[s], v, dv);
+      mma_left<DP, true>(left, 6, kt, s, b2.p[s], v, dv);
     }
     m += dm, v += dv;
   } else {  // the registers of two more sums are not there: the keys' first parts are read again
 #pragma unroll
     for (int s = 0; s < DP / 32; ++s) {
-      mma_left<DP, false>(tile, 0, kt, s, lane, b0.p[s], m, dm);
-      mma_left<DP, false>(tile, 3, kt, s, lane, b1.p[s], v, dv);
-      mma_left<DP, false>(tile, 6, kt, s, lane, b2.p[s], v, dv);
+      mma_left<DP, false>(left, 0, kt, s, b0.p[s], m, dm);
+      mma_left<DP, false>(left, 3, kt, s, b1.p[s], v, dv);
+      mma_left<DP, false>(left, 6, kt, s, b2.p[s], v, dv);
     }
     m = dm, v = dv;
 #pragma unroll
     for (int s = 0; s < DP / 32; ++s) {
-      m = mma_first<DP>(tile, 0, kt, s, lane, b0.p[s], m);
-      v = mma_first<DP>(tile, 3, kt, s, lane, b1.p[s], v);
-      v = mma_first<DP>(tile, 6, kt, s, lane, b2.p[s], v);
+      m = mma_first<DP>(left, 0, kt, s, b0.p[s], m);
+      v = mma_first<DP>(left, 3, kt, s, b1.p[s], v);
+      v = mma_first<DP>(left, 6, kt, s, b2.p[s], v);
     }
   }
 }
@@ -453,7 +462,7 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
   __syncthreads();
   int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile, buf ^= 1) {
-    const short* tile = lds + hidden(buf * Keys::halves);
+    const short* left = lds + hidden(buf * Keys::halves + 8 * lane);
     const bool more = key0 + kTile < to;
     if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 1, wave, hidden(lane), false, u);
     if (key0 < wave_to) {
@@ -463,14 +472,14 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
         // depend on their differences from the row's sums
         acc4 m[NC], v[NC];
         if constexpr (NC == 1) {
-          scores<DP>(tile, kt, lane, q[0], Q[0], P[0], m[0], v[0]);
+          scores<DP>(left, kt, q[0], Q[0], P[0], m[0], v[0]);
         } else {
           acc4 dm[NC], dv[NC];
 #pragma unroll
           for (int c = 0; c < NC; ++c) m[c] = v[c] = dm[c] = dv[c] = acc4{0, 0, 0, 0};
 #pragma unroll
           for (int st = 0; st < DP / 32; ++st) {
-            const short* at = tile + piece<DP>(0, kt, st) + 8 * lane;
+            const short* at = left + piece<DP>(0, kt, st);
 #pragma unroll
             for (int x = 0; x < 3; ++x)  // k q, k^2 Q, Sk P
 #pragma unroll
@@ -564,7 +573,7 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
   __syncthreads();
   int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile) {
-    const short* tile = lds + hidden(buf * KeysValues::halves);
+    const short *left = lds + hidden(buf * KeysValues::halves + 8 * lane), *turned = lds + hidden(buf * KeysValues::halves + turned_at(lane));
     const bool more = key0 + kTile < to;
     if constexpr (ahead) {
       if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), true, u);
@@ -575,7 +584,7 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
       for (int kt = 0; kt < 2; ++kt) {
         fence();
         acc4 m, v;
-        scores<DP>(tile, kt, lane, q, Q, P, m, v);
+        scores<DP>(left, kt, q, Q, P, m, v);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const Weight x = weigh(rectify(m[r], v[r]), rs);
@@ -593,13 +602,13 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
       {
         const Parts<3> b = split<3>(w);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) om[d] = mma_transposed<DP>(tile, 9, d, lane, b, om[d]);
+        for (int d = 0; d < DT; ++d) om[d] = mma_transposed<DP>(turned, 9, d, b, om[d]);
       }
       fence();
       {
         const Parts<3> b = split<3>(kw);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(tile, 12, d, lane, b, oS[d]);
+        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(turned, 12, d, b, oS[d]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) kw[i] = fmaf(w[i], w[i], kw[i]);
@@ -607,7 +616,7 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
       {
         const Parts<3> b = split<3>(kw);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(tile, 15, d, lane, b, oS[d]);
+        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(turned, 15, d, b, oS[d]);
       }
     }
     if (bufs == 2) buf ^= 1;
@@ -712,7 +721,7 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
   __syncthreads();
   int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile) {
-    const short* tile = lds + hidden(buf * KeysValues::halves);
+    const short *left = lds + hidden(buf * KeysValues::halves + 8 * lane), *turned = lds + hidden(buf * KeysValues::halves + turned_at(lane));
     const bool more = key0 + kTile < to;
     if constexpr (ahead) {
       if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), false, u);
@@ -723,7 +732,7 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
       for (int kt = 0; kt < 2; ++kt) {
         fence();
         acc4 m, v;
-        scores<DP>(tile, kt, lane, q, Q, P, m, v);
+        scores<DP>(left, kt, q, Q, P, m, v);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const Rectified z = rectify(m[r], v[r]);
@@ -735,8 +744,8 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
         acc4 e = {0, 0, 0, 0}, E = e;
 #pragma unroll
         for (int st = 0; st < DP / 32; ++st) {
-          e = mma_left<DP>(tile, 9, kt, st, lane, dm.p[st], e);
-          E = mma_left<DP>(tile, 12, kt, st, lane, dS.p[st], E);
+          e = mma_left<DP>(left, 9, kt, st, dm.p[st], e);
+          E = mma_left<DP>(left, 12, kt, st, dS.p[st], E);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[4 * kt + r] = e[r] * m[r], X[4 * kt + r] = E[r] * (m[r] * m[r]);
@@ -752,13 +761,13 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
       {
         const Parts<3> b = split<3>(x);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) om[d] = mma_transposed<DP>(tile, 0, d, lane, b, om[d]);
+        for (int d = 0; d < DT; ++d) om[d] = mma_transposed<DP>(turned, 0, d, b, om[d]);
       }
       fence();
       {
         const Parts<3> b = split<3>(X);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(tile, 3, d, lane, b, oS[d]);
+        for (int d = 0; d < DT; ++d) oS[d] = mma_transposed<DP>(turned, 3, d, b, oS[d]);
       }
     }
     if (bufs == 2) buf ^= 1;
@@ -893,7 +902,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   __syncthreads();
   int buf = 0;
   for (int64_t rho0 = from; rho0 < to; rho0 += kTile) {
-    const short* tile = lds + hidden(buf * Queries::halves);
+    const short *left = lds + hidden(buf * Queries::halves + 8 * lane), *turned = lds + hidden(buf * Queries::halves + turned_at(lane));
     const float* st = stats + buf * 5 * kTile;
     const bool more = rho0 + kTile < to;
     const bool busy = wave_key < s.len && rho0 + kTile > mine.first;
@@ -903,7 +912,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
       for (int kt = 0; kt < 2; ++kt) {
         fence();
         acc4 m, v;
-        scores<DP>(tile, kt, lane, k, K, Sk, m, v);
+        scores<DP>(left, kt, k, K, Sk, m, v);
         const float* const row = st + 16 * kt + 4 * k8;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -927,7 +936,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
           fence();
           acc4 e = {0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < S; ++i) e = mma_left<DP>(tile, 9, kt, i, lane, vm.p[i], e);
+          for (int i = 0; i < S; ++i) e = mma_left<DP>(left, 9, kt, i, vm.p[i], e);
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[4 * kt + r] = e[r] * J[4 * kt + r];
         }
@@ -935,14 +944,14 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
         {
           const Parts<3> b = split<3>(x);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) okm[d] = mma_transposed<DP>(tile, 0, d, lane, b, okm[d]);
+          for (int d = 0; d < DT; ++d) okm[d] = mma_transposed<DP>(turned, 0, d, b, okm[d]);
         }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           fence();
           acc4 E = {0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < S; ++i) E = mma_left<DP>(tile, 12, kt, i, lane, vv.p[i], E);
+          for (int i = 0; i < S; ++i) E = mma_left<DP>(left, 12, kt, i, vv.p[i], E);
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[4 * kt + r] = E[r] * (J[4 * kt + r] * J[4 * kt + r]);
         }
@@ -950,7 +959,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
         {
           const Parts<3> b = split<3>(x);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) okS[d] = mma_transposed<DP>(tile, 6, d, lane, b, okS[d]);
+          for (int d = 0; d < DT; ++d) okS[d] = mma_transposed<DP>(turned, 6, d, b, okS[d]);
         }
       }
       fence();
@@ -960,7 +969,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
         {
           const Parts<3> b = split<3>(a);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) ovm[d] = mma_transposed<DP>(tile, 9, d, lane, b, ovm[d]);
+          for (int d = 0; d < DT; ++d) ovm[d] = mma_transposed<DP>(turned, 9, d, b, ovm[d]);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] *= a[i];
@@ -968,7 +977,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
         {
           const Parts<3> b = split<3>(a);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) ovS[d] = mma_transposed<DP>(tile, 12, d, lane, b, ovS[d]);
+          for (int d = 0; d < DT; ++d) ovS[d] = mma_transposed<DP>(turned, 12, d, b, ovS[d]);
         }
       }
     }
