@@ -30,7 +30,7 @@
 // nor priorities between the waves changed that. (The shape of 32 rows and columns would run beside
 // vector work, 155 ns, but its right operands and sums of 64 features take more than the 256
 // registers of two waves a SIMD.) Measured: 2 x 4096 tokens, 16 heads of 64 over 4, causal: statistics
-// 0.73 ms, outputs 1.61, dq 1.65, dk and dv 2.47, joins 0.17: 97 TFLOP/s of fp32 products; on the fp32
+// 0.74 ms, outputs 1.62, dq 1.65, dk and dv 2.5, joins 0.17: 99 TFLOP/s of fp32 products; on the fp32
 // matrix cores, whose peak is 154, the same kernels took twice as long.
 #include "tagi_remax.h"
 #include "tagi_split_bf16.h"
