@@ -288,7 +288,7 @@ class RemaxAttention(QkvProjections):
             seen = at * on
         state.used += 1
         # a recorded graph's lengths go on beyond the host's count: it keeps the whole room
-        most = None if torch.cuda.is_current_stream_capturing() else -(-state.used // 1024) * 1024
+        most = None if torch.cuda.is_current_stream_capturing() else -(-state.used // 256) * 256
         mo, So = remax_attention_step(ops[0][:, 0], ops[1][:, 0], state.cache, state.table, seen, scale=self._scale,
                                       max_len=most)
         return mo.view(ma.shape), So.view(ma.shape)
