@@ -21,15 +21,15 @@
 // need no exchange until the end; and the registers of two products of 16 are the next product's
 // right operand as they are, whose left operand is the tile read transposed from LDS.
 //
-// What bounds it: instruction issue. A score of 64 features takes 18 MFMAs' 16th parts forward for
-// its moments (twice: statistics and weights) and 9 for the outputs, beside 66 vector instructions
-// for its moments and weight; a matrix instruction of this shape holds back a SIMD's vector
-// instructions for most of its 16 cycles (16 of them and 64 multiply-adds: 221 ns in turn, 117 and 144
-// alone; two waves, one each: 215), so the two add up: 3270 + 510 + 2300 cycles of a wave's tile of 32
-// keys, 6240 measured. Neither more waves, nor the two kinds interleaved instruction by instruction,
-// nor priorities between the waves changed that. (The shape of 32 rows and columns would run beside
-// vector work, 155 ns, but its right operands and sums of 64 features take more than the 256
-// registers of two waves a SIMD.) Measured: 2 x 4096 tokens, 16 heads of 64 over 4, causal: statistics
+// What bounds it: instruction issue. The outputs' kernel takes 144 matrix instructions for a wave's
+// tile of 16 rows and 32 keys of 64 features (half for the scores' moments, half for the outputs) and 800
+// vector instructions, 66 a score for its rectified moments and weight. A matrix instruction of this
+// shape holds back a SIMD's vector instructions for most of its 16 cycles (16 of them and 64
+// multiply-adds: 221 ns in turn, 117 and 144 alone; two waves, one each: 215), so the two add up: 3200 +
+// 510 (reciprocals, roots, exponentials) + 2300 cycles, 6240 measured. Neither more waves, nor the two
+// kinds interleaved instruction by instruction, nor priorities between the waves changed that. (The
+// shape of 32 rows and columns would run beside vector work, 155 ns, but its right operands and sums of
+// 64 features take more than the 256 registers of two waves a SIMD.) Measured: 2 x 4096 tokens, 16 heads of 64 over 4, causal: statistics
 // 0.74 ms, outputs 1.62, dq 1.65, dk and dv 2.5, joins 0.17: 99 TFLOP/s of fp32 products; on the fp32
 // matrix cores, whose peak is 154, the same kernels took twice as long.
 #include "tagi_remax.h"
