@@ -29,9 +29,10 @@
 // 510 (reciprocals, roots, exponentials) + 2300 cycles, 6240 measured. Neither more waves, nor the two
 // kinds interleaved instruction by instruction, nor priorities between the waves changed that. (The
 // shape of 32 rows and columns would run beside vector work, 155 ns, but its right operands and sums of
-// 64 features take more than the 256 registers of two waves a SIMD.) Measured: 2 x 4096 tokens, 16 heads of 64 over 4, causal: statistics
-// 0.74 ms, outputs 1.62, dq 1.65, dk and dv 2.5, joins 0.17: 99 TFLOP/s of fp32 products; on the fp32
-// matrix cores, whose peak is 154, the same kernels took twice as long.
+// 64 features take more than the 256 registers of two waves a SIMD.) Measured: 2 x 4096 tokens, 16
+// heads of 64 over 4, causal: statistics 0.74 ms, outputs 1.62, dq 1.65, dk and dv 2.5, joins 0.17: 99
+// TFLOP/s of fp32 products; on the fp32 matrix cores, whose peak is 154, the same kernels took twice
+// as long.
 #include "tagi_remax.h"
 #include "tagi_split_bf16.h"
 
@@ -573,7 +574,8 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
   __syncthreads();
   int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile) {
-    const short *left = lds + hidden(buf * KeysValues::halves + 8 * lane), *turned = lds + hidden(buf * KeysValues::halves + turned_at(lane));
+    const short *left = lds + hidden(buf * KeysValues::halves + 8 * lane),
+                *turned = lds + hidden(buf * KeysValues::halves + turned_at(lane));
     const bool more = key0 + kTile < to;
     if constexpr (ahead) {
       if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), true, u);
@@ -721,7 +723,8 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
   __syncthreads();
   int buf = 0;
   for (int key0 = from; key0 < to; key0 += kTile) {
-    const short *left = lds + hidden(buf * KeysValues::halves + 8 * lane), *turned = lds + hidden(buf * KeysValues::halves + turned_at(lane));
+    const short *left = lds + hidden(buf * KeysValues::halves + 8 * lane),
+                *turned = lds + hidden(buf * KeysValues::halves + turned_at(lane));
     const bool more = key0 + kTile < to;
     if constexpr (ahead) {
       if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 2, wave, hidden(lane), false, u);
@@ -819,7 +822,8 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   constexpr int bufs = 2 * Queries::bytes + 2 * 5 * kTile * 4 <= kLdsBytes ? 2 : 1;
   extern __shared__ __align__(16) short lds[];
   constexpr bool ahead = units_of<DP, W>(2) == 1;
-  float* const stats = reinterpret_cast<float*>(lds + bufs * Queries::halves);  // [buffer][5][kTile]: 1 / mt, vt, c_mt, 1 / s, limit
+  // [buffer][5][kTile]: 1 / mt, vt, c_mt, 1 / s, limit
+  float* const stats = reinterpret_cast<float*>(lds + bufs * Queries::halves);
   const Place p = place(A, (A.N + kKeys - 1) / kKeys);
   const Seq s = sequence(A, p.b);
   const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
@@ -902,7 +906,8 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   __syncthreads();
   int buf = 0;
   for (int64_t rho0 = from; rho0 < to; rho0 += kTile) {
-    const short *left = lds + hidden(buf * Queries::halves + 8 * lane), *turned = lds + hidden(buf * Queries::halves + turned_at(lane));
+    const short *left = lds + hidden(buf * Queries::halves + 8 * lane),
+                *turned = lds + hidden(buf * Queries::halves + turned_at(lane));
     const float* st = stats + buf * 5 * kTile;
     const bool more = rho0 + kTile < to;
     const bool busy = wave_key < s.len && rho0 + kTile > mine.first;

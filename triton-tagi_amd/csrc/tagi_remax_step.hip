@@ -229,8 +229,9 @@ __device__ __forceinline__ Right<HT> right_of(const float (&x)[8], int col) {
 template <int HT>
 __device__ __forceinline__ float over_parts(float x) {
   if constexpr (HT == 4) {
-    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));  // 8 columns on
-    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x124, 0xf, 0xf, true));  // 4 columns on
+    // row_ror: 8 columns on, then 4
+    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));
+    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x124, 0xf, 0xf, true));
   }
   return x;
 }
