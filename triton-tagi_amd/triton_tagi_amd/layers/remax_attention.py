@@ -32,12 +32,14 @@ from .rms_norm import RMSNorm
 @dataclass
 class AttentionState:
     """What a RemaxAttention keeps of a batch of sequences: ``lengths`` (B,) int64 tokens of each in
-    the pages that ``table`` names. ``used``: no length is above it, as the host counts them."""
+    the pages that ``table`` names. ``used``: no length is above it, as the host counts them; None
+    where it does not (a recorded graph's replays advance the lengths), and every call that is not
+    recorded reads them back."""
 
     cache: KVCache
     table: Tensor
     lengths: Tensor
-    used: int = 0
+    used: int | None = None
 
     @property
     def room(self) -> int:
@@ -226,12 +228,18 @@ class RemaxAttention(QkvProjections):
         width = -(-self.max_len // self.page_size)
         cache = new_kv_cache(batch * width, self.num_kv_heads, self.page_size, self.head_dim, self.cache_dtype, dev)
         table = torch.arange(batch * width, device=dev, dtype=torch.int32).view(batch, width)
-        return AttentionState(cache, table, torch.zeros(batch, device=dev, dtype=torch.int64))
+        return AttentionState(cache, table, torch.zeros(batch, device=dev, dtype=torch.int64), 0)
 
-    def _room(self, state: AttentionState, tokens: int) -> None:
-        if state.used + tokens > min(self.max_len, state.room):
-            raise ValueError(f"RemaxAttention: {state.used} + {tokens} tokens, max_len is "
-                             f"{min(self.max_len, state.room)}")
+    def _bound(self, state: AttentionState, tokens: int) -> int:
+        """No length is above it after ``tokens`` more, which the room has to hold. A recorded call keeps
+        the whole room: every replay finds other lengths, which are its caller's to bound."""
+        recorded = torch.cuda.is_current_stream_capturing()
+        limit, used = min(self.max_len, state.room), state.used
+        if used is None and not recorded:
+            used = int(state.lengths.max())
+        if used is not None and used + tokens > limit:
+            raise ValueError(f"RemaxAttention: {used} + {tokens} tokens, max_len is {limit}")
+        return state.room if recorded else used + tokens
 
     def prompt(self, ma: Tensor, Sa: Tensor, lengths: Tensor | None = None, state: AttentionState | None = None):
         """``forward`` after the tokens of ``state`` (none without) that keeps nothing for a backward:
@@ -244,11 +252,9 @@ class RemaxAttention(QkvProjections):
         if not fresh and (not isinstance(state, AttentionState) or state.lengths.shape[0] != B):
             raise ValueError(f"state: expected an AttentionState of {B} sequences")
         if fresh:
-            end = self.new_state(B, ma.device)
-        else:
-            self._room(state, T)
-            end = state.clone()
-        self._room(end, T)
+            state = self.new_state(B, ma.device)
+        bound = self._bound(state, T)
+        end = state if fresh else state.clone()
         starts = None if fresh else end.lengths
         _, ops = self._project(ma, Sa, self._positions(ma, starts, None))
         added = torch.full_like(end.lengths, T) if lengths is None else lengths.clamp(0, T).to(torch.int64)
@@ -256,22 +262,23 @@ class RemaxAttention(QkvProjections):
             raise ValueError(f"lengths: expected ({B},), got {tuple(added.shape)}")
         cache_write(end.cache, *ops[2:], end.table, starts, added)
         total = end.lengths + added
-        keys = ops[2:] if fresh else cache_read(end.cache, end.table, total, end.used + T)
+        keys = ops[2:] if fresh else cache_read(end.cache, end.table, total, bound)
         mo, So = remax_attention(*ops[:2], *keys, scale=self._scale, lengths=total, starts=starts)
-        end.lengths, end.used = total, end.used + T
+        end.lengths, end.used = total, None if torch.cuda.is_current_stream_capturing() else bound
         return mo.view(ma.shape), So.view(ma.shape), end
 
     def step(self, ma: Tensor, Sa: Tensor, state: AttentionState, active: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """One token of every sequence, (B, E) or (B, 1, E); ``state`` is advanced in place. ``active``
         (B,): sequences that are off keep their state and get zeros. A recorded graph's replays
-        advance the state without the host's count: at most ``max_len`` tokens are its caller's to keep."""
+        advance the state without the host: at most ``max_len`` tokens are its caller's to keep, and
+        calls on this state that are not recorded read its lengths back (a wait for the GPU)."""
         if ma.dim() not in (2, 3) or (ma.dim() == 3 and ma.shape[1] != 1):
             raise ValueError(f"RemaxAttention.step: expected (batch, features) or (batch, 1, features), "
                              f"got {tuple(ma.shape)}")
         B, E = ma.shape[0], ma.shape[-1]
         if not isinstance(state, AttentionState) or state.lengths.shape[0] != B:
             raise ValueError(f"state: expected an AttentionState of {B} sequences")
-        self._room(state, 1)
+        bound = self._bound(state, 1)
         at = state.lengths
         positions = self._positions(ma.reshape(B, 1, E), at, None)
         _, ops = self._project(ma.reshape(B, 1, E), None if Sa is None else Sa.reshape(B, 1, E), positions)
@@ -286,9 +293,11 @@ class RemaxAttention(QkvProjections):
             cache_write(state.cache, *ops[2:], state.table, at, on)
             at.add_(on)
             seen = at * on
-        state.used += 1
-        # a recorded graph's lengths go on beyond the host's count: it keeps the whole room
-        most = None if torch.cuda.is_current_stream_capturing() else -(-state.used // 256) * 256
+        if torch.cuda.is_current_stream_capturing():
+            state.used = None
+        elif state.used is not None:
+            state.used = bound
+        most = -(-bound // 256) * 256
         mo, So = remax_attention_step(ops[0][:, 0], ops[1][:, 0], state.cache, state.table, seen, scale=self._scale,
                                       max_len=most)
         return mo.view(ma.shape), So.view(ma.shape)
