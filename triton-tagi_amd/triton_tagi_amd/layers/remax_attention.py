@@ -34,7 +34,7 @@ class AttentionState:
     """What a RemaxAttention keeps of a batch of sequences: ``lengths`` (B,) int64 tokens of each in
     the pages that ``table`` names. ``used``: no length is above it, as the host counts them; None
     where it does not (a recorded graph's replays advance the lengths), and every call that is not
-    recorded reads them back."""
+    recorded reads them back, as it does where the count would not fit and the lengths may."""
 
     cache: KVCache
     table: Tensor
@@ -230,16 +230,19 @@ class RemaxAttention(QkvProjections):
         table = torch.arange(batch * width, device=dev, dtype=torch.int32).view(batch, width)
         return AttentionState(cache, table, torch.zeros(batch, device=dev, dtype=torch.int64), 0)
 
-    def _bound(self, state: AttentionState, tokens: int) -> int:
-        """No length is above it after ``tokens`` more, which the room has to hold. A recorded call keeps
-        the whole room: every replay finds other lengths, which are its caller's to bound."""
+    def _bound(self, state: AttentionState, tokens: int, added: Tensor | None = None) -> int:
+        """No length is above it after ``tokens`` more (of each sequence ``added`` (B,) where given), which
+        the room has to hold. The host counts every sequence as if it took all ``tokens``; where that
+        count does not fit, or there is none, the lengths are read back. A recorded call keeps the
+        whole room: every replay finds other lengths (and ``added``), which are its caller's to bound."""
         recorded = torch.cuda.is_current_stream_capturing()
-        limit, used = min(self.max_len, state.room), state.used
-        if used is None and not recorded:
-            used = int(state.lengths.max())
-        if used is not None and used + tokens > limit:
-            raise ValueError(f"RemaxAttention: {used} + {tokens} tokens, max_len is {limit}")
-        return state.room if recorded else used + tokens
+        limit = min(self.max_len, state.room)
+        most = None if state.used is None or (recorded and added is not None) else state.used + tokens
+        if not recorded and (most is None or most > limit):
+            most = int((state.lengths + (tokens if added is None else added)).max())
+        if most is not None and most > limit:
+            raise ValueError(f"RemaxAttention: a sequence of up to {most} tokens, max_len is {limit}")
+        return state.room if recorded else most
 
     def prompt(self, ma: Tensor, Sa: Tensor, lengths: Tensor | None = None, state: AttentionState | None = None):
         """``forward`` after the tokens of ``state`` (none without) that keeps nothing for a backward:
@@ -253,13 +256,13 @@ class RemaxAttention(QkvProjections):
             raise ValueError(f"state: expected an AttentionState of {B} sequences")
         if fresh:
             state = self.new_state(B, ma.device)
-        bound = self._bound(state, T)
+        added = torch.full_like(state.lengths, T) if lengths is None else lengths.clamp(0, T).to(torch.int64)
+        if tuple(added.shape) != (B,):
+            raise ValueError(f"lengths: expected ({B},), got {tuple(added.shape)}")
+        bound = self._bound(state, T, None if lengths is None else added)
         end = state if fresh else state.clone()
         starts = None if fresh else end.lengths
         _, ops = self._project(ma, Sa, self._positions(ma, starts, None))
-        added = torch.full_like(end.lengths, T) if lengths is None else lengths.clamp(0, T).to(torch.int64)
-        if tuple(added.shape) != (B,):
-            raise ValueError(f"lengths: expected ({B},), got {tuple(added.shape)}")
         cache_write(end.cache, *ops[2:], end.table, starts, added)
         total = end.lengths + added
         keys = ops[2:] if fresh else cache_read(end.cache, end.table, total, bound)
@@ -278,21 +281,18 @@ class RemaxAttention(QkvProjections):
         B, E = ma.shape[0], ma.shape[-1]
         if not isinstance(state, AttentionState) or state.lengths.shape[0] != B:
             raise ValueError(f"state: expected an AttentionState of {B} sequences")
-        bound = self._bound(state, 1)
-        at = state.lengths
-        positions = self._positions(ma.reshape(B, 1, E), at, None)
-        _, ops = self._project(ma.reshape(B, 1, E), None if Sa is None else Sa.reshape(B, 1, E), positions)
-        if active is None:
-            cache_write(state.cache, *ops[2:], state.table, at)
-            at.add_(1)
-            seen = at
-        else:
+        on = None
+        if active is not None:
             if active.dtype not in (torch.bool, torch.uint8) or tuple(active.shape) != (B,):
                 raise TypeError(f"active: expected a bool or uint8 tensor of ({B},)")
             on = (active != 0).to(torch.int64)
-            cache_write(state.cache, *ops[2:], state.table, at, on)
-            at.add_(on)
-            seen = at * on
+        bound = self._bound(state, 1, on)
+        at = state.lengths
+        positions = self._positions(ma.reshape(B, 1, E), at, None)
+        _, ops = self._project(ma.reshape(B, 1, E), None if Sa is None else Sa.reshape(B, 1, E), positions)
+        cache_write(state.cache, *ops[2:], state.table, at, on)
+        at.add_(1 if on is None else on)
+        seen = at if on is None else at * on
         if torch.cuda.is_current_stream_capturing():
             state.used = None
         elif state.used is not None:
