@@ -48,7 +48,7 @@ constexpr int kLdsBytes = 160 * 1024;
 // Walked by one block at most: the matrix cores cut sums off (they do not round them), and what is
 // lost of a sum of positive terms grows with their number (late rows' variances: 1.6e-6 after 2048
 // keys, 1e-6 after 1024; the join takes 23 us more of 6.2 ms at 4096 tokens). The gradients' terms have
-// both signs: 1e-6 after 2048. The splits are added in fp32.
+// both signs: 1e-6 after 2048. What blocks walked is added in fp32.
 constexpr int kMostWalked = 1024, kMostWalkedBack = 2048;
 
 struct Args {
@@ -59,7 +59,10 @@ struct Args {
   float *mo, *So, *rows, *dmk, *dSk, *dmv, *dSv;  // mo, So: dmq, dSq in the backward
   float *sums, *parts;  // workspace: [split][2][BG][M], [split][BG][M][2 D + 1] (or [..][N][4 D])
   int64_t B, M;         // M = T R rows of a key head
-  int T, N, H, G, R, D, splits, chunk;
+  int T, N, H, G, R, D;
+  // The walked side: launch l's split i has the chunk l splits + i; the statistics' split i, all of one
+  // launch, that of stat_chunk. parted: outputs are joined from parts.
+  int splits, chunk, launch, parted, stat_chunk;
   float c, c2;
 };
 
@@ -258,6 +261,10 @@ __device__ __forceinline__ void mma_left(const short* left, int first, int kt, i
 // of those in use.
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
+// Before a loop of a thousand instructions: from the middle of an instruction cache line they take 2%
+// longer (outputs of 64 features 1.46 -> 1.43 ms, dq 1.53 -> 1.49 at 2 x 4096 tokens).
+__device__ __forceinline__ void at_line() { asm volatile(".p2align 6"); }
+
 // Moments of the scores of 16 walked rows: m = a0 b0, v = a1 b1 + a2 b2 with a0, a1, a2 the parts
 // 0, 3, 6 of the tile.
 template <int DP>
@@ -440,8 +447,8 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
   const Seq s = sequence(A, p.b);
   const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
   const int64_t block0 = p.block * NC * kRows, wave0 = block0 + wave * NC * 16;
-  const int from = p.split * A.chunk;
-  auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
+  const int from = p.split * A.stat_chunk;
+  auto end = [&](int n) { return n < from + A.stat_chunk ? n : from + A.stat_chunk; };
   const int to = end(block_limit(A, s, block0, NC * kRows)), wave_to = end(block_limit(A, s, wave0, NC * 16));
   if (from >= to) return;
   Right<DP> q[NC], Q[NC], P[NC];
@@ -461,8 +468,14 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
   fetch_keys<DP, VEC, W>(A, p, from, to, 1, wave, lane, false, u);
   put_keys<DP, W>(lds, 1, wave, lane, false, u);
   __syncthreads();
-  int buf = 0;
+  float mts[NC] = {}, vts[NC] = {};  // sums of every kMostWalked keys: the rounding of many grows with their number
+  int buf = 0, stop = from + kMostWalked;
   for (int key0 = from; key0 < to; key0 += kTile, buf ^= 1) {
+    if (key0 == stop) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) mts[c] += mt[c], vts[c] += vt[c], mt[c] = vt[c] = 0.f;
+      stop += kMostWalked;
+    }
     const short* left = lds + hidden(buf * Keys::halves + 8 * lane);
     const bool more = key0 + kTile < to;
     if (more) fetch_keys<DP, VEC, W>(A, p, key0 + kTile, to, 1, wave, hidden(lane), false, u);
@@ -523,7 +536,7 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const float x = group_sum(mt[c]), y = group_sum(vt[c]);
+    const float x = group_sum(mts[c] + mt[c]), y = group_sum(vts[c] + vt[c]);
     const int64_t rho = wave0 + 16 * c + lane;
     if (k8 == 0 && rho < A.M) {
       float* o = A.sums + ((int64_t)p.split * 2 * A.B * A.G + p.bg) * A.M + rho;
@@ -532,12 +545,11 @@ __global__ void __launch_bounds__(64 * W) stats_kernel(const Args A) {
   }
 }
 
-// The splits that reach a row, and their sums in order.
-__device__ __forceinline__ int splits_to(const Args& A, int lim) { return (lim + A.chunk - 1) / A.chunk; }
+// The sums of the splits that reach a row, in order.
 __device__ __forceinline__ void add_sums(const Args& A, const Place& p, int64_t rho, int lim, float& mt, float& vt) {
   const float* o = A.sums + p.bg * A.M + rho;
   const int64_t step = A.B * A.G * A.M;
-  for (int i = 0; i < splits_to(A, lim); ++i, o += 2 * step) mt += o[0], vt += o[step];
+  for (int i = 0; i < (lim + A.stat_chunk - 1) / A.stat_chunk; ++i, o += 2 * step) mt += o[0], vt += o[step];
 }
 
 template <int DP, bool VEC, int W>
@@ -553,13 +565,13 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
   const Seq s = sequence(A, p.b);
   const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
   const int64_t block0 = p.block * kRows, wave0 = block0 + wave * 16, rho = wave0 + (lane & 15);
-  const int lim = row_limit(A, s, rho), from = p.split * A.chunk;
+  const int lim = row_limit(A, s, rho), from = (A.launch * A.splits + p.split) * A.chunk;
   auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
   const int to = end(block_limit(A, s, block0, kRows)), wave_to = end(block_limit(A, s, wave0, 16));
-  if (from >= to && p.split > 0) return;
+  if (from >= to && from > 0) return;
   float mt = 0.f, vt = 0.f;
   if (lim) add_sums(A, p, rho, lim, mt, vt);
-  if (p.split == 0 && k8 == 0 && rho < A.M)
+  if (from == 0 && k8 == 0 && rho < A.M)
     A.rows[stat_at(A, p.b, p.g, rho, 0)] = mt, A.rows[stat_at(A, p.b, p.g, rho, 1)] = vt;
   const RowSums rs = row_sums(mt, vt);
   Right<DP> q, Q, P;
@@ -573,6 +585,7 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
   if (from < to) pass_keys<DP, VEC, W>(A, p, from, to, lds, 2, wave, lane, true);
   __syncthreads();
   int buf = 0;
+  at_line();
   for (int key0 = from; key0 < to; key0 += kTile) {
     const short *left = lds + hidden(buf * KeysValues::halves + 8 * lane),
                 *turned = lds + hidden(buf * KeysValues::halves + turned_at(lane));
@@ -633,7 +646,7 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
   }
   sum = group_sum(sum);
   if (rho >= A.M) return;
-  if (A.splits > 1) {
+  if (A.parted) {
     float* o = A.parts + (((int64_t)p.split * A.B * A.G + p.bg) * A.M + rho) * (2 * A.D + 1);
     if (k8 == 0) o[2 * A.D] = sum;
 #pragma unroll
@@ -657,25 +670,30 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
     }
 }
 
-// The splits that reach a row added in order; a wave to a row. NORM: divided by the weights' sum.
+// The parts that reach a row added in order to what earlier launches left of it; a wave to a row. NORM:
+// divided by the weights' sum once they are complete.
 template <bool NORM>
 __global__ void __launch_bounds__(256) join_kernel(const Args A) {
   const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (i >= A.B * A.G * A.M) return;
   const int width = 2 * A.D + (NORM ? 1 : 0);
   const int64_t bg = i / A.M, rho = i - bg * A.M, b = bg / A.G, step = A.B * A.G * A.M * width;
-  const int g = (int)(bg - b * A.G), lane = threadIdx.x & 63, n = splits_to(A, row_limit(A, sequence(A, b), rho));
+  const int g = (int)(bg - b * A.G), lane = threadIdx.x & 63;
+  const int lim = row_limit(A, sequence(A, b), rho), chunks = (lim + A.chunk - 1) / A.chunk - A.launch * A.splits;
+  if (chunks <= 0 && A.launch > 0) return;  // complete
+  const int n = chunks < A.splits ? chunks : A.splits;
   const float* p = A.parts + i * width;
   float inv = 1.f;
   if constexpr (NORM) {
-    float sum = 0.f;
+    float* const to = A.rows + stat_at(A, b, g, rho, 2);
+    float sum = A.launch > 0 ? *to : 0.f;
     for (int k = 0; k < n; ++k) sum += p[k * step + 2 * A.D];
-    if (lane == 0) A.rows[stat_at(A, b, g, rho, 2)] = sum;
-    inv = fast_rcp(fmaxf(sum, kRemaxFloor));
+    if (lane == 0) *to = sum;
+    if (chunks <= A.splits) inv = fast_rcp(fmaxf(sum, kRemaxFloor));
   }
   const int64_t o = row_at(A, A.loq, b, g, rho);
   for (int f = lane; f < A.D; f += 64) {
-    float x = 0.f, y = 0.f;
+    float x = A.launch > 0 ? A.mo[o + f] : 0.f, y = A.launch > 0 ? A.So[o + f] : 0.f;
     for (int k = 0; k < n; ++k) x += p[k * step + f], y += p[k * step + A.D + f];
     A.mo[o + f] = x * inv, A.So[o + f] = y * (inv * inv);
   }
@@ -696,10 +714,10 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
   const Seq s = sequence(A, p.b);
   const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
   const int64_t block0 = p.block * kRows, wave0 = block0 + wave * 16, rho = wave0 + (lane & 15);
-  const int lim = row_limit(A, s, rho), from = p.split * A.chunk;
+  const int lim = row_limit(A, s, rho), from = (A.launch * A.splits + p.split) * A.chunk;
   auto end = [&](int n) { return n < from + A.chunk ? n : from + A.chunk; };
   const int to = end(block_limit(A, s, block0, kRows)), wave_to = end(block_limit(A, s, wave0, 16));
-  if (from >= to && p.split > 0) return;
+  if (from >= to && from > 0) return;
   float mt = 0.f, vt = 0.f, sum = 0.f;
   if (lim)
     mt = A.rows[stat_at(A, p.b, p.g, rho, 0)], vt = A.rows[stat_at(A, p.b, p.g, rho, 1)],
@@ -722,6 +740,7 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
   if (from < to) pass_keys<DP, VEC, W>(A, p, from, to, lds, 2, wave, lane, false);
   __syncthreads();
   int buf = 0;
+  at_line();
   for (int key0 = from; key0 < to; key0 += kTile) {
     const short *left = lds + hidden(buf * KeysValues::halves + 8 * lane),
                 *turned = lds + hidden(buf * KeysValues::halves + turned_at(lane));
@@ -784,7 +803,7 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args A) {
     __syncthreads();
   }
   if (rho >= A.M) return;
-  const bool whole = A.splits == 1;
+  const bool whole = !A.parted;
   float* const to_m = whole ? A.mo + row_at(A, A.loq, p.b, p.g, rho)
                             : A.parts + (((int64_t)p.split * A.B * A.G + p.bg) * A.M + rho) * (2 * A.D);
   float* const to_S = whole ? A.So + row_at(A, A.loq, p.b, p.g, rho) : to_m + A.D;
@@ -829,9 +848,9 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   const int wave = wave_id(), lane = threadIdx.x & 63, k8 = lane >> 4;
   const int key0 = (int)p.block * kKeys, wave_key = key0 + wave * 16, key = wave_key + (lane & 15);
   const RowRange all = rows_of(A, s, key0), mine = rows_of(A, s, wave_key);
-  const int64_t chunk0 = (int64_t)p.split * A.chunk, chunk1 = chunk0 + A.chunk;
+  const int64_t chunk0 = ((int64_t)A.launch * A.splits + p.split) * A.chunk, chunk1 = chunk0 + A.chunk;
   const int64_t from = all.first > chunk0 ? all.first : chunk0, to = all.end < chunk1 ? all.end : chunk1;
-  if (from >= to && A.splits > 1) return;
+  if (from >= to && A.parted) return;
   const bool on = key < s.len;
   constexpr int DK = KEYS ? DT : 1, DV = VALUES ? DT : 1;
   Right<DP> k, K, Sk, vm, vv;
@@ -905,6 +924,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   if (from < to) pass_rows(from, 0);
   __syncthreads();
   int buf = 0;
+  at_line();
   for (int64_t rho0 = from; rho0 < to; rho0 += kTile) {
     const short *left = lds + hidden(buf * Queries::halves + 8 * lane),
                 *turned = lds + hidden(buf * Queries::halves + turned_at(lane));
@@ -1011,7 +1031,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
     __syncthreads();
   }
   if (key >= A.N) return;
-  const bool whole = A.splits == 1;
+  const bool whole = !A.parted;
   const int64_t at = whole ? key_at(A.lokv, p.b, p.g, key) : (((int64_t)p.split * A.B * A.G + p.bg) * A.N + key) * (4 * A.D);
   auto put_out = [&](float* out, int i, const auto& x) {
     float* const o = (whole ? out : A.parts + i * A.D) + at;
@@ -1027,23 +1047,29 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   if constexpr (VALUES) put_out(A.dmv, 2, ovm), put_out(A.dSv, 3, ovS);
 }
 
-// The splits of rows that reach a key, in order; a wave to a key. kv_keys: keys of a dkv block.
+// The parts of the rows that see a key, in order, added to what earlier launches left; a wave to a key.
+// kv_keys: keys of a dkv block.
 __global__ void __launch_bounds__(256) join_keys_kernel(const Args A, int kv_keys) {
   const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (i >= A.B * A.G * A.N) return;
   const int64_t bg = i / A.N, b = bg / A.G, step = A.B * A.G * A.N * (4 * A.D);
   const int key = (int)(i - bg * A.N), g = (int)(bg - b * A.G);
   const RowRange r = rows_of(A, sequence(A, b), key / kv_keys * kv_keys);
-  const int k0 = (int)(r.first / A.chunk), k1 = (int)((r.end + A.chunk - 1) / A.chunk);
+  // chunks of rows, from those of this launch on
+  const int before = A.launch * A.splits, k0 = (int)(r.first / A.chunk) - before;
+  const int k1 = (int)((r.end + A.chunk - 1) / A.chunk) - before;
+  if (A.launch > 0 && (k1 <= 0 || k0 >= A.splits)) return;
+  const bool more = k0 < 0;
+  const int from = k0 < 0 ? 0 : k0, to = k1 < A.splits ? k1 : A.splits;
   const float* p = A.parts + i * (4 * A.D);
   const int64_t o = key_at(A.lokv, b, g, key);
   for (int f = threadIdx.x & 63; f < 4 * A.D; f += 64) {
-    float x = 0.f;
-    if (r.first < r.end)
-      for (int k = k0; k < k1; ++k) x += p[k * step + f];
     const int q = f / A.D;
-    float* out = q == 0 ? A.dmk : (q == 1 ? A.dSk : (q == 2 ? A.dmv : A.dSv));
-    out[o + f - q * A.D] = x;
+    float* const out = (q == 0 ? A.dmk : (q == 1 ? A.dSk : (q == 2 ? A.dmv : A.dSv))) + o + f - q * A.D;
+    float x = more ? *out : 0.f;
+    if (r.first < r.end)
+      for (int k = from; k < to; ++k) x += p[k * step + f];
+    *out = x;
   }
 }
 
@@ -1060,20 +1086,31 @@ constexpr int back_waves() {
 }
 int back_rows(int64_t D) { return 16 * (D > 64 ? 4 : 8); }
 
-// Splits of `walked` for blocks of `rows` of `own` on each of BG key heads: as many as fill the
+// Chunks of `walked` for blocks of `rows` of `own` on each of BG key heads: as many as fill the
 // GPU three times over, at least 256 walked each (a block's own operands are loaded and split again
-// for each) and at most `most`.
+// for each) and at most `most`. A launch's splits have their own parts in the workspace, 8192 blocks' worth
+// at most, so that it does not grow with both lengths; further chunks take further launches, whose last
+// rounds causal blocks leave half empty: 16384 tokens, 32 heads of 128 over 8, both directions, 360 ms and
+// 1.1 GB; 16384 blocks' worth 358 and 2.2; 4096 blocks' 369 and 0.5; all chunks at once 353 and 8.7.
 struct Splits {
-  int n, chunk;
+  int n, chunk, launches, stat_chunk;
+  bool parted() const { return n > 1 || launches > 1; }
 };
 Splits splits_of(int64_t own, int64_t rows, int64_t BG, int64_t walked, int64_t most) {
-  const int64_t blocks = cdiv(own, rows) * BG;
+  const int64_t blocks = cdiv(own, rows) * BG, room = cdiv(8192, blocks < 1 ? 1 : blocks);
   int64_t n = cdiv(768, blocks < 1 ? 1 : blocks);
   if (n > cdiv(walked, 256)) n = cdiv(walked, 256);
   if (n < cdiv(walked, most)) n = cdiv(walked, most);
   if (n < 1) n = 1;
-  const int64_t chunk = cdiv(cdiv(walked, n), kTile) * kTile;
-  return {(int)n, (int)(chunk < kTile ? kTile : chunk)};
+  const int64_t launches = cdiv(n, room), splits = cdiv(n, launches);
+  auto tiles = [&](int64_t chunks) {
+    const int64_t x = cdiv(cdiv(walked, chunks), kTile) * kTile;
+    return (int)(x < kTile ? kTile : x);
+  };
+  return {(int)splits, tiles(splits * launches), (int)launches, tiles(splits)};
+}
+void set(Args& a, const Splits& sp) {
+  a.splits = sp.n, a.chunk = sp.chunk, a.parted = sp.parted(), a.stat_chunk = sp.stat_chunk;
 }
 
 int check_sizes(const char* what, int64_t B, int64_t T, int64_t N, int64_t H, int64_t G, int64_t D) {
@@ -1104,7 +1141,7 @@ void go(K kernel, dim3 grid, int threads, int lds, hipStream_t s, const Args& a)
 constexpr int two_or_one(int bytes, int more) { return (2 * (bytes + more) <= kLdsBytes ? 2 : 1) * (bytes + more); }
 
 template <int DP, bool VEC>
-int forward(const char* what, Args a, hipStream_t s) {
+int forward(const char* what, Args a, int launches, hipStream_t s) {
   const int64_t BG = a.B * a.G;
   constexpr int NC = DP > 64 ? 1 : 2;
   dim3 grid;
@@ -1112,8 +1149,10 @@ int forward(const char* what, Args a, hipStream_t s) {
   dim3 out;
   if (int rc = grid_of(what, a.M, 16 * kOutWaves, BG, a.splits, 64 * kOutWaves, &out)) return rc;
   go(stats_kernel<DP, VEC, kStatsWaves, NC>, grid, 64 * kStatsWaves, 2 * Tile<DP, 9>::bytes, s, a);
-  go(outputs_kernel<DP, VEC, kOutWaves>, out, 64 * kOutWaves, two_or_one(Tile<DP, 18>::bytes, 0), s, a);
-  if (a.splits > 1) hipLaunchKernelGGL(join_kernel<true>, join_grid(BG * a.M), dim3(256), 0, s, a);
+  for (a.launch = 0; a.launch < launches; ++a.launch) {
+    go(outputs_kernel<DP, VEC, kOutWaves>, out, 64 * kOutWaves, two_or_one(Tile<DP, 18>::bytes, 0), s, a);
+    if (a.parted) hipLaunchKernelGGL(join_kernel<true>, join_grid(BG * a.M), dim3(256), 0, s, a);
+  }
   return TAGI_OK;
 }
 template <int DP, bool VEC>
@@ -1122,25 +1161,29 @@ int backward(const char* what, Args a, float* ws, hipStream_t s) {
   constexpr int W = back_waves<DP>(), rows = 16 * W;
   if (a.T) {
     const Splits sp = splits_of(a.M, rows, BG, a.N, kMostWalkedBack);
-    a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;
+    set(a, sp), a.parts = ws;
     dim3 grid;
     if (int rc = grid_of(what, a.M, rows, BG, sp.n, 64 * W, &grid)) return rc;
-    go(dq_kernel<DP, VEC, W>, grid, 64 * W, two_or_one(Tile<DP, 15>::bytes, 0), s, a);
-    if (sp.n > 1) hipLaunchKernelGGL(join_kernel<false>, join_grid(BG * a.M), dim3(256), 0, s, a);
+    for (a.launch = 0; a.launch < sp.launches; ++a.launch) {
+      go(dq_kernel<DP, VEC, W>, grid, 64 * W, two_or_one(Tile<DP, 15>::bytes, 0), s, a);
+      if (a.parted) hipLaunchKernelGGL(join_kernel<false>, join_grid(BG * a.M), dim3(256), 0, s, a);
+    }
   }
   if (a.N) {
     const Splits sp = splits_of(a.N, rows, BG, a.M, kMostWalkedBack);
-    a.splits = sp.n, a.chunk = sp.chunk, a.parts = ws;  // the stream's order keeps the joins apart
+    set(a, sp), a.parts = ws;  // the stream's order keeps the joins apart
     dim3 grid;
     if (int rc = grid_of(what, a.N, rows, BG, sp.n, 64 * W, &grid)) return rc;
     const int lds = two_or_one(Tile<DP, 15>::bytes, 5 * kTile * 4);
-    if constexpr (DP == 128) {
-      go(dkv_kernel<DP, VEC, W, true, false>, grid, 64 * W, lds, s, a);
-      go(dkv_kernel<DP, VEC, W, false, true>, grid, 64 * W, lds, s, a);
-    } else {
-      go(dkv_kernel<DP, VEC, W, true, true>, grid, 64 * W, lds, s, a);
+    for (a.launch = 0; a.launch < sp.launches; ++a.launch) {
+      if constexpr (DP == 128) {
+        go(dkv_kernel<DP, VEC, W, true, false>, grid, 64 * W, lds, s, a);
+        go(dkv_kernel<DP, VEC, W, false, true>, grid, 64 * W, lds, s, a);
+      } else {
+        go(dkv_kernel<DP, VEC, W, true, true>, grid, 64 * W, lds, s, a);
+      }
+      if (a.parted) hipLaunchKernelGGL(join_keys_kernel, join_grid(BG * a.N), dim3(256), 0, s, a, rows);
     }
-    if (sp.n > 1) hipLaunchKernelGGL(join_keys_kernel, join_grid(BG * a.N), dim3(256), 0, s, a, rows);
   }
   return TAGI_OK;
 }
@@ -1162,7 +1205,7 @@ extern "C" int64_t tagi_remax_attention_fwd_ws_bytes(int64_t B, int64_t T, int64
                                                      int64_t D) {
   if (B <= 0 || T <= 0 || N < 0 || H <= 0 || G <= 0 || D <= 0 || H % G) return 0;
   const Splits sp = splits_of(T * (H / G), 16 * kOutWaves, B * G, N, kMostWalked);
-  return 4 * B * H * T * sp.n * (2 + (sp.n > 1 ? 2 * D + 1 : 0));
+  return 4 * B * H * T * sp.n * (2 + (sp.parted() ? 2 * D + 1 : 0));
 }
 
 extern "C" int tagi_remax_attention_fwd(const float* mq, const float* Sq, const tagi_heads* lq, const float* mk,
@@ -1190,9 +1233,9 @@ extern "C" int tagi_remax_attention_fwd(const float* mq, const float* Sq, const 
   a.B = B, a.T = (int)T, a.N = (int)N, a.H = (int)H, a.G = (int)G, a.R = (int)(H / G), a.D = (int)D, a.M = T * (H / G);
   a.c = (float)scale, a.c2 = (float)(scale * scale);
   const Splits sp = splits_of(a.M, 16 * kOutWaves, B * G, N, kMostWalked);
-  a.splits = sp.n, a.chunk = sp.chunk;
+  set(a, sp);
   a.sums = static_cast<float*>(ws), a.parts = a.sums + 2 * a.splits * B * H * T;
-  if (int rc = BY_DIM(forward, what, a, s)) return rc;
+  if (int rc = BY_DIM(forward, what, a, sp.launches, s)) return rc;
   return check_launch(what);
 }
 
@@ -1200,9 +1243,8 @@ extern "C" int64_t tagi_remax_attention_bwd_ws_bytes(int64_t B, int64_t T, int64
                                                      int64_t D) {
   if (B <= 0 || T < 0 || N < 0 || H <= 0 || G <= 0 || D <= 0 || H % G) return 0;
   const int64_t M = T * (H / G), rows = back_rows(D);
-  const int q = splits_of(M, rows, B * G, N, kMostWalkedBack).n,
-            kv = splits_of(N, rows, B * G, M, kMostWalkedBack).n;
-  const int64_t a = q > 1 ? q * B * G * M * 2 * D : 0, b = kv > 1 ? kv * B * G * N * 4 * D : 0;
+  const Splits q = splits_of(M, rows, B * G, N, kMostWalkedBack), kv = splits_of(N, rows, B * G, M, kMostWalkedBack);
+  const int64_t a = q.parted() ? q.n * B * G * M * 2 * D : 0, b = kv.parted() ? kv.n * B * G * N * 4 * D : 0;
   return 4 * (a > b ? a : b);
 }
 
