@@ -851,7 +851,8 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args A) {
   const int64_t chunk0 = ((int64_t)A.launch * A.splits + p.split) * A.chunk, chunk1 = chunk0 + A.chunk;
   const int64_t from = all.first > chunk0 ? all.first : chunk0, to = all.end < chunk1 ? all.end : chunk1;
   if (from >= to && A.parted) return;
-  const bool on = key < s.len;
+  // zeros in place of a key behind the last query: whatever it holds would be NaN times a weight of 0
+  const bool on = key < s.len && (!A.causal || key < s.start + A.T);
   constexpr int DK = KEYS ? DT : 1, DV = VALUES ? DT : 1;
   Right<DP> k, K, Sk, vm, vv;
   load_right<DP, VEC>(A.mk, A.Sk, on ? key_at(A.lk, p.b, p.g, key) : 0, A.D, on, k8,
