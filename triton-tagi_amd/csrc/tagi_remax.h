@@ -20,6 +20,10 @@ constexpr float kRemaxFloor = 1e-6f;  // of means, variances, weights and their 
 // not change.
 constexpr float kVarFloor = 1e-20f;
 
+// The greater of the two, NaN where x is (fmaxf would give the floor): a mean and a weight that are NaN
+// reach the outputs.
+__device__ __forceinline__ float floored(float x, float floor) { return __builtin_elementwise_maximum(x, floor); }
+
 struct Rectified {
   float mm, vm;   // moments of max(z, 0), floored
   float cdf, rs;  // Phi(a), 1 / sqrt(v)
@@ -55,7 +59,7 @@ __device__ __forceinline__ Rectified rectify(float m, float v) {
   const float mean = fmaf(sd, f, up ? m : 0.0f);
   const float var = fmaf(-f, f, up ? 1.0f - fmaf(2.0f * x, f, q) : q);
   o.cdf = up ? 1.0f - tail : tail;
-  o.mm = fmaxf(mean, kRemaxFloor);
+  o.mm = floored(mean, kRemaxFloor);
   // where the floor lifts the mean by d, the variance is taken about the lifted one: less 2 d (mm -
   // m) and d^2, of which 2 d mm and d^2 are below 2e-6 of the variance's own floor
   o.vm = fmaxf(fmaf(-2.0f * m, mean - o.mm, v * var), kRemaxFloor);
@@ -68,7 +72,7 @@ struct RowSums {
 };
 __device__ __forceinline__ RowSums row_sums(float mt, float vt) {
   RowSums r;
-  r.inv_mt = fast_rcp(fmaxf(mt, kRemaxFloor));
+  r.inv_mt = fast_rcp(floored(mt, kRemaxFloor));
   r.vt = fmaxf(vt, kRemaxFloor);
   r.c_mt = fmaf(r.vt * r.inv_mt, r.inv_mt, 1.0f) * r.inv_mt;
   return r;
@@ -88,7 +92,7 @@ __device__ __forceinline__ Weight weigh(const Rectified& z, const RowSums& r) {
   Weight o;
   const float s = z.vm * r.inv_mt, d = z.mm + s;
   o.rd = fast_rcp(d);
-  o.w = fmaxf(z.mm * o.rd * z.mm * r.c_mt, kRemaxFloor);
+  o.w = floored(z.mm * o.rd * z.mm * r.c_mt, kRemaxFloor);
   const float p = z.mm * r.inv_mt;
   o.u = 1.0f - p;
   const float num = fmaf(r.vt - z.vm, fmaf(p, p, s * r.inv_mt), z.vm * (o.u * o.u));

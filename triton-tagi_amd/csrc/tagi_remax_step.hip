@@ -493,7 +493,7 @@ __device__ __forceinline__ void values_of(const Args& A) {
         for (int r = 0; r < HT; ++r) {
           if (HT > 4 && r >= n) continue;
           const Weight o = weigh(Rectified{z[r].x, z[r].y, 0.f, 0.f}, row[r]);
-          const bool there = key0 + lane < to && r < n && z[r].x > 0.f;
+          const bool there = key0 + lane < to && r < n && z[r].x != 0.f;
           const float w = there ? o.w : 0.f, k = there ? o.k : 0.f;
           total[r] += w;
           // the powers of two of the rows go into their weights

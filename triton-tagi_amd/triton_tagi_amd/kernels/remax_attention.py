@@ -13,7 +13,8 @@ dim's, which is 1; a mean and its variance share strides; other layouts are copi
 Query t of sequence b stands at position ``starts[b]`` + t (t without). It sees the keys j <
 ``lengths[b]`` (all without), with ``causal`` those up to its position. A query at or behind its
 sequence's length, or before 0, sees nothing: zeros, and no deltas; such queries and the keys behind
-a length may hold anything. Infinities and NaN inside a sequence may reach any of its queries.
+a length may hold anything. A NaN that a query sees makes its outputs NaN; infinities and NaN inside a
+sequence may reach any of its queries.
 
 ``remax_attention_step`` runs one query of every sequence over the pages of a cache (kv_cache.py).
 """
