@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -45,10 +46,45 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found (expected /opt/rocm/bin/hipcc)")
 
 
-def _run(cmd: list[str]) -> None:
+def _run(cmd: list[str]) -> str:
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"command failed ({proc.returncode}): {' '.join(cmd)}\n{proc.stdout}")
+    return proc.stdout
+
+
+# Units whose kernels keep everything in registers. In an earlier form of the attention kernels of four
+# waves (512 registers, half of them accumulation registers) operands of four registers that the compiler
+# had put into scratch memory came back wrong, for a reason that nobody has found in the source.
+NO_SCRATCH = ("tagi_remax_attention.hip", "tagi_remax_step.hip")
+
+
+def scratch_use(report: str) -> dict[str, int]:
+    """Bytes of scratch memory a lane of every kernel that a compiler's resource report names."""
+    use, name = {}, None
+    for line in report.splitlines():
+        m = re.search(r"remark:\s+(Function Name|ScratchSize \[bytes/lane\]): (\S+)", line)
+        if m is None:
+            continue
+        if m[1] == "Function Name":
+            name = m[2]
+        elif name is not None:
+            use[name] = int(m[2])
+    return use
+
+
+def compile_unit(hipcc: str, src: Path, obj: Path, defs: list[str]) -> None:
+    keep = src.name in NO_SCRATCH
+    report = _run([hipcc, *HIP_FLAGS, *defs, *(["-Rpass-analysis=kernel-resource-usage"] if keep else []), "-c", str(src),
+                   "-o", str(obj)])
+    if not keep:
+        return
+    use = scratch_use(report)
+    if not use:
+        raise RuntimeError(f"{src.name}: the compiler reported no kernel's resources")
+    bad = [f"{k}: {n} bytes a lane" for k, n in use.items() if n]
+    if bad:
+        raise RuntimeError(f"{src.name}: kernels in scratch memory\n" + "\n".join(bad))
 
 
 # tagi_gemm_inst.hip holds the GEMM kernels; it is compiled once per tile config (0..13)
@@ -84,7 +120,7 @@ def build(jobs: int | None = None, verbose: bool = True) -> Path:
         src, obj, defs = unit
         if verbose:
             print(f"[build] hipcc {src.name} {' '.join(defs)}".rstrip(), flush=True)
-        _run([hipcc, *HIP_FLAGS, *defs, "-c", str(src), "-o", str(obj)])
+        compile_unit(hipcc, src, obj, defs)
 
     # the instantiation units are the slowest: start them first
     with ThreadPoolExecutor(max_workers=jobs) as ex:

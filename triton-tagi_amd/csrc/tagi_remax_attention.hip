@@ -576,6 +576,10 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
   const RowSums rs = row_sums(mt, vt);
   Right<DP> q, Q, P;
   load_queries<DP, VEC>(A, lim ? row_at(A, A.lq, p.b, p.g, rho) : 0, lim > 0, k8, q, Q, P);
+  // Heads of 128: two of a query's 36 operands wait in LDS, the registers for them are not there.
+  static_assert(DP != 128 || bufs * KeysValues::bytes + 2 * 16 * 64 * W <= kLdsBytes, "they fit beside the tile");
+  bf8* const kept = reinterpret_cast<bf8*>(lds + bufs * KeysValues::halves) + threadIdx.x;
+  if constexpr (DP == 128) kept[0] = P.p[3].p[1], kept[64 * W] = P.p[3].p[2];
   const int whole = least(lim);
   float sum = 0.f;
   acc4 om[DT], oS[DT];
@@ -598,6 +602,7 @@ __global__ void __launch_bounds__(64 * W) outputs_kernel(const Args A) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         fence();
+        if constexpr (DP == 128) P.p[3].p[1] = kept[0], P.p[3].p[2] = kept[64 * W];
         acc4 m, v;
         scores<DP>(left, kt, q, Q, P, m, v);
 #pragma unroll
@@ -1076,8 +1081,8 @@ __global__ void __launch_bounds__(256) join_keys_kernel(const Args A, int kv_key
 
 // ------------------------------------------------------------------------------------ plans
 constexpr int kStatsWaves = 8, kOutWaves = 8;
-// Kernels of four waves keep what they have in 512 registers and nothing in scratch memory: operands of
-// four registers that the compiler had put there, beside accumulation registers, came back wrong.
+// Nothing lies in scratch memory (build.py refuses it here): in kernels of four waves operands of four
+// registers that the compiler had put there, beside accumulation registers, came back wrong.
 //
 // Waves of a backward block. Five right operands of 96 (128) features take 180 (240) registers: one
 // wave a SIMD has 512; eight waves would keep them in scratch memory.
@@ -1144,14 +1149,14 @@ constexpr int two_or_one(int bytes, int more) { return (2 * (bytes + more) <= kL
 template <int DP, bool VEC>
 int forward(const char* what, Args a, int launches, hipStream_t s) {
   const int64_t BG = a.B * a.G;
-  constexpr int NC = DP > 64 ? 1 : 2;
+  constexpr int NC = DP > 64 ? 1 : 2, kept = DP == 128 ? 2 * 16 * 64 * kOutWaves : 0;
   dim3 grid;
   if (int rc = grid_of(what, a.M, 16 * kStatsWaves * NC, BG, a.splits, 64 * kStatsWaves, &grid)) return rc;
   dim3 out;
   if (int rc = grid_of(what, a.M, 16 * kOutWaves, BG, a.splits, 64 * kOutWaves, &out)) return rc;
   go(stats_kernel<DP, VEC, kStatsWaves, NC>, grid, 64 * kStatsWaves, 2 * Tile<DP, 9>::bytes, s, a);
   for (a.launch = 0; a.launch < launches; ++a.launch) {
-    go(outputs_kernel<DP, VEC, kOutWaves>, out, 64 * kOutWaves, two_or_one(Tile<DP, 18>::bytes, 0), s, a);
+    go(outputs_kernel<DP, VEC, kOutWaves>, out, 64 * kOutWaves, two_or_one(Tile<DP, 18>::bytes, 0) + kept, s, a);
     if (a.parted) hipLaunchKernelGGL(join_kernel<true>, join_grid(BG * a.M), dim3(256), 0, s, a);
   }
   return TAGI_OK;

@@ -304,13 +304,16 @@ __device__ __forceinline__ void scores_of(const Args& A) {
   __shared__ float powers[kWaves][scaled_rows ? 2 * kWaveKeys : 1];
   __shared__ __align__(16) float tile[kWaves][2][HT * kRow];
   const int64_t b = blockIdx.z;
-  const int g = blockIdx.y, D = A.c.D, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, k8 = lane >> 4;
+  const int g = blockIdx.y, D = A.c.D, wave = threadIdx.x >> 6;
   const int len = length_of(A, b), from = ((int)blockIdx.x * kWaves + wave) * A.wave_keys;
   const int to = from + A.wave_keys < len ? from + A.wave_keys : len;
   int64_t* slot = slots[wave];
   float *pm = powers[wave], *pS = pm + (scaled_rows ? kWaveKeys : 0);
-  const int head = HT == 4 ? col & 3 : col;
   for (int r0 = 0; r0 < A.R; r0 += HT) {
+    int lane = threadIdx.x & 63;
+    // addresses are formed for each turn: where one turn takes the registers they would wait in scratch memory
+    if constexpr (HT > 4) asm volatile("" : "+v"(lane));
+    const int col = lane & 15, k8 = lane >> 4, head = HT == 4 ? col & 3 : col;
     const int n = A.R - r0 < HT ? A.R - r0 : HT;
     const int64_t h = b * A.H + g * A.R + r0;
     float mt[HT] = {}, vt[HT] = {};
