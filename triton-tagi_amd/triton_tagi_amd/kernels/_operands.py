@@ -39,6 +39,17 @@ def dense_like(t: Tensor, shape) -> Tensor:
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(shape)
 
 
+def written(ts, names, ref: Tensor, shape) -> None:
+    """Outputs of a caller's: one layout with a unit last stride, every element its own place."""
+    for t, n in zip(ts, names):
+        _lib.check_with(t, n, ref, shape)
+        st = t.stride()
+        if st != ts[0].stride() or (st[-1] != 1 and shape[-1] > 1):
+            raise ValueError(f"{', '.join(names)}: expected one layout with a last stride of 1, {n} has {st}")
+        if any(k == 0 and m > 1 for k, m in zip(st, shape)):
+            raise ValueError(f"{n}: an output's elements share their places, strides are {st}")
+
+
 def shape_of(t: Tensor, name: str, dims: int) -> torch.Size:
     _lib.check(t, name, contiguous=False)
     if t.dim() != dims or min(t.shape[-2:]) == 0:

@@ -25,7 +25,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._operands import counts, dense_like, finite_scale, heads, key_heads, mean, pair, shape_of
+from ._operands import counts, dense_like, finite_scale, heads, key_heads, mean, pair, shape_of, written
 from .kv_cache import KVCache, cache_struct, check_table
 
 
@@ -78,7 +78,7 @@ def remax_attention_backward(mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, mv:
     heads that share them."""
     dmq, dmk = (dense_like(t, t.shape) for t in (mq, mk))
     out = (dmq, torch.empty_like(dmq), dmk, *(torch.empty_like(dmk) for _ in range(3)))
-    remax_attention_backward_into(out, mq, Sq, mk, Sk, mv, delta_mo, delta_So, rows, scale, causal, lengths, starts)
+    _backward(out, mq, Sq, mk, Sk, mv, delta_mo, delta_So, rows, scale, causal, lengths, starts)
     return out
 
 
@@ -87,6 +87,15 @@ def remax_attention_backward_into(out, mq: Tensor, Sq: Tensor, mk: Tensor, Sk: T
                                   lengths: Tensor | None = None, starts: Tensor | None = None) -> None:
     """``remax_attention_backward`` into six tensors: the queries' two in one layout, the keys' and
     values' four in one, unit last strides."""
+    qs, ks = _sizes(mq, mk)
+    dmq, dSq, dmk, dSk, dmv, dSv = out
+    written((dmq, dSq), ("dmq", "dSq"), mq, qs)
+    written((dmk, dSk, dmv, dSv), ("dmk", "dSk", "dmv", "dSv"), mq, ks)
+    _backward(out, mq, Sq, mk, Sk, mv, delta_mo, delta_So, rows, scale, causal, lengths, starts)
+
+
+def _backward(out, mq: Tensor, Sq: Tensor, mk: Tensor, Sk: Tensor, mv: Tensor, delta_mo: Tensor, delta_So: Tensor,
+              rows: Tensor, scale: float, causal: bool, lengths: Tensor | None, starts: Tensor | None) -> None:
     qs, ks = _sizes(mq, mk)
     B, T, H, D = qs
     N, G = ks[1:3]

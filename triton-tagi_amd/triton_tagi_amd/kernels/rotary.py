@@ -20,7 +20,7 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ._operands import dense_like, heads, mean, pair, shape_of
+from ._operands import dense_like, heads, mean, pair, shape_of, written
 
 
 def rotary_frequencies(pairs: int, base: float = 10000.0, device="cuda") -> Tensor:
@@ -119,8 +119,8 @@ def qk_norm_rotary_backward(delta_mq: Tensor, delta_Sq: Tensor, delta_mk: Tensor
         dm = d inv g, dS = D (inv g)^2;  dmw = Sg sum d inv m, dSw = Sg^2 sum D (inv m)^2."""
     oqm, okm = (dense_like(t, t.shape) for t in (mq, mk))
     out = (oqm, torch.empty_like(oqm), okm, torch.empty_like(okm))
-    return (*out, *qk_norm_rotary_backward_into(out, delta_mq, delta_Sq, delta_mk, delta_Sk, mq, mk, inv, positions,
-                                                frequencies, weights, sections, interleaved))
+    return (*out, *_backward(out, delta_mq, delta_Sq, delta_mk, delta_Sk, mq, mk, inv, positions, frequencies, weights,
+                             sections, interleaved))
 
 
 def qk_norm_rotary_backward_into(out, delta_mq: Tensor, delta_Sq: Tensor, delta_mk: Tensor, delta_Sk: Tensor,
@@ -129,6 +129,17 @@ def qk_norm_rotary_backward_into(out, delta_mq: Tensor, delta_Sq: Tensor, delta_
                                  interleaved: bool = False) -> tuple[Tensor, ...]:
     """``qk_norm_rotary_backward`` into four tensors (a mean's and its variance's in one layout, unit
     last stride); returns the weights' deltas."""
+    qs, ks = _sizes(mq, mk)
+    oqm, oqS, okm, okS = out
+    written((oqm, oqS), ("dmq", "dSq"), mq, qs)
+    written((okm, okS), ("dmk", "dSk"), mq, ks)
+    return _backward(out, delta_mq, delta_Sq, delta_mk, delta_Sk, mq, mk, inv, positions, frequencies, weights, sections,
+                     interleaved)
+
+
+def _backward(out, delta_mq: Tensor, delta_Sq: Tensor, delta_mk: Tensor, delta_Sk: Tensor, mq: Tensor, mk: Tensor,
+              inv: Tensor | None, positions: Tensor | None, frequencies: Tensor | None, weights, sections,
+              interleaved: bool) -> tuple[Tensor, ...]:
     qs, ks = _sizes(mq, mk)
     B, T, H, D = qs
     G = ks[2]
