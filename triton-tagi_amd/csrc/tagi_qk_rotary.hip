@@ -23,7 +23,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr int kMaxAxes = 4;
-constexpr int kMaxBlocks = 1024;  // blocks of the backward, each with its own column sums
+// The backward: each block has its own column sums. 1024 of them fill the GPU; beyond, one thread adds up at
+// most kMostRows rows in fp32 (2^30 rows of one feature: 6e-5 wrong with 4096 rows a thread).
+constexpr int kMaxBlocks = 1024, kMostRows = 512;
 
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_fwd_kernel(const Args A) {
   }
 }
 
-// The column sums of the weights' deltas: a thread's rows in registers (at most a few hundred),
+// The column sums of the weights' deltas: a thread's rows in registers (at most kMostRows, or a token's),
 // a block's threads in a fixed order through LDS, the blocks' in float64 (column_sums_kernel).
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) qk_rotary_bwd_kernel(const Args A) {
@@ -302,8 +304,11 @@ int tokens_of(int64_t heads, int L) {
   return (int)(heads >= rows ? 1 : cdiv(rows, heads));
 }
 int64_t bwd_blocks(int64_t tokens, int64_t heads, int64_t D) {
-  const int64_t n = cdiv(tokens, tokens_of(heads, lanes_of(D)));
-  return n < kMaxBlocks ? n : kMaxBlocks;
+  const int L = lanes_of(D), TB = tokens_of(heads, L);
+  const int64_t n = cdiv(tokens, TB), rows = cdiv(TB * heads, kThreads / L);  // rows of a thread a turn
+  const int64_t turns = rows < kMostRows ? kMostRows / rows : 1, most = cdiv(n, turns);
+  const int64_t blocks = most > kMaxBlocks ? most : kMaxBlocks;
+  return n < blocks ? n : blocks;
 }
 
 int fill(const char* what, Args& a, int64_t B, int64_t T, int64_t H, int64_t G, int64_t D, const void* positions,
@@ -390,6 +395,7 @@ extern "C" int tagi_qk_rotary_bwd(const float* dmq, const float* dSq, const tagi
   TAGI_REQUIRE(a.tokens == 0 || G == 0 || (dmk && dSk && ldk && okm && okS && lok), "%s: null pointer", what);
   TAGI_REQUIRE(a.tokens == 0 || !wqm || (mq && lq && inv && (G == 0 || (mk && lk))), "%s: null pointer", what);
   const int64_t nblk = a.tokens ? bwd_blocks(a.tokens, H + G, D) : 0;
+  TAGI_REQUIRE(nblk * kThreads < (1ll << 32), "%s: too large", what);
   TAGI_REQUIRE(!wqm || !nblk || (ws && ws_bytes >= tagi_qk_rotary_bwd_ws_bytes(B, T, H, G, D)),
                "%s: workspace too small", what);
   hipStream_t s = (hipStream_t)stream;
