@@ -715,8 +715,8 @@ int tagi_qk_rotary_fwd(const float* mq, const float* Sq, const tagi_heads* lq, c
                        int interleaved, float eps, float* oqm, float* oqS, float* okm, float* okS,
                        float* inv, int64_t B, int64_t T, int64_t H, int64_t G, int64_t D,
                        tagi_stream_t stream);
-/* Its backward, inv held (rms_norm.py:115-134): deltas of the inputs (strides loq, lok), and with weights
- * their deltas (D each; queries' and keys', summed over tokens and heads, order fixed by the
+/* Its backward, inv held (rms_norm.py:115-134): deltas of the inputs (strides loq, lok; they may be dmq,
+ * dSq, dmk, dSk themselves with the same strides), and with weights their deltas (D each; queries' and keys', summed over tokens and heads, order fixed by the
  * sizes). mq, mk: the forward's input means (not read without weights). */
 int tagi_qk_rotary_bwd(const float* dmq, const float* dSq, const tagi_heads* ldq, const float* dmk,
                        const float* dSk, const tagi_heads* ldk, const float* mq,

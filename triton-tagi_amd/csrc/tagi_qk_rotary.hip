@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(kThreads) qk_rotary_bwd_kernel(const Args A) {
           da[j] *= wa, db[j] *= wb, ea[j] *= wa * wa, eb[j] *= wb * wb;
         }
       }
+      // the features that this lane has read: the outputs may be the deltas themselves
       const int64_t o = q ? head_at(A.loq, b, t, h) : head_at(A.lok, b, t, h - A.H);
       store_row<VEC>(A, (q ? A.oqm : A.okm) + o, lane, da, db);
       store_row<VEC>(A, (q ? A.oqS : A.okS) + o, lane, ea, eb);

@@ -128,7 +128,7 @@ def qk_norm_rotary_backward_into(out, delta_mq: Tensor, delta_Sq: Tensor, delta_
                                  frequencies: Tensor | None = None, weights=None, sections=None,
                                  interleaved: bool = False) -> tuple[Tensor, ...]:
     """``qk_norm_rotary_backward`` into four tensors (a mean's and its variance's in one layout, unit
-    last stride); returns the weights' deltas."""
+    last stride), which may be the four deltas themselves; returns the weights' deltas."""
     qs, ks = _sizes(mq, mk)
     oqm, oqS, okm, okS = out
     written((oqm, oqS), ("dmq", "dSq"), mq, qs)

@@ -188,14 +188,10 @@ class RemaxAttention(QkvProjections):
         # the deltas of Q, K and V side by side, for one projection backward
         dm, dS = (torch.empty(B, T, H + 2 * G, D, device=delta_mz.device, dtype=torch.float32) for _ in range(2))
         q, k, v = ((dm[:, :, a:b], dS[:, :, a:b]) for a, b in ((0, H), (H, H + G), (H + G, H + 2 * G)))
-        own = q, k  # the deltas of queries and keys as attention read them, before the norm
-        if c["rotary"] is not None:
-            own = (tuple(torch.empty(B, T, H, D, device=dm.device) for _ in range(2)),
-                   tuple(dm.new_empty(B, T, H + 2 * G, D)[:, :, H:H + G] for _ in range(2)))
-        remax_attention_backward_into((*own[0], *own[1], *v), *c["ops"], delta_mz.reshape(shape),
-                                      delta_Sz.reshape(shape), c["rows"], scale=self._scale, lengths=c["lengths"])
-        if c["rotary"] is not None:
-            dw = qk_norm_rotary_backward_into((*q, *k), *own[0], *own[1], *c["raw"], c["inv"], **c["rotary"])
+        remax_attention_backward_into((*q, *k, *v), *c["ops"], delta_mz.reshape(shape), delta_Sz.reshape(shape),
+                                      c["rows"], scale=self._scale, lengths=c["lengths"])
+        if c["rotary"] is not None:  # in place: queries and keys as attention read them, then before the norm
+            dw = qk_norm_rotary_backward_into((*q, *k), *q, *k, *c["raw"], c["inv"], **c["rotary"])
             if dw:
                 n, m = self._norms()
                 n.delta_mw, n.delta_Sw, m.delta_mw, m.delta_Sw = dw
