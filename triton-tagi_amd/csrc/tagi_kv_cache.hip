@@ -169,7 +169,7 @@ int sizes(const char* what, Args& a, int64_t B, int64_t T) {
   TAGI_REQUIRE(T >= 0 && T < (1ll << 31), "%s: bad sizes", what);
   a.B = B, a.rows = T * a.c.G, a.L = lanes_of(a.c.D);
   // fewer than 2^32 threads in one dimension
-  TAGI_REQUIRE(a.rows < (1ll << 32) / a.L, "%s: too large", what);
+  TAGI_REQUIRE(a.rows < (1ll << 32) / a.L && cdiv(a.rows, kThreads / a.L) * kThreads < (1ll << 32), "%s: too large", what);
   return TAGI_OK;
 }
 dim3 grid_of(const Args& a) {
