@@ -60,8 +60,9 @@ class RemaxAttention(QkvProjections):
         """``num_kv_heads``: key and value heads, a divisor of ``num_heads``. ``max_len``: tokens of a
         served sequence. ``qk_norm``: RMSNorm of each query and key head. ``rotary``: queries and keys
         turn by their positions, all pairs (u, u + head_dim / 2) of a head; ``rotary_sections`` splits
-        the pairs among several axes of positions, which ``forward`` then takes. ``cache_dtype``,
-        ``page_size``: of the cache that serving keeps."""
+        the pairs among several axes of positions, which this layer's ``forward`` then takes: a
+        ``Sequential`` passes none, and ``prompt`` and ``step`` know only the tokens' order, so they
+        refuse such a layer. ``cache_dtype``, ``page_size``: of the cache that serving keeps."""
         num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
         if embed_dim % num_heads != 0:
             raise ValueError(f"embed_dim ({embed_dim}) must be divisible by num_heads ({num_heads})")
