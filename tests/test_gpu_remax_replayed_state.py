@@ -116,3 +116,28 @@ def test_recorded_prompts(dev):
     part.copy_(x[:, 7:11]), tok.copy_(x[:, 11:12])
     graph.replay()
     near(pm, mu[:, 7:11], "prompt of a later state"), near(m[:, 0], mu[:, 11], "token of a later state")
+
+
+def test_recorded_first_prompts(dev):
+    """A first prompt of a padded batch and a token after it, recorded: every replay begins anew."""
+    net = network(max_len=32, page_size=4)
+    x = batch(3, 20, 9)[0].to(dev)
+    mu, _ = net.forward(x)
+    part, tok, n = x[:, :8].clone(), x[:, 8:9].clone(), torch.tensor([8, 8, 8], device=dev)
+    _, _, warm = net.prompt(part, lengths=n)
+    net.decode(tok, warm)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pm, _, states = net.prompt(part, lengths=n)
+        m, _ = net.decode(tok, states)
+    for cut in (8, 3, 6):
+        n.fill_(cut)
+        tok.copy_(x[:, cut:cut + 1])
+        for _ in range(2):
+            graph.replay()
+            near(pm[:, :cut], mu[:, :cut], f"prompt of {cut}"), near(m[:, 0], mu[:, cut], f"token after {cut}")
+            assert states[1][0].lengths.tolist() == [cut + 1] * 3
+            net.forward(x)
+        near(net.decode(x[:, cut + 1:cut + 2], states)[0][:, 0], mu[:, cut + 1], "eager token")
+        near(net.prompt(x[:, cut + 2:cut + 5], states=states)[0], mu[:, cut + 2:cut + 5], "eager prompt")
