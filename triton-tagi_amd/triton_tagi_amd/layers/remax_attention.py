@@ -267,6 +267,18 @@ class RemaxAttention(QkvProjections):
         end.lengths, end.used = total, None if torch.cuda.is_current_stream_capturing() else bound
         return mo.view(ma.shape), So.view(ma.shape), end
 
+    def _check_state(self, state, batch: int, active: Tensor | None) -> None:
+        if not isinstance(state, AttentionState) or state.lengths.shape[0] != batch:
+            raise ValueError(f"state: expected an AttentionState of {batch} sequences")
+        if active is not None and (active.dtype not in (torch.bool, torch.uint8) or tuple(active.shape) != (batch,)):
+            raise TypeError(f"active: expected a bool or uint8 tensor of ({batch},)")
+
+    def check_step(self, state: AttentionState, batch: int, active: Tensor | None = None) -> None:
+        """Refuses what ``step`` would refuse of a state, before any layer of a network has taken the token."""
+        self._check_state(state, batch, active)
+        if state.used is None or state.used >= min(self.max_len, state.room):  # else the count says enough
+            self._bound(state, 1, None if active is None else (active != 0).to(torch.int64))
+
     def step(self, ma: Tensor, Sa: Tensor, state: AttentionState, active: Tensor | None = None) -> tuple[Tensor, Tensor]:
         """One token of every sequence, (B, E) or (B, 1, E); ``state`` is advanced in place. ``active``
         (B,): sequences that are off keep their state and get zeros. A recorded graph's replays
@@ -276,13 +288,8 @@ class RemaxAttention(QkvProjections):
             raise ValueError(f"RemaxAttention.step: expected (batch, features) or (batch, 1, features), "
                              f"got {tuple(ma.shape)}")
         B, E = ma.shape[0], ma.shape[-1]
-        if not isinstance(state, AttentionState) or state.lengths.shape[0] != B:
-            raise ValueError(f"state: expected an AttentionState of {B} sequences")
-        on = None
-        if active is not None:
-            if active.dtype not in (torch.bool, torch.uint8) or tuple(active.shape) != (B,):
-                raise TypeError(f"active: expected a bool or uint8 tensor of ({B},)")
-            on = (active != 0).to(torch.int64)
+        self._check_state(state, B, active)
+        on = None if active is None else (active != 0).to(torch.int64)
         bound = self._bound(state, 1, on)
         at = state.lengths
         positions = self._positions(ma.reshape(B, 1, E), at, None)

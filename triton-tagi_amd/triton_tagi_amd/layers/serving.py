@@ -62,15 +62,29 @@ def run_prompt(layers, ma: Tensor, Sa: Tensor | None, lengths: Tensor | None, st
     return ma, Sa, out
 
 
-def run_step(layers, ma: Tensor, Sa: Tensor | None, states, active: Tensor | None):
-    """(ma, Sa) of one token of every sequence; the states are advanced in place."""
+def check_step(layers, states, batch: int, active: Tensor | None) -> None:
+    """A token that one layer has no room for is refused before another's state has taken it."""
     if len(states) != len(layers):
         raise ValueError(f"states: {len(states)} entries for {len(layers)} layers")
+    for layer, state in zip(layers, states):
+        if isinstance(layer, RemaxAttention):
+            layer.check_step(state, batch, active)
+        elif isinstance(layer, ResidualRMSNorm):
+            check_step(layer.layers, state, batch, active)
+
+
+def run_step(layers, ma: Tensor, Sa: Tensor | None, states, active: Tensor | None):
+    """(ma, Sa) of one token of every sequence; the states are advanced in place."""
+    check_step(layers, states, ma.shape[0], active)
+    return _run_step(layers, ma, Sa, states, active)
+
+
+def _run_step(layers, ma: Tensor, Sa: Tensor | None, states, active: Tensor | None):
     for layer, state in zip(layers, states):
         if isinstance(layer, _STATEFUL):
             ma, Sa = layer.step(ma, Sa, state, active)
         elif isinstance(layer, ResidualRMSNorm):
-            bm, bS = run_step(layer.layers, ma, Sa, state, active)
+            bm, bS = _run_step(layer.layers, ma, Sa, state, active)
             ma, Sa = layer._close(bm, bS, ma, Sa)[:2]
         else:
             ma, Sa = _tokenwise(layer, ma, Sa)
